@@ -285,7 +285,7 @@ def _run_own(s):
                  strides(s["out"]), _ptr(s["lse"]), *sizes, *grads)
         return {n: s[n] for n in ("out", "dq", "dk", "dv")}
     n = len(s["shapes"])
-    hyper = omb.MuonHyper(lr=RATE, momentum=case["momentum"], weight_decay=case["decay"], eps=EPS, nesterov=case["nesterov"], steps=STEPS, match_rms=1)
+    hyper = omb.MuonHyper(lr=RATE, momentum=case["momentum"], weight_decay=case["decay"], eps=EPS, grad_scale=1.0, nesterov=case["nesterov"], steps=STEPS, match_rms=1)
     lists = [(C.c_void_p * n)(*[t.data_ptr() for t in s[name]]) for name in ("p", "g", "m")]
     ctx.call("om_optim_muon_step", ctx.handle, omb.i32(n), *lists, None, omb.int_array([r for r, _ in s["shapes"]]),
              omb.int_array([c for _, c in s["shapes"]]), C.byref(hyper), None)
