@@ -549,6 +549,89 @@ int32_t om_attention_bwd_bf16(om_ctx* ctx, const uint16_t* g16, const float* g, 
                               const om_head_strides* dqs, float* dk, uint16_t* dk16, const om_head_strides* dks, float* dv,
                               uint16_t* dv16, const om_head_strides* dvs);
 
+/* ---- attention by rule ------------------------------------------------------------------------------------- */
+
+/* Which keys a query sees, and what is done to a score in front of the softmax, as a rule instead of a stored [lq, lk]
+ * matrix. Query i stands at position i + q_offset, key j at position j.
+ *   visible(i, j) = (j < prefix[b]  or  ((not causal or j <= i + q_offset) and (window == 0 or |i + q_offset - j| < window)))
+ *                   and q_documents[b, i] == k_documents[b, j] and q_documents[b, i] >= 0      (where documents are given)
+ *   score(i, j)   = s - slopes[head] * |i + q_offset - j|  with  s = scale q_i . k_j, or softcap * tanh(scale q_i . k_j / softcap)
+ * A row that sees no key gives zeros, a log-sum-exp of minus infinity and no gradients. A hidden score is never looked at, but
+ * rows of k and v (and of the output's gradient) have to be finite wherever they lie in range: a weight of zero times an
+ * infinite value is not a number, here as in the plain product. All pointers are device pointers and may be NULL. */
+typedef struct om_attention_rule {
+  int32_t causal;
+  int32_t window;             /* 0: none; else a positive number of positions */
+  int32_t q_offset;           /* |q_offset| <= 2^30; lk - lq puts the last query at the last key */
+  float softcap;              /* 0: none; else positive */
+  const float* slopes;        /* [h], of the query heads; constants: they get no gradient */
+  const int32_t* prefix;      /* [b]: keys before it are seen by every query of the sequence's documents */
+  const int32_t* q_documents; /* [b, lq]; both or none; a negative number marks padding, which neither sees nor is seen */
+  const int32_t* k_documents; /* [b, lk] */
+} om_attention_rule;
+/* out = softmax(score) v over the visible keys, with h query heads over hkv key heads (h a multiple of hkv: query head i reads
+ * key head i / (h / hkv)); stands beside om_attention_fwd_strided, which takes a stored mask and equal heads. Activations are
+ * addressed through om_head_strides; d is 1 to 256. Products, sums and exponentials are fp32 whatever the context's flags.
+ * lse [b, h, lq] (may be NULL) receives the row log-sum-exp for the backward. lk == 0 gives zeros. */
+int32_t om_rule_attention_fwd(om_ctx* ctx, const om_attention_rule* rule, const float* q, const om_head_strides* qs, const float* k,
+                              const om_head_strides* ks, const float* v, const om_head_strides* vs, int32_t b, int32_t h,
+                              int32_t hkv, int32_t lq, int32_t lk, int32_t d, float scale, float* out, const om_head_strides* os,
+                              float* lse);
+/* dq, dk, dv (each may be NULL) from g = dOut, the forward's output and its log-sum-exp; the gradient of a key head is the sum
+ * over its query heads in increasing order. Beside om_attention_bwd_strided_out. */
+int32_t om_rule_attention_bwd(om_ctx* ctx, const om_attention_rule* rule, const float* g, const om_head_strides* gs, const float* q,
+                              const om_head_strides* qs, const float* k, const om_head_strides* ks, const float* v,
+                              const om_head_strides* vs, const float* out, const om_head_strides* os, const float* lse, int32_t b,
+                              int32_t h, int32_t hkv, int32_t lq, int32_t lk, int32_t d, float scale, float* dq,
+                              const om_head_strides* dqs, float* dk, const om_head_strides* dks, float* dv,
+                              const om_head_strides* dvs);
+/* The same with bfloat16 operands: scores, softmax statistics and sums in fp32, the weights and the scores' gradients rounded to
+ * bfloat16 as operands of the products behind them. The forward writes out, out16 (same strides) or both, the backward each
+ * gradient as fp32, bfloat16 or both; the backward takes the output as bfloat16. */
+int32_t om_rule_attention_fwd_bf16(om_ctx* ctx, const om_attention_rule* rule, const uint16_t* q16, const om_head_strides* qs,
+                                   const uint16_t* k16, const om_head_strides* ks, const uint16_t* v16, const om_head_strides* vs,
+                                   int32_t b, int32_t h, int32_t hkv, int32_t lq, int32_t lk, int32_t d, float scale, float* out,
+                                   uint16_t* out16, const om_head_strides* os, float* lse);
+int32_t om_rule_attention_bwd_bf16(om_ctx* ctx, const om_attention_rule* rule, const uint16_t* g16, const om_head_strides* gs,
+                                   const uint16_t* q16, const om_head_strides* qs, const uint16_t* k16, const om_head_strides* ks,
+                                   const uint16_t* v16, const om_head_strides* vs, const uint16_t* out16, const om_head_strides* os,
+                                   const float* lse, int32_t b, int32_t h, int32_t hkv, int32_t lq, int32_t lk, int32_t d,
+                                   float scale, float* dq, uint16_t* dq16, const om_head_strides* dqs, float* dk, uint16_t* dk16,
+                                   const om_head_strides* dks, float* dv, uint16_t* dv16, const om_head_strides* dvs);
+
+/* ---- rotary positions -------------------------------------------------------------------------------------------- */
+
+/* How fast the pairs of columns turn: pair j by base^(-2 j / columns) radians a position, then
+ *   OM_ROTARY_PLAIN   nothing more (the other fields are not looked at);
+ *   OM_ROTARY_LINEAR  divided by factor (positions interpolated into the trained range);
+ *   OM_ROTARY_BASE    with the base raised to base * factor^(columns / (columns - 2)): the slowest pair is divided by factor;
+ *   OM_ROTARY_PARTS   pairs with fewer than low_turns turns over original_context positions divided by factor, those with more
+ *                     than high_turns left, and a linear blend in the number of turns between the two. */
+typedef enum om_rotary_scaling { OM_ROTARY_PLAIN = 0, OM_ROTARY_LINEAR = 1, OM_ROTARY_BASE = 2, OM_ROTARY_PARTS = 3 } om_rotary_scaling;
+typedef struct om_rotary_spec {
+  int32_t columns;            /* of a head that are turned: even, 2 to 256 */
+  int32_t scaling;            /* om_rotary_scaling */
+  double base;                /* above 1 */
+  double factor;              /* 1 or more */
+  double original_context;    /* positive */
+  double low_turns, high_turns; /* 0 <= low < high */
+} om_rotary_spec;
+/* Fills inv_freq_host[columns / 2] (host memory) in double. ctx is only where the error message goes and may be NULL. */
+int32_t om_rotary_frequencies(om_ctx* ctx, const om_rotary_spec* spec, double* inv_freq_host);
+/* y = x with the first 2 * pairs columns of every head turned by its token's angles: the pair (x0, x1) becomes
+ * (x0 cos - x1 sin, x0 sin + x1 cos) * magnitude, cos and sin of position * inv_freq_host[j]; the columns behind are copied.
+ * adjacent: pair j is columns (2 j, 2 j + 1), else (j, j + pairs). inverse: turned back by the same angles (times magnitude):
+ * the gradient of the forward call. The position of token (b, l) is first_position + positions[b * positions_batch_stride + l],
+ * or first_position + l where positions is NULL. Angles are reduced in double, so far positions lose nothing. x and y may be
+ * the same tensor with the same strides; inv_freq_host is read during the call. d >= 2 * pairs, pairs at most 128. */
+int32_t om_rotary(om_ctx* ctx, const float* x, const om_head_strides* xs, const int32_t* positions, int64_t positions_batch_stride,
+                  int32_t first_position, int32_t b, int32_t h, int32_t l, int32_t d, const double* inv_freq_host, int32_t pairs,
+                  int32_t adjacent, float magnitude, int32_t inverse, float* y, const om_head_strides* ys);
+int32_t om_rotary_bf16(om_ctx* ctx, const uint16_t* x16, const om_head_strides* xs, const int32_t* positions,
+                       int64_t positions_batch_stride, int32_t first_position, int32_t b, int32_t h, int32_t l, int32_t d,
+                       const double* inv_freq_host, int32_t pairs, int32_t adjacent, float magnitude, int32_t inverse, uint16_t* y16,
+                       const om_head_strides* ys);
+
 /* ---- pooling and convolution ---------------------------------------------------------------------------- */
 
 /* The 16 integers of ConvShape (src/OneModel/Kernels/Conv.cs:11-13) in the reference's order. */
@@ -700,6 +783,22 @@ int32_t om_optim_adam_step_b16(om_ctx* ctx, int32_t n_tensors, float* const* p_h
                                float* const* m_host, float* const* v_host, float* const* vmax_host,
                                uint16_t* const* p16_host, const int64_t* len_host, const om_adam_hyper* hyper_host,
                                const om_adam_hyper* hyper_dev);
+/* The update of weight matrices by their orthogonalised momentum (Muon), for the two-dimensional parameters of a model whose
+ * others go to om_optim_adam_step. Per matrix [rows, cols], row-major and contiguous, with g the gradient times grad_scale:
+ *   m = momentum m + (1 - momentum) g;  u = nesterov ? momentum m + (1 - momentum) g : m;  X = u / max(|u|, eps) (Frobenius norm),
+ *   steps times: G = X X^T (of the smaller side), X = 3.4445 X + (-4.7750 G + 2.0315 G G) X,
+ *   p = (1 - lr weight_decay) p - lr s X, with s = match_rms ? 0.2 sqrt(max(rows, cols)) : sqrt(max(1, rows / cols)).
+ * Products, norms and the state keep fp32 accuracy whatever the context's flags. p16_host (may be NULL, as may be its entries):
+ * the bfloat16 copies of the weights, refreshed by the update. hyper_dev (may be NULL): a device copy that the kernels read
+ * in place of hyper_host (so that a captured update follows a schedule); steps is always taken from hyper_host. A matrix with
+ * no elements is left alone; p, g and m of one call may not overlap. steps is 1 to 10, sides are at most 65536. */
+typedef struct om_muon_hyper {
+  float lr, momentum, weight_decay, eps, grad_scale;
+  int32_t nesterov, steps, match_rms;
+} om_muon_hyper;
+int32_t om_optim_muon_step(om_ctx* ctx, int32_t n_tensors, float* const* p_host, const float* const* g_host, float* const* m_host,
+                           uint16_t* const* p16_host, const int32_t* rows_host, const int32_t* cols_host,
+                           const om_muon_hyper* hyper_host, const om_muon_hyper* hyper_dev);
 typedef struct om_sgd_hyper {
   float lr, weight_decay, momentum, dampening, grad_scale;
   int32_t nesterov;

@@ -704,6 +704,8 @@ void RunBackwardOp(Engine& e, BackwardRecord& r, const Tensor& g) {
     case OpKind::BatchNorm: BatchNormBackward(r, g); break;
     case OpKind::Embedding: EmbeddingBackward(r, g); break;
     case OpKind::Attention: AttentionBackward(r, g); break;
+    case OpKind::Rotary: RotaryBackward(r, g); break;
+    case OpKind::RuleAttention: RuleAttentionBackward(r, g); break;
     case OpKind::Concat: {
       int axis = (int)r.Ints[0];
       int start = 0;

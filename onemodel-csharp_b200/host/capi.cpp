@@ -218,7 +218,23 @@ OMH_API int32_t omh_call(const char* op, int32_t n_in, omh_tensor* const* in, in
     else if (name == "feed_forward") r = Ops::FeedForward(T(0), T(1), T(2), T(3), T(4), I(0) != 0);
     else if (name == "attention") r = Ops::Attention(T(0), T(1), T(2), T(3), (float)F(0, 0));
     else if (name == "attention_heads") r = Ops::AttentionHeads(T(0), T(1), T(2), (int)I(0, 1), T(3), (float)F(0, 0));
-    else if (name == "concat") {
+    else if (name == "rotary" || name == "rotary_heads") {
+      // ints [columns, adjacent, first position, scaling, heads]; floats [base, factor, original context, low turns, high turns,
+      // magnitude]; inputs x, positions
+      RotarySpec s;
+      s.columns = (int)I(0); s.adjacent = I(1) != 0; s.firstPosition = (int)I(2); s.scaling = (int)I(3);
+      s.base = F(0, 10000.0); s.factor = F(1, 1.0); s.originalContext = F(2, 0.0); s.lowTurns = F(3, 1.0); s.highTurns = F(4, 32.0);
+      s.magnitude = (float)F(5, 1.0);
+      r = name == "rotary" ? Ops::Rotary(T(0), T(1), s) : Ops::RotaryHeads(T(0), (int)I(4), T(1), s);
+    } else if (name == "rule_attention" || name == "rule_attention_heads") {
+      // ints [causal, window, q offset, heads, key heads]; floats [cap, scale]; inputs q, k, v, prefix, the queries' and the keys'
+      // documents, slopes
+      AttentionRule a;
+      a.causal = I(0) != 0; a.window = (int)I(1); a.qOffset = (int)I(2); a.softcap = (float)F(0);
+      a.prefix = T(3); a.qDocuments = T(4); a.kDocuments = T(5); a.slopes = T(6);
+      r = name == "rule_attention" ? Ops::RuleAttention(T(0), T(1), T(2), a, (float)F(1))
+                                   : Ops::RuleAttentionHeads(T(0), T(1), T(2), (int)I(3), (int)I(4), a, (float)F(1));
+    } else if (name == "concat") {
       std::vector<Tensor> xs;
       for (int i = 0; i < n_in; i++) xs.push_back(T(i));
       r = Ops::Concat(xs, (int)I(0));
@@ -277,7 +293,8 @@ OMH_API int32_t omh_call(const char* op, int32_t n_in, omh_tensor* const* in, in
 struct omh_optim { std::unique_ptr<Optimizer> o; };
 
 // kind: 0 SGD (f: lr, momentum, dampening, weight_decay; i: nesterov), 1 Adam, 2 AdamW (f: lr, beta1, beta2, eps,
-// weight_decay; i: amsgrad), 3 SparseAdam (f: lr, beta1, beta2, eps).
+// weight_decay; i: amsgrad), 3 SparseAdam (f: lr, beta1, beta2, eps), 4 Muon (f: lr, momentum, weight_decay, eps; i: nesterov,
+// steps, match_rms).
 OMH_API int32_t omh_optim_create(int32_t kind, int32_t n, omh_tensor* const* params, const double* f, const int64_t* i,
                                  omh_optim** out) {
   return Guard([&] {
@@ -288,6 +305,7 @@ OMH_API int32_t omh_optim_create(int32_t kind, int32_t n, omh_tensor* const* par
     else if (kind == 1) o.reset(new Adam(ps, (float)f[0], (float)f[1], (float)f[2], (float)f[3], (float)f[4], false, i[0] != 0));
     else if (kind == 2) o.reset(new AdamW(ps, (float)f[0], (float)f[1], (float)f[2], (float)f[3], (float)f[4], i[0] != 0));
     else if (kind == 3) o.reset(new SparseAdam(ps, (float)f[0], (float)f[1], (float)f[2], (float)f[3]));
+    else if (kind == 4) o.reset(new Muon(ps, (float)f[0], (float)f[1], (float)f[2], i[0] != 0, (int)i[1], i[2] != 0, (float)f[3]));
     else throw InvalidOperationException("Unknown optimizer kind.");
     *out = new omh_optim{std::move(o)};
   });

@@ -183,12 +183,13 @@ std::array<int64_t, kMaxRank> ContiguousStrides(const Shape& s);
 // ---- autograd types ---------------------------------------------------------------------------------------------------
 // The reference's 43 kinds (Autograd.cs:7-97) plus the fused kinds this backend records in their place: Linear for
 // the Reshape/MatMul/Add chain of Ops.Linear, CrossEntropy for LogSoftmax+NllLoss, GlobalAvgPool for Mean over planes,
-// FeedForward for Linear -> Gelu -> Linear when the activation rides in the products' epilogues.
+// FeedForward for Linear -> Gelu -> Linear when the activation rides in the products' epilogues, and the decoder's Rotary and
+// RuleAttention, which the reference does not have.
 enum class OpKind {
   None = 0, Add, Sub, Mul, Div, Neg, Relu, MatMul, MaxPool2d, Cast, Slice, Permute, Reshape, Expand, Flip, Select, Gelu,
   Sigmoid, Tanh, Sum, Mean, Softmax, LogSoftmax, LayerNorm, BatchNorm, Conv2d, AvgPool2d, Concat, Embedding, NllLoss,
   Attention, Lstm, Gru, CtcLoss, ConvTranspose2d, Resize2d, Conv1d, BatchMatMul, Erf, Exp, Sqrt, Pow, Where, Gather,
-  Linear, CrossEntropy, Dropout, FeedForward
+  Linear, CrossEntropy, Dropout, FeedForward, Rotary, RuleAttention
 };
 
 struct AutogradMeta {
@@ -348,6 +349,25 @@ struct ConvTranspose2dParams {
   int strideH = 1, strideW = 1, padH = 0, padW = 0, outPadH = 0, outPadW = 0, dilH = 1, dilW = 1, groups = 1;
 };
 
+// The rule of om_attention_rule over tensors (empty: not given). Slopes are constants: they get no gradient.
+struct AttentionRule {
+  bool causal = false;
+  int window = 0, qOffset = 0;
+  float softcap = 0.f;
+  Tensor prefix, qDocuments, kDocuments, slopes;   // int32 [B], int32 [B,Lq], int32 [B,Lk], float32 [H]
+};
+// How om_rotary turns the heads: om_rotary_spec (columns 0: the whole head), the pairs' layout, and what positions start at.
+struct RotarySpec {
+  int columns = 0;
+  bool adjacent = false;
+  int firstPosition = 0;
+  int scaling = OM_ROTARY_PLAIN;
+  double base = 10000.0, factor = 1.0, originalContext = 0.0, lowTurns = 1.0, highTurns = 32.0;
+  float magnitude = 1.f;
+};
+void RotaryBackward(BackwardRecord& r, const Tensor& g);
+void RuleAttentionBackward(BackwardRecord& r, const Tensor& g);
+
 struct Ops {
   static Tensor Add(const Tensor& a, const Tensor& b);
   static Tensor Sub(const Tensor& a, const Tensor& b);
@@ -384,6 +404,13 @@ struct Ops {
   static Tensor Linear(const Tensor& x, const Tensor& weight, const Tensor& bias);
   static Tensor Attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask, float scale = 0.f);
   static Tensor AttentionHeads(const Tensor& q, const Tensor& k, const Tensor& v, int heads, const Tensor& mask, float scale = 0.f);
+  // Attention whose mask follows from a rule, with query heads that may share key heads: q [B,H,L,D], k and v [B,Hkv,Lk,D], or
+  // [B,L,H*D] and [B,Lk,Hkv*D] in the Heads form. Under bfloat16 products the operands are the tensors' bfloat16 copies.
+  static Tensor RuleAttention(const Tensor& q, const Tensor& k, const Tensor& v, const AttentionRule& rule, float scale = 0.f);
+  static Tensor RuleAttentionHeads(const Tensor& q, const Tensor& k, const Tensor& v, int heads, int keyHeads, const AttentionRule& rule, float scale = 0.f);
+  // The heads of x turned by their tokens' positions (int32 [L] or [B,L]; empty: 0, 1, ...).
+  static Tensor Rotary(const Tensor& x, const Tensor& positions, const RotarySpec& spec);
+  static Tensor RotaryHeads(const Tensor& x, int heads, const Tensor& positions, const RotarySpec& spec);
   // Several Linear layers over the same input whose weights (and biases) are adjacent in memory, as one product:
   // returns [..., sum of out features]. Throws when the parameters are not adjacent.
   // bf16_only_result: the caller consumes the result as bfloat16 only (the attention kernels of the bfloat16 tier); under
@@ -781,6 +808,29 @@ class SparseAdam : public Optimizer {
  private:
   float beta1_, beta2_, eps_, step_size_ = 0.f;
   std::vector<Tensor> m_, v_;
+};
+
+// The update of weight matrices by their orthogonalised momentum (om_optim_muon_step); not in the reference. Every parameter
+// is a matrix: a model's vectors, and its embedding tables, go to AdamW.
+class Muon : public Optimizer {
+ public:
+  Muon(std::vector<Tensor> parameters, float lr = 1e-3f, float momentum = 0.95f, float weightDecay = 0.1f, bool nesterov = true, int steps = 5,
+       bool matchRms = true, float eps = 1e-7f);
+  size_t HyperBytes() const override { return sizeof(om_muon_hyper); }
+  void FillHyper(void* host, int64_t step) const override;
+  std::vector<Tensor> StateTensors() const override { return buffers_; }
+  std::string Kind() const override { return "muon"; }
+  std::vector<std::pair<std::string, float>> HyperParameters() const override;
+  std::vector<StateEntry> NamedState() override;
+  float GradScale = 1.f;
+ protected:
+  bool WritesBf16Copies() const override { return true; }
+  void Launch(const std::vector<float*>& p, const std::vector<const float*>& g, const std::vector<int64_t>& len) override;
+ private:
+  float momentum_, eps_;
+  bool nesterov_, match_rms_;
+  int steps_;
+  std::vector<Tensor> buffers_;
 };
 
 struct GradClip {

@@ -295,6 +295,57 @@ void SparseAdam::UpdateSparse(int index, const Tensor& parameter, const RowSpars
   v_[(size_t)index].MarkModified();
 }
 
+// ---- Muon -----------------------------------------------------------------------------------------------------------
+Muon::Muon(std::vector<Tensor> parameters, float lr, float momentum, float weightDecay, bool nesterov, int steps, bool matchRms, float eps)
+    : Optimizer(std::move(parameters)), momentum_(momentum), eps_(eps), nesterov_(nesterov), match_rms_(matchRms), steps_(steps) {
+  LearningRate = lr;
+  WeightDecay = weightDecay;
+  if (!(momentum >= 0.f && momentum < 1.f)) throw ArgumentOutOfRangeException("The momentum must be in [0, 1).");
+  if (!(eps > 0.f) || !std::isfinite(eps)) throw ArgumentOutOfRangeException("Epsilon must be positive and finite.");
+  if (steps < 1 || steps > 10) throw ArgumentOutOfRangeException("Muon takes 1 to 10 steps.");
+  for (const Tensor& p : params_) {
+    if (p.Rank() != 2) throw TensorShapeException("Muon parameters must be matrices, not " + p.GetShape().ToString() + ".");
+    buffers_.push_back(Tensor::Zeros(DType::F32, p.GetShape()));
+  }
+}
+
+std::vector<std::pair<std::string, float>> Muon::HyperParameters() const {
+  return {{"lr", LearningRate}, {"momentum", momentum_}, {"weight_decay", WeightDecay}, {"epsilon", eps_}, {"nesterov", nesterov_ ? 1.f : 0.f},
+          {"steps", (float)steps_}, {"match_rms", match_rms_ ? 1.f : 0.f}};
+}
+std::vector<Optimizer::StateEntry> Muon::NamedState() {
+  std::vector<StateEntry> out;
+  for (size_t i = 0; i < buffers_.size(); i++) out.push_back({"momentum_buffer." + std::to_string(i), buffers_[i], nullptr});
+  return out;
+}
+
+void Muon::FillHyper(void* host, int64_t) const {
+  om_muon_hyper* h = (om_muon_hyper*)host;
+  h->lr = LearningRate;
+  h->momentum = momentum_;
+  h->weight_decay = WeightDecay;
+  h->eps = eps_;
+  h->grad_scale = GradScale;
+  h->nesterov = nesterov_;
+  h->steps = steps_;
+  h->match_rms = match_rms_;
+}
+
+void Muon::Launch(const std::vector<float*>& p, const std::vector<const float*>& g, const std::vector<int64_t>&) {
+  om_muon_hyper h;
+  FillHyper(&h, StepCount + 1);
+  std::vector<float*> m;
+  std::vector<int32_t> rows, cols;
+  for (int i : index_) {
+    m.push_back(buffers_[(size_t)i].Data());
+    rows.push_back(params_[(size_t)i].GetShape()[0]);
+    cols.push_back(params_[(size_t)i].GetShape()[1]);
+  }
+  Check(om_optim_muon_step(C(), (int32_t)p.size(), p.data(), g.data(), m.data(), p16_.size() == p.size() ? p16_.data() : nullptr, rows.data(),
+                           cols.data(), &h, (const om_muon_hyper*)HyperDevice));
+  for (int i : index_) buffers_[(size_t)i].MarkModified();
+}
+
 // ---- clipping -------------------------------------------------------------------------------------------------------
 // The values of a row-sparse gradient stand in for the gradient, each row counted once (Schedules.cs:33,72,130); the entries
 // behind its row count are zero, so the whole storage is normed and scaled.

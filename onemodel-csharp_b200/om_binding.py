@@ -174,6 +174,43 @@ class DeviceArray:
             pass
 
 
+class HeadStrides(C.Structure):
+    """om_head_strides: element strides of an activation seen as [B, H, L, D]."""
+    _fields_ = [("batch", C.c_int64), ("head", C.c_int64), ("row", C.c_int64)]
+
+
+class AttentionRule(C.Structure):
+    """om_attention_rule: which keys a query sees; pointers are device pointers."""
+    _fields_ = [("causal", C.c_int32), ("window", C.c_int32), ("q_offset", C.c_int32), ("softcap", C.c_float), ("slopes", C.c_void_p),
+                ("prefix", C.c_void_p), ("q_documents", C.c_void_p), ("k_documents", C.c_void_p)]
+
+
+ROTARY_SCALING = dict(plain=0, linear=1, base=2, parts=3)
+
+
+class RotarySpec(C.Structure):
+    """om_rotary_spec: how fast the pairs of columns turn."""
+    _fields_ = [("columns", C.c_int32), ("scaling", C.c_int32), ("base", C.c_double), ("factor", C.c_double), ("original_context", C.c_double),
+                ("low_turns", C.c_double), ("high_turns", C.c_double)]
+
+
+class MuonHyper(C.Structure):
+    """om_muon_hyper."""
+    _fields_ = [("lr", C.c_float), ("momentum", C.c_float), ("weight_decay", C.c_float), ("eps", C.c_float), ("grad_scale", C.c_float),
+                ("nesterov", C.c_int32), ("steps", C.c_int32), ("match_rms", C.c_int32)]
+
+
+def rotary_frequencies(columns, base=10000.0, scaling="plain", factor=1.0, original_context=0.0, low_turns=1.0, high_turns=32.0):
+    """The radians a position of every pair of columns (om_rotary_frequencies), as the array om_rotary takes."""
+    spec = RotarySpec(columns, ROTARY_SCALING[scaling], base, factor, original_context, low_turns, high_turns)
+    out = (C.c_double * 128)()
+    st = kernel_lib().om_rotary_frequencies(None, C.byref(spec), out)
+    if st != 0:
+        _raise(st, f"om_rotary_frequencies refuses columns {columns}, base {base}, scaling {scaling}, factor {factor}, context {original_context}, "
+                   f"turns {low_turns} to {high_turns}")
+    return out
+
+
 def i32(v):
     return C.c_int32(int(v))
 
@@ -380,7 +417,7 @@ class RowSparseGradient:
 
 
 class Optimizer:
-    """Sgd / Adam / AdamW / SparseAdam of RecursiveAI.OneModel.Training (Optimizers.cs)."""
+    """Sgd / Adam / AdamW / SparseAdam of RecursiveAI.OneModel.Training (Optimizers.cs), and Muon, which the reference does not have."""
 
     def __init__(self, kind, params, floats, ints):
         self.params = list(params)
@@ -405,6 +442,11 @@ class Optimizer:
     @staticmethod
     def sparse_adam(params, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8):
         return Optimizer(3, params, [lr, beta1, beta2, eps], [0])
+
+    @staticmethod
+    def muon(params, lr=1e-3, momentum=0.95, weight_decay=0.1, nesterov=True, steps=5, match_rms=True, eps=1e-7):
+        """The update of weight matrices by their orthogonalised momentum; a model's other parameters go to adamw."""
+        return Optimizer(4, params, [lr, momentum, weight_decay, eps], [1 if nesterov else 0, steps, 1 if match_rms else 0])
 
     def step(self):
         _hcheck(host_lib().omh_optim_step(self.h))
