@@ -9,7 +9,7 @@ constexpr int RULE_GRAIN = 64;   // rows per entry of the document ranges: every
 
 struct RuleArgs {
   int causal, window, q_offset;
-  float softcap, scale;
+  float softcap, inv_softcap, scale;
   const float* slopes;
   const int32_t* prefix;
   const int32_t *q_docs, *k_docs;
@@ -69,7 +69,8 @@ __device__ __forceinline__ int rule_documents(const RuleArgs& r, int b, int i0, 
   if (qhi < 0 || khi < 0 || qlo > khi || klo > qhi) return 0;
   return whole ? 2 : 1;
 }
-// 0: nothing of the tile is visible; 1: some may be; 2: all of it is, and it lies inside the matrix.
+// 0: nothing of the tile is visible; 1: some may be; 2: every query of the sequence in it sees all of its keys, none of them beyond
+// the last.
 __device__ __forceinline__ int rule_tile(const RuleArgs& r, int prefix, int b, int i0, int nq, int j0, int nk) {
   const int i1 = min(i0 + nq * RULE_GRAIN, r.lq), j1 = min(j0 + nk * RULE_GRAIN, r.lk);
   if (i0 >= i1 || j0 >= j1) return 0;
@@ -77,7 +78,7 @@ __device__ __forceinline__ int rule_tile(const RuleArgs& r, int prefix, int b, i
   if (!(j0 < s.prefix || (j0 < s.hi && j1 > s.lo))) return 0;
   const int docs = rule_documents(r, b, i0, nq, j0, nk);
   if (docs != 2) return docs;
-  if (i1 - i0 != nq * RULE_GRAIN || j1 - j0 != nk * RULE_GRAIN) return 1;
+  if (j1 - j0 != nk * RULE_GRAIN) return 1;
   if (j1 <= s.prefix) return 2;
   const long long p0 = (long long)i0 + r.q_offset, p1 = (long long)i1 - 1 + r.q_offset;
   if (r.causal && j1 - 1 > p0) return 1;
@@ -112,7 +113,21 @@ struct RuleCall {
 int32_t rule_check(om_ctx* ctx, const char* who, const om_attention_rule* rule, int b, int h, int hkv, int lq, int lk, int d, float scale);
 int32_t rule_operand(om_ctx* ctx, const char* who, const void* p, const om_head_strides* s, int d);
 int32_t rule_result(om_ctx* ctx, const char* who, const om_head_strides* s, int b, int h, int l, int d);
+// Row dots rowsum(dO o O) beside the log-sum-exp times `unit`, [b * h][rule_rows_pitch(lq)] float2: what the backward kernels read.
+__host__ __device__ constexpr int rule_rows_pitch(int lq) { return (lq + 127) / 128 * 128; }
 int32_t rule_begin(om_ctx* ctx, const om_attention_rule* rule, int b, int h, int hkv, int lq, int lk, int d, float scale, RuleCall* call);
 void rule_end(om_ctx* ctx, RuleCall* call);
+// The tensor-pipe kernels for bfloat16 operands (om_rule_attention16.cu): whether they take a call, and the call. Pointers to
+// operands and bfloat16 results are to 2-byte elements; `rows` as above with log2 e for the unit.
+bool rule16_fwd_takes(const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
+                      const om_head_strides* vs, const float* out, const void* out16, const om_head_strides* os);
+int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
+                   const om_head_strides* vs, float* out, void* out16, const om_head_strides* os, float* lse);
+bool rule16_bwd_takes(const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
+                      const om_head_strides* ks, const void* v, const om_head_strides* vs, const float* dq, const void* dq16, const om_head_strides* dqs,
+                      const float* dk, const void* dk16, const om_head_strides* dks, const float* dv, const void* dv16, const om_head_strides* dvs);
+int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
+                   const om_head_strides* ks, const void* v, const om_head_strides* vs, const float2* rows, float* dq, void* dq16,
+                   const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs);
 
 }  // namespace om

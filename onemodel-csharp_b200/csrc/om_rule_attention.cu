@@ -59,7 +59,7 @@ int32_t rule_check(om_ctx* ctx, const char* who, const om_attention_rule* rule, 
   if (d < 1 || d > 256) return fail(ctx, OM_ERR_UNSUPPORTED, "%s: head dimension %d (1 to 256 are built)", who, d);
   if (h > 0 && (hkv == 0 || h % hkv)) return fail(ctx, OM_ERR_SHAPE, "%s: %d query heads do not share %d key heads evenly", who, h, hkv);
   if ((int64_t)b * h > 65535) return fail(ctx, OM_ERR_UNSUPPORTED, "%s: more than 65535 heads in one call", who);
-  if ((int64_t)b * h * (((int64_t)lq + 63) / 64 * 64) > INT_MAX) return fail(ctx, OM_ERR_UNSUPPORTED, "%s: more than 2^31 rows in one call", who);
+  if ((int64_t)b * h * (((int64_t)lq + 127) / 128 * 128) > INT_MAX) return fail(ctx, OM_ERR_UNSUPPORTED, "%s: more than 2^31 rows in one call", who);
   if (!isfinite(scale)) return fail(ctx, OM_ERR_ARG, "%s: the scale must be finite", who);
   if (rule->window < 0) return fail(ctx, OM_ERR_ARG, "%s: a negative window", who);
   if (rule->q_offset < -(1 << 30) || rule->q_offset > (1 << 30)) return fail(ctx, OM_ERR_ARG, "%s: q_offset %d is beyond 2^30", who, rule->q_offset);
@@ -88,6 +88,7 @@ int32_t rule_begin(om_ctx* ctx, const om_attention_rule* rule, int b, int h, int
   r.window = rule->window;
   r.q_offset = rule->q_offset;
   r.softcap = rule->softcap;
+  r.inv_softcap = rule->softcap > 0.f ? 1.f / rule->softcap : 0.f;
   r.scale = scale;
   r.slopes = rule->slopes;
   r.prefix = rule->prefix;
@@ -226,7 +227,7 @@ struct RaParams {
   float *out, *lse;               // forward
   __nv_bfloat16* out16;
   const float* lse_in;            // backward
-  const float2* rows;             // [b * h][nq64 * 64]: log-sum-exp (plus infinity for a row that sees nothing) and row dot
+  const float2* rows;             // [b * h][rule_rows_pitch(lq)]: log-sum-exp (plus infinity for a row that sees nothing) and row dot
   float *dq, *dk, *dv;
   __nv_bfloat16 *dq16, *dk16, *dv16;
   RaStrides dqs, dks, dvs;
@@ -315,12 +316,12 @@ rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
   ra_store<BM, DP>(p.out, p.out16, p.os, bi * p.os.batch + hi * p.os.head, i0, r.lq, p.d, ty, tx, acc, 1.f);
 }
 
-// Row dots rowsum(dO o O) beside the log-sum-exp, [b * h][nq64 * 64]; rows behind the last query get plus infinity and 0, so that
-// a weight recomputed from them is 0. A warp per row.
+// Row dots rowsum(dO o O) beside the log-sum-exp times `unit` (log2 e for the kernels that work with powers of two); rows behind
+// the last query, and those that see no key, get plus infinity and 0, so that a weight recomputed from them is 0. A warp per row.
 template <typename T>
 __global__ void __launch_bounds__(256)
-rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float* lse, int h, int lq, int lq_pad, int d, long long total,
-                 float2* __restrict__ rows) {
+rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float* lse, int h, int lq, int lq_pad, int d, float unit,
+                 long long total, float2* __restrict__ rows) {
   pdl_enter();
   const int lane = threadIdx.x & 31;
   for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
@@ -335,7 +336,7 @@ rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float
       for (int c = lane; c < d; c += 32) dot = fmaf(ra_value<T>(gp[c]), ra_value<T>(op[c]), dot);
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, x);
-      e = lse[bh * lq + i];
+      e = lse[bh * lq + i] * unit;
       if (e == -INFINITY) {
         e = INFINITY;
         dot = 0.f;
@@ -399,7 +400,7 @@ rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
   for (int gi = 0; gi < group; gi++) {
     const int head = hk * group + gi;
     const float slope = r.slopes ? r.slopes[head] : 0.f;
-    const float2* rows = p.rows + ((long long)bi * p.h + head) * r.nq64 * RULE_GRAIN;
+    const float2* rows = p.rows + ((long long)bi * p.h + head) * rule_rows_pitch(r.lq);
     for (int i0 = lo / BM * BM; i0 < hi; i0 += BM) {
       if (BM >= RULE_GRAIN ? rule_tile(r, prefix, bi, i0, NT, j0, NT) == 0 : rule_documents(r, bi, i0, 1, j0, 1) == 0) continue;
       __syncthreads();
@@ -431,7 +432,7 @@ rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
   const int bh = blockIdx.y, bi = bh / p.h, hi = bh - bi * p.h, hk = hi / (p.h / p.hkv);
   const int prefix = r.prefix ? r.prefix[bi] : 0;
   const float slope = r.slopes ? r.slopes[hi] : 0.f;
-  const float2* rows = p.rows + (long long)bh * r.nq64 * RULE_GRAIN;
+  const float2* rows = p.rows + (long long)bh * rule_rows_pitch(r.lq);
   ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + hi * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec);
   ra_load<T, BM, DP>(G, p.g + bi * p.gs.batch + hi * p.gs.head, p.gs.row, i0, r.lq, p.d, p.vec);
   if (r.q_docs)
@@ -546,6 +547,11 @@ static int32_t rule_fwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   ProfileScope prof(ctx, "om_rule_attention_fwd", 4.0 * b * h * (double)lq * lk * d, sizeof(T) * (2.0 * b * h * (double)lq * d + 2.0 * b * hkv * (double)lk * d));
   RuleCall call;
   OM_TRY(rule_begin(ctx, rule, b, h, hkv, lq, lk, d, scale, &call));
+  if (sizeof(T) == 2 && rule16_fwd_takes(call, q, qs, k, ks, v, vs, out, out16, os)) {
+    const int32_t st = rule16_fwd(ctx, call, q, qs, k, ks, v, vs, out, out16, os, lse);
+    rule_end(ctx, &call);
+    return st;
+  }
   RaParams<T> p = {};
   p.r = call.r; p.b = b; p.h = h; p.hkv = hkv; p.d = d;
   p.q = q; p.k = k; p.v = v; p.qs = ra_strides(qs); p.ks = ra_strides(ks); p.vs = ra_strides(vs);
@@ -589,12 +595,20 @@ static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   ProfileScope prof(ctx, "om_rule_attention_bwd", 10.0 * b * h * (double)lq * lk * d, sizeof(T) * (4.0 * b * h * (double)lq * d + 4.0 * b * hkv * (double)lk * d));
   RuleCall call;
   OM_TRY(rule_begin(ctx, rule, b, h, hkv, lq, lk, d, scale, &call));
-  const int lq_pad = call.r.nq64 * RULE_GRAIN;
+  const int lq_pad = rule_rows_pitch(lq);
   float2* rows = nullptr;
   int32_t st = pool_alloc(ctx, sizeof(float2) * (size_t)b * h * lq_pad, false, (void**)&rows);
   if (st == OM_OK) {
     const long long total = (long long)b * h * lq_pad;
-    launch_chained(ctx, rule_rows_kernel<T>, grid_for(ctx, total, 8, 16), 256, 0, g, ra_strides(gs), out, ra_strides(os), lse, h, lq, lq_pad, d, total, rows);
+    const bool tensor = sizeof(T) == 2 && rule16_bwd_takes(call, g, gs, q, qs, k, ks, v, vs, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs);
+    launch_chained(ctx, rule_rows_kernel<T>, grid_for(ctx, total, 8, 16), 256, 0, g, ra_strides(gs), out, ra_strides(os), lse, h, lq, lq_pad, d,
+                   tensor ? 1.4426950408889634f : 1.f, total, rows);
+    if (tensor) {
+      st = rule16_bwd(ctx, call, g, gs, q, qs, k, ks, v, vs, rows, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs);
+      pool_free(ctx, rows);
+      rule_end(ctx, &call);
+      return st;
+    }
     RaParams<T> p = {};
     p.r = call.r; p.b = b; p.h = h; p.hkv = hkv; p.d = d;
     p.q = q; p.k = k; p.v = v; p.g = g; p.qs = ra_strides(qs); p.ks = ra_strides(ks); p.vs = ra_strides(vs); p.gs = ra_strides(gs);

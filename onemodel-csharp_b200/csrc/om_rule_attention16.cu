@@ -1,0 +1,1184 @@
+// Attention by rule with bfloat16 operands on the tensor pipe (tcgen05), forward and backward, for head dimensions up to 128.
+//
+// Forward: a CTA holds 256 queries as two tiles of 128 and walks the tiles of 128 keys that the rule lets them see. Four warps per
+// query tile keep the running maximum and sum of a row per thread; while one tile's rows turn scores into weights the tensor pipe
+// works on the other's:  S = Q K^T (fp32 in tensor memory) -> weights exp2(S - m), rounded to bfloat16 over the scores they came
+// from, in tensor memory -> O += P V with P read from there. O stays in tensor memory; it is rescaled only when a row's maximum has
+// grown by more than 2^8 over the one in use, which changes no result: numerator and denominator share the factor.
+// With few rows the walk over the keys is split over CTAs that leave their sums, maxima and O for rule16_join_kernel, and the query
+// heads that share a key head become rows of one tile, so that keys and values are read once.
+//
+// Backward: the weights come back from the forward's log-sum-exp, once in rule16_dkv_kernel (a CTA per 128 keys walks the queries of
+// all heads that share them; rows are keys: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q) and once in rule16_dq_kernel (a
+// CTA per 128 queries walks the keys: dQ += dS K). Seven products for five, but no partial sums through memory: a part of dQ per
+// (query tile, key tile) is 128 KB of traffic against 0.3 us of tensor time for the two products that are done again.
+// P and dS are rounded to bfloat16 as operands (the only roundings of the backward besides the results').
+//
+// Every wait is bounded (om_tc.cuh). All sums are fp32 in an order that the shapes alone decide.
+#include <cuda_bf16.h>
+#include <math.h>
+
+#include "om_rule.cuh"
+#include "om_tc.cuh"
+
+namespace om {
+
+constexpr int R16_T = 128;                         // rows of every tile
+constexpr int R16_CHUNK = R16_T * 128;             // bytes of a [128 x 64] bfloat16 block, 128-byte swizzled rows
+constexpr int R16_THREADS = 320;                   // warps 0-7: rows; warp 8: MMA issue; warp 9: TMA
+constexpr float R16_LOG2E = 1.4426950408889634f, R16_LN2 = 0.6931471805599453f;
+
+__device__ __forceinline__ void r16_arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory"); }
+__device__ __forceinline__ float r16_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float r16_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// tanh(x) = 1 - 2 / (exp(2 x) + 1): off by 2^-22 at most, absolutely, which a cap times it carries into a score.
+__device__ __forceinline__ float r16_tanh(float x) { return fmaf(-2.f, r16_rcp(r16_ex2(x * (2.f * R16_LOG2E)) + 1.f), 1.f); }
+__device__ __forceinline__ uint32_t r16_pack(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Shared-memory descriptors share their upper word (stride offset 1024 bytes, version 1, 128-byte swizzle); the lower one is
+// (address >> 4) with the leading offset, one block of 64 columns for MN-major operands.
+constexpr uint32_t R16_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr uint32_t R16_LBO_K = 1u << 16, R16_LBO_MN = ((uint32_t)R16_CHUNK >> 4) << 16;
+__device__ __forceinline__ uint32_t r16_desc_k(const void* p) { return (smem_u32(p) >> 4) | R16_LBO_K; }
+__device__ __forceinline__ uint32_t r16_desc_mn(const void* p) { return (smem_u32(p) >> 4) | R16_LBO_MN; }
+// kind::f16 with bfloat16 operands and fp32 sums, M = 128.
+__device__ __forceinline__ constexpr uint32_t r16_idesc(bool b_mn, int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(R16_T >> 4) << 24);
+}
+__device__ __forceinline__ void r16_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(R16_DESC_HI), "r"(0u)
+      : "memory");
+}
+// A from tensor memory: row r in lane r, elements 2 c and 2 c + 1 of the contraction in column c.
+__device__ __forceinline__ void r16_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%6, %6, %6, %6}, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(R16_DESC_HI), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void r16_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void r16_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void r16_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D[128 x 128] = A B^T over the head's columns, both operands K-major in shared memory.
+template <int DP>
+__device__ __forceinline__ void r16_scores(uint32_t d, uint32_t a_k, uint32_t b_k) {
+  constexpr uint32_t idesc = r16_idesc(false, R16_T);
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ks++) {
+    const uint32_t o = (uint32_t)(ks / 4) * (R16_CHUNK >> 4) + (uint32_t)(ks % 4) * 2;
+    r16_mma_ss(d, a_k + o, b_k + o, idesc, ks > 0 ? 1u : 0u);
+  }
+}
+// D[128 x DP] (+)= A B over the tile's 128 rows of B, A in tensor memory (elements 64 h ... of the contraction at column 64 h or,
+// packed, 32 h), B MN-major in shared memory.
+template <int DP, int HALF>
+__device__ __forceinline__ void r16_gather(uint32_t d, uint32_t a, uint32_t b_mn, uint32_t accumulate) {
+  constexpr uint32_t idesc = r16_idesc(true, DP);
+#pragma unroll
+  for (int ks = 0; ks < R16_T / 16; ks++)
+    r16_mma_ts(d, a + (uint32_t)((ks / 4) * HALF + (ks % 4) * 8), b_mn + (uint32_t)ks * 128u, idesc, ks > 0 ? 1u : accumulate);
+}
+template <int DP>
+__device__ __forceinline__ void r16_load_tile(uint8_t* dst, const CUtensorMap* map, int row0, int head, int batch, uint64_t* bar) {
+#pragma unroll
+  for (int c = 0; c < DP / 64; c++) tma_load_4d(dst + c * R16_CHUNK, map, c * 64, row0, head, batch, bar);
+}
+
+// Which of the indices at, at + 1, ... of one row's other axis are seen: [0, prefix), [lo, hi), none beyond `end`.
+struct R16Row {
+  int prefix, lo, hi, end, doc;
+};
+__device__ __forceinline__ R16Row r16_query_row(const RuleArgs& r, int prefix, int b, int i) {
+  R16Row w;
+  const RuleSpan s = rule_keys(r, prefix, i, i + 1);
+  w.prefix = s.prefix;
+  w.lo = s.lo;
+  w.hi = s.hi;
+  w.end = r.lk;
+  w.doc = r.q_docs && i < r.lq ? r.q_docs[(long long)b * r.lq + i] : -1;
+  return w;
+}
+__device__ __forceinline__ R16Row r16_key_row(const RuleArgs& r, int prefix, int b, int j) {
+  R16Row w;
+  w.prefix = 0;
+  rule_queries(r, prefix, j, j + 1, &w.lo, &w.hi);
+  w.end = r.lq;
+  w.doc = r.k_docs && j < r.lk ? r.k_docs[(long long)b * r.lk + j] : -1;
+  return w;
+}
+__device__ __forceinline__ bool r16_sees(const R16Row& w, int at, const int32_t* docs) {
+  const bool near = (at >= w.lo && at < w.hi) || at < w.prefix;
+  return near && at < w.end && (!docs || (w.doc >= 0 && docs[at] == w.doc));
+}
+// The score in powers of two of a product, and the cap's derivative.
+__device__ __forceinline__ float r16_score(const RuleArgs& r, float slope, int far, float dot, float* dcap) {
+  float s = dot * r.scale;
+  if (r.softcap > 0.f) {
+    const float t = r16_tanh(s * r.inv_softcap);
+    *dcap = fmaf(-t, t, 1.f);
+    s = r.softcap * t;
+  } else {
+    *dcap = 1.f;
+  }
+  return fmaf(-slope, (float)abs(far), s) * R16_LOG2E;
+}
+
+// A row of N fp32 values to fp32 and bfloat16 results, both 16 bytes at a time; columns behind d stay unwritten (d is a multiple of 8).
+template <int N>
+__device__ __forceinline__ void r16_write(const uint32_t (&v)[N], float factor, float* out, __nv_bfloat16* out16, long long at, int col, int d) {
+#pragma unroll
+  for (int c = 0; c < N; c += 8) {
+    if (col + c >= d) break;
+    float f[8];
+#pragma unroll
+    for (int u = 0; u < 8; u++) f[u] = __uint_as_float(v[c + u]) * factor;
+    if (out) {
+      *reinterpret_cast<float4*>(out + at + c) = make_float4(f[0], f[1], f[2], f[3]);
+      *reinterpret_cast<float4*>(out + at + c + 4) = make_float4(f[4], f[5], f[6], f[7]);
+    }
+    if (out16) *reinterpret_cast<uint4*>(out16 + at + c) = make_uint4(r16_pack(f[0], f[1]), r16_pack(f[2], f[3]), r16_pack(f[4], f[5]), r16_pack(f[6], f[7]));
+  }
+}
+
+// A wait of all 32 rows of a warp: they go on together or not at all (what follows is issued by the whole warp).
+__device__ __forceinline__ bool r16_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, where));
+}
+
+struct R16Strides {
+  long long batch, head, row;
+};
+struct R16Fwd {
+  RuleArgs r;
+  int h, hkv, d;
+  int packed;                     // rows of a tile are (head of the group, query): h / hkv * lq of them
+  int splits;
+  float* out;
+  __nv_bfloat16* out16;
+  R16Strides os;
+  float* lse;
+  float* part;                    // [splits][b * h * lq][d] and [splits][b * h * lq] (maximum, sum) where splits > 1
+  float2* part_ml;
+  long long rows;                 // b * h * lq
+  int32_t* status;
+};
+
+// The tiles of keys that the queries of a CTA walk, in order: next() leaves the first key of the next one and what each of the two
+// query tiles sees of it (rule_tile's answer), or returns false.
+struct R16Walk {
+  const RuleArgs& r;
+  int prefix, b, i0, both, at, last;
+  int see[2];
+  __device__ __forceinline__ bool next() {
+    for (; at < last; at += R16_T) {
+      see[0] = rule_tile(r, prefix, b, i0, 2, at, 2);
+      see[1] = both ? rule_tile(r, prefix, b, i0 + R16_T, 2, at, 2) : 0;
+      if (see[0] | see[1]) {
+        at += R16_T;
+        return true;
+      }
+    }
+    return false;
+  }
+  __device__ __forceinline__ int tile() const { return at - R16_T; }
+};
+
+template <int DP>
+struct R16FwdShape {
+  static constexpr int TILE = DP / 64 * R16_CHUNK;
+  static constexpr int STAGES = DP == 128 ? 5 : 8;       // of K and V tiles in turn
+  static constexpr int BARS = (2 + STAGES) * TILE;
+  static constexpr int SMEM = BARS + 256 + 1024;
+};
+
+template <int DP, bool EXTRA>
+__global__ void __launch_bounds__(R16_THREADS, 1)
+rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const __grid_constant__ R16Fwd p) {
+  typedef R16FwdShape<DP> W;
+  constexpr uint32_t COL_S = 0, COL_O = 256;             // S (and P over it) of tile g at 128 g, O of tile g at 256 + 128 g
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t *slot_q = smem, *ring = smem + 2 * W::TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
+  uint64_t *bar_q = bars, *bar_s = bars + 1 /* [2] */, *bar_p = bars + 3 /* [2] */, *bar_o = bars + 5 /* [2] */, *bar_full = bars + 7 /* [STAGES] */,
+           *bar_empty = bar_full + W::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_empty + W::STAGES);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const RuleArgs& r = p.r;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = p.h / p.hkv;
+  const int split = blockIdx.z;
+  int bi, hi, hk, i0;
+  if (p.packed) {
+    bi = blockIdx.y / p.hkv;
+    hk = blockIdx.y - bi * p.hkv;
+    hi = hk * group;
+    i0 = 0;
+  } else {
+    bi = blockIdx.y / p.h;
+    hi = blockIdx.y - bi * p.h;
+    hk = hi / group;
+    i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * 2 * R16_T;      // the longest walks of a causal mask first
+  }
+  const int both = !p.packed && i0 + R16_T < r.lq;
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar_q, 1);
+    for (int a = 0; a < 2; a++) {
+      mbar_init(&bar_s[a], 1);
+      mbar_init(&bar_p[a], 128);
+      mbar_init(&bar_o[a], 1);
+    }
+    for (int a = 0; a < W::STAGES; a++) {
+      mbar_init(&bar_full[a], 1);
+      mbar_init(&bar_empty[a], 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  const int prefix = r.prefix ? r.prefix[bi] : 0;
+  R16Walk walk{r, prefix, bi, i0, both, 0, 0, {0, 0}};
+  {
+    const RuleSpan span = rule_keys(r, prefix, i0, min(p.packed ? r.lq : i0 + 2 * R16_T, r.lq));
+    const int first = span.prefix > 0 ? 0 : span.lo / R16_T, last = (max(span.prefix, span.hi) + R16_T - 1) / R16_T;
+    const int per = max(0, last - first + p.splits - 1) / p.splits;
+    walk.at = (first + split * per) * R16_T;
+    walk.last = min(first + (split + 1) * per, last) * R16_T;
+  }
+
+  if (warp == 9) {
+    if (lane == 0) {
+      if (p.packed) {
+        mbar_expect_tx(bar_q, (uint32_t)(DP / 64) * (uint32_t)(group * r.lq) * 128u);
+        r16_load_tile<DP>(slot_q, &map_q, 0, hi, bi, bar_q);
+      } else {
+        mbar_expect_tx(bar_q, (uint32_t)W::TILE * (both ? 2u : 1u));
+        r16_load_tile<DP>(slot_q, &map_q, i0, hi, bi, bar_q);
+        if (both) r16_load_tile<DP>(slot_q + W::TILE, &map_q, i0 + R16_T, hi, bi, bar_q);
+      }
+      int s = 0;
+      uint32_t phase = 0;
+      bool ok = true, again = false;
+      while (ok && walk.next()) {
+        for (int kv = 0; kv < 2 && ok; kv++) {
+          if (again) ok = mbar_wait(&bar_empty[s], phase ^ 1u, abort_flag, p.status, 61);
+          if (!ok) break;
+          mbar_expect_tx(&bar_full[s], W::TILE);
+          r16_load_tile<DP>(ring + s * W::TILE, kv ? &map_v : &map_k, walk.tile(), hk, bi, &bar_full[s]);
+          if (++s == W::STAGES) {
+            s = 0;
+            phase ^= 1u;
+            again = true;
+          }
+        }
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      bool ok = mbar_wait(bar_q, 0, abort_flag, p.status, 62);
+      int s = 0;                                          // the ring's next tile
+      uint32_t phase = 0, p_phase[2] = {0, 0}, o_phase[2] = {0, 0}, sums[2] = {0, 0};
+      bool pending[2] = {false, false};
+      auto take = [&]() {
+        const int at = s;
+        ok = mbar_wait(&bar_full[s], phase, abort_flag, p.status, 63);
+        if (++s == W::STAGES) {
+          s = 0;
+          phase ^= 1u;
+        }
+        return at;
+      };
+      auto scores = [&](int g, int k_stage) {
+        if (pending[g]) {                                 // the product that reads this tile's weights is complete
+          ok = mbar_wait(&bar_o[g], o_phase[g], abort_flag, p.status, 64);
+          if (!ok) return;
+          o_phase[g] ^= 1u;
+          pending[g] = false;
+        }
+        tc_fence_after();
+        r16_scores<DP>(tmem + COL_S + 128u * g, r16_desc_k(slot_q + g * W::TILE), r16_desc_k(ring + k_stage * W::TILE));
+        umma_commit(&bar_s[g]);
+      };
+      bool more = ok && walk.next();
+      int see[2] = {walk.see[0], walk.see[1]};
+      if (more) {
+        const int ks = take();
+        for (int g = 0; g < 2 && ok; g++)
+          if (see[g]) scores(g, ks);
+        if (ok) umma_commit(&bar_empty[ks]);
+      }
+      while (ok && more) {
+        const int vs = take();
+        if (!ok) break;
+        more = walk.next();
+        int ks = -1;
+        for (int g = 0; g < 2 && ok; g++) {
+          if (see[g]) {
+            ok = mbar_wait(&bar_p[g], p_phase[g], abort_flag, p.status, 65);
+            if (!ok) break;
+            p_phase[g] ^= 1u;
+            tc_fence_after();
+            r16_gather<DP, 32>(tmem + COL_O + 128u * g, tmem + COL_S + 128u * g, r16_desc_mn(ring + vs * W::TILE), sums[g] > 0 ? 1u : 0u);
+            umma_commit(&bar_o[g]);
+            sums[g]++;
+            pending[g] = true;
+          }
+          if (more && walk.see[g]) {
+            if (ks < 0) ks = take();
+            if (ok) scores(g, ks);
+          }
+        }
+        if (!ok) break;
+        umma_commit(&bar_empty[vs]);
+        if (ks >= 0) umma_commit(&bar_empty[ks]);
+        see[0] = walk.see[0];
+        see[1] = walk.see[1];
+      }
+      if (!ok) *abort_flag = 1;
+    }
+  } else {
+    const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    int i = i0 + g * R16_T + row, head = hi;
+    bool valid = i < r.lq;
+    if (p.packed) {
+      const int gi = row / r.lq;
+      i = row - gi * r.lq;
+      head = hi + gi;
+      valid = g == 0 && gi < group;
+    }
+    if (p.packed && !valid) {
+      i = 0;
+      head = hi;
+    }
+    const float slope = EXTRA && r.slopes ? r.slopes[head] : 0.f;
+    const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
+    const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+    const uint32_t t_s = lane_base + COL_S + 128u * g, t_o = lane_base + COL_O + 128u * g;
+    const float mult = EXTRA ? 1.f : r.scale * R16_LOG2E;
+    float m = -INFINITY, l = 0.f;
+    uint32_t count = 0;
+    bool ok = true;
+    while (ok && walk.next()) {
+      if (!walk.see[g]) continue;
+      ok = r16_wait(&bar_s[g], count & 1u, abort_flag, p.status, 66);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; c++) tmem_ld_32x32b_x32(t_s + 32u * c, x[c]);
+      tmem_ld_wait();
+      const int j0 = walk.tile();
+      if (EXTRA) {
+        const int far = i + r.q_offset - j0;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int u = 0; u < 32; u++) {
+            float dcap;
+            x[c][u] = __float_as_uint(r16_score(r, slope, far - (c * 32 + u), __uint_as_float(x[c][u]), &dcap));
+          }
+      }
+      if (walk.see[g] == 1) {
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+          for (int u = 0; u < 32; u++)
+            if (!r16_sees(seen, j0 + c * 32 + u, docs)) x[c][u] = 0xff800000u;
+      }
+      float top = __uint_as_float(x[0][0]);
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int u = 0; u < 32; u++) top = fmaxf(top, __uint_as_float(x[c][u]));
+      top *= mult;
+      float shrink = 1.f;
+      if (top > m + 8.f || m == -INFINITY) {
+        shrink = r16_ex2(m - (top == -INFINITY ? 0.f : top));      // m = -inf: 0
+        m = fmaxf(m, top);
+      }
+      if (count > 0 && __any_sync(0xffffffffu, shrink != 1.f)) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int u = 0; u < 32; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * shrink);
+          r16_st32(t_o + (uint32_t)c, o);
+        }
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        uint32_t w[32];
+#pragma unroll
+        for (int u = 0; u < 32; u++) {
+          const float a = r16_ex2(fmaf(__uint_as_float(x[2 * half + u / 16][(2 * u) % 32]), mult, -base));
+          const float b = r16_ex2(fmaf(__uint_as_float(x[2 * half + u / 16][(2 * u + 1) % 32]), mult, -base));
+          sum[(2 * u) & 3] += a;
+          sum[(2 * u + 1) & 3] += b;
+          w[u] = r16_pack(a, b);
+        }
+        r16_st32(t_s + 32u * half, w);
+      }
+      l = fmaf(l, shrink, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+      r16_st_wait();
+      tc_fence_before();
+      r16_arrive(&bar_p[g]);
+      count++;
+    }
+    if (ok && count > 0) ok = r16_wait(&bar_o[g], (count - 1) & 1u, abort_flag, p.status, 67);
+    if (ok) {
+      tc_fence_after();
+      const long long at_row = ((long long)bi * p.h + head) * r.lq + i;
+      float inv = l == 0.f ? 0.f : 1.f / l;
+      float* out = p.out;
+      __nv_bfloat16* out16 = p.out16;
+      long long at = bi * p.os.batch + head * p.os.head + (long long)i * p.os.row;
+      if (p.splits > 1) {
+        inv = 1.f;
+        out = p.part;
+        out16 = nullptr;
+        at = ((long long)split * p.rows + at_row) * p.d;
+        if (valid) p.part_ml[(long long)split * p.rows + at_row] = make_float2(m, l);
+      } else if (p.lse && valid) {
+        p.lse[at_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * R16_LN2;
+      }
+      if (g == 0 || both) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          __syncwarp();
+          if (count > 0) {
+            tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
+            tmem_ld_wait();
+          }
+          if (count == 0 || l == 0.f) {
+#pragma unroll
+            for (int u = 0; u < 32; u++) o[u] = 0u;
+          }
+          if (valid) r16_write(o, inv, out, out16, at + c, c, p.d);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// The parts of split walks: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s in increasing order of the splits. A warp per row.
+__global__ void __launch_bounds__(256)
+rule16_join_kernel(const __grid_constant__ R16Fwd p) {
+  pdl_enter();
+  const int lane = threadIdx.x & 31;
+  for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < p.rows; row += (long long)gridDim.x * 8) {
+    float m = -INFINITY;
+    for (int s = 0; s < p.splits; s++) {
+      const float2 v = p.part_ml[s * p.rows + row];
+      if (v.y != 0.f) m = fmaxf(m, v.x);
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int c = lane * 4;
+    for (int s = 0; s < p.splits; s++) {
+      const float2 v = p.part_ml[s * p.rows + row];
+      if (v.y == 0.f) continue;                       // this part saw nothing
+      const float f = r16_ex2(v.x - base);
+      l = fmaf(v.y, f, l);
+      if (c < p.d) {
+        const float4 o = *reinterpret_cast<const float4*>(p.part + (s * p.rows + row) * p.d + c);
+        acc = make_float4(fmaf(o.x, f, acc.x), fmaf(o.y, f, acc.y), fmaf(o.z, f, acc.z), fmaf(o.w, f, acc.w));
+      }
+    }
+    const long long bh = row / p.r.lq;
+    const int i = (int)(row - bh * p.r.lq), bi = (int)(bh / p.h), hi = (int)(bh - (long long)bi * p.h);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (c < p.d) {
+      const long long at = bi * p.os.batch + hi * p.os.head + (long long)i * p.os.row + c;
+      acc = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      if (p.out) *reinterpret_cast<float4*>(p.out + at) = acc;
+      if (p.out16) *reinterpret_cast<uint2*>(p.out16 + at) = make_uint2(r16_pack(acc.x, acc.y), r16_pack(acc.z, acc.w));
+    }
+    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * R16_LN2;
+  }
+}
+
+// ---- backward -------------------------------------------------------------------------------------------------------------------
+
+struct R16Bwd {
+  RuleArgs r;
+  int h, hkv, d;
+  const float2* rows;             // [b * h][pitch]: log-sum-exp in powers of two, row dot
+  int pitch;
+  float *d0, *d1;                 // dv and dk, or dq and nothing
+  __nv_bfloat16 *d0_16, *d1_16;
+  R16Strides s0, s1;
+  int32_t* status;
+};
+
+template <int DP>
+struct R16BwdShape {
+  static constexpr int TILE = DP / 64 * R16_CHUNK;
+  static constexpr int RING_A = 3, RING_B = 2;           // tiles that two products read (Q or K), and the others (dO or V)
+  static constexpr int BARS = (2 + RING_A + RING_B) * TILE;
+  static constexpr int SMEM = BARS + 256 + 1024;
+};
+
+// Scores of one row (64 of them, half a tile) to weights: packed as bfloat16 in w where they are wanted, and in x, times the cap's
+// derivative, for r16_gradients. Rows are keys (COLUMNS: log-sum-exp and row dot go with the column) or queries.
+template <bool EXTRA, bool COLUMNS>
+__device__ __forceinline__ void r16_weights(const RuleArgs& r, uint32_t (&x)[2][32], uint32_t (&w)[32], const float2* rows, float lse, float slope, int far, float mult,
+                                            bool partial, const R16Row& seen, int at, const int32_t* docs) {
+#pragma unroll
+  for (int c = 0; c < 2; c++)
+#pragma unroll
+    for (int u = 0; u < 32; u += 2) {
+      float e[2] = {lse, lse}, p[2];
+      if (COLUMNS) {
+        const float4 v = *reinterpret_cast<const float4*>(rows + c * 32 + u);
+        e[0] = v.x;
+        e[1] = v.z;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        float s = __uint_as_float(x[c][u + t]), dcap = 1.f;
+        if (EXTRA) s = r16_score(r, slope, COLUMNS ? far + (c * 32 + u + t) : far - (c * 32 + u + t), s, &dcap);
+        p[t] = r16_ex2(fmaf(s, mult, -e[t]));
+        float d = EXTRA ? p[t] * dcap : p[t];
+        if (partial && !r16_sees(seen, at + c * 32 + u + t, docs)) p[t] = d = 0.f;
+        x[c][u + t] = __float_as_uint(d);
+      }
+      if (COLUMNS) w[c * 16 + u / 2] = r16_pack(p[0], p[1]);
+    }
+}
+// dS = weight (dP - dot), 32 of them, packed. partial: some are hidden, and 0 whatever dP is there.
+template <bool COLUMNS>
+__device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uint32_t (&dp)[32], uint32_t* w, const float2* rows, float dot, bool partial) {
+#pragma unroll
+  for (int u = 0; u < 32; u += 2) {
+    float d[2] = {dot, dot};
+    if (COLUMNS) {
+      const float4 v = *reinterpret_cast<const float4*>(rows + u);
+      d[0] = v.y;
+      d[1] = v.w;
+    }
+    float a = __uint_as_float(x[u]) * (__uint_as_float(dp[u]) - d[0]), b = __uint_as_float(x[u + 1]) * (__uint_as_float(dp[u + 1]) - d[1]);
+    if (partial) {
+      a = x[u] == 0u ? 0.f : a;
+      b = x[u + 1] == 0u ? 0.f : b;
+    }
+    w[u / 2] = r16_pack(a, b);
+  }
+}
+
+template <int DP, bool EXTRA>
+__global__ void __launch_bounds__(R16_THREADS, 1)
+rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                  const __grid_constant__ CUtensorMap map_g, const __grid_constant__ R16Bwd p) {
+  typedef R16BwdShape<DP> W;
+  constexpr uint32_t COL_S = 0, COL_DP = 128, COL_DV = 256, COL_DK = 384;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t *slot_k = smem, *slot_v = smem + W::TILE, *ring_q = smem + 2 * W::TILE, *ring_g = ring_q + W::RING_A * W::TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
+  uint64_t *bar_kv = bars, *bar_s = bars + 1, *bar_dp = bars + 2, *bar_p = bars + 3, *bar_ds = bars + 4, *bar_dv = bars + 5, *bar_dk = bars + 6,
+           *bar_done = bars + 7, *full_q = bars + 8 /* [3] */, *empty_q = bars + 11, *full_g = bars + 14 /* [2] */, *empty_g = bars + 16;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const RuleArgs& r = p.r;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int j0 = blockIdx.x * R16_T, bi = blockIdx.y / p.hkv, hk = blockIdx.y - bi * p.hkv, group = p.h / p.hkv;
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar_kv, 1);
+    mbar_init(bar_s, 1);
+    mbar_init(bar_dp, 1);
+    mbar_init(bar_p, 256);
+    mbar_init(bar_ds, 256);
+    mbar_init(bar_dv, 1);
+    mbar_init(bar_dk, 1);
+    mbar_init(bar_done, 1);
+    for (int a = 0; a < 3; a++) {
+      mbar_init(&full_q[a], 1);
+      mbar_init(&empty_q[a], 1);
+    }
+    for (int a = 0; a < 2; a++) {
+      mbar_init(&full_g[a], 1);
+      mbar_init(&empty_g[a], 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  const int prefix = r.prefix ? r.prefix[bi] : 0;
+  int q_lo, q_hi;
+  rule_queries(r, prefix, j0, min(j0 + R16_T, r.lk), &q_lo, &q_hi);
+  q_lo = q_lo / R16_T * R16_T;
+  // The tiles of queries of the heads in order: (head of the group, first query, what of the tile is visible).
+  struct {
+    int gi, at, see;
+  } step = {0, q_lo, 0};
+  auto next = [&]() {
+    for (; step.gi < group; step.gi++, step.at = q_lo)
+      for (; step.at < q_hi; step.at += R16_T) {
+        step.see = rule_tile(r, prefix, bi, step.at, 2, j0, 2);
+        if (step.see) {
+          step.at += R16_T;
+          return true;
+        }
+      }
+    return false;
+  };
+
+  if (warp == 9) {
+    if (lane == 0) {
+      mbar_expect_tx(bar_kv, 2 * W::TILE);
+      r16_load_tile<DP>(slot_k, &map_k, j0, hk, bi, bar_kv);
+      r16_load_tile<DP>(slot_v, &map_v, j0, hk, bi, bar_kv);
+      int a = 0, b = 0, n = 0;
+      uint32_t pa = 0, pb = 0;
+      bool ok = true;
+      for (; ok && next(); n++) {
+        const int at = step.at - R16_T, head = hk * group + step.gi;
+        if (n >= W::RING_A) ok = mbar_wait(&empty_q[a], pa ^ 1u, abort_flag, p.status, 71);
+        if (!ok) break;
+        mbar_expect_tx(&full_q[a], W::TILE);
+        r16_load_tile<DP>(ring_q + a * W::TILE, &map_q, at, head, bi, &full_q[a]);
+        if (++a == W::RING_A) {
+          a = 0;
+          pa ^= 1u;
+        }
+        if (n >= W::RING_B) ok = mbar_wait(&empty_g[b], pb ^ 1u, abort_flag, p.status, 72);
+        if (!ok) break;
+        mbar_expect_tx(&full_g[b], W::TILE);
+        r16_load_tile<DP>(ring_g + b * W::TILE, &map_g, at, head, bi, &full_g[b]);
+        if (++b == W::RING_B) {
+          b = 0;
+          pb ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      bool ok = mbar_wait(bar_kv, 0, abort_flag, p.status, 73);
+      bool more = ok && next();
+      int a = 0, b = 0;
+      uint32_t pa = 0, pb = 0, n = 0;
+      if (more) {
+        ok = mbar_wait(&full_q[0], 0, abort_flag, p.status, 74);
+        if (ok) {
+          tc_fence_after();
+          r16_scores<DP>(tmem + COL_S, r16_desc_k(slot_k), r16_desc_k(ring_q));
+          umma_commit(bar_s);
+          ok = mbar_wait(&full_g[0], 0, abort_flag, p.status, 75);
+        }
+        if (ok) {
+          tc_fence_after();
+          r16_scores<DP>(tmem + COL_DP, r16_desc_k(slot_v), r16_desc_k(ring_g));
+          umma_commit(bar_dp);
+        }
+      }
+      for (; ok && more; n++) {
+        more = next();
+        const int a1 = a + 1 == W::RING_A ? 0 : a + 1, b1 = b + 1 == W::RING_B ? 0 : b + 1;
+        const uint32_t pa1 = a1 == 0 ? pa ^ 1u : pa, pb1 = b1 == 0 ? pb ^ 1u : pb;
+        // dV += P^T dO, then the next tile's scores as soon as that product has read P (which lies over them).
+        if (!(ok = mbar_wait(bar_p, n & 1u, abort_flag, p.status, 76))) break;
+        tc_fence_after();
+        r16_gather<DP, 64>(tmem + COL_DV, tmem + COL_S, r16_desc_mn(ring_g + b * W::TILE), n > 0 ? 1u : 0u);
+        umma_commit(bar_dv);
+        umma_commit(&empty_g[b]);
+        if (more) {
+          if (!(ok = mbar_wait(&full_q[a1], pa1, abort_flag, p.status, 74) && mbar_wait(bar_dv, n & 1u, abort_flag, p.status, 77))) break;
+          tc_fence_after();
+          r16_scores<DP>(tmem + COL_S, r16_desc_k(slot_k), r16_desc_k(ring_q + a1 * W::TILE));
+          umma_commit(bar_s);
+        }
+        // dK += dS^T Q, then the next dP over the dS it has read.
+        if (!(ok = mbar_wait(bar_ds, n & 1u, abort_flag, p.status, 78))) break;
+        tc_fence_after();
+        r16_gather<DP, 64>(tmem + COL_DK, tmem + COL_DP, r16_desc_mn(ring_q + a * W::TILE), n > 0 ? 1u : 0u);
+        umma_commit(bar_dk);
+        umma_commit(&empty_q[a]);
+        if (more) {
+          if (!(ok = mbar_wait(&full_g[b1], pb1, abort_flag, p.status, 75) && mbar_wait(bar_dk, n & 1u, abort_flag, p.status, 79))) break;
+          tc_fence_after();
+          r16_scores<DP>(tmem + COL_DP, r16_desc_k(slot_v), r16_desc_k(ring_g + b1 * W::TILE));
+          umma_commit(bar_dp);
+        }
+        a = a1;
+        b = b1;
+        pa = pa1;
+        pb = pb1;
+      }
+      if (ok) umma_commit(bar_done);
+      else *abort_flag = 1;
+    }
+  } else {
+    const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane, j = j0 + row;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+    const R16Row seen = r16_key_row(r, prefix, bi, min(j, r.lk - 1));
+    const int32_t* docs = r.q_docs ? r.q_docs + (long long)bi * r.lq : nullptr;
+    const float mult = EXTRA ? 1.f : r.scale * R16_LOG2E;
+    bool ok = true;
+    uint32_t n = 0;
+    for (; ok && next(); n++) {
+      const int head = hk * group + step.gi, at = step.at - R16_T + g * 64;
+      const float slope = EXTRA && r.slopes ? r.slopes[head] : 0.f;
+      const float2* rows = p.rows + ((long long)bi * p.h + head) * p.pitch + at;
+      if (!(ok = r16_wait(bar_s, n & 1u, abort_flag, p.status, 80))) break;
+      tc_fence_after();
+      uint32_t x[2][32], w[32];
+      tmem_ld_32x32b_x32(lane_base + COL_S + 64u * g, x[0]);
+      tmem_ld_32x32b_x32(lane_base + COL_S + 64u * g + 32u, x[1]);
+      tmem_ld_wait();
+      r16_weights<EXTRA, true>(r, x, w, rows, 0.f, slope, at + r.q_offset - j, mult, step.see == 1, seen, at, docs);
+      r16_st32(lane_base + COL_S + 64u * g, w);
+      r16_st_wait();
+      tc_fence_before();
+      r16_arrive(bar_p);
+      if (!(ok = r16_wait(bar_dp, n & 1u, abort_flag, p.status, 81))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        uint32_t dp[32];
+        tmem_ld_32x32b_x32(lane_base + COL_DP + 64u * g + 32u * c, dp);
+        tmem_ld_wait();
+        r16_gradients<true>(x[c], dp, w + c * 16, rows + c * 32, 0.f, step.see == 1);
+      }
+      r16_st32(lane_base + COL_DP + 64u * g, w);
+      r16_st_wait();
+      tc_fence_before();
+      r16_arrive(bar_ds);
+    }
+    if (ok) ok = r16_wait(bar_done, 0, abort_flag, p.status, 82);
+    if (ok) {
+      tc_fence_after();
+      // dV by the first four warps, dK by the others.
+      float* out = g == 0 ? p.d0 : p.d1;
+      __nv_bfloat16* out16 = g == 0 ? p.d0_16 : p.d1_16;
+      const R16Strides& s = g == 0 ? p.s0 : p.s1;
+      if (out || out16) {
+#pragma unroll 1
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          __syncwarp();
+          if (n > 0) {
+            tmem_ld_32x32b_x32(lane_base + (g == 0 ? COL_DV : COL_DK) + (uint32_t)c, o);
+            tmem_ld_wait();
+          } else {
+#pragma unroll
+            for (int u = 0; u < 32; u++) o[u] = 0u;
+          }
+          if (j < r.lk) r16_write(o, g == 0 ? 1.f : r.scale, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int DP, bool EXTRA>
+__global__ void __launch_bounds__(R16_THREADS, 1)
+rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                 const __grid_constant__ CUtensorMap map_g, const __grid_constant__ R16Bwd p) {
+  typedef R16BwdShape<DP> W;
+  constexpr uint32_t COL_S = 0 /* two buffers */, COL_DP = 256, COL_DQ = 384;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint8_t *slot_q = smem, *slot_g = smem + W::TILE, *ring_k = smem + 2 * W::TILE, *ring_v = ring_k + W::RING_A * W::TILE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
+  uint64_t *bar_qg = bars, *bar_s = bars + 1 /* [2] */, *bar_dp = bars + 3, *bar_read = bars + 4, *bar_ds = bars + 5, *bar_dq = bars + 6 /* [2] */,
+           *bar_done = bars + 8, *full_k = bars + 9 /* [3] */, *empty_k = bars + 12, *full_v = bars + 15 /* [2] */, *empty_v = bars + 17;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const RuleArgs& r = p.r;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * R16_T, bi = blockIdx.y / p.h, hi = blockIdx.y - bi * p.h, hk = hi / (p.h / p.hkv);
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar_qg, 1);
+    mbar_init(bar_dp, 1);
+    mbar_init(bar_read, 256);
+    mbar_init(bar_ds, 256);
+    mbar_init(bar_done, 1);
+    for (int a = 0; a < 2; a++) {
+      mbar_init(&bar_s[a], 1);
+      mbar_init(&bar_dq[a], 1);
+      mbar_init(&full_v[a], 1);
+      mbar_init(&empty_v[a], 1);
+    }
+    for (int a = 0; a < 3; a++) {
+      mbar_init(&full_k[a], 1);
+      mbar_init(&empty_k[a], 1);
+    }
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  const int prefix = r.prefix ? r.prefix[bi] : 0;
+  R16Walk walk{r, prefix, bi, i0, 0, 0, 0, {0, 0}};
+  {
+    const RuleSpan span = rule_keys(r, prefix, i0, min(i0 + R16_T, r.lq));
+    walk.at = span.prefix > 0 ? 0 : span.lo / R16_T * R16_T;
+    walk.last = max(span.prefix, span.hi);
+  }
+
+  if (warp == 9) {
+    if (lane == 0) {
+      mbar_expect_tx(bar_qg, 2 * W::TILE);
+      r16_load_tile<DP>(slot_q, &map_q, i0, hi, bi, bar_qg);
+      r16_load_tile<DP>(slot_g, &map_g, i0, hi, bi, bar_qg);
+      int a = 0, b = 0, n = 0;
+      uint32_t pa = 0, pb = 0;
+      bool ok = true;
+      for (; ok && walk.next(); n++) {
+        if (n >= W::RING_A) ok = mbar_wait(&empty_k[a], pa ^ 1u, abort_flag, p.status, 83);
+        if (!ok) break;
+        mbar_expect_tx(&full_k[a], W::TILE);
+        r16_load_tile<DP>(ring_k + a * W::TILE, &map_k, walk.tile(), hk, bi, &full_k[a]);
+        if (++a == W::RING_A) {
+          a = 0;
+          pa ^= 1u;
+        }
+        if (n >= W::RING_B) ok = mbar_wait(&empty_v[b], pb ^ 1u, abort_flag, p.status, 84);
+        if (!ok) break;
+        mbar_expect_tx(&full_v[b], W::TILE);
+        r16_load_tile<DP>(ring_v + b * W::TILE, &map_v, walk.tile(), hk, bi, &full_v[b]);
+        if (++b == W::RING_B) {
+          b = 0;
+          pb ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 8) {
+    if (lane == 0) {
+      bool ok = mbar_wait(bar_qg, 0, abort_flag, p.status, 85);
+      bool more = ok && walk.next();
+      int a = 0, b = 0;
+      uint32_t pa = 0, pb = 0, n = 0;
+      if (more) {
+        ok = mbar_wait(&full_k[0], 0, abort_flag, p.status, 86);
+        if (ok) {
+          tc_fence_after();
+          r16_scores<DP>(tmem + COL_S, r16_desc_k(slot_q), r16_desc_k(ring_k));
+          umma_commit(&bar_s[0]);
+          ok = mbar_wait(&full_v[0], 0, abort_flag, p.status, 87);
+        }
+        if (ok) {
+          tc_fence_after();
+          r16_scores<DP>(tmem + COL_DP, r16_desc_k(slot_g), r16_desc_k(ring_v));
+          umma_commit(bar_dp);
+          umma_commit(&empty_v[0]);
+        }
+      }
+      for (; ok && more; n++) {
+        more = walk.next();
+        const int a1 = a + 1 == W::RING_A ? 0 : a + 1, b1 = b + 1 == W::RING_B ? 0 : b + 1;
+        const uint32_t pa1 = a1 == 0 ? pa ^ 1u : pa, pb1 = b1 == 0 ? pb ^ 1u : pb, buf = n & 1u;
+        if (more) {
+          // The next tile's scores into the other buffer, whose dS the product of the tile before has read.
+          ok = mbar_wait(&full_k[a1], pa1, abort_flag, p.status, 86);
+          if (ok && n > 0) ok = mbar_wait(&bar_dq[buf ^ 1u], ((n - 1) >> 1) & 1u, abort_flag, p.status, 88);
+          if (!ok) break;
+          tc_fence_after();
+          r16_scores<DP>(tmem + COL_S + 128u * (buf ^ 1u), r16_desc_k(slot_q), r16_desc_k(ring_k + a1 * W::TILE));
+          umma_commit(&bar_s[buf ^ 1u]);
+          // The next dP once the rows have read this one.
+          if (!(ok = mbar_wait(&full_v[b1], pb1, abort_flag, p.status, 87) && mbar_wait(bar_read, n & 1u, abort_flag, p.status, 89))) break;
+          tc_fence_after();
+          r16_scores<DP>(tmem + COL_DP, r16_desc_k(slot_g), r16_desc_k(ring_v + b1 * W::TILE));
+          umma_commit(bar_dp);
+          umma_commit(&empty_v[b1]);
+        }
+        if (!(ok = mbar_wait(bar_ds, n & 1u, abort_flag, p.status, 90))) break;
+        tc_fence_after();
+        r16_gather<DP, 64>(tmem + COL_DQ, tmem + COL_S + 128u * buf, r16_desc_mn(ring_k + a * W::TILE), n > 0 ? 1u : 0u);
+        umma_commit(&bar_dq[buf]);
+        umma_commit(&empty_k[a]);
+        a = a1;
+        b = b1;
+        pa = pa1;
+        pb = pb1;
+      }
+      if (ok) umma_commit(bar_done);
+      else *abort_flag = 1;
+    }
+  } else {
+    const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane, i = i0 + row;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
+    const float slope = EXTRA && r.slopes ? r.slopes[hi] : 0.f;
+    const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
+    const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
+    const float mult = EXTRA ? 1.f : r.scale * R16_LOG2E;
+    const float2 stat = p.rows[((long long)bi * p.h + hi) * p.pitch + i];
+    bool ok = true;
+    uint32_t n = 0;
+    for (; ok && walk.next(); n++) {
+      const int at = walk.tile() + g * 64;
+      const uint32_t t_s = lane_base + COL_S + 128u * (n & 1u) + 64u * g;
+      if (!(ok = r16_wait(&bar_s[n & 1u], (n >> 1) & 1u, abort_flag, p.status, 91))) break;
+      tc_fence_after();
+      uint32_t x[2][32], w[32];
+      tmem_ld_32x32b_x32(t_s, x[0]);
+      tmem_ld_32x32b_x32(t_s + 32u, x[1]);
+      tmem_ld_wait();
+      r16_weights<EXTRA, false>(r, x, w, nullptr, stat.x, slope, i + r.q_offset - at, mult, walk.see[0] == 1, seen, at, docs);
+      if (!(ok = r16_wait(bar_dp, n & 1u, abort_flag, p.status, 92))) break;
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        uint32_t dp[32];
+        tmem_ld_32x32b_x32(lane_base + COL_DP + 64u * g + 32u * c, dp);
+        tmem_ld_wait();
+        if (c == 1) {
+          tc_fence_before();
+          r16_arrive(bar_read);
+        }
+        r16_gradients<false>(x[c], dp, w + c * 16, nullptr, stat.y, walk.see[0] == 1);
+      }
+      r16_st32(t_s, w);
+      r16_st_wait();
+      tc_fence_before();
+      r16_arrive(bar_ds);
+    }
+    if (ok) ok = r16_wait(bar_done, 0, abort_flag, p.status, 93);
+    if (ok) {
+      tc_fence_after();
+      // Half of dQ's columns by each four warps.
+#pragma unroll 1
+      for (int c = g * (DP / 2); c < (g + 1) * (DP / 2); c += 32) {
+        uint32_t o[32];
+        __syncwarp();
+        if (n > 0) {
+          tmem_ld_32x32b_x32(lane_base + COL_DQ + (uint32_t)c, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int u = 0; u < 32; u++) o[u] = 0u;
+        }
+        if (i < r.lq) r16_write(o, r.scale, p.d0, p.d0_16, bi * p.s0.batch + hi * p.s0.head + (long long)i * p.s0.row + c, c, p.d);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------------
+
+// Rank-4 map over a bfloat16 activation seen as [B, H, L, D] through element strides; box = [64 columns, rows, heads, 1]. Columns
+// behind D and rows behind L come as zeros.
+static bool r16_map(CUtensorMap* map, const void* base, int d, int l, int heads, int batch, const om_head_strides* s, int box_rows, int box_heads) {
+  cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)l, (cuuint64_t)heads, (cuuint64_t)batch};
+  const cuuint64_t row = (cuuint64_t)s->row * 2;
+  cuuint64_t strides[3] = {row, heads > 1 ? (cuuint64_t)s->head * 2 : row, batch > 1 ? (cuuint64_t)s->batch * 2 : row};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, (cuuint32_t)box_heads, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// What TMA addresses: a 16-byte aligned base, strides that are positive multiples of 16 bytes below 2^40.
+static bool r16_operand(const void* p, const om_head_strides* s, int heads, int batch) {
+  auto fits = [](int64_t v) { return v > 0 && v % 8 == 0 && v < (1ll << 38); };
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && fits(s->row) && (heads == 1 || fits(s->head)) && (batch == 1 || fits(s->batch));
+}
+// Rows of results are written 16 bytes at a time.
+static bool r16_result(const float* p, const void* p16, const om_head_strides* s) {
+  if (p && ((reinterpret_cast<uintptr_t>(p) & 15) || s->row % 4 || s->head % 4 || s->batch % 4)) return false;
+  return !p16 || !((reinterpret_cast<uintptr_t>(p16) & 15) || s->row % 8 || s->head % 8 || s->batch % 8);
+}
+static bool r16_shape(const RuleCall& c) { return encode_fn() && c.d % 8 == 0 && c.d <= 128 && c.r.scale > 0.f; }
+static R16Strides r16_strides(const om_head_strides* s) { return R16Strides{s->batch, s->head, s->row}; }
+
+bool rule16_fwd_takes(const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
+                      const om_head_strides* vs, const float* out, const void* out16, const om_head_strides* os) {
+  return r16_shape(c) && r16_operand(q, qs, c.h, c.b) && r16_operand(k, ks, c.hkv, c.b) && r16_operand(v, vs, c.hkv, c.b) && r16_result(out, out16, os);
+}
+bool rule16_bwd_takes(const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
+                      const om_head_strides* ks, const void* v, const om_head_strides* vs, const float* dq, const void* dq16, const om_head_strides* dqs,
+                      const float* dk, const void* dk16, const om_head_strides* dks, const float* dv, const void* dv16, const om_head_strides* dvs) {
+  return r16_shape(c) && r16_operand(g, gs, c.h, c.b) && r16_operand(q, qs, c.h, c.b) && r16_operand(k, ks, c.hkv, c.b) && r16_operand(v, vs, c.hkv, c.b) &&
+         (!(dq || dq16) || r16_result(dq, dq16, dqs)) && (!(dk || dk16) || r16_result(dk, dk16, dks)) && (!(dv || dv16) || r16_result(dv, dv16, dvs));
+}
+
+template <typename K>
+static int32_t r16_room(om_ctx* ctx, K kernel, int smem) {
+  OM_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  return OM_OK;
+}
+
+template <int DP, bool EXTRA>
+static int32_t r16_fwd(om_ctx* ctx, dim3 grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const R16Fwd& p) {
+  OM_TRY(r16_room(ctx, rule16_fwd_kernel<DP, EXTRA>, R16FwdShape<DP>::SMEM));
+  launch_chained(ctx, rule16_fwd_kernel<DP, EXTRA>, grid, R16_THREADS, R16FwdShape<DP>::SMEM, mq, mk, mv, p);
+  return OM_OK;
+}
+
+int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
+                   const om_head_strides* vs, float* out, void* out16, const om_head_strides* os, float* lse) {
+  const int group = c.h / c.hkv, lq = c.r.lq, lk = c.r.lk;
+  R16Fwd p = {};
+  p.r = c.r; p.h = c.h; p.hkv = c.hkv; p.d = c.d;
+  p.out = out; p.out16 = reinterpret_cast<__nv_bfloat16*>(out16); p.os = r16_strides(os); p.lse = lse;
+  p.rows = (long long)c.b * c.h * lq;
+  p.status = ctx->status_dev;
+  // Heads that share keys as rows of one tile where they fit it: keys and values are read once for all of them.
+  p.packed = (long long)group * lq <= R16_T && (group > 1);
+  dim3 grid(p.packed ? 1u : (unsigned)ceil_div(lq, 2 * R16_T), (unsigned)(c.b * (p.packed ? c.hkv : c.h)), 1);
+  // A walk is split where the CTAs leave SMs without one, four tiles of keys a part at least: a part costs its CTA's start and a
+  // row of O per query in memory, twice.
+  const int64_t ctas = (int64_t)grid.x * grid.y;
+  const int64_t span = c.r.window && !c.r.prefix ? std::min<int64_t>(lk, 2ll * c.r.window + lq) : lk;
+  const int64_t tiles = ceil_div(span, R16_T);
+  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count / std::max<int64_t>(ctas, 1), tiles / 4));
+  grid.z = (unsigned)p.splits;
+  CUtensorMap mq, mk, mv;
+  if (!r16_map(&mq, q, c.d, lq, c.h, c.b, qs, p.packed ? lq : R16_T, p.packed ? group : 1) || !r16_map(&mk, k, c.d, lk, c.hkv, c.b, ks, R16_T, 1) ||
+      !r16_map(&mv, v, c.d, lk, c.hkv, c.b, vs, R16_T, 1))
+    return fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the operands of om_rule_attention_fwd_bf16");
+  char* part = nullptr;
+  if (p.splits > 1) {
+    const size_t ml = ((size_t)p.splits * p.rows * sizeof(float2) + 255) & ~(size_t)255;
+    OM_TRY(pool_alloc(ctx, ml + (size_t)p.splits * p.rows * c.d * sizeof(float), false, (void**)&part));
+    p.part_ml = reinterpret_cast<float2*>(part);
+    p.part = reinterpret_cast<float*>(part + ml);
+  }
+  const bool extra = c.r.softcap > 0.f || c.r.slopes;
+  int32_t st;
+  if (c.d <= 64) st = extra ? r16_fwd<64, true>(ctx, grid, mq, mk, mv, p) : r16_fwd<64, false>(ctx, grid, mq, mk, mv, p);
+  else st = extra ? r16_fwd<128, true>(ctx, grid, mq, mk, mv, p) : r16_fwd<128, false>(ctx, grid, mq, mk, mv, p);
+  if (p.splits > 1) {
+    if (st == OM_OK) launch_chained(ctx, rule16_join_kernel, grid_for(ctx, p.rows, 8), 256, 0, p);
+    pool_free(ctx, part);
+  }
+  OM_TRY(st);
+  OM_LAUNCH_CHECK(ctx, "om_rule_attention_fwd_bf16");
+  return OM_OK;
+}
+
+template <int DP, bool EXTRA>
+static int32_t r16_bwd(om_ctx* ctx, const RuleCall& c, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg,
+                       const R16Bwd& kv, const R16Bwd& q) {
+  const int smem = R16BwdShape<DP>::SMEM;
+  if (kv.d0 || kv.d0_16 || kv.d1 || kv.d1_16) {
+    OM_TRY(r16_room(ctx, rule16_dkv_kernel<DP, EXTRA>, smem));
+    launch_chained(ctx, rule16_dkv_kernel<DP, EXTRA>, dim3((unsigned)ceil_div(c.r.lk, R16_T), (unsigned)(c.b * c.hkv)), R16_THREADS, smem, mq, mk, mv, mg, kv);
+  }
+  if (q.d0 || q.d0_16) {
+    OM_TRY(r16_room(ctx, rule16_dq_kernel<DP, EXTRA>, smem));
+    launch_chained(ctx, rule16_dq_kernel<DP, EXTRA>, dim3((unsigned)ceil_div(c.r.lq, R16_T), (unsigned)(c.b * c.h)), R16_THREADS, smem, mq, mk, mv, mg, q);
+  }
+  return OM_OK;
+}
+
+int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
+                   const om_head_strides* ks, const void* v, const om_head_strides* vs, const float2* rows, float* dq, void* dq16,
+                   const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs) {
+  const int lq = c.r.lq, lk = c.r.lk;
+  CUtensorMap mq, mk, mv, mg;
+  if (!r16_map(&mq, q, c.d, lq, c.h, c.b, qs, R16_T, 1) || !r16_map(&mk, k, c.d, lk, c.hkv, c.b, ks, R16_T, 1) ||
+      !r16_map(&mv, v, c.d, lk, c.hkv, c.b, vs, R16_T, 1) || !r16_map(&mg, g, c.d, lq, c.h, c.b, gs, R16_T, 1))
+    return fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the operands of om_rule_attention_bwd_bf16");
+  R16Bwd kv = {};
+  kv.r = c.r; kv.h = c.h; kv.hkv = c.hkv; kv.d = c.d; kv.rows = rows; kv.pitch = rule_rows_pitch(lq); kv.status = ctx->status_dev;
+  R16Bwd one = kv;
+  kv.d0 = dv; kv.d1 = dk; kv.d0_16 = reinterpret_cast<__nv_bfloat16*>(dv16); kv.d1_16 = reinterpret_cast<__nv_bfloat16*>(dk16);
+  if (dv || dv16) kv.s0 = r16_strides(dvs);
+  if (dk || dk16) kv.s1 = r16_strides(dks);
+  one.d0 = dq; one.d0_16 = reinterpret_cast<__nv_bfloat16*>(dq16);
+  if (dq || dq16) one.s0 = r16_strides(dqs);
+  const bool extra = c.r.softcap > 0.f || c.r.slopes;
+  int32_t st;
+  if (c.d <= 64) st = extra ? r16_bwd<64, true>(ctx, c, mq, mk, mv, mg, kv, one) : r16_bwd<64, false>(ctx, c, mq, mk, mv, mg, kv, one);
+  else st = extra ? r16_bwd<128, true>(ctx, c, mq, mk, mv, mg, kv, one) : r16_bwd<128, false>(ctx, c, mq, mk, mv, mg, kv, one);
+  OM_TRY(st);
+  OM_LAUNCH_CHECK(ctx, "om_rule_attention_bwd_bf16");
+  return OM_OK;
+}
+
+}  // namespace om
