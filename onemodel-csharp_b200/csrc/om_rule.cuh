@@ -113,8 +113,13 @@ struct RuleCall {
 int32_t rule_check(om_ctx* ctx, const char* who, const om_attention_rule* rule, int b, int h, int hkv, int lq, int lk, int d, float scale);
 int32_t rule_operand(om_ctx* ctx, const char* who, const void* p, const om_head_strides* s, int d);
 int32_t rule_result(om_ctx* ctx, const char* who, const om_head_strides* s, int b, int h, int l, int d);
-// Row dots rowsum(dO o O) beside the log-sum-exp times `unit`, [b * h][rule_rows_pitch(lq)] float2: what the backward kernels read.
-__host__ __device__ constexpr int rule_rows_pitch(int lq) { return (lq + 127) / 128 * 128; }
+// What the backward kernels read of the queries: per (batch, head) and 128 queries, the log-sum-exps times a unit and behind them the
+// row dots rowsum(dO o O), 256 floats.
+__host__ __device__ constexpr int rule_row_tiles(int lq) { return (lq + 127) / 128; }
+__device__ __forceinline__ float2 rule_row(const float* rows, long long bh, int lq, int i) {
+  const float* t = rows + (bh * rule_row_tiles(lq) + i / 128) * 256 + i % 128;
+  return make_float2(t[0], t[128]);
+}
 int32_t rule_begin(om_ctx* ctx, const om_attention_rule* rule, int b, int h, int hkv, int lq, int lk, int d, float scale, RuleCall* call);
 void rule_end(om_ctx* ctx, RuleCall* call);
 // The tensor-pipe kernels for bfloat16 operands (om_rule_attention16.cu): whether they take a call, and the call. Pointers to
@@ -127,7 +132,7 @@ bool rule16_bwd_takes(const RuleCall& c, const void* g, const om_head_strides* g
                       const om_head_strides* ks, const void* v, const om_head_strides* vs, const float* dq, const void* dq16, const om_head_strides* dqs,
                       const float* dk, const void* dk16, const om_head_strides* dks, const float* dv, const void* dv16, const om_head_strides* dvs);
 int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
-                   const om_head_strides* ks, const void* v, const om_head_strides* vs, const float2* rows, float* dq, void* dq16,
+                   const om_head_strides* ks, const void* v, const om_head_strides* vs, const float* rows, float* dq, void* dq16,
                    const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs);
 
 }  // namespace om

@@ -227,7 +227,7 @@ struct RaParams {
   float *out, *lse;               // forward
   __nv_bfloat16* out16;
   const float* lse_in;            // backward
-  const float2* rows;             // [b * h][rule_rows_pitch(lq)]: log-sum-exp (plus infinity for a row that sees nothing) and row dot
+  const float* rows;              // log-sum-exps (plus infinity for a row that sees nothing) and row dots, read by rule_row
   float *dq, *dk, *dv;
   __nv_bfloat16 *dq16, *dk16, *dv16;
   RaStrides dqs, dks, dvs;
@@ -321,7 +321,7 @@ rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
 template <typename T>
 __global__ void __launch_bounds__(256)
 rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float* lse, int h, int lq, int lq_pad, int d, float unit,
-                 long long total, float2* __restrict__ rows) {
+                 long long total, float* __restrict__ rows) {
   pdl_enter();
   const int lane = threadIdx.x & 31;
   for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
@@ -342,14 +342,17 @@ rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float
         dot = 0.f;
       }
     }
-    if (lane == 0) rows[w] = make_float2(e, dot);
+    if (lane == 0) {
+      rows[w / 128 * 256 + w % 128] = e;
+      rows[w / 128 * 256 + w % 128 + 128] = dot;
+    }
   }
 }
 
 // The weights and the scores' gradients of one tile into P and S, [query][key].
 template <typename T, int BM, int DP>
 __device__ __forceinline__ void ra_gradients(const RaParams<T>& p, const float* Q, const float* K, const float* V, const float* G, float* P, float* S,
-                                             const float2* rows, const int* qdoc, const int* kdoc, int prefix, float slope, int i0, int j0, int ty, int tx) {
+                                             long long bh, const int* qdoc, const int* kdoc, int prefix, float slope, int i0, int j0, int ty, int tx) {
   constexpr int R = BM / 16, LW = BM + 4;
   const RuleArgs& r = p.r;
   float s[R][R], dp[R][R];
@@ -358,7 +361,7 @@ __device__ __forceinline__ void ra_gradients(const RaParams<T>& p, const float* 
 #pragma unroll
   for (int a = 0; a < R; a++) {
     const int i = i0 + ty * R + a;
-    const float2 row = i < r.lq ? rows[i] : make_float2(INFINITY, 0.f);
+    const float2 row = i < r.lq ? rule_row(p.rows, bh, r.lq, i) : make_float2(INFINITY, 0.f);
 #pragma unroll
     for (int c = 0; c < R; c++) {
       const int j = j0 + tx + 16 * c;
@@ -400,7 +403,6 @@ rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
   for (int gi = 0; gi < group; gi++) {
     const int head = hk * group + gi;
     const float slope = r.slopes ? r.slopes[head] : 0.f;
-    const float2* rows = p.rows + ((long long)bi * p.h + head) * rule_rows_pitch(r.lq);
     for (int i0 = lo / BM * BM; i0 < hi; i0 += BM) {
       if (BM >= RULE_GRAIN ? rule_tile(r, prefix, bi, i0, NT, j0, NT) == 0 : rule_documents(r, bi, i0, 1, j0, 1) == 0) continue;
       __syncthreads();
@@ -409,7 +411,7 @@ rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
       if (r.q_docs)
         for (int e = threadIdx.x; e < BM; e += 256) qdoc[e] = i0 + e < r.lq ? r.q_docs[(long long)bi * r.lq + i0 + e] : -1;
       __syncthreads();
-      ra_gradients<T, BM, DP>(p, Q, K, V, G, P, S, rows, qdoc, kdoc, prefix, slope, i0, j0, ty, tx);
+      ra_gradients<T, BM, DP>(p, Q, K, V, G, P, S, (long long)bi * p.h + head, qdoc, kdoc, prefix, slope, i0, j0, ty, tx);
       __syncthreads();
       ra_product<BM, DP, true>(P, G, ty, tx, dv);
       ra_product<BM, DP, true>(S, Q, ty, tx, dk);
@@ -432,7 +434,6 @@ rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
   const int bh = blockIdx.y, bi = bh / p.h, hi = bh - bi * p.h, hk = hi / (p.h / p.hkv);
   const int prefix = r.prefix ? r.prefix[bi] : 0;
   const float slope = r.slopes ? r.slopes[hi] : 0.f;
-  const float2* rows = p.rows + (long long)bh * rule_rows_pitch(r.lq);
   ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + hi * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec);
   ra_load<T, BM, DP>(G, p.g + bi * p.gs.batch + hi * p.gs.head, p.gs.row, i0, r.lq, p.d, p.vec);
   if (r.q_docs)
@@ -453,7 +454,7 @@ rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
     if (r.k_docs)
       for (int e = threadIdx.x; e < BM; e += 256) kdoc[e] = j0 + e < r.lk ? r.k_docs[(long long)bi * r.lk + j0 + e] : -1;
     __syncthreads();
-    ra_gradients<T, BM, DP>(p, Q, K, V, G, nullptr, S, rows, qdoc, kdoc, prefix, slope, i0, j0, ty, tx);
+    ra_gradients<T, BM, DP>(p, Q, K, V, G, nullptr, S, bh, qdoc, kdoc, prefix, slope, i0, j0, ty, tx);
     __syncwarp();
     ra_product<BM, DP, false>(S, K, ty, tx, dq);
   }
@@ -595,9 +596,9 @@ static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   ProfileScope prof(ctx, "om_rule_attention_bwd", 10.0 * b * h * (double)lq * lk * d, sizeof(T) * (4.0 * b * h * (double)lq * d + 4.0 * b * hkv * (double)lk * d));
   RuleCall call;
   OM_TRY(rule_begin(ctx, rule, b, h, hkv, lq, lk, d, scale, &call));
-  const int lq_pad = rule_rows_pitch(lq);
-  float2* rows = nullptr;
-  int32_t st = pool_alloc(ctx, sizeof(float2) * (size_t)b * h * lq_pad, false, (void**)&rows);
+  const int lq_pad = rule_row_tiles(lq) * 128;
+  float* rows = nullptr;
+  int32_t st = pool_alloc(ctx, 2 * sizeof(float) * (size_t)b * h * lq_pad, false, (void**)&rows);
   if (st == OM_OK) {
     const long long total = (long long)b * h * lq_pad;
     const bool tensor = sizeof(T) == 2 && rule16_bwd_takes(call, g, gs, q, qs, k, ks, v, vs, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs);

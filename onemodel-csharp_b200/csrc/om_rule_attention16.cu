@@ -120,6 +120,10 @@ __device__ __forceinline__ void r16_load_tile(uint8_t* dst, const CUtensorMap* m
   for (int c = 0; c < DP / 64; c++) tma_load_4d(dst + c * R16_CHUNK, map, c * 64, row0, head, batch, bar);
 }
 
+__device__ __forceinline__ void r16_load_rows(float* dst, const float* src, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 1024, [%2];" ::"r"(smem_u32(dst)), "l"(src), "r"(smem_u32(bar)) : "memory");
+}
+
 // Which of the indices at, at + 1, ... of one row's other axis are seen: [0, prefix), [lo, hi), none beyond `end`.
 struct R16Row {
   int prefix, lo, hi, end, doc;
@@ -142,9 +146,42 @@ __device__ __forceinline__ R16Row r16_key_row(const RuleArgs& r, int prefix, int
   w.doc = r.k_docs && j < r.lk ? r.k_docs[(long long)b * r.lk + j] : -1;
   return w;
 }
-__device__ __forceinline__ bool r16_sees(const R16Row& w, int at, const int32_t* docs) {
-  const bool near = (at >= w.lo && at < w.hi) || at < w.prefix;
-  return near && at < w.end && (!docs || (w.doc >= 0 && docs[at] == w.doc));
+// Bit u: index at + u of the 32 from `at` on is seen.
+__device__ __forceinline__ uint32_t r16_below(int n) { return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t r16_bits(const R16Row& w, int at, const int32_t* docs) {
+  uint32_t v = ((r16_below(w.hi - at) & ~r16_below(w.lo - at)) | r16_below(w.prefix - at)) & r16_below(w.end - at);
+  if (docs) {
+    uint32_t same = 0;
+#pragma unroll 8
+    for (int u = 0; u < 32; u++)
+      if (at + u < w.end) same |= (docs[at + u] == w.doc ? 1u : 0u) << u;
+    v &= w.doc >= 0 ? same : 0u;
+  }
+  return v;
+}
+__device__ __forceinline__ void r16_hide(uint32_t (&x)[32], uint32_t bits) {
+#pragma unroll
+  for (int u = 0; u < 32; u++)
+    if (!((bits >> u) & 1u)) x[u] = 0xff800000u;
+}
+// Two fp32 operations an instruction.
+__device__ __forceinline__ uint64_t r16_two(float a, float b) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ void r16_fma2(float& a, float& b, uint32_t x, uint32_t y, uint64_t m, uint64_t c) {
+  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tfma.rn.f32x2 t, t, %4, %5;\n\tmov.b64 {%0, %1}, t;\n\t}" : "=f"(a), "=f"(b) : "r"(x), "r"(y), "l"(m), "l"(c));
+}
+__device__ __forceinline__ uint64_t r16_add2(uint64_t s, float a, float b) {
+  uint64_t v;
+  asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%2, %3};\n\tadd.rn.f32x2 %0, %1, t;\n\t}" : "=l"(v) : "l"(s), "f"(a), "f"(b));
+  return v;
+}
+__device__ __forceinline__ float r16_max3(float a, float b, float c) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
 }
 // The score in powers of two of a product, and the cap's derivative.
 __device__ __forceinline__ float r16_score(const RuleArgs& r, float slope, int far, float dot, float* dcap) {
@@ -247,15 +284,15 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int split = blockIdx.z;
   int bi, hi, hk, i0;
   if (p.packed) {
-    bi = blockIdx.y / p.hkv;
-    hk = blockIdx.y - bi * p.hkv;
+    bi = blockIdx.x / p.hkv;
+    hk = blockIdx.x - bi * p.hkv;
     hi = hk * group;
     i0 = 0;
   } else {
-    bi = blockIdx.y / p.h;
-    hi = blockIdx.y - bi * p.h;
+    bi = blockIdx.x / p.h;
+    hi = blockIdx.x - bi * p.h;
     hk = hi / group;
-    i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * 2 * R16_T;      // the longest walks of a causal mask first
+    i0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 2 * R16_T;      // the longest walks of a causal mask first
   }
   const int both = !p.packed && i0 + R16_T < r.lq;
 
@@ -429,16 +466,17 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       if (walk.see[g] == 1) {
 #pragma unroll
-        for (int c = 0; c < 4; c++)
-#pragma unroll
-          for (int u = 0; u < 32; u++)
-            if (!r16_sees(seen, j0 + c * 32 + u, docs)) x[c][u] = 0xff800000u;
+        for (int c = 0; c < 4; c++) r16_hide(x[c], r16_bits(seen, j0 + c * 32, docs));
       }
-      float top = __uint_as_float(x[0][0]);
+      float tops[4];
 #pragma unroll
-      for (int c = 0; c < 4; c++)
+      for (int c = 0; c < 4; c++) {
+        float t = fmaxf(__uint_as_float(x[c][0]), __uint_as_float(x[c][1]));
 #pragma unroll
-        for (int u = 0; u < 32; u++) top = fmaxf(top, __uint_as_float(x[c][u]));
+        for (int u = 2; u < 32; u += 2) t = r16_max3(t, __uint_as_float(x[c][u]), __uint_as_float(x[c][u + 1]));
+        tops[c] = t;
+      }
+      float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       top *= mult;
       float shrink = 1.f;
       if (top > m + 8.f || m == -INFINITY) {
@@ -457,21 +495,24 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t mult2 = r16_two(mult, mult), base2 = r16_two(-base, -base);
+      uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         uint32_t w[32];
 #pragma unroll
         for (int u = 0; u < 32; u++) {
-          const float a = r16_ex2(fmaf(__uint_as_float(x[2 * half + u / 16][(2 * u) % 32]), mult, -base));
-          const float b = r16_ex2(fmaf(__uint_as_float(x[2 * half + u / 16][(2 * u + 1) % 32]), mult, -base));
-          sum[(2 * u) & 3] += a;
-          sum[(2 * u + 1) & 3] += b;
+          float a, b;
+          r16_fma2(a, b, x[2 * half + u / 16][(2 * u) % 32], x[2 * half + u / 16][(2 * u + 1) % 32], mult2, base2);
+          a = r16_ex2(a);
+          b = r16_ex2(b);
+          sum[u & 1] = r16_add2(sum[u & 1], a, b);
           w[u] = r16_pack(a, b);
         }
         r16_st32(t_s + 32u * half, w);
       }
-      l = fmaf(l, shrink, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+      const float2 s0 = *reinterpret_cast<const float2*>(&sum[0]), s1 = *reinterpret_cast<const float2*>(&sum[1]);
+      l = fmaf(l, shrink, (s0.x + s0.y) + (s1.x + s1.y));
       r16_st_wait();
       tc_fence_before();
       r16_arrive(&bar_p[g]);
@@ -563,8 +604,8 @@ rule16_join_kernel(const __grid_constant__ R16Fwd p) {
 struct R16Bwd {
   RuleArgs r;
   int h, hkv, d;
-  const float2* rows;             // [b * h][pitch]: log-sum-exp in powers of two, row dot
-  int pitch;
+  const float* rows;              // [b * h][tiles of 128 queries][2][128]: log-sum-exp in powers of two, row dots
+  int tiles;
   float *d0, *d1;                 // dv and dk, or dq and nothing
   __nv_bfloat16 *d0_16, *d1_16;
   R16Strides s0, s1;
@@ -574,56 +615,66 @@ struct R16Bwd {
 template <int DP>
 struct R16BwdShape {
   static constexpr int TILE = DP / 64 * R16_CHUNK;
-  static constexpr int RING_A = 3, RING_B = 2;           // tiles that two products read (Q or K), and the others (dO or V)
-  static constexpr int BARS = (2 + RING_A + RING_B) * TILE;
+  static constexpr int RING = 2;
+  static constexpr int ROWS = (2 + 2 * RING) * TILE;     // the queries' log-sum-exps and row dots, 1 KB a stage
+  static constexpr int BARS = ROWS + RING * 1024;
   static constexpr int SMEM = BARS + 256 + 1024;
 };
 
 // Scores of one row (64 of them, half a tile) to weights: packed as bfloat16 in w where they are wanted, and in x, times the cap's
-// derivative, for r16_gradients. Rows are keys (COLUMNS: log-sum-exp and row dot go with the column) or queries.
+// derivative, for r16_gradients. Rows are keys (COLUMNS: the log-sum-exps go with the columns) or queries.
 template <bool EXTRA, bool COLUMNS>
-__device__ __forceinline__ void r16_weights(const RuleArgs& r, uint32_t (&x)[2][32], uint32_t (&w)[32], const float2* rows, float lse, float slope, int far, float mult,
+__device__ __forceinline__ void r16_weights(const RuleArgs& r, uint32_t (&x)[2][32], uint32_t (&w)[32], const float* lses, float lse, float slope, int far, float mult,
                                             bool partial, const R16Row& seen, int at, const int32_t* docs) {
+  float dcap[EXTRA ? 64 : 1];
+  if (EXTRA) {
 #pragma unroll
-  for (int c = 0; c < 2; c++)
+    for (int u = 0; u < 64; u++)
+      x[u / 32][u % 32] = __float_as_uint(r16_score(r, slope, COLUMNS ? far + u : far - u, __uint_as_float(x[u / 32][u % 32]), &dcap[EXTRA ? u : 0]));
+  }
+  if (partial) {
 #pragma unroll
-    for (int u = 0; u < 32; u += 2) {
-      float e[2] = {lse, lse}, p[2];
-      if (COLUMNS) {
-        const float4 v = *reinterpret_cast<const float4*>(rows + c * 32 + u);
-        e[0] = v.x;
-        e[1] = v.z;
-      }
+    for (int c = 0; c < 2; c++) r16_hide(x[c], r16_bits(seen, at + c * 32, docs));
+  }
+  const uint64_t mult2 = r16_two(mult, mult);
 #pragma unroll
-      for (int t = 0; t < 2; t++) {
-        float s = __uint_as_float(x[c][u + t]), dcap = 1.f;
-        if (EXTRA) s = r16_score(r, slope, COLUMNS ? far + (c * 32 + u + t) : far - (c * 32 + u + t), s, &dcap);
-        p[t] = r16_ex2(fmaf(s, mult, -e[t]));
-        float d = EXTRA ? p[t] * dcap : p[t];
-        if (partial && !r16_sees(seen, at + c * 32 + u + t, docs)) p[t] = d = 0.f;
-        x[c][u + t] = __float_as_uint(d);
-      }
-      if (COLUMNS) w[c * 16 + u / 2] = r16_pack(p[0], p[1]);
+  for (int u = 0; u < 64; u += 4) {
+    float e[4] = {lse, lse, lse, lse}, p[4];
+    if (COLUMNS) {
+      const float4 v = *reinterpret_cast<const float4*>(lses + u);
+      e[0] = v.x; e[1] = v.y; e[2] = v.z; e[3] = v.w;
     }
+#pragma unroll
+    for (int t = 0; t < 4; t += 2) {
+      r16_fma2(p[t], p[t + 1], x[u / 32][(u + t) % 32], x[u / 32][(u + t + 1) % 32], mult2, r16_two(-e[t], -e[t + 1]));
+      p[t] = r16_ex2(p[t]);
+      p[t + 1] = r16_ex2(p[t + 1]);
+      if (COLUMNS) w[(u + t) / 2] = r16_pack(p[t], p[t + 1]);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; t++) x[u / 32][(u + t) % 32] = __float_as_uint(EXTRA ? p[t] == 0.f ? 0.f : p[t] * dcap[EXTRA ? u + t : 0] : p[t]);
+  }
 }
 // dS = weight (dP - dot), 32 of them, packed. partial: some are hidden, and 0 whatever dP is there.
 template <bool COLUMNS>
-__device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uint32_t (&dp)[32], uint32_t* w, const float2* rows, float dot, bool partial) {
+__device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uint32_t (&dp)[32], uint32_t* w, const float* dots, float dot, bool partial) {
+  float v[32];
 #pragma unroll
-  for (int u = 0; u < 32; u += 2) {
-    float d[2] = {dot, dot};
+  for (int u = 0; u < 32; u += 4) {
+    float d[4] = {dot, dot, dot, dot};
     if (COLUMNS) {
-      const float4 v = *reinterpret_cast<const float4*>(rows + u);
-      d[0] = v.y;
-      d[1] = v.w;
+      const float4 f = *reinterpret_cast<const float4*>(dots + u);
+      d[0] = f.x; d[1] = f.y; d[2] = f.z; d[3] = f.w;
     }
-    float a = __uint_as_float(x[u]) * (__uint_as_float(dp[u]) - d[0]), b = __uint_as_float(x[u + 1]) * (__uint_as_float(dp[u + 1]) - d[1]);
-    if (partial) {
-      a = x[u] == 0u ? 0.f : a;
-      b = x[u + 1] == 0u ? 0.f : b;
-    }
-    w[u / 2] = r16_pack(a, b);
+#pragma unroll
+    for (int t = 0; t < 4; t++) v[u + t] = __uint_as_float(x[u + t]) * (__uint_as_float(dp[u + t]) - d[t]);
   }
+  if (partial) {
+#pragma unroll
+    for (int u = 0; u < 32; u++) v[u] = x[u] == 0u ? 0.f : v[u];
+  }
+#pragma unroll
+  for (int u = 0; u < 32; u += 2) w[u / 2] = r16_pack(v[u], v[u + 1]);
 }
 
 template <int DP, bool EXTRA>
@@ -634,15 +685,16 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   constexpr uint32_t COL_S = 0, COL_DP = 128, COL_DV = 256, COL_DK = 384;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t *slot_k = smem, *slot_v = smem + W::TILE, *ring_q = smem + 2 * W::TILE, *ring_g = ring_q + W::RING_A * W::TILE;
+  uint8_t *slot_k = smem, *slot_v = smem + W::TILE, *ring_q = smem + 2 * W::TILE, *ring_g = ring_q + W::RING * W::TILE;
+  float* ring_rows = reinterpret_cast<float*>(smem + W::ROWS);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
   uint64_t *bar_kv = bars, *bar_s = bars + 1, *bar_dp = bars + 2, *bar_p = bars + 3, *bar_ds = bars + 4, *bar_dv = bars + 5, *bar_dk = bars + 6,
-           *bar_done = bars + 7, *full_q = bars + 8 /* [3] */, *empty_q = bars + 11, *full_g = bars + 14 /* [2] */, *empty_g = bars + 16;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+           *bar_done = bars + 7, *full_q = bars + 8 /* [2] */, *empty_q = bars + 10, *full_g = bars + 12, *empty_g = bars + 14, *full_r = bars + 16, *empty_r = bars + 18;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const RuleArgs& r = p.r;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int j0 = blockIdx.x * R16_T, bi = blockIdx.y / p.hkv, hk = blockIdx.y - bi * p.hkv, group = p.h / p.hkv;
+  const int j0 = blockIdx.y * R16_T, bi = blockIdx.x / p.hkv, hk = blockIdx.x - bi * p.hkv, group = p.h / p.hkv;   // the longest walks of a causal mask first
 
   if (threadIdx.x == 0) {
     mbar_init(bar_kv, 1);
@@ -653,11 +705,11 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     mbar_init(bar_dv, 1);
     mbar_init(bar_dk, 1);
     mbar_init(bar_done, 1);
-    for (int a = 0; a < 3; a++) {
+    for (int a = 0; a < W::RING; a++) {
       mbar_init(&full_q[a], 1);
       mbar_init(&empty_q[a], 1);
-    }
-    for (int a = 0; a < 2; a++) {
+      mbar_init(&full_r[a], 1);
+      mbar_init(&empty_r[a], 256);
       mbar_init(&full_g[a], 1);
       mbar_init(&empty_g[a], 1);
     }
@@ -705,19 +757,23 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       bool ok = true;
       for (; ok && next(); n++) {
         const int at = step.at - R16_T, head = hk * group + step.gi;
-        if (n >= W::RING_A) ok = mbar_wait(&empty_q[a], pa ^ 1u, abort_flag, p.status, 71);
+        if (n >= W::RING) ok = mbar_wait(&empty_q[a], pa ^ 1u, abort_flag, p.status, 71);
         if (!ok) break;
         mbar_expect_tx(&full_q[a], W::TILE);
         r16_load_tile<DP>(ring_q + a * W::TILE, &map_q, at, head, bi, &full_q[a]);
-        if (++a == W::RING_A) {
+        if (n >= W::RING) ok = mbar_wait(&empty_r[a], pa ^ 1u, abort_flag, p.status, 70);
+        if (!ok) break;
+        mbar_expect_tx(&full_r[a], 1024);
+        r16_load_rows(ring_rows + a * 256, p.rows + (((long long)bi * p.h + head) * p.tiles + at / R16_T) * 256, &full_r[a]);
+        if (++a == W::RING) {
           a = 0;
           pa ^= 1u;
         }
-        if (n >= W::RING_B) ok = mbar_wait(&empty_g[b], pb ^ 1u, abort_flag, p.status, 72);
+        if (n >= W::RING) ok = mbar_wait(&empty_g[b], pb ^ 1u, abort_flag, p.status, 72);
         if (!ok) break;
         mbar_expect_tx(&full_g[b], W::TILE);
         r16_load_tile<DP>(ring_g + b * W::TILE, &map_g, at, head, bi, &full_g[b]);
-        if (++b == W::RING_B) {
+        if (++b == W::RING) {
           b = 0;
           pb ^= 1u;
         }
@@ -745,7 +801,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       for (; ok && more; n++) {
         more = next();
-        const int a1 = a + 1 == W::RING_A ? 0 : a + 1, b1 = b + 1 == W::RING_B ? 0 : b + 1;
+        const int a1 = a + 1 == W::RING ? 0 : a + 1, b1 = b + 1 == W::RING ? 0 : b + 1;
         const uint32_t pa1 = a1 == 0 ? pa ^ 1u : pa, pb1 = b1 == 0 ? pb ^ 1u : pb;
         // dV += P^T dO, then the next tile's scores as soon as that product has read P (which lies over them).
         if (!(ok = mbar_wait(bar_p, n & 1u, abort_flag, p.status, 76))) break;
@@ -790,8 +846,8 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     for (; ok && next(); n++) {
       const int head = hk * group + step.gi, at = step.at - R16_T + g * 64;
       const float slope = EXTRA && r.slopes ? r.slopes[head] : 0.f;
-      const float2* rows = p.rows + ((long long)bi * p.h + head) * p.pitch + at;
-      if (!(ok = r16_wait(bar_s, n & 1u, abort_flag, p.status, 80))) break;
+      const float* rows = ring_rows + (n & 1u) * 256 + g * 64;
+      if (!(ok = r16_wait(&full_r[n & 1u], (n >> 1) & 1u, abort_flag, p.status, 94) && r16_wait(bar_s, n & 1u, abort_flag, p.status, 80))) break;
       tc_fence_after();
       uint32_t x[2][32], w[32];
       tmem_ld_32x32b_x32(lane_base + COL_S + 64u * g, x[0]);
@@ -809,8 +865,9 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         uint32_t dp[32];
         tmem_ld_32x32b_x32(lane_base + COL_DP + 64u * g + 32u * c, dp);
         tmem_ld_wait();
-        r16_gradients<true>(x[c], dp, w + c * 16, rows + c * 32, 0.f, step.see == 1);
+        r16_gradients<true>(x[c], dp, w + c * 16, rows + 128 + c * 32, 0.f, step.see == 1);
       }
+      r16_arrive(&empty_r[n & 1u]);
       r16_st32(lane_base + COL_DP + 64u * g, w);
       r16_st_wait();
       tc_fence_before();
@@ -856,15 +913,15 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   constexpr uint32_t COL_S = 0 /* two buffers */, COL_DP = 256, COL_DQ = 384;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t *slot_q = smem, *slot_g = smem + W::TILE, *ring_k = smem + 2 * W::TILE, *ring_v = ring_k + W::RING_A * W::TILE;
+  uint8_t *slot_q = smem, *slot_g = smem + W::TILE, *ring_k = smem + 2 * W::TILE, *ring_v = ring_k + W::RING * W::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
   uint64_t *bar_qg = bars, *bar_s = bars + 1 /* [2] */, *bar_dp = bars + 3, *bar_read = bars + 4, *bar_ds = bars + 5, *bar_dq = bars + 6 /* [2] */,
-           *bar_done = bars + 8, *full_k = bars + 9 /* [3] */, *empty_k = bars + 12, *full_v = bars + 15 /* [2] */, *empty_v = bars + 17;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+           *bar_done = bars + 8, *full_k = bars + 9 /* [2] */, *empty_k = bars + 11, *full_v = bars + 13, *empty_v = bars + 15;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const RuleArgs& r = p.r;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * R16_T, bi = blockIdx.y / p.h, hi = blockIdx.y - bi * p.h, hk = hi / (p.h / p.hkv);
+  const int i0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * R16_T, bi = blockIdx.x / p.h, hi = blockIdx.x - bi * p.h, hk = hi / (p.h / p.hkv);
 
   if (threadIdx.x == 0) {
     mbar_init(bar_qg, 1);
@@ -877,8 +934,6 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       mbar_init(&bar_dq[a], 1);
       mbar_init(&full_v[a], 1);
       mbar_init(&empty_v[a], 1);
-    }
-    for (int a = 0; a < 3; a++) {
       mbar_init(&full_k[a], 1);
       mbar_init(&empty_k[a], 1);
     }
@@ -913,19 +968,19 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       uint32_t pa = 0, pb = 0;
       bool ok = true;
       for (; ok && walk.next(); n++) {
-        if (n >= W::RING_A) ok = mbar_wait(&empty_k[a], pa ^ 1u, abort_flag, p.status, 83);
+        if (n >= W::RING) ok = mbar_wait(&empty_k[a], pa ^ 1u, abort_flag, p.status, 83);
         if (!ok) break;
         mbar_expect_tx(&full_k[a], W::TILE);
         r16_load_tile<DP>(ring_k + a * W::TILE, &map_k, walk.tile(), hk, bi, &full_k[a]);
-        if (++a == W::RING_A) {
+        if (++a == W::RING) {
           a = 0;
           pa ^= 1u;
         }
-        if (n >= W::RING_B) ok = mbar_wait(&empty_v[b], pb ^ 1u, abort_flag, p.status, 84);
+        if (n >= W::RING) ok = mbar_wait(&empty_v[b], pb ^ 1u, abort_flag, p.status, 84);
         if (!ok) break;
         mbar_expect_tx(&full_v[b], W::TILE);
         r16_load_tile<DP>(ring_v + b * W::TILE, &map_v, walk.tile(), hk, bi, &full_v[b]);
-        if (++b == W::RING_B) {
+        if (++b == W::RING) {
           b = 0;
           pb ^= 1u;
         }
@@ -954,7 +1009,7 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       for (; ok && more; n++) {
         more = walk.next();
-        const int a1 = a + 1 == W::RING_A ? 0 : a + 1, b1 = b + 1 == W::RING_B ? 0 : b + 1;
+        const int a1 = a + 1 == W::RING ? 0 : a + 1, b1 = b + 1 == W::RING ? 0 : b + 1;
         const uint32_t pa1 = a1 == 0 ? pa ^ 1u : pa, pb1 = b1 == 0 ? pb ^ 1u : pb, buf = n & 1u;
         if (more) {
           // The next tile's scores into the other buffer, whose dS the product of the tile before has read.
@@ -991,7 +1046,8 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
     const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
     const float mult = EXTRA ? 1.f : r.scale * R16_LOG2E;
-    const float2 stat = p.rows[((long long)bi * p.h + hi) * p.pitch + i];
+    const float* stats = p.rows + (((long long)bi * p.h + hi) * p.tiles + i0 / R16_T) * 256 + row;
+    const float2 stat = make_float2(stats[0], stats[128]);
     bool ok = true;
     uint32_t n = 0;
     for (; ok && walk.next(); n++) {
@@ -1072,7 +1128,10 @@ static bool r16_result(const float* p, const void* p16, const om_head_strides* s
   if (p && ((reinterpret_cast<uintptr_t>(p) & 15) || s->row % 4 || s->head % 4 || s->batch % 4)) return false;
   return !p16 || !((reinterpret_cast<uintptr_t>(p16) & 15) || s->row % 8 || s->head % 8 || s->batch % 8);
 }
-static bool r16_shape(const RuleCall& c) { return encode_fn() && c.d % 8 == 0 && c.d <= 128 && c.r.scale > 0.f; }
+// Tiles are the grid's second axis: 65535 of them.
+static bool r16_shape(const RuleCall& c) {
+  return encode_fn() && c.d % 8 == 0 && c.d <= 128 && c.r.scale > 0.f && c.r.lq <= 65535 * R16_T && c.r.lk <= 65535 * R16_T;
+}
 static R16Strides r16_strides(const om_head_strides* s) { return R16Strides{s->batch, s->head, s->row}; }
 
 bool rule16_fwd_takes(const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
@@ -1109,7 +1168,7 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
   p.status = ctx->status_dev;
   // Heads that share keys as rows of one tile where they fit it: keys and values are read once for all of them.
   p.packed = (long long)group * lq <= R16_T && (group > 1);
-  dim3 grid(p.packed ? 1u : (unsigned)ceil_div(lq, 2 * R16_T), (unsigned)(c.b * (p.packed ? c.hkv : c.h)), 1);
+  dim3 grid((unsigned)(c.b * (p.packed ? c.hkv : c.h)), p.packed ? 1u : (unsigned)ceil_div(lq, 2 * R16_T), 1);
   // A walk is split where the CTAs leave SMs without one, four tiles of keys a part at least: a part costs its CTA's start and a
   // row of O per query in memory, twice.
   const int64_t ctas = (int64_t)grid.x * grid.y;
@@ -1147,17 +1206,17 @@ static int32_t r16_bwd(om_ctx* ctx, const RuleCall& c, const CUtensorMap& mq, co
   const int smem = R16BwdShape<DP>::SMEM;
   if (kv.d0 || kv.d0_16 || kv.d1 || kv.d1_16) {
     OM_TRY(r16_room(ctx, rule16_dkv_kernel<DP, EXTRA>, smem));
-    launch_chained(ctx, rule16_dkv_kernel<DP, EXTRA>, dim3((unsigned)ceil_div(c.r.lk, R16_T), (unsigned)(c.b * c.hkv)), R16_THREADS, smem, mq, mk, mv, mg, kv);
+    launch_chained(ctx, rule16_dkv_kernel<DP, EXTRA>, dim3((unsigned)(c.b * c.hkv), (unsigned)ceil_div(c.r.lk, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, kv);
   }
   if (q.d0 || q.d0_16) {
     OM_TRY(r16_room(ctx, rule16_dq_kernel<DP, EXTRA>, smem));
-    launch_chained(ctx, rule16_dq_kernel<DP, EXTRA>, dim3((unsigned)ceil_div(c.r.lq, R16_T), (unsigned)(c.b * c.h)), R16_THREADS, smem, mq, mk, mv, mg, q);
+    launch_chained(ctx, rule16_dq_kernel<DP, EXTRA>, dim3((unsigned)(c.b * c.h), (unsigned)ceil_div(c.r.lq, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, q);
   }
   return OM_OK;
 }
 
 int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
-                   const om_head_strides* ks, const void* v, const om_head_strides* vs, const float2* rows, float* dq, void* dq16,
+                   const om_head_strides* ks, const void* v, const om_head_strides* vs, const float* rows, float* dq, void* dq16,
                    const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs) {
   const int lq = c.r.lq, lk = c.r.lk;
   CUtensorMap mq, mk, mv, mg;
@@ -1165,7 +1224,7 @@ int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_
       !r16_map(&mv, v, c.d, lk, c.hkv, c.b, vs, R16_T, 1) || !r16_map(&mg, g, c.d, lq, c.h, c.b, gs, R16_T, 1))
     return fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the operands of om_rule_attention_bwd_bf16");
   R16Bwd kv = {};
-  kv.r = c.r; kv.h = c.h; kv.hkv = c.hkv; kv.d = c.d; kv.rows = rows; kv.pitch = rule_rows_pitch(lq); kv.status = ctx->status_dev;
+  kv.r = c.r; kv.h = c.h; kv.hkv = c.hkv; kv.d = c.d; kv.rows = rows; kv.tiles = rule_row_tiles(lq); kv.status = ctx->status_dev;
   R16Bwd one = kv;
   kv.d0 = dv; kv.d1 = dk; kv.d0_16 = reinterpret_cast<__nv_bfloat16*>(dv16); kv.d1_16 = reinterpret_cast<__nv_bfloat16*>(dk16);
   if (dv || dv16) kv.s0 = r16_strides(dvs);
