@@ -48,42 +48,88 @@ __device__ __forceinline__ void rule_queries(const RuleArgs& r, int prefix, int 
   *lo = (int)min(a, (long long)r.lq);
   *hi = (int)max(b, 0ll);
 }
-// Documents of queries [i0, i0 + 64 nq) and keys [j0, j0 + 64 nk): 0 none in common, 1 perhaps some, 2 one and the same throughout.
-__device__ __forceinline__ int rule_documents(const RuleArgs& r, int b, int i0, int nq, int j0, int nk) {
-  if (!r.q_docs) return 2;
-  int qlo = INT32_MAX, qhi = -1, klo = INT32_MAX, khi = -1, one = -2;
-  bool whole = true;
-  for (int t = i0 / RULE_GRAIN; t < min(i0 / RULE_GRAIN + nq, r.nq64); t++) {
-    const int4 v = r.q_ranges[(long long)b * r.nq64 + t];
-    qlo = min(qlo, v.x);
-    qhi = max(qhi, v.y);
-    if (one == -2) one = v.z;
-    whole = whole && v.z >= 0 && v.z == one;
+// What a fixed tile of queries (or of keys) sees of the other axis, as whole numbers that a walk over that axis compares with: the
+// indices below `pre` and those in [lo, hi) are seen by some of its rows, those below `all_pre` and those in [all_lo, all_hi) by all.
+struct RuleTile {
+  int pre, lo, hi, all_pre, all_lo, all_hi, end;
+  int doc_lo, doc_hi, doc;               // documents of its rows; `doc` where they are one and the same, else -1
+  const int4* other;                     // the other axis's documents, per 64 indices (null: no documents)
+  int n64;
+};
+__device__ __forceinline__ int rule_clamp(long long v, int end) { return (int)max(0ll, min(v, (long long)end)); }
+__device__ __forceinline__ void rule_tile_documents(RuleTile& t, const int4* mine, int m64, int first, int n, const int4* other, int n64) {
+  t.other = other;
+  t.n64 = n64;
+  t.doc_lo = INT32_MAX;
+  t.doc_hi = t.doc = -1;
+  if (!other) return;
+  for (int e = first / RULE_GRAIN; e < min(first / RULE_GRAIN + n, m64); e++) {
+    const int4 v = mine[e];
+    t.doc_lo = min(t.doc_lo, v.x);
+    t.doc_hi = max(t.doc_hi, v.y);
+    t.doc = e == first / RULE_GRAIN || v.z == t.doc ? v.z : -1;
   }
-  for (int t = j0 / RULE_GRAIN; t < min(j0 / RULE_GRAIN + nk, r.nk64); t++) {
-    const int4 v = r.k_ranges[(long long)b * r.nk64 + t];
-    klo = min(klo, v.x);
-    khi = max(khi, v.y);
-    whole = whole && v.z == one;
-  }
-  if (qhi < 0 || khi < 0 || qlo > khi || klo > qhi) return 0;
-  return whole ? 2 : 1;
 }
-// 0: nothing of the tile is visible; 1: some may be; 2: every query of the sequence in it sees all of its keys, none of them beyond
-// the last.
-__device__ __forceinline__ int rule_tile(const RuleArgs& r, int prefix, int b, int i0, int nq, int j0, int nk) {
-  const int i1 = min(i0 + nq * RULE_GRAIN, r.lq), j1 = min(j0 + nk * RULE_GRAIN, r.lk);
-  if (i0 >= i1 || j0 >= j1) return 0;
+// Queries [i0, i0 + 64 n).
+__device__ __forceinline__ RuleTile rule_query_tile(const RuleArgs& r, int prefix, int b, int i0, int n) {
+  RuleTile t;
+  const int i1 = min(i0 + n * RULE_GRAIN, r.lq);
   const RuleSpan s = rule_keys(r, prefix, i0, i1);
-  if (!(j0 < s.prefix || (j0 < s.hi && j1 > s.lo))) return 0;
-  const int docs = rule_documents(r, b, i0, nq, j0, nk);
-  if (docs != 2) return docs;
-  if (j1 - j0 != nk * RULE_GRAIN) return 1;
-  if (j1 <= s.prefix) return 2;
+  t.end = r.lk;
+  t.pre = t.all_pre = s.prefix;
+  t.lo = s.lo;
+  t.hi = i0 < i1 ? s.hi : 0;
   const long long p0 = (long long)i0 + r.q_offset, p1 = (long long)i1 - 1 + r.q_offset;
-  if (r.causal && j1 - 1 > p0) return 1;
-  if (r.window && (p1 - j0 >= r.window || j1 - 1 - p0 >= r.window)) return 1;
-  return 2;
+  long long lo = 0, hi = r.lk;
+  if (r.causal) hi = min(hi, p0 + 1);
+  if (r.window) {
+    lo = max(lo, p1 - r.window + 1);
+    hi = min(hi, p0 + r.window);
+  }
+  t.all_lo = rule_clamp(lo, r.lk);
+  t.all_hi = rule_clamp(hi, r.lk);
+  if (i0 >= i1) t.pre = 0;
+  rule_tile_documents(t, r.q_docs ? r.q_ranges + (long long)b * r.nq64 : nullptr, r.nq64, i0, n, r.q_docs ? r.k_ranges + (long long)b * r.nk64 : nullptr, r.nk64);
+  return t;
+}
+// Keys [j0, j0 + 64 n).
+__device__ __forceinline__ RuleTile rule_key_tile(const RuleArgs& r, int prefix, int b, int j0, int n) {
+  RuleTile t;
+  const int j1 = min(j0 + n * RULE_GRAIN, r.lk);
+  t.end = r.lq;
+  t.pre = t.all_pre = 0;
+  rule_queries(r, prefix, j0, j1, &t.lo, &t.hi);
+  long long lo = 0, hi = r.lq;
+  if (j1 > prefix) {
+    if (r.causal) lo = max(lo, (long long)j1 - 1 - r.q_offset);
+    if (r.window) {
+      lo = max(lo, (long long)j1 - r.window - r.q_offset);
+      hi = min(hi, (long long)j0 + r.window - r.q_offset);
+    }
+  }
+  t.all_lo = rule_clamp(lo, r.lq);
+  t.all_hi = rule_clamp(hi, r.lq);
+  rule_tile_documents(t, r.q_docs ? r.k_ranges + (long long)b * r.nk64 : nullptr, r.nk64, j0, n, r.q_docs ? r.q_ranges + (long long)b * r.nq64 : nullptr, r.nq64);
+  return t;
+}
+// What the tile sees of indices [at, at + 64 n): 0 nothing, 1 perhaps some, 2 all of its rows see all of those in range (FULL: and
+// all of them are in range).
+template <bool FULL>
+__device__ __forceinline__ int rule_see(const RuleTile& t, int at, int n) {
+  const int to = min(at + n * RULE_GRAIN, t.end);
+  if (at >= to || !(at < t.pre || (at < t.hi && to > t.lo))) return 0;
+  const bool all = (to <= t.all_pre || (at >= t.all_lo && to <= t.all_hi)) && (!FULL || to == at + n * RULE_GRAIN);
+  if (!t.other) return all ? 2 : 1;
+  int lo = INT32_MAX, hi = -1;
+  bool same = t.doc >= 0;
+  for (int e = at / RULE_GRAIN; e < min(at / RULE_GRAIN + n, t.n64); e++) {
+    const int4 v = t.other[e];
+    lo = min(lo, v.x);
+    hi = max(hi, v.y);
+    same = same && v.z == t.doc;
+  }
+  if (hi < 0 || t.doc_hi < 0 || lo > t.doc_hi || hi < t.doc_lo) return 0;
+  return all && same ? 2 : 1;
 }
 // One pair, both inside the matrix; doc: the query's document (any value where there are none).
 __device__ __forceinline__ bool rule_visible(const RuleArgs& r, int prefix, int i, int j, int q_doc, int k_doc) {

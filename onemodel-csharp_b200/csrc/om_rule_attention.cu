@@ -237,7 +237,7 @@ template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
   extern __shared__ __align__(16) float sm[];
-  constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4, NT = BM / RULE_GRAIN > 0 ? BM / RULE_GRAIN : 1;
+  constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *Q = sm, *K = Q + BM * LD, *V = K + BM * LD, *P = V + BM * LD;
   int* kdoc = reinterpret_cast<int*>(P + BM * LW);
   const RuleArgs& r = p.r;
@@ -258,12 +258,12 @@ rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
 #pragma unroll
     for (int c = 0; c < RaCols<DP>::N; c++) acc[a][c] = 0.f;
   }
+  const RuleTile tile = rule_query_tile(r, prefix, bi, i0 / RULE_GRAIN * RULE_GRAIN, 1);
   const RuleSpan span = rule_keys(r, prefix, i0, min(i0 + BM, r.lq));
   const int first = span.prefix > 0 ? 0 : span.lo / BM * BM, last = max(span.prefix, span.hi);
   for (int j0 = first; j0 < last; j0 += BM) {
     // The document ranges go by 64 rows: a tile of 32 asks for the 64 that hold it.
-    if (BM >= RULE_GRAIN ? rule_tile(r, prefix, bi, i0, NT, j0, NT) == 0
-                         : !(j0 < span.prefix || (j0 < span.hi && j0 + BM > span.lo)) || rule_documents(r, bi, i0, 1, j0, 1) == 0) continue;
+    if (rule_see<false>(tile, j0 / RULE_GRAIN * RULE_GRAIN, 1) == 0) continue;
     __syncthreads();
     ra_load<T, BM, DP>(K, p.k + bi * p.ks.batch + hk * p.ks.head, p.ks.row, j0, r.lk, p.d, p.vec);
     ra_load<T, BM, DP>(V, p.v + bi * p.vs.batch + hk * p.vs.head, p.vs.row, j0, r.lk, p.d, p.vec);
@@ -317,36 +317,68 @@ rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
 }
 
 // Row dots rowsum(dO o O) beside the log-sum-exp times `unit` (log2 e for the kernels that work with powers of two); rows behind
-// the last query, and those that see no key, get plus infinity and 0, so that a weight recomputed from them is 0. A warp per row.
-template <typename T>
+// the last query, and those that see no key, get plus infinity and 0, so that a weight recomputed from them is 0. A power of two of
+// lanes per row, each with 16 bytes at a time (N elements; one where rows do not start on that grid), two rows in flight per lane.
+template <typename T, int N>
 __global__ void __launch_bounds__(256)
-rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float* lse, int h, int lq, int lq_pad, int d, float unit,
+rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float* lse, int h, int lq, int lq_pad, int d, int lanes, float unit,
                  long long total, float* __restrict__ rows) {
   pdl_enter();
-  const int lane = threadIdx.x & 31;
-  for (long long w = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); w < total; w += (long long)gridDim.x * 8) {
-    const long long bh = w / lq_pad;
-    const int i = (int)(w - bh * lq_pad);
-    const long long bi = bh / h;
-    const int hi = (int)(bh - bi * h);
-    float dot = 0.f, e = INFINITY;
-    if (i < lq) {
-      const T* gp = g + bi * gs.batch + hi * gs.head + (long long)i * gs.row;
-      const T* op = o + bi * os.batch + hi * os.head + (long long)i * os.row;
-      for (int c = lane; c < d; c += 32) dot = fmaf(ra_value<T>(gp[c]), ra_value<T>(op[c]), dot);
+  struct alignas(N * sizeof(T)) Vec {
+    T v[N];
+  };
+  const int sub = threadIdx.x & (lanes - 1), per_cta = 256 / lanes;
+  for (long long w0 = (long long)blockIdx.x * 2 * per_cta + threadIdx.x / lanes; w0 < total; w0 += (long long)gridDim.x * 2 * per_cta) {
+    float dot[2] = {0.f, 0.f};
+    long long at[2], bhs[2];
+    int is[2];
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, x);
-      e = lse[bh * lq + i] * unit;
-      if (e == -INFINITY) {
-        e = INFINITY;
-        dot = 0.f;
+    for (int u = 0; u < 2; u++) {
+      at[u] = w0 + u * per_cta;
+      bhs[u] = at[u] / lq_pad;
+      is[u] = at[u] < total ? (int)(at[u] - bhs[u] * lq_pad) : lq;
+      if (is[u] < lq) {
+        const long long bi = bhs[u] / h;
+        const int hi = (int)(bhs[u] - bi * h);
+        const T* gp = g + bi * gs.batch + hi * gs.head + (long long)is[u] * gs.row;
+        const T* op = o + bi * os.batch + hi * os.head + (long long)is[u] * os.row;
+        for (int c = sub * N; c < d; c += lanes * N) {
+          const Vec a = *reinterpret_cast<const Vec*>(gp + c), b = *reinterpret_cast<const Vec*>(op + c);
+#pragma unroll
+          for (int e = 0; e < N; e++) dot[u] = fmaf(ra_value<T>(a.v[e]), ra_value<T>(b.v[e]), dot[u]);
+        }
       }
     }
-    if (lane == 0) {
-      rows[w / 128 * 256 + w % 128] = e;
-      rows[w / 128 * 256 + w % 128 + 128] = dot;
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      for (int x = lanes >> 1; x > 0; x >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], x);
+      if (sub == 0 && at[u] < total) {
+        float e = is[u] < lq ? lse[bhs[u] * lq + is[u]] * unit : -INFINITY;
+        if (e == -INFINITY) {
+          e = INFINITY;
+          dot[u] = 0.f;
+        }
+        rows[at[u] / 128 * 256 + at[u] % 128] = e;
+        rows[at[u] / 128 * 256 + at[u] % 128 + 128] = dot[u];
+      }
     }
   }
+}
+template <typename T>
+static void launch_rows(om_ctx* ctx, const T* g, const om_head_strides* gs, const T* o, const om_head_strides* os, const float* lse, int b, int h, int lq, int d,
+                        float unit, float* rows) {
+  const int lq_pad = rule_row_tiles(lq) * 128;
+  const long long total = (long long)b * h * lq_pad;          // a multiple of 128: no warp runs over the end alone
+  constexpr int N = 16 / sizeof(T);
+  auto grid16 = [&](const T* p, const om_head_strides* s) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s->row % N == 0 && s->head % N == 0 && s->batch % N == 0;
+  };
+  const bool vec = d % N == 0 && grid16(g, gs) && grid16(o, os);
+  int lanes = 1;
+  while (lanes < 32 && lanes * (vec ? N : 1) < d) lanes *= 2;
+  const int grid = grid_for(ctx, total, 2 * 256 / lanes, 16);
+  if (vec) launch_chained(ctx, rule_rows_kernel<T, N>, grid, 256, 0, g, ra_strides(gs), o, ra_strides(os), lse, h, lq, lq_pad, d, lanes, unit, total, rows);
+  else launch_chained(ctx, rule_rows_kernel<T, 1>, grid, 256, 0, g, ra_strides(gs), o, ra_strides(os), lse, h, lq, lq_pad, d, lanes, unit, total, rows);
 }
 
 // The weights and the scores' gradients of one tile into P and S, [query][key].
@@ -381,7 +413,7 @@ template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
   extern __shared__ __align__(16) float sm[];
-  constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4, NT = BM / RULE_GRAIN > 0 ? BM / RULE_GRAIN : 1;
+  constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *K = sm, *V = K + BM * LD, *Q = V + BM * LD, *G = Q + BM * LD, *P = G + BM * LD, *S = P + BM * LW;
   int *qdoc = reinterpret_cast<int*>(S + BM * LW), *kdoc = qdoc + BM;
   const RuleArgs& r = p.r;
@@ -398,13 +430,14 @@ rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
   for (int a = 0; a < R; a++)
 #pragma unroll
     for (int c = 0; c < RaCols<DP>::N; c++) dk[a][c] = dv[a][c] = 0.f;
+  const RuleTile tile = rule_key_tile(r, prefix, bi, j0 / RULE_GRAIN * RULE_GRAIN, 1);
   int lo, hi;
   rule_queries(r, prefix, j0, min(j0 + BM, r.lk), &lo, &hi);
   for (int gi = 0; gi < group; gi++) {
     const int head = hk * group + gi;
     const float slope = r.slopes ? r.slopes[head] : 0.f;
     for (int i0 = lo / BM * BM; i0 < hi; i0 += BM) {
-      if (BM >= RULE_GRAIN ? rule_tile(r, prefix, bi, i0, NT, j0, NT) == 0 : rule_documents(r, bi, i0, 1, j0, 1) == 0) continue;
+      if (rule_see<false>(tile, i0 / RULE_GRAIN * RULE_GRAIN, 1) == 0) continue;
       __syncthreads();
       ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + head * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec);
       ra_load<T, BM, DP>(G, p.g + bi * p.gs.batch + head * p.gs.head, p.gs.row, i0, r.lq, p.d, p.vec);
@@ -425,7 +458,7 @@ template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
   extern __shared__ __align__(16) float sm[];
-  constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4, NT = BM / RULE_GRAIN > 0 ? BM / RULE_GRAIN : 1;
+  constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *Q = sm, *G = Q + BM * LD, *K = G + BM * LD, *V = K + BM * LD, *S = V + BM * LD;
   int *qdoc = reinterpret_cast<int*>(S + BM * LW), *kdoc = qdoc + BM;
   const RuleArgs& r = p.r;
@@ -443,11 +476,11 @@ rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
   for (int a = 0; a < R; a++)
 #pragma unroll
     for (int c = 0; c < RaCols<DP>::N; c++) dq[a][c] = 0.f;
+  const RuleTile tile = rule_query_tile(r, prefix, bi, i0 / RULE_GRAIN * RULE_GRAIN, 1);
   const RuleSpan span = rule_keys(r, prefix, i0, min(i0 + BM, r.lq));
   const int first = span.prefix > 0 ? 0 : span.lo / BM * BM, last = max(span.prefix, span.hi);
   for (int j0 = first; j0 < last; j0 += BM) {
-    if (BM >= RULE_GRAIN ? rule_tile(r, prefix, bi, i0, NT, j0, NT) == 0
-                         : !(j0 < span.prefix || (j0 < span.hi && j0 + BM > span.lo)) || rule_documents(r, bi, i0, 1, j0, 1) == 0) continue;
+    if (rule_see<false>(tile, j0 / RULE_GRAIN * RULE_GRAIN, 1) == 0) continue;
     __syncthreads();
     ra_load<T, BM, DP>(K, p.k + bi * p.ks.batch + hk * p.ks.head, p.ks.row, j0, r.lk, p.d, p.vec);
     ra_load<T, BM, DP>(V, p.v + bi * p.vs.batch + hk * p.vs.head, p.vs.row, j0, r.lk, p.d, p.vec);
@@ -600,10 +633,8 @@ static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   float* rows = nullptr;
   int32_t st = pool_alloc(ctx, 2 * sizeof(float) * (size_t)b * h * lq_pad, false, (void**)&rows);
   if (st == OM_OK) {
-    const long long total = (long long)b * h * lq_pad;
     const bool tensor = sizeof(T) == 2 && rule16_bwd_takes(call, g, gs, q, qs, k, ks, v, vs, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs);
-    launch_chained(ctx, rule_rows_kernel<T>, grid_for(ctx, total, 8, 16), 256, 0, g, ra_strides(gs), out, ra_strides(os), lse, h, lq, lq_pad, d,
-                   tensor ? 1.4426950408889634f : 1.f, total, rows);
+    launch_rows<T>(ctx, g, gs, out, os, lse, b, h, lq, d, tensor ? 1.4426950408889634f : 1.f, rows);
     if (tensor) {
       st = rule16_bwd(ctx, call, g, gs, q, qs, k, ks, v, vs, rows, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs);
       pool_free(ctx, rows);
