@@ -2,38 +2,59 @@
 //
 // A matrix is worked on as X [m, n] with m <= n (transposed where it is taller). One step is
 //   G = X X^T,  Y = -4.7750 G + 2.0315 G G,  X' = 3.4445 X + Y X,
-// three products; G and Y are symmetric, so the tiles above the diagonal are mirrored instead of computed. All matrices of a
+// three products; G and Y are symmetric, so their blocks above the diagonal are mirrored instead of computed. All matrices of a
 // call go through each launch together: a launch covers the tiles of one product of up to MU_TENSORS matrices, whatever their
 // shapes, so a step costs three launches for a whole model.
+//
+// The products run on the tensor pipe with fp32 accuracy: a value v is kept as two half-precision numbers, h = half(v) and
+// l = half(v - h), 22 significant bits together, and a product is h h' + h l' + l h' (what is left out is 2^-22 of it). Five steps
+// raise an error in the direction of a small singular value up to 3.4445^5 = 485 times, which is why plain half or bfloat16
+// operands (2^-11, 2^-8) would leave few digits of the update. Every matrix of a step is bounded (|X| <= 1.2, |G| <= 1.5, |Y| <= 3 in the
+// spectral norm, so element by element), and is stored times a power of two that puts its usual elements in the middle of the
+// half's range. Three products at the 16-bit rate bound it: 3/1664 s a TFLOP; two planes of 2 bytes are what fp32 would read.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <math.h>
 
 #include <vector>
 
-#include "om_common.cuh"
+#include "om_tc.cuh"
 
 namespace om {
 
 constexpr int MU_TENSORS = 32;
 constexpr float MU_A = 3.4445f, MU_B = -4.7750f, MU_C = 2.0315f;   // the quintic's coefficients
 constexpr int MU_CHUNK = 8192;                                     // elements of one partial sum of squares
-constexpr int MU_T = 64;                                           // tile
+constexpr int MU_BM = 128, MU_BK = 64;                             // rows of a tile of a product, terms of a stage
+constexpr float MU_SX = 1024.f, MU_SG = 4096.f;                    // X is stored times the first, G and Y times the second
+constexpr int MU_THREADS = 192;                                    // warps 0-3: results; warp 4: MMA issue; warp 5: TMA
 
+// A matrix as two planes of halves, the second `plane` elements behind the first, rows `ld` apart.
+struct MuonPlanes {
+  __half* p;
+  long long plane;
+  int ld;
+};
 struct MuonTensor {
   float *p, *m;
   const float* g;
   uint16_t* p16;
   int rows, cols;        // as the caller has them
-  float *x, *x2, *gram, *poly;   // [mm, nn], [mm, nn], [mm, mm], [mm, mm] with mm <= nn
+  int mm, nn;            // sides of X, mm <= nn
   double* partial;       // [ceil(rows * cols / MU_CHUNK)]
-  int mm, nn;
+  MuonPlanes x, x2, gram, poly;   // [mm, nn], [mm, nn], [mm, mm], [mm, mm]
 };
 struct MuonList {
   om_muon_hyper hyper;
   const om_muon_hyper* hyper_dev;
+  int32_t* status;
   int count;
   long long end[MU_TENSORS];      // work items of this launch up to and with tensor i
   MuonTensor t[MU_TENSORS];
+};
+// The operands of one launch's products: A's tiles, and B's.
+struct MuonMaps {
+  CUtensorMap a[MU_TENSORS], b[MU_TENSORS];
 };
 __device__ __forceinline__ om_muon_hyper mu_hyper(const MuonList& l) { return l.hyper_dev ? *l.hyper_dev : l.hyper; }
 __device__ __forceinline__ int mu_find(const MuonList& l, long long item, long long* local) {
@@ -46,6 +67,7 @@ __device__ __forceinline__ int mu_find(const MuonList& l, long long item, long l
 // m = momentum m + (1 - momentum) g, and the sum of squares of u over this chunk (in double: the chunks of a large matrix
 // differ by orders of magnitude in what they add).
 __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constant__ MuonList l) {
+  pdl_enter();
   long long chunk;
   const MuonTensor& t = l.t[mu_find(l, blockIdx.x, &chunk)];
   const om_muon_hyper h = mu_hyper(l);
@@ -69,13 +91,26 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constan
   }
 }
 
-// X = u / max(|u|, eps), transposed where the matrix is taller than wide.
+__device__ __forceinline__ void mu_split(float v, __half* h, __half* l) {
+  *h = __float2half_rn(v);
+  *l = __float2half_rn(v - __half2float(*h));
+}
+// Tile (row block, column block) of 64 x 64 of the caller's matrix.
+__device__ __forceinline__ void mu_block(const MuonTensor& t, long long tile, int* r0, int* c0) {
+  const int across = (t.cols + 63) / 64;
+  *r0 = (int)(tile / across) * 64;
+  *c0 = (int)(tile % across) * 64;
+}
+
+// X = u / max(|u|, eps) as two planes, transposed where the matrix is taller than wide.
 __global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__ MuonList l) {
-  long long chunk;
-  const MuonTensor& t = l.t[mu_find(l, blockIdx.x, &chunk)];
+  pdl_enter();
+  long long tile;
+  const MuonTensor& t = l.t[mu_find(l, blockIdx.x, &tile)];
   const om_muon_hyper h = mu_hyper(l);
-  const long long n = (long long)t.rows * t.cols, chunks = (n + MU_CHUNK - 1) / MU_CHUNK;
+  const long long chunks = ((long long)t.rows * t.cols + MU_CHUNK - 1) / MU_CHUNK;
   __shared__ double s[8];
+  __shared__ float block[64][65];
   double sum = 0.0;
   for (long long c = threadIdx.x; c < chunks; c += 256) sum += t.partial[c];
 #pragma unroll
@@ -85,75 +120,280 @@ __global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__
   sum = 0.0;
   for (int w = 0; w < 8; w++) sum += s[w];
   const float norm = fmaxf((float)sqrt(sum), h.eps);
-  const long long e1 = min(chunk * MU_CHUNK + MU_CHUNK, n);
-  for (long long e = chunk * MU_CHUNK + threadIdx.x; e < e1; e += 256) {
-    const float m = t.m[e], u = h.nesterov ? fmaf(m, h.momentum, t.g[e] * h.grad_scale * (1.f - h.momentum)) : m;
-    const long long o = t.rows > t.cols ? e % t.cols * t.rows + e / t.cols : e;
-    t.x[o] = u / norm;
+  int r0, c0;
+  mu_block(t, tile, &r0, &c0);
+  const bool turn = t.rows > t.cols;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+    const int r = r0 + e / 64, c = c0 + e % 64;
+    if (r >= t.rows || c >= t.cols) continue;
+    const long long at = (long long)r * t.cols + c;
+    const float m = t.m[at], u = h.nesterov ? fmaf(m, h.momentum, t.g[at] * h.grad_scale * (1.f - h.momentum)) : m;
+    block[e / 64][e % 64] = u / norm * MU_SX;
   }
-}
-
-// One product of a step over every matrix. KIND 0: gram = x x^T; 1: poly = B gram + C gram gram; 2: x2 = A x + poly x.
-template <int KIND>
-__global__ void __launch_bounds__(256) muon_product_kernel(const __grid_constant__ MuonList l) {
-  long long tile;
-  const MuonTensor& t = l.t[mu_find(l, blockIdx.x, &tile)];
-  const int M = t.mm, N = KIND == 2 ? t.nn : t.mm, K = KIND == 0 ? t.nn : t.mm;
-  const int tiles_n = (N + MU_T - 1) / MU_T;
-  const int r0 = (int)(tile / tiles_n) * MU_T, c0 = (int)(tile % tiles_n) * MU_T;
-  const float *A = KIND == 0 ? t.x : KIND == 1 ? t.gram : t.poly, *B = KIND == 1 ? t.gram : t.x;
-  const int lda = K, ldb = KIND == 0 ? K : N;
-  __shared__ float As[16][MU_T + 4], Bs[16][MU_T + 4];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < K; k0 += 16) {
-    for (int e = threadIdx.x; e < 16 * MU_T; e += 256) {
-      const int r = e >> 4, k = e & 15;
-      As[k][r] = r0 + r < M && k0 + k < K ? A[(long long)(r0 + r) * lda + k0 + k] : 0.f;
-      if (KIND == 0) {
-        Bs[k][r] = c0 + r < N && k0 + k < K ? B[(long long)(c0 + r) * ldb + k0 + k] : 0.f;
-      } else {
-        const int c = e & 63, kk = e >> 6;
-        Bs[kk][c] = c0 + c < N && k0 + kk < K ? B[(long long)(k0 + kk) * ldb + c0 + c] : 0.f;
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; k++)
-#pragma unroll
-      for (int a = 0; a < 4; a++)
-#pragma unroll
-        for (int b = 0; b < 4; b++) acc[a][b] = fmaf(As[k][ty * 4 + a], Bs[k][tx * 4 + b], acc[a][b]);
-    __syncthreads();
+  __syncthreads();
+#pragma unroll 4
+  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+    const int a = e / 64, b = e % 64;                     // row and column of this tile of X
+    const int xr = (turn ? c0 : r0) + a, xc = (turn ? r0 : c0) + b;
+    if (xr >= t.mm || xc >= t.nn) continue;
+    __half hi, lo;
+    mu_split(turn ? block[b][a] : block[a][b], &hi, &lo);
+    const long long at = (long long)xr * t.x.ld + xc;
+    t.x.p[at] = hi;
+    t.x.p[t.x.plane + at] = lo;
   }
-  for (int a = 0; a < 4; a++)
-    for (int b = 0; b < 4; b++) {
-      const int r = r0 + ty * 4 + a, c = c0 + tx * 4 + b;
-      if (r >= M || c >= N) continue;
-      const long long o = (long long)r * N + c;
-      if (KIND == 0) t.gram[o] = acc[a][b];
-      if (KIND == 1) t.poly[o] = fmaf(MU_C, acc[a][b], MU_B * t.gram[o]);
-      if (KIND == 2) t.x2[o] = fmaf(MU_A, t.x[o], acc[a][b]);
-    }
 }
 
 // p = (1 - lr weight_decay) p - lr s X, with the bfloat16 copy where it is wanted.
 __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant__ MuonList l) {
-  long long chunk;
-  const MuonTensor& t = l.t[mu_find(l, blockIdx.x, &chunk)];
+  pdl_enter();
+  long long tile;
+  const MuonTensor& t = l.t[mu_find(l, blockIdx.x, &tile)];
   const om_muon_hyper h = mu_hyper(l);
   const float s = h.match_rms ? 0.2f * sqrtf((float)max(t.rows, t.cols)) : sqrtf(fmaxf(1.f, (float)t.rows / (float)t.cols));
   const float keep = 1.f - h.lr * h.weight_decay, rate = h.lr * s;
-  const long long n = (long long)t.rows * t.cols, e1 = min(chunk * MU_CHUNK + MU_CHUNK, n);
-  for (long long e = chunk * MU_CHUNK + threadIdx.x; e < e1; e += 256) {
-    const long long o = t.rows > t.cols ? e % t.cols * t.rows + e / t.cols : e;
-    const float p = fmaf(-rate, t.x[o], t.p[e] * keep);
-    t.p[e] = p;
+  __shared__ float block[64][65];
+  int r0, c0;
+  mu_block(t, tile, &r0, &c0);
+  const bool turn = t.rows > t.cols;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+    const int a = e / 64, b = e % 64;
+    const int xr = (turn ? c0 : r0) + a, xc = (turn ? r0 : c0) + b;
+    if (xr >= t.mm || xc >= t.nn) continue;
+    const long long at = (long long)xr * t.x.ld + xc;
+    const float v = (__half2float(t.x.p[at]) + __half2float(t.x.p[t.x.plane + at])) * (1.f / MU_SX);
+    if (turn) block[b][a] = v;
+    else block[a][b] = v;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+    const int r = r0 + e / 64, c = c0 + e % 64;
+    if (r >= t.rows || c >= t.cols) continue;
+    const long long at = (long long)r * t.cols + c;
+    const float p = fmaf(-rate, block[e / 64][e % 64], t.p[at] * keep);
+    t.p[at] = p;
     if (t.p16) {
       const __nv_bfloat16 v = __float2bfloat16_rn(p);
-      t.p16[e] = *reinterpret_cast<const uint16_t*>(&v);
+      t.p16[at] = *reinterpret_cast<const uint16_t*>(&v);
     }
   }
+}
+
+// ---- products ---------------------------------------------------------------------------------------------------------------------
+
+constexpr uint32_t MU_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);     // stride offset 1024 bytes, version 1, 128-byte swizzle
+__device__ __forceinline__ void mu_mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n\t}"
+      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(MU_DESC_HI), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mu_load(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)), "l"(map),
+               "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+               : "memory");
+}
+// 32 values of a row of planes (from a column that is a multiple of 8; the pitch is one too, so whole groups of 8 lie within it).
+__device__ __forceinline__ void mu_read(const MuonPlanes& x, long long at, int valid, float (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 32; c += 8) {
+    uint4 h = make_uint4(0, 0, 0, 0), l = h;
+    if (c < valid) {
+      h = *reinterpret_cast<const uint4*>(x.p + at + c);
+      l = *reinterpret_cast<const uint4*>(x.p + x.plane + at + c);
+    }
+    const __half2 *hp = reinterpret_cast<const __half2*>(&h), *lp = reinterpret_cast<const __half2*>(&l);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const float2 a = __half22float2(hp[u]), b = __half22float2(lp[u]);
+      v[c + 2 * u] = a.x + b.x;
+      v[c + 2 * u + 1] = a.y + b.y;
+    }
+  }
+}
+
+template <int BN>
+struct MuonShape {
+  static constexpr int PLANE_A = MU_BM * MU_BK * 2, PLANE_B = BN * MU_BK * 2;
+  static constexpr int STAGE = 2 * (PLANE_A + PLANE_B), STAGES = BN == 256 ? 2 : 3;
+  static constexpr int SMEM = STAGES * STAGE + 128 + 1024;
+};
+
+// Blocks of 128 rows by BN columns of one product over every matrix. KIND 0: gram = x x^T; 1: poly = B gram + C gram gram (both
+// symmetric: only what lies on and below the diagonal of blocks of 128, the rest mirrored from there); 2: x2 = A x + poly x.
+template <int KIND, int BN>
+__global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __grid_constant__ MuonList l, const __grid_constant__ MuonMaps maps) {
+  typedef MuonShape<BN> W;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::STAGES * W::STAGE);
+  uint64_t *bar_full = bars, *bar_empty = bars + W::STAGES, *bar_done = bars + 2 * W::STAGES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * W::STAGES + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < W::STAGES; s++) {
+      mbar_init(&bar_full[s], 1);
+      mbar_init(&bar_empty[s], 1);
+    }
+    mbar_init(bar_done, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 4) {
+    tmem_alloc(tmem_slot, BN);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_trigger();
+  pdl_wait();
+
+  long long tile;
+  const int which = mu_find(l, blockIdx.x, &tile);
+  const MuonTensor& t = l.t[which];
+  const int M = t.mm, N = KIND == 2 ? t.nn : t.mm, K = KIND == 0 ? t.nn : t.mm;
+  int r0, c0;
+  if (KIND == 2) {
+    const int down = (M + MU_BM - 1) / MU_BM;            // down the rows first: the CTAs of a round share columns of X
+    c0 = (int)(tile / down) * BN;
+    r0 = (int)(tile % down) * MU_BM;
+  } else {
+    int rb = 0;
+    for (;; rb++) {
+      const int across = ((rb + 1) * MU_BM + BN - 1) / BN;
+      if (tile < across) break;
+      tile -= across;
+    }
+    r0 = rb * MU_BM;
+    c0 = (int)tile * BN;
+  }
+  const int steps = (K + MU_BK - 1) / MU_BK;
+
+  if (warp == 5) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int k = 0; ok && k < steps; k++) {
+        const int s = k % W::STAGES;
+        if (k >= W::STAGES) ok = mbar_wait(&bar_empty[s], (uint32_t)((k / W::STAGES) & 1) ^ 1u, abort_flag, l.status, 101);
+        if (!ok) break;
+        uint8_t* at = smem + s * W::STAGE;
+        mbar_expect_tx(&bar_full[s], W::STAGE);
+#pragma unroll
+        for (int plane = 0; plane < 2; plane++) {
+          mu_load(at + plane * W::PLANE_A, &maps.a[which], k * MU_BK, r0, plane, &bar_full[s]);
+          uint8_t* b = at + 2 * W::PLANE_A + plane * W::PLANE_B;
+          if (KIND == 2) {
+#pragma unroll
+            for (int c = 0; c < BN / 64; c++) mu_load(b + c * 64 * 128, &maps.b[which], c0 + c * 64, k * MU_BK, plane, &bar_full[s]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < BN / 128; c++) mu_load(b + c * 128 * 128, &maps.a[which], k * MU_BK, c0 + c * 128, plane, &bar_full[s]);
+          }
+        }
+      }
+    }
+  } else if (warp == 4) {
+    if (lane == 0) {
+      // Half-precision operands, fp32 sums; B is K-major (rows of the same matrix) or MN-major (X as it lies).
+      constexpr uint32_t idesc = (1u << 4) | ((KIND == 2 ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(MU_BM >> 4) << 24);
+      constexpr uint32_t lbo_b = KIND == 2 ? ((64u * 128u) >> 4) << 16 : 1u << 16, step_b = KIND == 2 ? (16u * 128u) >> 4 : 2u;
+      bool ok = true;
+      for (int k = 0; ok && k < steps; k++) {
+        const int s = k % W::STAGES;
+        if (!(ok = mbar_wait(&bar_full[s], (uint32_t)(k / W::STAGES) & 1u, abort_flag, l.status, 102))) break;
+        tc_fence_after();
+        const uint32_t a_h = (smem_u32(smem + s * W::STAGE) >> 4) | 1u << 16, a_l = a_h + (W::PLANE_A >> 4);
+        const uint32_t b_h = (smem_u32(smem + s * W::STAGE + 2 * W::PLANE_A) >> 4) | lbo_b, b_l = b_h + (W::PLANE_B >> 4);
+#pragma unroll
+        for (int ks = 0; ks < MU_BK / 16; ks++) {
+          const uint32_t ao = ks * 2u, bo = ks * step_b;
+          mu_mma(tmem, a_h + ao, b_h + bo, idesc, (k > 0 || ks > 0) ? 1u : 0u);
+          mu_mma(tmem, a_h + ao, b_l + bo, idesc, 1u);
+          mu_mma(tmem, a_l + ao, b_h + bo, idesc, 1u);
+        }
+        umma_commit(&bar_empty[s]);
+      }
+      if (ok) umma_commit(bar_done);
+      else *abort_flag = 1;
+    }
+  } else {
+    const int r = r0 + warp * 32 + lane;
+    bool ok = mbar_wait(bar_done, 0, abort_flag, l.status, 103);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      tc_fence_after();
+      const MuonPlanes& out = KIND == 0 ? t.gram : KIND == 1 ? t.poly : t.x2;
+      const MuonPlanes& in = KIND == 1 ? t.gram : t.x;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        const int col = c0 + c;
+        if (col >= N || (KIND != 2 && col >= r0 + MU_BM)) break;   // the same for the whole warp
+        uint32_t acc[32];
+        __syncwarp();
+        tmem_ld_32x32b_x32(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, acc);
+        tmem_ld_wait();
+        float v[32];
+        const long long at = (long long)r * out.ld + col;
+        if (KIND != 0) mu_read(in, at, r < M ? N - col : 0, v);
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int u = 0; u < 32; u += 2) {
+          __half h[2], w[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float x = __uint_as_float(acc[u + e]);
+            const float y = KIND == 0 ? x * (MU_SG / (MU_SX * MU_SX)) : KIND == 1 ? fmaf(MU_C / MU_SG, x, MU_B * v[u + e]) : fmaf(1.f / MU_SG, x, MU_A * v[u + e]);
+            mu_split(y, &h[e], &w[e]);
+          }
+          hi[u / 2] = (uint32_t)__half_as_ushort(h[0]) | (uint32_t)__half_as_ushort(h[1]) << 16;
+          lo[u / 2] = (uint32_t)__half_as_ushort(w[0]) | (uint32_t)__half_as_ushort(w[1]) << 16;
+        }
+        if (r < M) {
+#pragma unroll
+          for (int u = 0; u < 32; u += 8)
+            if (col + u < N) {                            // the pitch holds whole groups of 8
+              *reinterpret_cast<uint4*>(out.p + at + u) = make_uint4(hi[u / 2], hi[u / 2 + 1], hi[u / 2 + 2], hi[u / 2 + 3]);
+              *reinterpret_cast<uint4*>(out.p + out.plane + at + u) = make_uint4(lo[u / 2], lo[u / 2 + 1], lo[u / 2 + 2], lo[u / 2 + 3]);
+            }
+          if (KIND != 2 && col / MU_BM < r0 / MU_BM) {
+            // Mirrored: the lanes of a warp are adjacent there.
+#pragma unroll
+            for (int u = 0; u < 32; u++) {
+              if (col + u >= N) break;
+              const long long to = (long long)(col + u) * out.ld + r;
+              out.p[to] = __ushort_as_half((unsigned short)(hi[u / 2] >> (16 * (u & 1))));
+              out.p[out.plane + to] = __ushort_as_half((unsigned short)(lo[u / 2] >> (16 * (u & 1))));
+            }
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, BN);
+  }
+}
+
+// Map of planes [2][rows][cols]: boxes of 64 columns by `box_rows` rows, zeros behind the matrix.
+static bool mu_map(CUtensorMap* map, const MuonPlanes& x, int rows, int cols, int box_rows) {
+  cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, 2};
+  cuuint64_t strides[2] = {(cuuint64_t)x.ld * 2, (cuuint64_t)x.plane * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, estr[3] = {1, 1, 1};
+  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, x.p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename F>
@@ -161,6 +401,31 @@ static int64_t mu_items(MuonList& l, F items) {
   long long end = 0;
   for (int i = 0; i < l.count; i++) l.end[i] = end += items(l.t[i]);
   return end;
+}
+
+template <int KIND, int BN>
+static int32_t mu_launch(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
+  const int64_t n = mu_items(l, [](const MuonTensor& t) {
+    const int64_t rb = ceil_div(t.mm, MU_BM);
+    if (KIND == 2) return rb * ceil_div(t.nn, BN);
+    int64_t all = 0;
+    for (int64_t r = 0; r < rb; r++) all += ceil_div((r + 1) * MU_BM, BN);
+    return all;
+  });
+  OM_CUDA(ctx, cudaFuncSetAttribute(muon_product_kernel<KIND, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, MuonShape<BN>::SMEM));
+  launch_chained(ctx, muon_product_kernel<KIND, BN>, (unsigned)n, MU_THREADS, MuonShape<BN>::SMEM, l, maps);
+  return OM_OK;
+}
+// Tiles of 128 x 256 use a stage's operands for twice the products, and a product of 256 columns is the tensor pipe's full rate; tiles
+// of 128 x 128 where the wider ones would leave SMs without one.
+template <int KIND>
+static int32_t mu_product(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
+  int64_t wide = 0;
+  for (int i = 0; i < l.count; i++) {
+    const int64_t rb = ceil_div(l.t[i].mm, MU_BM), nb = ceil_div(KIND == 2 ? l.t[i].nn : l.t[i].mm, 256);
+    wide += KIND == 2 ? rb * nb : (rb * nb + rb) / 2;
+  }
+  return wide >= ctx->sm_count ? mu_launch<KIND, 256>(ctx, l, maps) : mu_launch<KIND, 128>(ctx, l, maps);
 }
 
 }  // namespace om
@@ -193,6 +458,7 @@ int32_t om_optim_muon_step(om_ctx* ctx, int32_t n_tensors, float* const* p_host,
     MuonList l = {};
     l.hyper = *hyper_host;
     l.hyper_dev = hyper_dev;
+    l.status = ctx->status_dev;
     std::vector<size_t> offset;
     size_t total = 0;
     auto room = [&](size_t n) {
@@ -206,35 +472,54 @@ int32_t om_optim_muon_step(om_ctx* ctx, int32_t n_tensors, float* const* p_host,
       t.p = p_host[at]; t.g = g_host[at]; t.m = m_host[at]; t.p16 = p16_host ? p16_host[at] : nullptr;
       t.rows = rows_host[at]; t.cols = cols_host[at];
       t.mm = std::min(t.rows, t.cols); t.nn = std::max(t.rows, t.cols);
-      const size_t mn = (size_t)t.mm * t.nn, mm = (size_t)t.mm * t.mm;
-      for (size_t n : {4 * mn, 4 * mn, 4 * mm, 4 * mm, 8 * ((mn + MU_CHUNK - 1) / MU_CHUNK)}) offset.push_back(room(n));
+      t.x.ld = t.x2.ld = (t.nn + 7) & ~7;                // 16-byte pitches: what TMA addresses
+      t.gram.ld = t.poly.ld = (t.mm + 7) & ~7;
+      t.x.plane = t.x2.plane = (long long)t.mm * t.x.ld;
+      t.gram.plane = t.poly.plane = (long long)t.mm * t.gram.ld;
+      const size_t x = 4 * (size_t)t.x.plane, g = 4 * (size_t)t.gram.plane;
+      for (size_t n : {x, x, g, g, 8 * (size_t)ceil_div((int64_t)t.mm * t.nn, MU_CHUNK)}) offset.push_back(room(n));
     }
     if (l.count == 0) break;
     char* work = nullptr;
     OM_TRY(pool_alloc(ctx, total, false, (void**)&work));
-    for (int i = 0; i < l.count; i++) {
+    MuonMaps gram, poly, apply[2];
+    bool mapped = encode_fn() != nullptr;
+    for (int i = 0; i < l.count && mapped; i++) {
       MuonTensor& t = l.t[i];
       const size_t* o = offset.data() + 5 * i;
-      t.x = (float*)(work + o[0]); t.x2 = (float*)(work + o[1]); t.gram = (float*)(work + o[2]); t.poly = (float*)(work + o[3]);
+      t.x.p = (__half*)(work + o[0]); t.x2.p = (__half*)(work + o[1]); t.gram.p = (__half*)(work + o[2]); t.poly.p = (__half*)(work + o[3]);
       t.partial = (double*)(work + o[4]);
+      mapped = mu_map(&poly.a[i], t.gram, t.mm, t.mm, MU_BM) && mu_map(&apply[0].a[i], t.poly, t.mm, t.mm, MU_BM) &&
+               mu_map(&apply[0].b[i], t.x, t.mm, t.nn, MU_BK) && mu_map(&apply[1].b[i], t.x2, t.mm, t.nn, MU_BK) &&
+               mu_map(&gram.a[i], t.x, t.mm, t.nn, MU_BM) && mu_map(&gram.b[i], t.x2, t.mm, t.nn, MU_BM);
+      if (mapped) {
+        apply[1].a[i] = apply[0].a[i];
+        poly.b[i] = poly.a[i];
+      }
     }
-    auto chunks = [](const MuonTensor& t) { return ceil_div((int64_t)t.rows * t.cols, MU_CHUNK); };
-    auto square = [](const MuonTensor& t) { return ceil_div(t.mm, MU_T) * ceil_div(t.mm, MU_T); };
-    auto wide = [](const MuonTensor& t) { return ceil_div(t.mm, MU_T) * ceil_div(t.nn, MU_T); };
-    int64_t n = mu_items(l, chunks);
-    muon_momentum_kernel<<<(unsigned)n, 256, 0, ctx->stream>>>(l);
-    muon_start_kernel<<<(unsigned)n, 256, 0, ctx->stream>>>(l);
-    for (int s = 0; s < hyper_host->steps; s++) {
-      n = mu_items(l, square);
-      muon_product_kernel<0><<<(unsigned)n, 256, 0, ctx->stream>>>(l);
-      muon_product_kernel<1><<<(unsigned)n, 256, 0, ctx->stream>>>(l);
-      n = mu_items(l, wide);
-      muon_product_kernel<2><<<(unsigned)n, 256, 0, ctx->stream>>>(l);
-      for (int i = 0; i < l.count; i++) std::swap(l.t[i].x, l.t[i].x2);
+    int32_t st = mapped ? OM_OK : fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for om_optim_muon_step");
+    if (st == OM_OK) {
+      int64_t n = mu_items(l, [](const MuonTensor& t) { return ceil_div((int64_t)t.rows * t.cols, MU_CHUNK); });
+      launch_chained(ctx, muon_momentum_kernel, (unsigned)n, 256, 0, l);
+      auto blocks = [](const MuonTensor& t) { return ceil_div(t.rows, 64) * ceil_div(t.cols, 64); };
+      n = mu_items(l, blocks);
+      launch_chained(ctx, muon_start_kernel, (unsigned)n, 256, 0, l);
+      for (int s = 0; s < hyper_host->steps && st == OM_OK; s++) {
+        st = mu_product<0>(ctx, l, gram);
+        if (st == OM_OK) st = mu_product<1>(ctx, l, poly);
+        if (st == OM_OK) st = mu_product<2>(ctx, l, apply[s & 1]);
+        for (int i = 0; i < l.count; i++) {
+          std::swap(l.t[i].x, l.t[i].x2);
+          std::swap(gram.a[i], gram.b[i]);
+        }
+      }
+      if (st == OM_OK) {
+        n = mu_items(l, blocks);
+        launch_chained(ctx, muon_finish_kernel, (unsigned)n, 256, 0, l);
+      }
     }
-    n = mu_items(l, chunks);
-    muon_finish_kernel<<<(unsigned)n, 256, 0, ctx->stream>>>(l);
     pool_free(ctx, work);
+    OM_TRY(st);
     OM_LAUNCH_CHECK(ctx, "om_optim_muon_step");
   }
   return OM_OK;
