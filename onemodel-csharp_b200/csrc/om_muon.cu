@@ -9,7 +9,9 @@
 // The products run on the tensor pipe with fp32 accuracy: a value v is kept as two half-precision numbers, h = half(v) and
 // l = half(v - h), 22 significant bits together, and a product is h h' + h l' + l h' (what is left out is 2^-22 of it). Five steps
 // raise an error in the direction of a small singular value up to 3.4445^5 = 485 times, which is why plain half or bfloat16
-// operands (2^-11, 2^-8) would leave few digits of the update. Every matrix of a step is bounded (|X| <= 1.2, |G| <= 1.5, |Y| <= 3 in the
+// operands (2^-11, 2^-8) would leave few digits of the update. The tensor core cuts each sum it adds to off, an error that grows with the
+// number of additions: h h' has an accumulator of its own and the two small products another, a third of the additions
+// (4096 terms: the weights' error against 64 bits 8.7e-7 in one accumulator, 7.1e-7 in two, at the same speed). Every matrix of a step is bounded (|X| <= 1.2, |G| <= 1.5, |Y| <= 3 in the
 // spectral norm, so element by element), and is stored times a power of two that puts its usual elements in the middle of the
 // half's range. Three products at the 16-bit rate bound it: 3/1664 s a TFLOP; two planes of 2 bytes are what fp32 would read.
 #include <cuda_bf16.h>
@@ -27,7 +29,8 @@ constexpr float MU_A = 3.4445f, MU_B = -4.7750f, MU_C = 2.0315f;   // the quinti
 constexpr int MU_CHUNK = 8192;                                     // elements of one partial sum of squares
 constexpr int MU_BM = 128, MU_BK = 64;                             // rows of a tile of a product, terms of a stage
 constexpr float MU_SX = 1024.f, MU_SG = 4096.f;                    // X is stored times the first, G and Y times the second
-constexpr int MU_THREADS = 192;                                    // warps 0-3: results; warp 4: MMA issue; warp 5: TMA
+constexpr int MU_EPI = 8;                                          // warps 0-7: results, half of a tile's columns each four; warp 8: MMA issue; warp 9: TMA
+constexpr int MU_THREADS = 32 * (MU_EPI + 2);
 
 // A matrix as two planes of halves, the second `plane` elements behind the first, rows `ld` apart.
 struct MuonPlanes {
@@ -41,6 +44,7 @@ struct MuonTensor {
   uint16_t* p16;
   int rows, cols;        // as the caller has them
   int mm, nn;            // sides of X, mm <= nn
+  int quads;             // rows of p, m and g start where four elements move at once
   double* partial;       // [ceil(rows * cols / MU_CHUNK)]
   MuonPlanes x, x2, gram, poly;   // [mm, nn], [mm, nn], [mm, mm], [mm, mm]
 };
@@ -73,11 +77,23 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constan
   const om_muon_hyper h = mu_hyper(l);
   const long long n = (long long)t.rows * t.cols, e0 = chunk * MU_CHUNK, e1 = min(e0 + MU_CHUNK, n);
   double sum = 0.0;
-  for (long long e = e0 + threadIdx.x; e < e1; e += 256) {
-    const float g = t.g[e] * h.grad_scale * (1.f - h.momentum), m = fmaf(t.m[e], h.momentum, g);
-    t.m[e] = m;
+  auto one = [&](float g, float& m) {
+    g = g * h.grad_scale * (1.f - h.momentum);
+    m = fmaf(m, h.momentum, g);
     const float u = h.nesterov ? fmaf(m, h.momentum, g) : m;
-    sum += (double)u * u;
+    return u * u;
+  };
+  if (t.quads) {
+#pragma unroll 4
+    for (long long e = e0 + 4 * threadIdx.x; e < e1; e += 1024) {
+      const float4 g = *reinterpret_cast<const float4*>(t.g + e);
+      float4 m = *reinterpret_cast<float4*>(t.m + e);
+      const float a = one(g.x, m.x), b = one(g.y, m.y), c = one(g.z, m.z), d = one(g.w, m.w);
+      *reinterpret_cast<float4*>(t.m + e) = m;
+      sum += ((double)a + b) + ((double)c + d);
+    }
+  } else {
+    for (long long e = e0 + threadIdx.x; e < e1; e += 256) sum += one(t.g[e], t.m[e]);
   }
   __shared__ double s[8];
 #pragma unroll
@@ -123,25 +139,42 @@ __global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__
   int r0, c0;
   mu_block(t, tile, &r0, &c0);
   const bool turn = t.rows > t.cols;
+  auto one = [&](float m, float g) { return (h.nesterov ? fmaf(m, h.momentum, g * h.grad_scale * (1.f - h.momentum)) : m) / norm * MU_SX; };
+  if (t.quads) {
+#pragma unroll
+    for (int e = threadIdx.x; e < 64 * 16; e += 256) {
+      const int a = e / 16, b = e % 16 * 4;
+      if (r0 + a >= t.rows || c0 + b >= t.cols) continue;
+      const long long at = (long long)(r0 + a) * t.cols + c0 + b;
+      const float4 m = *reinterpret_cast<const float4*>(t.m + at), g = h.nesterov ? *reinterpret_cast<const float4*>(t.g + at) : m;
+      block[a][b] = one(m.x, g.x);
+      block[a][b + 1] = one(m.y, g.y);
+      block[a][b + 2] = one(m.z, g.z);
+      block[a][b + 3] = one(m.w, g.w);
+    }
+  } else {
 #pragma unroll 4
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    const int r = r0 + e / 64, c = c0 + e % 64;
-    if (r >= t.rows || c >= t.cols) continue;
-    const long long at = (long long)r * t.cols + c;
-    const float m = t.m[at], u = h.nesterov ? fmaf(m, h.momentum, t.g[at] * h.grad_scale * (1.f - h.momentum)) : m;
-    block[e / 64][e % 64] = u / norm * MU_SX;
+    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+      const int r = r0 + e / 64, c = c0 + e % 64;
+      if (r >= t.rows || c >= t.cols) continue;
+      const long long at = (long long)r * t.cols + c;
+      block[e / 64][e % 64] = one(t.m[at], t.g[at]);
+    }
   }
   __syncthreads();
-#pragma unroll 4
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    const int a = e / 64, b = e % 64;                     // row and column of this tile of X
+  // Eight values of a row of X at a time: the pitch holds whole groups of 8.
+#pragma unroll
+  for (int e = threadIdx.x; e < 64 * 8; e += 256) {
+    const int a = e / 8, b = e % 8 * 8;
     const int xr = (turn ? c0 : r0) + a, xc = (turn ? r0 : c0) + b;
     if (xr >= t.mm || xc >= t.nn) continue;
-    __half hi, lo;
-    mu_split(turn ? block[b][a] : block[a][b], &hi, &lo);
+    uint4 hi, lo;
+    __half *hp = reinterpret_cast<__half*>(&hi), *lp = reinterpret_cast<__half*>(&lo);
+#pragma unroll
+    for (int u = 0; u < 8; u++) mu_split(xc + u < t.nn ? (turn ? block[b + u][a] : block[a][b + u]) : 0.f, hp + u, lp + u);
     const long long at = (long long)xr * t.x.ld + xc;
-    t.x.p[at] = hi;
-    t.x.p[t.x.plane + at] = lo;
+    *reinterpret_cast<uint4*>(t.x.p + at) = hi;
+    *reinterpret_cast<uint4*>(t.x.p + t.x.plane + at) = lo;
   }
 }
 
@@ -157,27 +190,48 @@ __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant_
   int r0, c0;
   mu_block(t, tile, &r0, &c0);
   const bool turn = t.rows > t.cols;
-#pragma unroll 4
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    const int a = e / 64, b = e % 64;
+#pragma unroll
+  for (int e = threadIdx.x; e < 64 * 8; e += 256) {
+    const int a = e / 8, b = e % 8 * 8;
     const int xr = (turn ? c0 : r0) + a, xc = (turn ? r0 : c0) + b;
     if (xr >= t.mm || xc >= t.nn) continue;
     const long long at = (long long)xr * t.x.ld + xc;
-    const float v = (__half2float(t.x.p[at]) + __half2float(t.x.p[t.x.plane + at])) * (1.f / MU_SX);
-    if (turn) block[b][a] = v;
-    else block[a][b] = v;
+    const uint4 hi = *reinterpret_cast<const uint4*>(t.x.p + at), lo = *reinterpret_cast<const uint4*>(t.x.p + t.x.plane + at);
+    const __half *hp = reinterpret_cast<const __half*>(&hi), *lp = reinterpret_cast<const __half*>(&lo);
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const float v = (__half2float(hp[u]) + __half2float(lp[u])) * (1.f / MU_SX);
+      if (turn) block[b + u][a] = v;
+      else block[a][b + u] = v;
+    }
   }
   __syncthreads();
+  auto half16 = [](float v) {
+    const __nv_bfloat16 b = __float2bfloat16_rn(v);
+    return *reinterpret_cast<const uint16_t*>(&b);
+  };
+  if (t.quads) {
+#pragma unroll
+    for (int e = threadIdx.x; e < 64 * 16; e += 256) {
+      const int a = e / 16, b = e % 16 * 4;
+      if (r0 + a >= t.rows || c0 + b >= t.cols) continue;
+      const long long at = (long long)(r0 + a) * t.cols + c0 + b;
+      float4 p = *reinterpret_cast<float4*>(t.p + at);
+      p = make_float4(fmaf(-rate, block[a][b], p.x * keep), fmaf(-rate, block[a][b + 1], p.y * keep), fmaf(-rate, block[a][b + 2], p.z * keep),
+                      fmaf(-rate, block[a][b + 3], p.w * keep));
+      *reinterpret_cast<float4*>(t.p + at) = p;
+      if (t.p16)
+        *reinterpret_cast<uint2*>(t.p16 + at) = make_uint2((uint32_t)half16(p.x) | (uint32_t)half16(p.y) << 16, (uint32_t)half16(p.z) | (uint32_t)half16(p.w) << 16);
+    }
+  } else {
 #pragma unroll 4
-  for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-    const int r = r0 + e / 64, c = c0 + e % 64;
-    if (r >= t.rows || c >= t.cols) continue;
-    const long long at = (long long)r * t.cols + c;
-    const float p = fmaf(-rate, block[e / 64][e % 64], t.p[at] * keep);
-    t.p[at] = p;
-    if (t.p16) {
-      const __nv_bfloat16 v = __float2bfloat16_rn(p);
-      t.p16[at] = *reinterpret_cast<const uint16_t*>(&v);
+    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
+      const int r = r0 + e / 64, c = c0 + e % 64;
+      if (r >= t.rows || c >= t.cols) continue;
+      const long long at = (long long)r * t.cols + c;
+      const float p = fmaf(-rate, block[e / 64][e % 64], t.p[at] * keep);
+      t.p[at] = p;
+      if (t.p16) t.p16[at] = half16(p);
     }
   }
 }
@@ -200,23 +254,23 @@ __device__ __forceinline__ void mu_load(void* dst, const CUtensorMap* map, int c
                "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
                : "memory");
 }
-// 32 values of a row of planes (from a column that is a multiple of 8; the pitch is one too, so whole groups of 8 lie within it).
-__device__ __forceinline__ void mu_read(const MuonPlanes& x, long long at, int valid, float (&v)[32]) {
+// 32 values of a row of planes, as they lie (from a column that is a multiple of 8; the pitch is one too, so whole groups of 8 lie within
+// it), and their sums.
+struct MuonRow {
+  uint4 h[4], l[4];
+};
+__device__ __forceinline__ void mu_fetch(const MuonPlanes& x, long long at, int valid, MuonRow& v) {
 #pragma unroll
-  for (int c = 0; c < 32; c += 8) {
-    uint4 h = make_uint4(0, 0, 0, 0), l = h;
-    if (c < valid) {
-      h = *reinterpret_cast<const uint4*>(x.p + at + c);
-      l = *reinterpret_cast<const uint4*>(x.p + x.plane + at + c);
-    }
-    const __half2 *hp = reinterpret_cast<const __half2*>(&h), *lp = reinterpret_cast<const __half2*>(&l);
-#pragma unroll
-    for (int u = 0; u < 4; u++) {
-      const float2 a = __half22float2(hp[u]), b = __half22float2(lp[u]);
-      v[c + 2 * u] = a.x + b.x;
-      v[c + 2 * u + 1] = a.y + b.y;
+  for (int c = 0; c < 4; c++) {
+    v.h[c] = v.l[c] = make_uint4(0, 0, 0, 0);
+    if (8 * c < valid) {
+      v.h[c] = *reinterpret_cast<const uint4*>(x.p + at + 8 * c);
+      v.l[c] = *reinterpret_cast<const uint4*>(x.p + x.plane + at + 8 * c);
     }
   }
+}
+__device__ __forceinline__ float mu_value(const MuonRow& v, int u) {
+  return __half2float(reinterpret_cast<const __half*>(v.h)[u]) + __half2float(reinterpret_cast<const __half*>(v.l)[u]);
 }
 
 template <int BN>
@@ -247,8 +301,8 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 4) {
-    tmem_alloc(tmem_slot, BN);
+  if (warp == MU_EPI) {
+    tmem_alloc(tmem_slot, 2 * BN);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -279,7 +333,7 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
   }
   const int steps = (K + MU_BK - 1) / MU_BK;
 
-  if (warp == 5) {
+  if (warp == MU_EPI + 1) {
     if (lane == 0) {
       bool ok = true;
       for (int k = 0; ok && k < steps; k++) {
@@ -302,7 +356,7 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
         }
       }
     }
-  } else if (warp == 4) {
+  } else if (warp == MU_EPI) {
     if (lane == 0) {
       // Half-precision operands, fp32 sums; B is K-major (rows of the same matrix) or MN-major (X as it lies).
       constexpr uint32_t idesc = (1u << 4) | ((KIND == 2 ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(MU_BM >> 4) << 24);
@@ -317,9 +371,10 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
 #pragma unroll
         for (int ks = 0; ks < MU_BK / 16; ks++) {
           const uint32_t ao = ks * 2u, bo = ks * step_b;
-          mu_mma(tmem, a_h + ao, b_h + bo, idesc, (k > 0 || ks > 0) ? 1u : 0u);
-          mu_mma(tmem, a_h + ao, b_l + bo, idesc, 1u);
-          mu_mma(tmem, a_l + ao, b_h + bo, idesc, 1u);
+          const uint32_t more = (k > 0 || ks > 0) ? 1u : 0u;
+          mu_mma(tmem, a_h + ao, b_h + bo, idesc, more);
+          mu_mma(tmem + BN, a_h + ao, b_l + bo, idesc, more);
+          mu_mma(tmem + BN, a_l + ao, b_h + bo, idesc, 1u);
         }
         umma_commit(&bar_empty[s]);
       }
@@ -327,32 +382,41 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
       else *abort_flag = 1;
     }
   } else {
-    const int r = r0 + warp * 32 + lane;
-    bool ok = mbar_wait(bar_done, 0, abort_flag, l.status, 103);
+    const int r = r0 + (warp & 3) * 32 + lane, first = (warp >> 2) * (BN / 2);
+    const uint32_t t_acc = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const MuonPlanes& out = KIND == 0 ? t.gram : KIND == 1 ? t.poly : t.x2;
+    const MuonPlanes& in = KIND == 1 ? t.gram : t.x;
+    // What the result adds to is fetched a block of 32 columns ahead, the first one under the products.
+    MuonRow next;
+    if (KIND != 0) mu_fetch(in, (long long)r * in.ld + c0 + first, r < M ? N - (c0 + first) : 0, next);
+    bool ok = true;
+    if (lane == 0) ok = mbar_wait(bar_done, 0, abort_flag, l.status, 103);
     ok = __all_sync(0xffffffffu, ok);
     if (ok) {
       tc_fence_after();
-      const MuonPlanes& out = KIND == 0 ? t.gram : KIND == 1 ? t.poly : t.x2;
-      const MuonPlanes& in = KIND == 1 ? t.gram : t.x;
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
+      for (int c = first; c < first + BN / 2; c += 32) {
         const int col = c0 + c;
         if (col >= N || (KIND != 2 && col >= r0 + MU_BM)) break;   // the same for the whole warp
-        uint32_t acc[32];
+        uint32_t acc[32], small[32];
         __syncwarp();
-        tmem_ld_32x32b_x32(tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)c, acc);
+        tmem_ld_32x32b_x32(t_acc + (uint32_t)c, acc);
+        tmem_ld_32x32b_x32(t_acc + (uint32_t)(BN + c), small);
         tmem_ld_wait();
-        float v[32];
         const long long at = (long long)r * out.ld + col;
-        if (KIND != 0) mu_read(in, at, r < M ? N - col : 0, v);
+        MuonRow v;
+        if (KIND != 0) {
+          v = next;
+          if (c + 32 < first + BN / 2) mu_fetch(in, at + 32, r < M ? N - (col + 32) : 0, next);
+        }
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int u = 0; u < 32; u += 2) {
           __half h[2], w[2];
 #pragma unroll
           for (int e = 0; e < 2; e++) {
-            const float x = __uint_as_float(acc[u + e]);
-            const float y = KIND == 0 ? x * (MU_SG / (MU_SX * MU_SX)) : KIND == 1 ? fmaf(MU_C / MU_SG, x, MU_B * v[u + e]) : fmaf(1.f / MU_SG, x, MU_A * v[u + e]);
+            const float x = __uint_as_float(acc[u + e]) + __uint_as_float(small[u + e]);
+            const float y = KIND == 0 ? x * (MU_SG / (MU_SX * MU_SX)) : KIND == 1 ? fmaf(MU_C / MU_SG, x, MU_B * mu_value(v, u + e)) : fmaf(1.f / MU_SG, x, MU_A * mu_value(v, u + e));
             mu_split(y, &h[e], &w[e]);
           }
           hi[u / 2] = (uint32_t)__half_as_ushort(h[0]) | (uint32_t)__half_as_ushort(h[1]) << 16;
@@ -381,9 +445,9 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == MU_EPI) {
     tc_fence_after();
-    tmem_dealloc(tmem, BN);
+    tmem_dealloc(tmem, 2 * BN);
   }
 }
 
@@ -472,6 +536,8 @@ int32_t om_optim_muon_step(om_ctx* ctx, int32_t n_tensors, float* const* p_host,
       t.p = p_host[at]; t.g = g_host[at]; t.m = m_host[at]; t.p16 = p16_host ? p16_host[at] : nullptr;
       t.rows = rows_host[at]; t.cols = cols_host[at];
       t.mm = std::min(t.rows, t.cols); t.nn = std::max(t.rows, t.cols);
+      t.quads = t.cols % 4 == 0 && ((reinterpret_cast<uintptr_t>(t.p) | reinterpret_cast<uintptr_t>(t.g) | reinterpret_cast<uintptr_t>(t.m)) & 15) == 0 &&
+                (reinterpret_cast<uintptr_t>(t.p16) & 7) == 0;
       t.x.ld = t.x2.ld = (t.nn + 7) & ~7;                // 16-byte pitches: what TMA addresses
       t.gram.ld = t.poly.ld = (t.mm + 7) & ~7;
       t.x.plane = t.x2.plane = (long long)t.mm * t.x.ld;
