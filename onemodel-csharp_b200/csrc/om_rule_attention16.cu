@@ -1,12 +1,14 @@
 // Attention by rule with bfloat16 operands on the tensor pipe (tcgen05), forward and backward, for head dimensions up to 128.
 //
-// Forward: a CTA holds 256 queries as two tiles of 128 and walks the keys that the rule lets them see, 64 at a time. Eight warps per
-// query tile keep the running maximum and sum of its rows, two threads a row. Scores S = Q K^T come to tensor memory in fp32; the rows
-// take them to registers, which frees their place for the next scores at once, and put the weights exp2(S - m), rounded to bfloat16,
-// into one of two places beside them, from where O += P V reads them. So the tensor pipe works on the next scores of both tiles and on
-// the products behind while the rows form exponentials, and every reuse of a place in tensor memory has a barrier of its own. O stays
-// in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 over the one in use, which changes no result:
-// numerator and denominator share the factor.
+// Forward: a CTA holds 256 queries as two tiles of 128 and walks the tiles of 128 keys that the rule lets them see. Four warps per query
+// tile keep the running maximum and sum of a row per thread; while one tile's rows turn scores into weights the tensor pipe works on
+// the other's: S = Q K^T in fp32 in tensor memory -> weights exp2(S - m), rounded to bfloat16, in tensor memory -> O += P V with P read
+// from there. Up to a head dimension of 64 the weights have a place of their own, so the next scores come while the rows are still at
+// these; with 128 columns of O they lie over the scores they came from, and the next scores wait for the product that reads them.
+// O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 over the one in use, which changes no
+// result: numerator and denominator share the factor. Rows go through their scores twice, 32 at a time (128 in registers would spill,
+// and what spills does not fit the L1 that the operands leave). Steps of 64 keys, with everything in places of its own, were measured
+// too and slower at 128 columns: a product of 128 x 64 takes the tensor pipe as long as one of 128 x 128.
 // With few rows the walk over the keys is split over CTAs that leave their sums, maxima and O for rule16_join_kernel, and the query
 // heads that share a key head become rows of one tile, so that keys and values are read once.
 //
@@ -14,8 +16,7 @@
 // all heads that share them; rows are keys: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q) and once in rule16_dq_kernel (a
 // CTA per 128 queries walks the keys: dQ += dS K). Seven products for five, but no partial sums through memory: a part of dQ per
 // (query tile, key tile) is 128 KB of traffic against 0.3 us of tensor time for the two products that are done again.
-// Two sets of eight warps of rows take turns, so that a set has two steps' time for one. P and dS are rounded to bfloat16 as operands
-// (the only roundings of the backward besides the results').
+// P and dS are rounded to bfloat16 as operands (the only roundings of the backward besides the results').
 //
 // What a CTA sees of the other axis is worked out before its walk, a byte per 128 indices: worked out along the way it cost the rows as
 // much as their exponentials. Every wait is bounded (om_tc.cuh). All sums are fp32 in an order that the shapes alone decide.
@@ -29,8 +30,8 @@ namespace om {
 
 constexpr int R16_T = 128;                         // rows of every tile
 constexpr int R16_CHUNK = R16_T * 128;             // bytes of a [128 x 64] bfloat16 block, 128-byte swizzled rows
-constexpr int R16_ROW_WARPS = 16;
-constexpr int R16_THREADS = 32 * (R16_ROW_WARPS + 2);   // warps 0-15: rows; warp 16: MMA issue; warp 17: TMA
+constexpr int R16_ROW_WARPS = 8;
+constexpr int R16_THREADS = 32 * (R16_ROW_WARPS + 2);   // warps 0-7: rows; warp 8: MMA issue; warp 9: TMA
 constexpr int R16_PLAN = 1024;                     // tiles of the other axis that a CTA walks at most
 constexpr float R16_LOG2E = 1.4426950408889634f, R16_LN2 = 0.6931471805599453f;
 
@@ -45,8 +46,6 @@ __device__ __forceinline__ float r16_rcp(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh(x) = 1 - 2 / (exp(2 x) + 1): off by 2^-22 at most, absolutely, which a cap times it carries into a score.
-__device__ __forceinline__ float r16_tanh(float x) { return fmaf(-2.f, r16_rcp(r16_ex2(x * (2.f * R16_LOG2E)) + 1.f), 1.f); }
 __device__ __forceinline__ uint32_t r16_pack(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -101,23 +100,25 @@ __device__ __forceinline__ void r16_st16(uint32_t taddr, const uint32_t (&r)[16]
 }
 __device__ __forceinline__ void r16_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// D[128 x 64] = A B^T over the head's columns, both operands K-major in shared memory; b_k: 64 rows of B.
+// D[128 x 128] = A B^T over the head's columns, both operands K-major in shared memory.
 template <int DP>
 __device__ __forceinline__ void r16_scores(uint32_t d, uint32_t a_k, uint32_t b_k) {
-  constexpr uint32_t idesc = r16_idesc(false, 64);
+  constexpr uint32_t idesc = r16_idesc(false, R16_T);
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ks++) {
     const uint32_t o = (uint32_t)(ks / 4) * (R16_CHUNK >> 4) + (uint32_t)(ks % 4) * 2;
     r16_mma_ss(d, a_k + o, b_k + o, idesc, ks > 0 ? 1u : 0u);
   }
 }
-constexpr uint32_t R16_HALF_K = (64u * 128u) >> 4, R16_HALF_MN = (64u * 128u) >> 4;   // the second 64 rows of a tile
-// D[128 x DP] (+)= A B over 64 rows of B: A [128 x 64] packed in 32 columns of tensor memory, B MN-major in shared memory.
-template <int DP>
+// D[128 x DP] (+)= A B over the 128 rows of B: A in tensor memory, B MN-major in shared memory. Where A lies over what it came from, a
+// row thread packs the results of its COLS columns over the first half of them: elements COLS t ... of the contraction are at COLS t.
+template <int DP, int COLS>
 __device__ __forceinline__ void r16_gather(uint32_t d, uint32_t a, uint32_t b_mn, uint32_t accumulate) {
   constexpr uint32_t idesc = r16_idesc(true, DP);
+  constexpr int STEPS = COLS / 16;
 #pragma unroll
-  for (int ks = 0; ks < 4; ks++) r16_mma_ts(d, a + (uint32_t)ks * 8u, b_mn + (uint32_t)ks * 128u, idesc, ks > 0 ? 1u : accumulate);
+  for (int ks = 0; ks < R16_T / 16; ks++)
+    r16_mma_ts(d, a + (uint32_t)((ks / STEPS) * COLS + (ks % STEPS) * 8), b_mn + (uint32_t)ks * 128u, idesc, ks > 0 ? 1u : accumulate);
 }
 template <int DP>
 __device__ __forceinline__ void r16_load_tile(uint8_t* dst, const CUtensorMap* map, int row0, int head, int batch, uint64_t* bar) {
@@ -188,17 +189,31 @@ __device__ __forceinline__ float r16_max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
   return v;
 }
-// The score in powers of two of a product, and the cap's derivative.
-__device__ __forceinline__ float r16_score(const RuleArgs& r, float slope, int far, float dot, float* dcap) {
-  float s = dot * r.scale;
-  if (r.softcap > 0.f) {
-    const float t = r16_tanh(s * r.inv_softcap);
+// What is done to a product in front of the softmax: 0 scaled, 1 and lowered with the distance, 2 capped (and lowered). Scores are in powers
+// of two: scale, cap and slope come times log2 e. `far`: the signed distance of the first index of a run, as a float (a conversion for
+// every score would take the unit that the exponentials need).
+struct R16Score {
+  float scale, turns, cap, slope;                        // turns: of the tanh's argument, 2 log2 e scale / cap
+};
+template <int MODE>
+__device__ __forceinline__ R16Score r16_score_of(const RuleArgs& r, int head) {
+  R16Score c;
+  c.scale = r.scale * R16_LOG2E;
+  c.turns = 2.f * R16_LOG2E * r.scale * r.inv_softcap;
+  c.cap = r.softcap * R16_LOG2E;
+  c.slope = MODE > 0 && r.slopes ? r.slopes[head] * R16_LOG2E : 0.f;
+  return c;
+}
+template <int MODE>
+__device__ __forceinline__ float r16_score(const R16Score& c, float far, float dot, float* dcap) {
+  float s = dot * c.scale;
+  if (MODE == 2) {
+    // tanh(x) = 1 - 2 / (exp(2 x) + 1): off by 2^-22 at most, absolutely, which the cap times it carries into a score.
+    const float t = fmaf(-2.f, r16_rcp(r16_ex2(dot * c.turns) + 1.f), 1.f);
     *dcap = fmaf(-t, t, 1.f);
-    s = r.softcap * t;
-  } else {
-    *dcap = 1.f;
+    s = c.cap * t;
   }
-  return fmaf(-slope, (float)abs(far), s) * R16_LOG2E;
+  return fmaf(-c.slope, fabsf(far), s);
 }
 
 // A row of N fp32 values to fp32 and bfloat16 results, both 16 bytes at a time; columns behind d stay unwritten (d is a multiple of 8).
@@ -252,27 +267,18 @@ struct R16Fwd {
   int32_t* status;
 };
 
-// A CTA's plan: the steps of its walk in order, a step being 64 indices of the other axis that some row tile sees anything of.
-constexpr uint32_t R16_OPENS = 1u << 12, R16_CLOSES = 1u << 13;      // the first, the last step of its tile of 128
-__device__ __forceinline__ int r16_tile_of(uint32_t step) { return (int)(step & 1023u); }
-__device__ __forceinline__ uint32_t r16_half_of(uint32_t step) { return (step >> 10) & 1u; }
-__device__ __forceinline__ int r16_sees_of(uint32_t step, int tile) { return (int)(step >> (16 + 2 * tile)) & 3; }
-// By one warp: `see(tile, half)` gives rule_see's answers, two bits a row tile. Returns the number of steps.
+// A CTA's plan: the tiles of 128 of the other axis that some row tile sees anything of, in order, with rule_see's answer for each row
+// tile (two bits, from bit 10 on). Made by one warp; returns their number.
+__device__ __forceinline__ int r16_tile_of(uint32_t step) { return (int)(step & (R16_PLAN - 1)); }
+__device__ __forceinline__ int r16_sees_of(uint32_t step, int tile) { return (int)(step >> (10 + 2 * tile)) & 3; }
 template <typename F>
-__device__ __forceinline__ int r16_plan(uint32_t* steps, int tiles, int lane, F see) {
+__device__ __forceinline__ int r16_plan(uint16_t* steps, int tiles, int lane, F see) {
   int n = 0;
   for (int t0 = 0; t0 < tiles; t0 += 32) {
     const int t = t0 + lane;
-    uint32_t a = 0, b = 0;
-    if (t < tiles) {
-      a = see(t, 0);
-      b = see(t, 1);
-    }
-    const uint32_t first = __ballot_sync(0xffffffffu, a != 0), second = __ballot_sync(0xffffffffu, b != 0), below = (1u << lane) - 1u;
-    int at = n + __popc(first & below) + __popc(second & below);
-    if (a) steps[at++] = (uint32_t)t | R16_OPENS | (b ? 0u : R16_CLOSES) | a << 16;
-    if (b) steps[at] = (uint32_t)t | 1u << 10 | (a ? 0u : R16_OPENS) | R16_CLOSES | b << 16;
-    n += __popc(first) + __popc(second);
+    const uint32_t a = t < tiles ? see(t) : 0u, some = __ballot_sync(0xffffffffu, a != 0);
+    if (a) steps[n + __popc(some & ((1u << lane) - 1u))] = (uint16_t)((uint32_t)t | a << 10);
+    n += __popc(some);
   }
   return n;
 }
@@ -281,28 +287,26 @@ template <int DP>
 struct R16FwdShape {
   static constexpr int TILE = DP / 64 * R16_CHUNK;
   static constexpr int STAGES = DP == 128 ? 4 : 8;       // of K and V tiles in turn
-  static constexpr int MAXIMA = (2 + STAGES) * TILE;     // [parity][query tile][half][128] floats, and the halves' sums in the end
-  static constexpr int RULES = MAXIMA + 4096;
+  static constexpr bool APART = DP == 64;                // the weights have columns of their own
+  static constexpr int RULES = (2 + STAGES) * TILE;
   static constexpr int PLAN = RULES + 128;
-  static constexpr int BARS = PLAN + 2 * R16_PLAN * 4 + 16;
-  static constexpr int SMEM = BARS + 512 + 1024;
+  static constexpr int BARS = PLAN + R16_PLAN * 2 + 16;
+  static constexpr int SMEM = BARS + 512;
 };
 
-template <int DP, bool EXTRA>
+template <int DP, int MODE>
 __global__ void __launch_bounds__(R16_THREADS, 1)
 rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const __grid_constant__ R16Fwd p) {
   typedef R16FwdShape<DP> W;
-  // Of query tile g at 64 g: the scores; at 128 + 64 g: the two places of its weights, 32 columns each; at 256 + 128 g: O.
-  constexpr uint32_t COL_S = 0, COL_P = 128, COL_O = 256;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  // Scores of query tile g at 128 g, weights at 128 g too or at 256 + 64 g, O behind.
+  constexpr uint32_t COL_S = 0, COL_P = W::APART ? 256 : 0, P_STEP = W::APART ? 64 : 128, COL_O = W::APART ? 384 : 256, O_STEP = W::APART ? 64 : 128;
+  extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *slot_q = smem, *ring = smem + 2 * W::TILE;
-  uint32_t* steps = reinterpret_cast<uint32_t*>(smem + W::PLAN);
-  float* maxima = reinterpret_cast<float*>(smem + W::MAXIMA);
+  uint16_t* steps = reinterpret_cast<uint16_t*>(smem + W::PLAN);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
-  uint64_t *bar_q = bars, *bar_s = bars + 1 /* [tile] */, *bar_read = bars + 3 /* [tile] */, *bar_p = bars + 5 /* [tile][place] */, *bar_o = bars + 9 /* [tile][place] */,
-           *bar_max = bars + 13 /* [tile][quad] */, *bar_full = bars + 21 /* [STAGES] */, *bar_empty = bar_full + W::STAGES;
+  uint64_t *bar_q = bars, *bar_s = bars + 1 /* [tile] */, *bar_read = bars + 3 /* [tile] */, *bar_p = bars + 5 /* [tile] */, *bar_o = bars + 7 /* [tile] */,
+           *bar_full = bars + 9 /* [STAGES] */, *bar_empty = bar_full + W::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_empty + W::STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const RuleArgs& r = p.r;
@@ -328,12 +332,9 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     for (int a = 0; a < 2; a++) {
       mbar_init(&bar_s[a], 1);
       mbar_init(&bar_read[a], R16_ROW_WARPS / 2);
-    }
-    for (int a = 0; a < 4; a++) {
       mbar_init(&bar_p[a], R16_ROW_WARPS / 2);
       mbar_init(&bar_o[a], 1);
     }
-    for (int a = 0; a < 8; a++) mbar_init(&bar_max[a], 2);
     for (int a = 0; a < W::STAGES; a++) {
       mbar_init(&bar_full[a], 1);
       mbar_init(&bar_empty[a], 1);
@@ -362,18 +363,14 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   last = min(first + per, last);
   __syncthreads();
   if (warp == 0) {
-    const int n = r16_plan(steps, last - first, lane, [&](int t, int e) {
-      const int at = (first + t) * R16_T + e * 64;
-      return (uint32_t)(rule_see<true>(tiles[0], at, 1) | rule_see<true>(tiles[1], at, 1) << 2);
+    const int n = r16_plan(steps, last - first, lane, [&](int t) {
+      return (uint32_t)(rule_see<true>(tiles[0], (first + t) * R16_T, 2) | rule_see<true>(tiles[1], (first + t) * R16_T, 2) << 2);
     });
-    if (lane == 0) steps[2 * R16_PLAN] = (uint32_t)n;
+    if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
-  const int walk = (int)steps[2 * R16_PLAN];
+  const int walk = (int)steps[R16_PLAN];
 
-  const int g = (warp >> 3) & 1, half = (warp >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
-  float m = -INFINITY, l = 0.f;
-  uint32_t count = 0;
   bool ok = true;
   if (warp == R16_ROW_WARPS + 1) {
     if (lane == 0) {
@@ -390,7 +387,6 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       bool again = false;
       for (int n = 0; ok && n < walk; n++) {
         const uint32_t step = steps[n];
-        if (!(step & R16_OPENS)) continue;
         for (int kv = 0; kv < 2 && ok; kv++) {
           if (again) ok = r16_bar(&bar_empty[s], phase ^ 1u, abort_flag, p.status, 61);
           if (!ok) break;
@@ -407,7 +403,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   } else if (warp == R16_ROW_WARPS) {
     if (lane == 0) {
       ok = r16_bar(bar_q, 0, abort_flag, p.status, 62);
-      int s = 0, ks = 0, vs = 0;                          // the ring's next tile, and those of the steps at hand
+      int s = 0;                                          // the ring's next tile
       uint32_t phase = 0, scored[2] = {0, 0}, summed[2] = {0, 0};
       auto take = [&]() {
         const int at = s;
@@ -418,106 +414,125 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         return at;
       };
-      // The scores of a step for every query tile that sees something of it.
-      auto scores = [&](uint32_t step) {
-        if (step & R16_OPENS) ks = take();
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          if (!ok || !r16_sees_of(step, t)) continue;
-          // The rows have taken the scores before to registers.
-          if (scored[t] > 0) ok = r16_bar(&bar_read[t], (scored[t] - 1) & 1u, abort_flag, p.status, 64);
-          if (!ok) break;
-          tc_fence_after();
-          r16_scores<DP>(tmem + COL_S + 64u * t, r16_desc_k(slot_q + t * W::TILE), r16_desc_k(ring + ks * W::TILE) + r16_half_of(step) * R16_HALF_K);
-          umma_commit(&bar_s[t]);
-          scored[t]++;
+      auto scores = [&](const int t, int ks) {
+        if (scored[t] > 0) {
+          // APART: the rows have taken the scores before. Else the product that reads the weights over them is complete.
+          ok = W::APART ? r16_bar(&bar_read[t], (scored[t] - 1) & 1u, abort_flag, p.status, 64) : r16_bar(&bar_o[t], (summed[t] - 1) & 1u, abort_flag, p.status, 64);
+          if (!ok) return;
         }
-        if (ok && (step & R16_CLOSES)) umma_commit(&bar_empty[ks]);
+        tc_fence_after();
+        r16_scores<DP>(tmem + COL_S + 128u * t, r16_desc_k(slot_q + t * W::TILE), r16_desc_k(ring + ks * W::TILE));
+        umma_commit(&bar_s[t]);
+        scored[t]++;
+      };
+      auto product = [&](const int t, int vs) {
+        ok = r16_bar(&bar_p[t], summed[t] & 1u, abort_flag, p.status, 65);
+        if (!ok) return;
+        tc_fence_after();
+        r16_gather<DP, 128>(tmem + COL_O + O_STEP * t, tmem + COL_P + P_STEP * t, r16_desc_mn(ring + vs * W::TILE), summed[t] > 0 ? 1u : 0u);
+        umma_commit(&bar_o[t]);
+        summed[t]++;
       };
       uint32_t step = walk > 0 ? steps[0] : 0u;
-      if (ok && walk > 0) scores(step);
+      if (ok && walk > 0) {
+        const int ks = take();
+        if (ok && r16_sees_of(step, 0)) scores(0, ks);
+        if (ok && r16_sees_of(step, 1)) scores(1, ks);
+        if (ok) umma_commit(&bar_empty[ks]);
+      }
       for (int n = 0; ok && n < walk; n++) {
-        const uint32_t ahead = n + 1 < walk ? steps[n + 1] : 0u;
-        if (step & R16_OPENS) vs = take();
-        if (ok && n + 1 < walk) scores(ahead);
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-          if (!ok || !r16_sees_of(step, t)) continue;
-          const uint32_t place = summed[t] & 1u;
-          ok = r16_bar(&bar_p[t * 2 + place], (summed[t] >> 1) & 1u, abort_flag, p.status, 65);
-          if (!ok) break;
-          tc_fence_after();
-          r16_gather<DP>(tmem + COL_O + 128u * t, tmem + COL_P + 64u * t + 32u * place, r16_desc_mn(ring + vs * W::TILE) + r16_half_of(step) * R16_HALF_MN,
-                         summed[t] > 0 ? 1u : 0u);
-          umma_commit(&bar_o[t * 2 + place]);
-          summed[t]++;
+        const bool more = n + 1 < walk;
+        const uint32_t ahead = more ? steps[n + 1] : 0u;
+        const int vs = take(), ks = more ? take() : 0;
+        if (W::APART) {
+          if (ok && r16_sees_of(ahead, 0)) scores(0, ks);
+          if (ok && r16_sees_of(ahead, 1)) scores(1, ks);
+          if (ok && r16_sees_of(step, 0)) product(0, vs);
+          if (ok && r16_sees_of(step, 1)) product(1, vs);
+        } else {
+          if (ok && r16_sees_of(step, 0)) product(0, vs);
+          if (ok && r16_sees_of(ahead, 0)) scores(0, ks);
+          if (ok && r16_sees_of(step, 1)) product(1, vs);
+          if (ok && r16_sees_of(ahead, 1)) scores(1, ks);
         }
-        if (ok && (step & R16_CLOSES)) umma_commit(&bar_empty[vs]);
+        if (!ok) break;
+        umma_commit(&bar_empty[vs]);
+        if (more) umma_commit(&bar_empty[ks]);
         step = ahead;
       }
       if (!ok) *abort_flag = 1;
     }
   } else {
+    const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     int i = i0 + g * R16_T + row, head = hi;
+    bool valid = i < r.lq;
     if (p.packed) {
       const int gi = row / r.lq;
-      i = g == 0 && gi < group ? row - gi * r.lq : 0;
-      head = g == 0 && gi < group ? hi + gi : hi;
+      valid = g == 0 && gi < group;
+      i = valid ? row - gi * r.lq : 0;
+      head = valid ? hi + gi : hi;
     }
-    const float slope = EXTRA && r.slopes ? r.slopes[head] : 0.f;
+    const R16Score score = r16_score_of<MODE>(r, head);
     const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
     const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t t_s = lane_base + COL_S + 64u * g + 32u * half, t_p = lane_base + COL_P + 64u * g + 16u * half,
-                   t_o = lane_base + COL_O + 128u * g + (uint32_t)(DP / 2) * half;
-    const float mult = EXTRA ? 1.f : r.scale * R16_LOG2E;
+    const uint32_t t_s = lane_base + COL_S + 128u * g, t_p = lane_base + COL_P + P_STEP * g, t_o = lane_base + COL_O + O_STEP * g;
+    const float mult = MODE ? 1.f : r.scale * R16_LOG2E;
     const uint64_t mult2 = r16_two(mult, mult);
+    float m = -INFINITY, l = 0.f;
+    uint32_t count = 0;
     for (int n = 0; ok && n < walk; n++) {
       const uint32_t step = steps[n];
       const int sees = r16_sees_of(step, g);
       if (!sees) continue;
+      const int j0 = (first + r16_tile_of(step)) * R16_T;
       if (!(ok = r16_wait(&bar_s[g], count & 1u, abort_flag, p.status, 66))) break;
       tc_fence_after();
-      uint32_t x[32];
-      tmem_ld_32x32b_x32(t_s, x);
-      tmem_ld_wait();
-      r16_arrive_warp(&bar_read[g], lane);
-      const int j = (first + r16_tile_of(step)) * R16_T + (int)r16_half_of(step) * 64 + half * 32;
-      if (EXTRA) {
-        const int far = i + r.q_offset - j;
+      float tops[4];
+      {
+        uint32_t x[2][32];
+        tmem_ld_32x32b_x32(t_s, x[0]);
+        tmem_ld_wait();
 #pragma unroll
-        for (int u = 0; u < 32; u++) {
-          float dcap;
-          x[u] = __float_as_uint(r16_score(r, slope, far - u, __uint_as_float(x[u]), &dcap));
+        for (int c = 0; c < 4; c++) {
+          uint32_t(&v)[32] = x[c & 1];
+          if (c < 3) tmem_ld_32x32b_x32(t_s + 32u * (c + 1), x[(c + 1) & 1]);
+          if (MODE) {
+            const float far = (float)(i + r.q_offset - j0 - 32 * c);
+#pragma unroll
+            for (int u = 0; u < 32; u++) {
+              float dcap;
+              v[u] = __float_as_uint(r16_score<MODE>(score, far - (float)u, __uint_as_float(v[u]), &dcap));
+            }
+          }
+          if (sees == 1) r16_hide(v, r16_bits(seen, j0 + c * 32, docs));
+          if (MODE || sees == 1) r16_st32(t_s + 32u * c, v);
+          float t[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            t[e] = fmaxf(__uint_as_float(v[8 * e]), __uint_as_float(v[8 * e + 1]));
+#pragma unroll
+            for (int u = 2; u < 8; u += 2) t[e] = r16_max3(t[e], __uint_as_float(v[8 * e + u]), __uint_as_float(v[8 * e + u + 1]));
+          }
+          tops[c] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+          if (c < 3) tmem_ld_wait();
         }
+        if (MODE || sees == 1) r16_st_wait();
       }
-      if (sees == 1) r16_hide(x, r16_bits(seen, j, docs));
-      float t[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        t[e] = fmaxf(__uint_as_float(x[8 * e]), __uint_as_float(x[8 * e + 1]));
-#pragma unroll
-        for (int u = 2; u < 8; u += 2) t[e] = r16_max3(t[e], __uint_as_float(x[8 * e + u]), __uint_as_float(x[8 * e + u + 1]));
-      }
-      float top = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-      // The other half of the row is with another warp.
-      float* slots = maxima + ((count & 1u) * 2 + g) * 256;
-      slots[half * 128 + row] = top;
-      __syncwarp();
-      if (lane == 0) r16_arrive(&bar_max[g * 4 + quad]);
-      if (!(ok = r16_wait(&bar_max[g * 4 + quad], count & 1u, abort_flag, p.status, 68))) break;
-      top = fmaxf(top, slots[(half ^ 1) * 128 + row]) * mult;
+      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mult;
       const bool grown = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
+      // The product before has read the weights' place and is in O (in the other layout these scores came after it anyway).
+      if (W::APART && count > 0) {
+        if (!(ok = r16_wait(&bar_o[g], (count - 1) & 1u, abort_flag, p.status, 69))) break;
+        tc_fence_after();
+      }
       if (__any_sync(0xffffffffu, grown)) {
         const float shrink = grown ? r16_ex2(m - top) : 1.f;      // m = -inf: 0
         if (grown) m = top;
         l *= shrink;
         if (count > 0) {
-          const uint32_t before = count - 1;
-          if (!(ok = r16_wait(&bar_o[g * 2 + (before & 1u)], (before >> 1) & 1u, abort_flag, p.status, 69))) break;
-          tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < DP / 2; c += 32) {
+          for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
             tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
             tmem_ld_wait();
@@ -530,71 +545,68 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const float base = m == -INFINITY ? 0.f : m;
       const uint64_t base2 = r16_two(-base, -base);
       uint64_t sum[2] = {0ull, 0ull};
-      uint32_t w[16];
+      {
+        uint32_t x[2][32];
+        tmem_ld_32x32b_x32(t_s, x[0]);
+        tmem_ld_wait();
 #pragma unroll
-      for (int u = 0; u < 16; u++) {
-        float a, b;
-        r16_fma2(a, b, x[2 * u], x[2 * u + 1], mult2, base2);
-        a = r16_ex2(a);
-        b = r16_ex2(b);
-        sum[u & 1] = r16_add2(sum[u & 1], a, b);
-        w[u] = r16_pack(a, b);
+        for (int c = 0; c < 4; c++) {
+          uint32_t(&v)[32] = x[c & 1];
+          if (c < 3) tmem_ld_32x32b_x32(t_s + 32u * (c + 1), x[(c + 1) & 1]);
+          uint32_t w[16];
+#pragma unroll
+          for (int u = 0; u < 16; u++) {
+            float a, b;
+            r16_fma2(a, b, v[2 * u], v[2 * u + 1], mult2, base2);
+            a = r16_ex2(a);
+            b = r16_ex2(b);
+            sum[u & 1] = r16_add2(sum[u & 1], a, b);
+            w[u] = r16_pack(a, b);
+          }
+          if (c < 3) tmem_ld_wait();                      // what the weights may lie over has been read
+          if (W::APART && c == 2) r16_arrive_warp(&bar_read[g], lane);
+          r16_st16(t_p + 16u * c, w);
+        }
       }
       const float2 s0 = *reinterpret_cast<const float2*>(&sum[0]), s1 = *reinterpret_cast<const float2*>(&sum[1]);
       l += (s0.x + s0.y) + (s1.x + s1.y);
-      const uint32_t place = count & 1u;
-      // The product before last has read this place.
-      if (count >= 2 && !(ok = r16_wait(&bar_o[g * 2 + place], ((count - 2) >> 1) & 1u, abort_flag, p.status, 60))) break;
-      tc_fence_after();
-      r16_st16(t_p + 32u * place, w);
       r16_st_wait();
-      r16_arrive_warp(&bar_p[g * 2 + place], lane);
+      r16_arrive_warp(&bar_p[g], lane);
       count++;
     }
-    if (ok && count > 0) ok = r16_wait(&bar_o[g * 2 + ((count - 1) & 1u)], ((count - 1) >> 1) & 1u, abort_flag, p.status, 67);
-    tc_fence_after();
-    maxima[(g * 2 + half) * 128 + row] = l;
-  }
-  __syncthreads();
-  if (warp < R16_ROW_WARPS && ok && (g == 0 || both)) {
-    int i = i0 + g * R16_T + row, head = hi;
-    bool valid = i < r.lq;
-    if (p.packed) {
-      const int gi = row / r.lq;
-      i = row - gi * r.lq;
-      head = hi + gi;
-      valid = gi < group;
-    }
-    l += maxima[(g * 2 + (half ^ 1)) * 128 + row];
-    const uint32_t t_o = tmem + ((uint32_t)(quad * 32) << 16) + COL_O + 128u * g + (uint32_t)(DP / 2) * half;
-    const long long at_row = ((long long)bi * p.h + head) * r.lq + i;
-    float inv = l == 0.f ? 0.f : 1.f / l;
-    float* out = p.out;
-    __nv_bfloat16* out16 = p.out16;
-    long long at = bi * p.os.batch + head * p.os.head + (long long)i * p.os.row;
-    if (p.splits > 1) {
-      inv = 1.f;
-      out = p.part;
-      out16 = nullptr;
-      at = ((long long)split * p.rows + at_row) * p.d;
-      if (valid && half == 0) p.part_ml[(long long)split * p.rows + at_row] = make_float2(m, l);
-    } else if (p.lse && valid && half == 0) {
-      p.lse[at_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * R16_LN2;
-    }
+    if (ok && count > 0) ok = r16_wait(&bar_o[g], (count - 1) & 1u, abort_flag, p.status, 67);
+    if (ok) {
+      tc_fence_after();
+      const long long at_row = ((long long)bi * p.h + head) * r.lq + i;
+      float inv = l == 0.f ? 0.f : 1.f / l;
+      float* out = p.out;
+      __nv_bfloat16* out16 = p.out16;
+      long long at = bi * p.os.batch + head * p.os.head + (long long)i * p.os.row;
+      if (p.splits > 1) {
+        inv = 1.f;
+        out = p.part;
+        out16 = nullptr;
+        at = ((long long)split * p.rows + at_row) * p.d;
+        if (valid) p.part_ml[(long long)split * p.rows + at_row] = make_float2(m, l);
+      } else if (p.lse && valid) {
+        p.lse[at_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * R16_LN2;
+      }
+      if (g == 0 || both) {
 #pragma unroll 1
-    for (int c = 0; c < DP / 2; c += 32) {
-      uint32_t o[32];
-      __syncwarp();
-      if (count > 0) {
-        tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
-        tmem_ld_wait();
-      }
-      if (count == 0 || l == 0.f) {
+        for (int c = 0; c < DP; c += 32) {
+          uint32_t o[32];
+          __syncwarp();
+          if (count > 0) {
+            tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
+            tmem_ld_wait();
+          }
+          if (count == 0 || l == 0.f) {
 #pragma unroll
-        for (int u = 0; u < 32; u++) o[u] = 0u;
+            for (int u = 0; u < 32; u++) o[u] = 0u;
+          }
+          if (valid) r16_write(o, inv, out, out16, at + c, c, p.d);
+        }
       }
-      const int col = half * (DP / 2) + c;
-      if (valid) r16_write(o, inv, out, out16, at + col, col, p.d);
     }
   }
   tc_fence_before();
@@ -656,27 +668,29 @@ struct R16Bwd {
   int32_t* status;
 };
 
-template <int DP>
+// Two stationary tiles, a ring of the tiles that two products read, the second one late (Q, or K), and a ring of the others (dO, or V).
+// dQ's kernel has room for a third K at 128 columns; with two, the next scores waited for a load that waited for the product before.
+template <int DP, bool KEYS>
 struct R16BwdShape {
   static constexpr int TILE = DP / 64 * R16_CHUNK;
-  static constexpr int RING = 2;
-  static constexpr int ROWS = (2 + 2 * RING) * TILE;     // the queries' log-sum-exps and row dots, 1 KB a stage
-  static constexpr int RULES = ROWS + RING * 1024;
+  static constexpr int RING_A = DP == 64 ? 4 : KEYS ? 2 : 3, RING_B = DP == 64 ? 4 : 2;
+  static constexpr int ROWS = (2 + RING_A + RING_B) * TILE;     // the queries' log-sum-exps and row dots, 1 KB a stage
+  static constexpr int RULES = ROWS + (KEYS ? RING_A * 1024 : 0);
   static constexpr int PLAN = RULES + 64;
-  static constexpr int BARS = PLAN + 2 * R16_PLAN * 4 + 16;
-  static constexpr int SMEM = BARS + 256 + 1024;
+  static constexpr int BARS = PLAN + R16_PLAN * 2 + 16;
+  static constexpr int SMEM = BARS + 256;
 };
 
 // Scores of one row (32 of them, a quarter of a tile) to weights: packed as bfloat16 in w where they are wanted, and in x, times the
 // cap's derivative, for r16_gradients. Rows are keys (COLUMNS: the log-sum-exps go with the columns) or queries.
-template <bool EXTRA, bool COLUMNS>
-__device__ __forceinline__ void r16_weights(const RuleArgs& r, uint32_t (&x)[32], uint32_t (&w)[16], const float* lses, float lse, float slope, int far, float mult,
+template <int MODE, bool COLUMNS>
+__device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)[32], uint32_t (&w)[16], const float* lses, float lse, float far, float mult,
                                             bool partial, const R16Row& seen, int at, const int32_t* docs) {
-  float dcap[EXTRA ? 32 : 1];
-  if (EXTRA) {
+  float dcap[MODE == 2 ? 32 : 1];
+  if (MODE) {
 #pragma unroll
     for (int u = 0; u < 32; u++)
-      x[u] = __float_as_uint(r16_score(r, slope, COLUMNS ? far + u : far - u, __uint_as_float(x[u]), &dcap[EXTRA ? u : 0]));
+      x[u] = __float_as_uint(r16_score<MODE>(score, COLUMNS ? far + (float)u : far - (float)u, __uint_as_float(x[u]), &dcap[MODE == 2 ? u : 0]));
   }
   if (partial) r16_hide(x, r16_bits(seen, at, docs));
   const uint64_t mult2 = r16_two(mult, mult);
@@ -695,7 +709,7 @@ __device__ __forceinline__ void r16_weights(const RuleArgs& r, uint32_t (&x)[32]
       if (COLUMNS) w[(u + t) / 2] = r16_pack(p[t], p[t + 1]);
     }
 #pragma unroll
-    for (int t = 0; t < 4; t++) x[u + t] = __float_as_uint(EXTRA ? p[t] == 0.f ? 0.f : p[t] * dcap[EXTRA ? u + t : 0] : p[t]);
+    for (int t = 0; t < 4; t++) x[u + t] = __float_as_uint(MODE == 2 ? p[t] == 0.f ? 0.f : p[t] * dcap[MODE == 2 ? u + t : 0] : p[t]);
   }
 }
 // dS = weight (dP - dot), 32 of them, packed. partial: some are hidden, and 0 whatever dP is there.
@@ -720,23 +734,20 @@ __device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uin
   for (int u = 0; u < 32; u += 2) w[u / 2] = r16_pack(v[u], v[u + 1]);
 }
 
-template <int DP, bool EXTRA>
+template <int DP, int MODE>
 __global__ void __launch_bounds__(R16_THREADS, 1)
 rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const __grid_constant__ CUtensorMap map_g, const __grid_constant__ R16Bwd p) {
-  typedef R16BwdShape<DP> W;
-  // Scores, dP; two places each of P and dS (32 columns) that the two sets of rows fill in turn; the sums.
-  constexpr uint32_t COL_S = 0, COL_DP = 64, COL_P = 128, COL_DS = 192, COL_DV = 256, COL_DK = 384;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t *slot_k = smem, *slot_v = smem + W::TILE, *ring_q = smem + 2 * W::TILE, *ring_g = ring_q + W::RING * W::TILE;
-  uint32_t* steps = reinterpret_cast<uint32_t*>(smem + W::PLAN);
+  typedef R16BwdShape<DP, true> W;
+  constexpr uint32_t COL_S = 0 /* and P over it */, COL_DP = 128 /* and dS */, COL_DV = 256, COL_DK = 384;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *slot_k = smem, *slot_v = smem + W::TILE, *ring_q = smem + 2 * W::TILE, *ring_g = ring_q + W::RING_A * W::TILE;
+  uint16_t* steps = reinterpret_cast<uint16_t*>(smem + W::PLAN);
   float* ring_rows = reinterpret_cast<float*>(smem + W::ROWS);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
-  // By the step's parity but for the first and the last line: a set of rows waits for its own steps only.
-  uint64_t *bar_kv = bars, *bar_done = bars + 1, *bar_s = bars + 2, *bar_dp = bars + 4, *read_s = bars + 6, *read_dp = bars + 8, *bar_p = bars + 10, *bar_ds = bars + 12,
-           *bar_dv = bars + 14, *bar_dk = bars + 16, *full_q = bars + 18, *empty_q = bars + 20, *full_g = bars + 22, *empty_g = bars + 24;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+  uint64_t *bar_kv = bars, *bar_done = bars + 1, *bar_s = bars + 2, *bar_dp = bars + 3, *bar_p = bars + 4, *bar_ds = bars + 5, *bar_dv = bars + 6, *bar_dk = bars + 7,
+           *full_q = bars + 8, *empty_q = full_q + W::RING_A, *full_g = empty_q + W::RING_A, *empty_g = full_g + W::RING_B;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty_g + W::RING_B);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const RuleArgs& r = p.r;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -745,15 +756,14 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   if (threadIdx.x == 0) {
     mbar_init(bar_kv, 1);
     mbar_init(bar_done, 1);
-    for (int a = 0; a < 2; a++) {
-      mbar_init(&bar_s[a], 1);
-      mbar_init(&bar_dp[a], 1);
-      mbar_init(&read_s[a], R16_ROW_WARPS / 2);
-      mbar_init(&read_dp[a], R16_ROW_WARPS / 2);
-      mbar_init(&bar_p[a], R16_ROW_WARPS / 2);
-      mbar_init(&bar_ds[a], R16_ROW_WARPS / 2);
-      mbar_init(&bar_dv[a], 1);
-      mbar_init(&bar_dk[a], 1);
+    mbar_init(bar_s, 1);
+    mbar_init(bar_dp, 1);
+    mbar_init(bar_p, R16_ROW_WARPS);
+    mbar_init(bar_ds, R16_ROW_WARPS);
+    mbar_init(bar_dv, 1);
+    mbar_init(bar_dk, 1);
+    static_assert(W::RING_A == W::RING_B, "one stage number serves both rings");
+    for (int a = 0; a < W::RING_A; a++) {
       mbar_init(&full_q[a], 1);
       mbar_init(&empty_q[a], 1);
       mbar_init(&full_g[a], 1);
@@ -779,21 +789,19 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   __syncthreads();
   const int first = tile->lo / R16_T, tiles = max(0, (min(tile->hi, r.lq) + R16_T - 1) / R16_T - first);
   if (warp == 0) {
-    const int n = r16_plan(steps, tiles, lane, [&](int t, int e) { return (uint32_t)rule_see<false>(*tile, (first + t) * R16_T + e * 64, 1); });
-    if (lane == 0) steps[2 * R16_PLAN] = (uint32_t)n;
+    const int n = r16_plan(steps, tiles, lane, [&](int t) { return (uint32_t)rule_see<false>(*tile, (first + t) * R16_T, 2); });
+    if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
   // The same steps for every head that shares the keys, head by head.
-  const int round = (int)steps[2 * R16_PLAN], walk = round * group;
-  int gi = 0, k = -1, turn = -1;                         // the head, its step, and the number of its tile in the rings
+  const int round = (int)steps[R16_PLAN], walk = round * group;
+  int gi = 0, k = -1;                                    // the head, and its step
   auto forth = [&]() {
     if (++k == round) {
       k = 0;
       gi++;
     }
-    const uint32_t step = steps[k];
-    if (step & R16_OPENS) turn++;
-    return step;
+    return (uint32_t)steps[k];
   };
 
   bool ok = true;
@@ -804,16 +812,15 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       r16_load_tile<DP>(slot_v, &map_v, j0, hk, bi, bar_kv);
       for (int n = 0; ok && n < walk; n++) {
         const uint32_t step = forth();
-        if (!(step & R16_OPENS)) continue;
-        const int a = turn % W::RING, head = hk * group + gi, at = first + r16_tile_of(step);
-        const uint32_t before = ((turn / W::RING) & 1u) ^ 1u;
+        const int a = n % W::RING_A, head = hk * group + gi, at = first + r16_tile_of(step);
+        const uint32_t before = ((n / W::RING_A) & 1u) ^ 1u;
         // The keys' gradient of the tile before in this stage has read it, after the rows were done with its log-sum-exps and dots.
-        if (turn >= W::RING) ok = r16_bar(&empty_q[a], before, abort_flag, p.status, 71);
+        if (n >= W::RING_A) ok = r16_bar(&empty_q[a], before, abort_flag, p.status, 71);
         if (!ok) break;
         mbar_expect_tx(&full_q[a], W::TILE + 1024);
         r16_load_tile<DP>(ring_q + a * W::TILE, &map_q, at * R16_T, head, bi, &full_q[a]);
         r16_load_rows(ring_rows + a * 256, p.rows + (((long long)bi * p.h + head) * p.tiles + at) * 256, &full_q[a]);
-        if (turn >= W::RING) ok = r16_bar(&empty_g[a], before, abort_flag, p.status, 72);
+        if (n >= W::RING_A) ok = r16_bar(&empty_g[a], before, abort_flag, p.status, 72);
         if (!ok) break;
         mbar_expect_tx(&full_g[a], W::TILE);
         r16_load_tile<DP>(ring_g + a * W::TILE, &map_g, at * R16_T, head, bi, &full_g[a]);
@@ -822,106 +829,107 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   } else if (warp == R16_ROW_WARPS) {
     if (lane == 0) {
       ok = r16_bar(bar_kv, 0, abort_flag, p.status, 73);
-      auto scores = [&](int n, uint32_t step, uint64_t* full, uint64_t* read, uint64_t* bar, const uint8_t* keep, const uint8_t* ring, uint32_t col) {
-        const int a = turn % W::RING;
-        if (step & R16_OPENS) ok = ok && r16_bar(&full[a], (turn / W::RING) & 1u, abort_flag, p.status, 74);
-        if (ok && n > 0) ok = r16_bar(&read[(n - 1) & 1], ((n - 1) >> 1) & 1u, abort_flag, p.status, 75);   // the rows have taken the ones before
+      auto scores = [&](int n, uint64_t* full, uint64_t* bar, const uint8_t* keep, const uint8_t* ring, uint32_t col) {
+        const int a = n % W::RING_A;
+        ok = ok && r16_bar(&full[a], (n / W::RING_A) & 1u, abort_flag, p.status, 74);
         if (!ok) return;
         tc_fence_after();
-        r16_scores<DP>(tmem + col, r16_desc_k(keep), r16_desc_k(ring + a * W::TILE) + r16_half_of(step) * R16_HALF_K);
-        umma_commit(&bar[n & 1]);
+        r16_scores<DP>(tmem + col, r16_desc_k(keep), r16_desc_k(ring + a * W::TILE));
+        umma_commit(bar);
       };
-      uint32_t step = walk > 0 ? forth() : 0u;
       if (ok && walk > 0) {
-        scores(0, step, full_q, read_s, bar_s, slot_k, ring_q, COL_S);
-        scores(0, step, full_g, read_dp, bar_dp, slot_v, ring_g, COL_DP);
+        scores(0, full_q, bar_s, slot_k, ring_q, COL_S);
+        scores(0, full_g, bar_dp, slot_v, ring_g, COL_DP);
       }
       for (int n = 0; ok && n < walk; n++) {
-        const int a = turn % W::RING;
-        const uint32_t set = n & 1, phase = (n >> 1) & 1u, half = r16_half_of(step) * R16_HALF_MN;
-        const uint32_t ahead = n + 1 < walk ? forth() : 0u;
-        if (n + 1 < walk) scores(n + 1, ahead, full_q, read_s, bar_s, slot_k, ring_q, COL_S);
-        // dV += P^T dO
-        if (!(ok = ok && r16_bar(&bar_p[set], phase, abort_flag, p.status, 76))) break;
+        const int a = n % W::RING_A;
+        const uint32_t phase = n & 1u;
+        const bool more = n + 1 < walk;
+        // dV += P^T dO, then the next scores as soon as it has read P, which lies over these.
+        if (!(ok = r16_bar(bar_p, phase, abort_flag, p.status, 76))) break;
         tc_fence_after();
-        r16_gather<DP>(tmem + COL_DV, tmem + COL_P + 32u * set, r16_desc_mn(ring_g + a * W::TILE) + half, n > 0 ? 1u : 0u);
-        umma_commit(&bar_dv[set]);
-        if (step & R16_CLOSES) umma_commit(&empty_g[a]);
-        if (n + 1 < walk) scores(n + 1, ahead, full_g, read_dp, bar_dp, slot_v, ring_g, COL_DP);
-        // dK += dS^T Q
-        if (!(ok = ok && r16_bar(&bar_ds[set], phase, abort_flag, p.status, 78))) break;
+        r16_gather<DP, 64>(tmem + COL_DV, tmem + COL_S, r16_desc_mn(ring_g + a * W::TILE), n > 0 ? 1u : 0u);
+        umma_commit(bar_dv);
+        umma_commit(&empty_g[a]);
+        if (more) {
+          ok = r16_bar(bar_dv, phase, abort_flag, p.status, 77);
+          scores(n + 1, full_q, bar_s, slot_k, ring_q, COL_S);
+        }
+        // dK += dS^T Q, then the next dP.
+        if (!(ok = ok && r16_bar(bar_ds, phase, abort_flag, p.status, 78))) break;
         tc_fence_after();
-        r16_gather<DP>(tmem + COL_DK, tmem + COL_DS + 32u * set, r16_desc_mn(ring_q + a * W::TILE) + half, n > 0 ? 1u : 0u);
-        umma_commit(&bar_dk[set]);
-        if (step & R16_CLOSES) umma_commit(&empty_q[a]);
-        step = ahead;
+        r16_gather<DP, 64>(tmem + COL_DK, tmem + COL_DP, r16_desc_mn(ring_q + a * W::TILE), n > 0 ? 1u : 0u);
+        umma_commit(bar_dk);
+        umma_commit(&empty_q[a]);
+        if (more) {
+          ok = r16_bar(bar_dk, phase, abort_flag, p.status, 79);
+          scores(n + 1, full_g, bar_dp, slot_v, ring_g, COL_DP);
+        }
       }
       if (ok) umma_commit(bar_done);
       else *abort_flag = 1;
     }
   } else {
-    const int set = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, row = quad * 32 + lane, j = j0 + row;
+    const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane, j = j0 + row;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t t_s = lane_base + COL_S + 32u * half, t_dp = lane_base + COL_DP + 32u * half, t_p = lane_base + COL_P + 32u * set + 16u * half,
-                   t_ds = lane_base + COL_DS + 32u * set + 16u * half;
+    const uint32_t t_s = lane_base + COL_S + 64u * half, t_dp = lane_base + COL_DP + 64u * half;
     const R16Row seen = r16_key_row(r, prefix, bi, min(j, r.lk - 1));
     const int32_t* docs = r.q_docs ? r.q_docs + (long long)bi * r.lq : nullptr;
-    const float mult = EXTRA ? 1.f : r.scale * R16_LOG2E;
+    const float mult = MODE ? 1.f : r.scale * R16_LOG2E;
     for (int n = 0; ok && n < walk; n++) {
-      const uint32_t step = forth();
-      if ((n & 1) != set) continue;
-      const int a = turn % W::RING, in = (int)r16_half_of(step) * 64 + half * 32, at = (first + r16_tile_of(step)) * R16_T + in;
-      const uint32_t phase = (n >> 1) & 1u;
+      const uint32_t step = forth(), phase = n & 1u;
+      const int a = n % W::RING_A, at = (first + r16_tile_of(step)) * R16_T + half * 64;
       const bool partial = r16_sees_of(step, 0) == 1;
-      const float slope = EXTRA && r.slopes ? r.slopes[hk * group + gi] : 0.f;
-      const float* rows = ring_rows + a * 256 + in;
+      const R16Score score = r16_score_of<MODE>(r, hk * group + gi);
+      const float* rows = ring_rows + a * 256 + half * 64;
       // The queries' log-sum-exps came with the queries, which the scores have waited for; this wait makes them seen here.
-      if (!(ok = r16_wait(&full_q[a], (turn / W::RING) & 1u, abort_flag, p.status, 94) && r16_wait(&bar_s[set], phase, abort_flag, p.status, 80))) break;
+      if (!(ok = r16_wait(&full_q[a], (n / W::RING_A) & 1u, abort_flag, p.status, 94) && r16_wait(bar_s, phase, abort_flag, p.status, 80))) break;
       tc_fence_after();
-      uint32_t x[32], w[16];
-      tmem_ld_32x32b_x32(t_s, x);
+      uint32_t x[2][32], w[16];
+      tmem_ld_32x32b_x32(t_s, x[0]);
+      tmem_ld_32x32b_x32(t_s + 32u, x[1]);
       tmem_ld_wait();
-      r16_arrive_warp(&read_s[set], lane);
-      r16_weights<EXTRA, true>(r, x, w, rows, 0.f, slope, at + r.q_offset - j, mult, partial, seen, at, docs);
-      // The products of this set's step before have read the places of P and dS.
-      if (n >= 2 && !(ok = r16_wait(&bar_dv[set], phase ^ 1u, abort_flag, p.status, 95))) break;
-      tc_fence_after();
-      r16_st16(t_p, w);
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        r16_weights<MODE, true>(score, x[c], w, rows + c * 32, 0.f, (float)(at + c * 32 + r.q_offset - j), mult, partial, seen, at + c * 32, docs);
+        r16_st16(t_s + 16u * c, w);
+      }
       r16_st_wait();
-      r16_arrive_warp(&bar_p[set], lane);
-      if (!(ok = r16_wait(&bar_dp[set], phase, abort_flag, p.status, 81))) break;
+      r16_arrive_warp(bar_p, lane);
+      if (!(ok = r16_wait(bar_dp, phase, abort_flag, p.status, 81))) break;
       tc_fence_after();
-      uint32_t dp[32];
-      tmem_ld_32x32b_x32(t_dp, dp);
+      uint32_t dp[2][32];
+      tmem_ld_32x32b_x32(t_dp, dp[0]);
       tmem_ld_wait();
-      r16_arrive_warp(&read_dp[set], lane);
-      r16_gradients<true>(x, dp, w, rows + 128, 0.f, partial);
-      if (n >= 2 && !(ok = r16_wait(&bar_dk[set], phase ^ 1u, abort_flag, p.status, 96))) break;
-      tc_fence_after();
-      r16_st16(t_ds, w);
+      tmem_ld_32x32b_x32(t_dp + 32u, dp[1]);
+      r16_gradients<true>(x[0], dp[0], w, rows + 128, 0.f, partial);
+      tmem_ld_wait();
+      r16_st16(t_dp, w);
+      r16_gradients<true>(x[1], dp[1], w, rows + 160, 0.f, partial);
+      r16_st16(t_dp + 16u, w);
       r16_st_wait();
-      r16_arrive_warp(&bar_ds[set], lane);
+      r16_arrive_warp(bar_ds, lane);
     }
     if (ok) ok = r16_wait(bar_done, 0, abort_flag, p.status, 82);
     if (ok) {
       tc_fence_after();
-      // dV by the first set, dK by the other, half of the columns each.
-      float* out = set == 0 ? p.d0 : p.d1;
-      __nv_bfloat16* out16 = set == 0 ? p.d0_16 : p.d1_16;
-      const R16Strides& s = set == 0 ? p.s0 : p.s1;
+      // dV by the first four warps, dK by the others.
+      float* out = half == 0 ? p.d0 : p.d1;
+      __nv_bfloat16* out16 = half == 0 ? p.d0_16 : p.d1_16;
+      const R16Strides& s = half == 0 ? p.s0 : p.s1;
       if (out || out16) {
 #pragma unroll 1
-        for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
+        for (int c = 0; c < DP; c += 32) {
           uint32_t o[32];
           __syncwarp();
           if (walk > 0) {
-            tmem_ld_32x32b_x32(lane_base + (set == 0 ? COL_DV : COL_DK) + (uint32_t)c, o);
+            tmem_ld_32x32b_x32(lane_base + (half == 0 ? COL_DV : COL_DK) + (uint32_t)c, o);
             tmem_ld_wait();
           } else {
 #pragma unroll
             for (int u = 0; u < 32; u++) o[u] = 0u;
           }
-          if (j < r.lk) r16_write(o, set == 0 ? 1.f : r.scale, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
+          if (j < r.lk) r16_write(o, half == 0 ? 1.f : r.scale, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
         }
       }
     }
@@ -934,21 +942,19 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   }
 }
 
-template <int DP, bool EXTRA>
+template <int DP, int MODE>
 __global__ void __launch_bounds__(R16_THREADS, 1)
 rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_g, const __grid_constant__ R16Bwd p) {
-  typedef R16BwdShape<DP> W;
-  // Two places each of scores, dP (64 columns) and dS (32): the two sets of rows take the steps in turn.
-  constexpr uint32_t COL_S = 0, COL_DP = 128, COL_DS = 256, COL_DQ = 384;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t *slot_q = smem, *slot_g = smem + W::TILE, *ring_k = smem + 2 * W::TILE, *ring_v = ring_k + W::RING * W::TILE;
-  uint32_t* steps = reinterpret_cast<uint32_t*>(smem + W::PLAN);
+  typedef R16BwdShape<DP, false> W;
+  constexpr uint32_t COL_S = 0 /* two places, and dS over either */, COL_DP = 256, COL_DQ = 384;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *slot_q = smem, *slot_g = smem + W::TILE, *ring_k = smem + 2 * W::TILE, *ring_v = ring_k + W::RING_A * W::TILE;
+  uint16_t* steps = reinterpret_cast<uint16_t*>(smem + W::PLAN);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
-  uint64_t *bar_qg = bars, *bar_done = bars + 1, *bar_s = bars + 2, *bar_dp = bars + 4, *read_s = bars + 6, *read_dp = bars + 8, *bar_ds = bars + 10, *bar_dq = bars + 12,
-           *full_k = bars + 14, *empty_k = bars + 16, *full_v = bars + 18, *empty_v = bars + 20;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 22);
+  uint64_t *bar_qg = bars, *bar_done = bars + 1, *bar_s = bars + 2 /* [place] */, *bar_ds = bars + 4 /* [place] */, *bar_dq = bars + 6 /* [place] */, *bar_dp = bars + 8,
+           *read_dp = bars + 9, *full_k = bars + 10, *empty_k = full_k + W::RING_A, *full_v = empty_k + W::RING_A, *empty_v = full_v + W::RING_B;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(empty_v + W::RING_B);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const RuleArgs& r = p.r;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -957,17 +963,20 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   if (threadIdx.x == 0) {
     mbar_init(bar_qg, 1);
     mbar_init(bar_done, 1);
+    mbar_init(bar_dp, 1);
+    mbar_init(read_dp, R16_ROW_WARPS);
     for (int a = 0; a < 2; a++) {
       mbar_init(&bar_s[a], 1);
-      mbar_init(&bar_dp[a], 1);
-      mbar_init(&read_s[a], R16_ROW_WARPS / 2);
-      mbar_init(&read_dp[a], R16_ROW_WARPS / 2);
-      mbar_init(&bar_ds[a], R16_ROW_WARPS / 2);
+      mbar_init(&bar_ds[a], R16_ROW_WARPS);
       mbar_init(&bar_dq[a], 1);
-      mbar_init(&full_v[a], 1);
-      mbar_init(&empty_v[a], 1);
+    }
+    for (int a = 0; a < W::RING_A; a++) {
       mbar_init(&full_k[a], 1);
       mbar_init(&empty_k[a], 1);
+    }
+    for (int a = 0; a < W::RING_B; a++) {
+      mbar_init(&full_v[a], 1);
+      mbar_init(&empty_v[a], 1);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -989,12 +998,11 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __syncthreads();
   const int first = tile->pre > 0 ? 0 : tile->lo / R16_T, tiles = max(0, (min(max(tile->pre, tile->hi), r.lk) + R16_T - 1) / R16_T - first);
   if (warp == 0) {
-    const int n = r16_plan(steps, tiles, lane, [&](int t, int e) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T + e * 64, 1); });
-    if (lane == 0) steps[2 * R16_PLAN] = (uint32_t)n;
+    const int n = r16_plan(steps, tiles, lane, [&](int t) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T, 2); });
+    if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
-  const int walk = (int)steps[2 * R16_PLAN];
-  int turn = -1;                                         // the number of a step's tile in the rings
+  const int walk = (int)steps[R16_PLAN];
 
   bool ok = true;
   if (warp == R16_ROW_WARPS + 1) {
@@ -1003,97 +1011,91 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       r16_load_tile<DP>(slot_q, &map_q, i0, hi, bi, bar_qg);
       r16_load_tile<DP>(slot_g, &map_g, i0, hi, bi, bar_qg);
       for (int n = 0; ok && n < walk; n++) {
-        const uint32_t step = steps[n];
-        if (!(step & R16_OPENS)) continue;
-        const int a = ++turn % W::RING, at = (first + r16_tile_of(step)) * R16_T;
-        const uint32_t before = ((turn / W::RING) & 1u) ^ 1u;
-        if (turn >= W::RING) ok = r16_bar(&empty_k[a], before, abort_flag, p.status, 83);
+        const int a = n % W::RING_A, b = n % W::RING_B, at = (first + r16_tile_of(steps[n])) * R16_T;
+        if (n >= W::RING_A) ok = r16_bar(&empty_k[a], ((n / W::RING_A) & 1u) ^ 1u, abort_flag, p.status, 83);
         if (!ok) break;
         mbar_expect_tx(&full_k[a], W::TILE);
         r16_load_tile<DP>(ring_k + a * W::TILE, &map_k, at, hk, bi, &full_k[a]);
-        if (turn >= W::RING) ok = r16_bar(&empty_v[a], before, abort_flag, p.status, 84);
+        if (n >= W::RING_B) ok = r16_bar(&empty_v[b], ((n / W::RING_B) & 1u) ^ 1u, abort_flag, p.status, 84);
         if (!ok) break;
-        mbar_expect_tx(&full_v[a], W::TILE);
-        r16_load_tile<DP>(ring_v + a * W::TILE, &map_v, at, hk, bi, &full_v[a]);
+        mbar_expect_tx(&full_v[b], W::TILE);
+        r16_load_tile<DP>(ring_v + b * W::TILE, &map_v, at, hk, bi, &full_v[b]);
       }
     }
   } else if (warp == R16_ROW_WARPS) {
     if (lane == 0) {
       ok = r16_bar(bar_qg, 0, abort_flag, p.status, 85);
-      // Scores and dP of a step, into the places that this set's step before has been taken from.
-      auto scores = [&](int n, uint32_t step) {
-        if (step & R16_OPENS) turn++;
-        const int a = turn % W::RING;
-        const uint32_t phase = (turn / W::RING) & 1u, set = n & 1, before = ((n >> 1) & 1u) ^ 1u, half = r16_half_of(step) * R16_HALF_K;
-        if (step & R16_OPENS) ok = r16_bar(&full_k[a], phase, abort_flag, p.status, 86);
-        if (ok && n >= 2) ok = r16_bar(&read_s[set], before, abort_flag, p.status, 87);
+      auto scores = [&](int n) {
+        const int a = n % W::RING_A, b = n % W::RING_B;
+        const uint32_t place = n & 1u;
+        // Over the gradients of the step before last, which their product has read.
+        ok = r16_bar(&full_k[a], (n / W::RING_A) & 1u, abort_flag, p.status, 86) && (n < 2 || r16_bar(&bar_dq[place], ((n - 2) >> 1) & 1u, abort_flag, p.status, 87));
         if (!ok) return;
         tc_fence_after();
-        r16_scores<DP>(tmem + COL_S + 64u * set, r16_desc_k(slot_q), r16_desc_k(ring_k + a * W::TILE) + half);
-        umma_commit(&bar_s[set]);
-        if (step & R16_OPENS) ok = r16_bar(&full_v[a], phase, abort_flag, p.status, 88);
-        if (ok && n >= 2) ok = r16_bar(&read_dp[set], before, abort_flag, p.status, 89);
+        r16_scores<DP>(tmem + COL_S + 128u * place, r16_desc_k(slot_q), r16_desc_k(ring_k + a * W::TILE));
+        umma_commit(&bar_s[place]);
+        // Once the rows have taken the dP before.
+        ok = r16_bar(&full_v[b], (n / W::RING_B) & 1u, abort_flag, p.status, 88) && (n < 1 || r16_bar(read_dp, (n - 1) & 1u, abort_flag, p.status, 89));
         if (!ok) return;
         tc_fence_after();
-        r16_scores<DP>(tmem + COL_DP + 64u * set, r16_desc_k(slot_g), r16_desc_k(ring_v + a * W::TILE) + half);
-        umma_commit(&bar_dp[set]);
-        if (step & R16_CLOSES) umma_commit(&empty_v[a]);
+        r16_scores<DP>(tmem + COL_DP, r16_desc_k(slot_g), r16_desc_k(ring_v + b * W::TILE));
+        umma_commit(bar_dp);
+        umma_commit(&empty_v[b]);
       };
-      uint32_t step = walk > 0 ? steps[0] : 0u;
-      if (ok && walk > 0) scores(0, step);
+      if (ok && walk > 0) scores(0);
       for (int n = 0; ok && n < walk; n++) {
-        const int a = turn % W::RING;
-        const uint32_t set = n & 1, ahead = n + 1 < walk ? steps[n + 1] : 0u;
-        if (n + 1 < walk) scores(n + 1, ahead);
-        if (!(ok = ok && r16_bar(&bar_ds[set], (n >> 1) & 1u, abort_flag, p.status, 90))) break;
+        const uint32_t place = n & 1u;
+        if (n + 1 < walk) scores(n + 1);
+        if (!(ok = ok && r16_bar(&bar_ds[place], (n >> 1) & 1u, abort_flag, p.status, 90))) break;
         tc_fence_after();
-        r16_gather<DP>(tmem + COL_DQ, tmem + COL_DS + 32u * set, r16_desc_mn(ring_k + a * W::TILE) + r16_half_of(step) * R16_HALF_MN, n > 0 ? 1u : 0u);
-        umma_commit(&bar_dq[set]);
-        if (step & R16_CLOSES) umma_commit(&empty_k[a]);
-        step = ahead;
+        r16_gather<DP, 64>(tmem + COL_DQ, tmem + COL_S + 128u * place, r16_desc_mn(ring_k + (n % W::RING_A) * W::TILE), n > 0 ? 1u : 0u);
+        umma_commit(&bar_dq[place]);
+        umma_commit(&empty_k[n % W::RING_A]);
       }
       if (ok) umma_commit(bar_done);
       else *abort_flag = 1;
     }
   } else {
-    const int set = warp >> 3, half = (warp >> 2) & 1, quad = warp & 3, row = quad * 32 + lane, i = i0 + row;
-    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t t_s = lane_base + COL_S + 64u * set + 32u * half, t_dp = lane_base + COL_DP + 64u * set + 32u * half, t_ds = lane_base + COL_DS + 32u * set + 16u * half;
-    const float slope = EXTRA && r.slopes ? r.slopes[hi] : 0.f;
+    const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane, i = i0 + row;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), t_dp = lane_base + COL_DP + 64u * half;
+    const R16Score score = r16_score_of<MODE>(r, hi);
     const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
     const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
-    const float mult = EXTRA ? 1.f : r.scale * R16_LOG2E;
+    const float mult = MODE ? 1.f : r.scale * R16_LOG2E;
     const float2 stat = rule_row(p.rows, (long long)bi * p.h + hi, r.lq, i);
-    for (int n = set; ok && n < walk; n += 2) {
-      const uint32_t step = steps[n];
-      const int at = (first + r16_tile_of(step)) * R16_T + (int)r16_half_of(step) * 64 + half * 32;
-      const uint32_t phase = (n >> 1) & 1u;
+    for (int n = 0; ok && n < walk; n++) {
+      const uint32_t step = steps[n], place = n & 1u, phase = (n >> 1) & 1u, t_s = lane_base + COL_S + 128u * place + 64u * half;
+      const int at = (first + r16_tile_of(step)) * R16_T + half * 64;
       const bool partial = r16_sees_of(step, 0) == 1;
-      if (!(ok = r16_wait(&bar_s[set], phase, abort_flag, p.status, 91))) break;
+      if (!(ok = r16_wait(&bar_s[place], phase, abort_flag, p.status, 91))) break;
       tc_fence_after();
-      uint32_t x[32], dp[32], w[16];
-      tmem_ld_32x32b_x32(t_s, x);
+      uint32_t x[2][32], dp[2][32], w[16];
+      tmem_ld_32x32b_x32(t_s, x[0]);
+      tmem_ld_32x32b_x32(t_s + 32u, x[1]);
       tmem_ld_wait();
-      r16_arrive_warp(&read_s[set], lane);
-      r16_weights<EXTRA, false>(r, x, w, nullptr, stat.x, slope, i + r.q_offset - at, mult, partial, seen, at, docs);
-      if (!(ok = r16_wait(&bar_dp[set], phase, abort_flag, p.status, 92))) break;
+#pragma unroll
+      for (int c = 0; c < 2; c++)
+        r16_weights<MODE, false>(score, x[c], w, nullptr, stat.x, (float)(i + r.q_offset - at - c * 32), mult, partial, seen, at + c * 32, docs);
+      if (!(ok = r16_wait(bar_dp, n & 1u, abort_flag, p.status, 92))) break;
       tc_fence_after();
-      tmem_ld_32x32b_x32(t_dp, dp);
+      tmem_ld_32x32b_x32(t_dp, dp[0]);
+      tmem_ld_32x32b_x32(t_dp + 32u, dp[1]);
       tmem_ld_wait();
-      r16_arrive_warp(&read_dp[set], lane);
-      r16_gradients<false>(x, dp, w, nullptr, stat.y, partial);
-      if (n >= 2 && !(ok = r16_wait(&bar_dq[set], phase ^ 1u, abort_flag, p.status, 97))) break;    // the product has read the gradients before
-      tc_fence_after();
-      r16_st16(t_ds, w);
+      r16_arrive_warp(read_dp, lane);
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        r16_gradients<false>(x[c], dp[c], w, nullptr, stat.y, partial);
+        r16_st16(t_s + 16u * c, w);
+      }
       r16_st_wait();
-      r16_arrive_warp(&bar_ds[set], lane);
+      r16_arrive_warp(&bar_ds[place], lane);
     }
     if (ok) ok = r16_wait(bar_done, 0, abort_flag, p.status, 93);
     if (ok) {
       tc_fence_after();
-      // A quarter of dQ's columns by each four warps.
+      // Half of dQ's columns by each four warps.
 #pragma unroll 1
-      for (int c = (set * 2 + half) * 32; c < DP; c += 128) {
+      for (int c = half * (DP / 2); c < (half + 1) * (DP / 2); c += 32) {
         uint32_t o[32];
         __syncwarp();
         if (walk > 0) {
@@ -1162,11 +1164,17 @@ static int32_t r16_room(om_ctx* ctx, K kernel, int smem) {
   return OM_OK;
 }
 
-template <int DP, bool EXTRA>
+template <int DP, int MODE>
 static int32_t r16_fwd(om_ctx* ctx, dim3 grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const R16Fwd& p) {
-  OM_TRY(r16_room(ctx, rule16_fwd_kernel<DP, EXTRA>, R16FwdShape<DP>::SMEM));
-  launch_chained(ctx, rule16_fwd_kernel<DP, EXTRA>, grid, R16_THREADS, R16FwdShape<DP>::SMEM, mq, mk, mv, p);
+  OM_TRY(r16_room(ctx, rule16_fwd_kernel<DP, MODE>, R16FwdShape<DP>::SMEM));
+  launch_chained(ctx, rule16_fwd_kernel<DP, MODE>, grid, R16_THREADS, R16FwdShape<DP>::SMEM, mq, mk, mv, p);
   return OM_OK;
+}
+
+template <int DP>
+static int32_t r16_fwd_by_mode(om_ctx* ctx, dim3 grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const R16Fwd& p) {
+  if (p.r.softcap > 0.f) return r16_fwd<DP, 2>(ctx, grid, mq, mk, mv, p);
+  return p.r.slopes ? r16_fwd<DP, 1>(ctx, grid, mq, mk, mv, p) : r16_fwd<DP, 0>(ctx, grid, mq, mk, mv, p);
 }
 
 int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
@@ -1199,10 +1207,7 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
     p.part_ml = reinterpret_cast<float2*>(part);
     p.part = reinterpret_cast<float*>(part + ml);
   }
-  const bool extra = c.r.softcap > 0.f || c.r.slopes;
-  int32_t st;
-  if (c.d <= 64) st = extra ? r16_fwd<64, true>(ctx, grid, mq, mk, mv, p) : r16_fwd<64, false>(ctx, grid, mq, mk, mv, p);
-  else st = extra ? r16_fwd<128, true>(ctx, grid, mq, mk, mv, p) : r16_fwd<128, false>(ctx, grid, mq, mk, mv, p);
+  const int32_t st = c.d <= 64 ? r16_fwd_by_mode<64>(ctx, grid, mq, mk, mv, p) : r16_fwd_by_mode<128>(ctx, grid, mq, mk, mv, p);
   if (p.splits > 1) {
     if (st == OM_OK) launch_chained(ctx, rule16_join_kernel, grid_for(ctx, p.rows, 8), 256, 0, p);
     pool_free(ctx, part);
@@ -1212,19 +1217,27 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
   return OM_OK;
 }
 
-template <int DP, bool EXTRA>
+template <int DP, int MODE>
 static int32_t r16_bwd(om_ctx* ctx, const RuleCall& c, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg,
                        const R16Bwd& kv, const R16Bwd& q) {
-  const int smem = R16BwdShape<DP>::SMEM;
   if (kv.d0 || kv.d0_16 || kv.d1 || kv.d1_16) {
-    OM_TRY(r16_room(ctx, rule16_dkv_kernel<DP, EXTRA>, smem));
-    launch_chained(ctx, rule16_dkv_kernel<DP, EXTRA>, dim3((unsigned)(c.b * c.hkv), (unsigned)ceil_div(c.r.lk, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, kv);
+    constexpr int smem = R16BwdShape<DP, true>::SMEM;
+    OM_TRY(r16_room(ctx, rule16_dkv_kernel<DP, MODE>, smem));
+    launch_chained(ctx, rule16_dkv_kernel<DP, MODE>, dim3((unsigned)(c.b * c.hkv), (unsigned)ceil_div(c.r.lk, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, kv);
   }
   if (q.d0 || q.d0_16) {
-    OM_TRY(r16_room(ctx, rule16_dq_kernel<DP, EXTRA>, smem));
-    launch_chained(ctx, rule16_dq_kernel<DP, EXTRA>, dim3((unsigned)(c.b * c.h), (unsigned)ceil_div(c.r.lq, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, q);
+    constexpr int smem = R16BwdShape<DP, false>::SMEM;
+    OM_TRY(r16_room(ctx, rule16_dq_kernel<DP, MODE>, smem));
+    launch_chained(ctx, rule16_dq_kernel<DP, MODE>, dim3((unsigned)(c.b * c.h), (unsigned)ceil_div(c.r.lq, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, q);
   }
   return OM_OK;
+}
+
+template <int DP>
+static int32_t r16_bwd_by_mode(om_ctx* ctx, const RuleCall& c, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg,
+                               const R16Bwd& kv, const R16Bwd& q) {
+  if (c.r.softcap > 0.f) return r16_bwd<DP, 2>(ctx, c, mq, mk, mv, mg, kv, q);
+  return c.r.slopes ? r16_bwd<DP, 1>(ctx, c, mq, mk, mv, mg, kv, q) : r16_bwd<DP, 0>(ctx, c, mq, mk, mv, mg, kv, q);
 }
 
 int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
@@ -1243,10 +1256,7 @@ int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_
   if (dk || dk16) kv.s1 = r16_strides(dks);
   one.d0 = dq; one.d0_16 = reinterpret_cast<__nv_bfloat16*>(dq16);
   if (dq || dq16) one.s0 = r16_strides(dqs);
-  const bool extra = c.r.softcap > 0.f || c.r.slopes;
-  int32_t st;
-  if (c.d <= 64) st = extra ? r16_bwd<64, true>(ctx, c, mq, mk, mv, mg, kv, one) : r16_bwd<64, false>(ctx, c, mq, mk, mv, mg, kv, one);
-  else st = extra ? r16_bwd<128, true>(ctx, c, mq, mk, mv, mg, kv, one) : r16_bwd<128, false>(ctx, c, mq, mk, mv, mg, kv, one);
+  const int32_t st = c.d <= 64 ? r16_bwd_by_mode<64>(ctx, c, mq, mk, mv, mg, kv, one) : r16_bwd_by_mode<128>(ctx, c, mq, mk, mv, mg, kv, one);
   OM_TRY(st);
   OM_LAUNCH_CHECK(ctx, "om_rule_attention_bwd_bf16");
   return OM_OK;
