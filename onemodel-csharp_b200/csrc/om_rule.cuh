@@ -168,17 +168,33 @@ __device__ __forceinline__ float2 rule_row(const float* rows, long long bh, int 
 }
 int32_t rule_begin(om_ctx* ctx, const om_attention_rule* rule, int b, int h, int hkv, int lq, int lk, int d, float scale, RuleCall* call);
 void rule_end(om_ctx* ctx, RuleCall* call);
+struct RulePlanes {
+  const void* p[4];               // q, k, v, g
+  om_head_strides q, k;           // of q and g, of k and v
+  const float* units;
+  const int32_t* plain;
+  void *small, *large;
+};
 // The tensor-pipe kernels for bfloat16 operands (om_rule_attention16.cu): whether they take a call, and the call. Pointers to
 // operands and bfloat16 results are to 2-byte elements; `rows` as above with log2 e for the unit.
 bool rule16_fwd_takes(const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
                       const om_head_strides* vs, const float* out, const void* out16, const om_head_strides* os);
 int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
-                   const om_head_strides* vs, float* out, void* out16, const om_head_strides* os, float* lse);
+                   const om_head_strides* vs, float* out, void* out16, const om_head_strides* os, float* lse, const RulePlanes* planes);
 bool rule16_bwd_takes(const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
                       const om_head_strides* ks, const void* v, const om_head_strides* vs, const float* dq, const void* dq16, const om_head_strides* dqs,
                       const float* dk, const void* dk16, const om_head_strides* dks, const float* dv, const void* dv16, const om_head_strides* dvs);
 int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
                    const om_head_strides* ks, const void* v, const om_head_strides* vs, const float* rows, float* dq, void* dq16,
-                   const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs);
+                   const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs,
+                   const RulePlanes* planes);
+// fp32 operands as two planes of halves for the same kernels: whether a call is taken, the planes (freed by rule16_planes_end once
+// what reads them is queued), and whether a result can be written. Where the flag `plain` gets set on the device the kernels leave
+// the call to the fp32 ones, which have to be queued behind them with that flag.
+bool rule16_planes_take(const RuleCall& c, bool backward);
+bool rule16_result_fits(const float* p, const om_head_strides* s);
+int32_t rule16_planes(om_ctx* ctx, const RuleCall& c, const float* q, const om_head_strides* qs, const float* k, const om_head_strides* ks, const float* v,
+                      const om_head_strides* vs, const float* g, const om_head_strides* gs, RulePlanes* out);
+void rule16_planes_end(om_ctx* ctx, RulePlanes* planes);
 
 }  // namespace om

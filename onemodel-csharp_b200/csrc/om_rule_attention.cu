@@ -231,11 +231,14 @@ struct RaParams {
   float *dq, *dk, *dv;
   __nv_bfloat16 *dq16, *dk16, *dv16;
   RaStrides dqs, dks, dvs;
+  const int32_t* plain;           // not NULL: the tensor-pipe kernels in front have done the call unless this is set
+  float unit;                     // of the log-sum-exps in `rows` (log2 e where those kernels read them too)
 };
 
 template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
+  if (p.plain && ld_global(p.plain) == 0) return;
   extern __shared__ __align__(16) float sm[];
   constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *Q = sm, *K = Q + BM * LD, *V = K + BM * LD, *P = V + BM * LD;
@@ -400,7 +403,7 @@ __device__ __forceinline__ void ra_gradients(const RaParams<T>& p, const float* 
       float w = 0.f, ds = 0.f;
       if (i < r.lq && j < r.lk && rule_visible(r, prefix, i, j, r.q_docs ? qdoc[ty * R + a] : 0, r.k_docs ? kdoc[tx + 16 * c] : 0)) {
         float dcap;
-        w = expf(rule_score(r, slope, i, j, s[a][c], &dcap) - row.x);
+        w = expf(rule_score(r, slope, i, j, s[a][c], &dcap) - row.x * p.unit);
         ds = (w * (dp[a][c] - row.y)) * dcap;
       }
       if (P) P[(ty * R + a) * LW + tx + 16 * c] = w;
@@ -412,6 +415,7 @@ __device__ __forceinline__ void ra_gradients(const RaParams<T>& p, const float* 
 template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
+  if (p.plain && ld_global(p.plain) == 0) return;
   extern __shared__ __align__(16) float sm[];
   constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *K = sm, *V = K + BM * LD, *Q = V + BM * LD, *G = Q + BM * LD, *P = G + BM * LD, *S = P + BM * LW;
@@ -457,6 +461,7 @@ rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
 template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
+  if (p.plain && ld_global(p.plain) == 0) return;
   extern __shared__ __align__(16) float sm[];
   constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *Q = sm, *G = Q + BM * LD, *K = G + BM * LD, *V = K + BM * LD, *S = V + BM * LD;
@@ -582,7 +587,7 @@ static int32_t rule_fwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   RuleCall call;
   OM_TRY(rule_begin(ctx, rule, b, h, hkv, lq, lk, d, scale, &call));
   if (sizeof(T) == 2 && rule16_fwd_takes(call, q, qs, k, ks, v, vs, out, out16, os)) {
-    const int32_t st = rule16_fwd(ctx, call, q, qs, k, ks, v, vs, out, out16, os, lse);
+    const int32_t st = rule16_fwd(ctx, call, q, qs, k, ks, v, vs, out, out16, os, lse, nullptr);
     rule_end(ctx, &call);
     return st;
   }
@@ -591,7 +596,15 @@ static int32_t rule_fwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   p.q = q; p.k = k; p.v = v; p.qs = ra_strides(qs); p.ks = ra_strides(ks); p.vs = ra_strides(vs);
   p.vec = d % 4 == 0 && ra_quads(q, qs, sizeof(T)) && ra_quads(k, ks, sizeof(T)) && ra_quads(v, vs, sizeof(T));
   p.out = out; p.out16 = out16; p.os = ra_strides(os); p.lse = lse;
-  const int32_t st = ra_fwd_by_width<T>(ctx, p);
+  RulePlanes planes = {};
+  int32_t st = OM_OK;
+  if (sizeof(T) == 4 && rule16_planes_take(call, false) && rule16_result_fits(out, os)) {
+    st = rule16_planes(ctx, call, (const float*)q, qs, (const float*)k, ks, (const float*)v, vs, nullptr, nullptr, &planes);
+    if (st == OM_OK) st = rule16_fwd(ctx, call, planes.p[0], &planes.q, planes.p[1], &planes.k, planes.p[2], &planes.k, out, nullptr, os, lse, &planes);
+    p.plain = planes.plain;
+  }
+  if (st == OM_OK) st = ra_fwd_by_width<T>(ctx, p);
+  rule16_planes_end(ctx, &planes);
   rule_end(ctx, &call);
   return st;
 }
@@ -634,9 +647,10 @@ static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   int32_t st = pool_alloc(ctx, 2 * sizeof(float) * (size_t)b * h * lq_pad, false, (void**)&rows);
   if (st == OM_OK) {
     const bool tensor = sizeof(T) == 2 && rule16_bwd_takes(call, g, gs, q, qs, k, ks, v, vs, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs);
-    launch_rows<T>(ctx, g, gs, out, os, lse, b, h, lq, d, tensor ? 1.4426950408889634f : 1.f, rows);
+    const bool apart = sizeof(T) == 4 && rule16_planes_take(call, true) && rule16_result_fits(dq, dqs) && rule16_result_fits(dk, dks) && rule16_result_fits(dv, dvs);
+    launch_rows<T>(ctx, g, gs, out, os, lse, b, h, lq, d, tensor || apart ? 1.4426950408889634f : 1.f, rows);
     if (tensor) {
-      st = rule16_bwd(ctx, call, g, gs, q, qs, k, ks, v, vs, rows, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs);
+      st = rule16_bwd(ctx, call, g, gs, q, qs, k, ks, v, vs, rows, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs, nullptr);
       pool_free(ctx, rows);
       rule_end(ctx, &call);
       return st;
@@ -650,7 +664,17 @@ static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* r
     if (dq || dq16) p.dqs = ra_strides(dqs);
     if (dk || dk16) p.dks = ra_strides(dks);
     if (dv || dv16) p.dvs = ra_strides(dvs);
-    st = ra_bwd_by_width<T>(ctx, p);
+    p.unit = apart ? 0.6931471805599453f : 1.f;
+    RulePlanes planes = {};
+    if (apart) {
+      st = rule16_planes(ctx, call, (const float*)q, qs, (const float*)k, ks, (const float*)v, vs, (const float*)g, gs, &planes);
+      if (st == OM_OK)
+        st = rule16_bwd(ctx, call, planes.p[3], &planes.q, planes.p[0], &planes.q, planes.p[1], &planes.k, planes.p[2], &planes.k, rows, dq, nullptr, dqs, dk, nullptr, dks, dv,
+                        nullptr, dvs, &planes);
+      p.plain = planes.plain;
+    }
+    if (st == OM_OK) st = ra_bwd_by_width<T>(ctx, p);
+    rule16_planes_end(ctx, &planes);
     pool_free(ctx, rows);
   }
   rule_end(ctx, &call);

@@ -18,9 +18,16 @@
 // (query tile, key tile) is 128 KB of traffic against 0.3 us of tensor time for the two products that are done again.
 // P and dS are rounded to bfloat16 as operands (the only roundings of the backward besides the results').
 //
+// fp32 operands of heads up to 64 columns run on the same kernels (PL = 2) with fp32 accuracy: every value as two half-precision numbers
+// h + l, 22 significant bits, side by side in a row of 128 columns where two blocks of 64 lie otherwise, and a product as h h' + h l' +
+// l h'. Weights and gradients of scores are taken apart the same way. A power of two per (batch, key head) brings each operand's
+// largest value to 2^14 ... 2^15, so values down to 2^-14 of it keep all 22 bits; rule16_split_kernel, which makes the planes, sets a flag
+// where a row's own largest is smaller than that (or not finite), and then these kernels do nothing and the fp32 ones behind them work.
+//
 // What a CTA sees of the other axis is worked out before its walk, a byte per 128 indices: worked out along the way it cost the rows as
 // much as their exponentials. Every wait is bounded (om_tc.cuh). All sums are fp32 in an order that the shapes alone decide.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <math.h>
 
 #include "om_rule.cuh"
@@ -57,9 +64,9 @@ constexpr uint32_t R16_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
 constexpr uint32_t R16_LBO_K = 1u << 16, R16_LBO_MN = ((uint32_t)R16_CHUNK >> 4) << 16;
 __device__ __forceinline__ uint32_t r16_desc_k(const void* p) { return (smem_u32(p) >> 4) | R16_LBO_K; }
 __device__ __forceinline__ uint32_t r16_desc_mn(const void* p) { return (smem_u32(p) >> 4) | R16_LBO_MN; }
-// kind::f16 with bfloat16 operands and fp32 sums, M = 128.
-__device__ __forceinline__ constexpr uint32_t r16_idesc(bool b_mn, int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(R16_T >> 4) << 24);
+// kind::f16 with bfloat16 (PL = 1) or half-precision operands and fp32 sums, M = 128.
+__device__ __forceinline__ constexpr uint32_t r16_idesc(int pl, bool b_mn, int n) {
+  return (1u << 4) | (pl == 1 ? (1u << 7) | (1u << 10) : 0u) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(R16_T >> 4) << 24);
 }
 __device__ __forceinline__ void r16_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -100,30 +107,93 @@ __device__ __forceinline__ void r16_st16(uint32_t taddr, const uint32_t (&r)[16]
 }
 __device__ __forceinline__ void r16_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Bytes of a tile of 128 rows.
+template <int DP, int PL>
+constexpr int r16_tile_bytes() { return (PL == 2 ? 2 : DP / 64) * R16_CHUNK; }
 // D[128 x 128] = A B^T over the head's columns, both operands K-major in shared memory.
-template <int DP>
+template <int DP, int PL>
 __device__ __forceinline__ void r16_scores(uint32_t d, uint32_t a_k, uint32_t b_k) {
-  constexpr uint32_t idesc = r16_idesc(false, R16_T);
+  constexpr uint32_t idesc = r16_idesc(PL, false, R16_T), CH = R16_CHUNK >> 4;
+  if (PL == 2) {
 #pragma unroll
-  for (int ks = 0; ks < DP / 16; ks++) {
-    const uint32_t o = (uint32_t)(ks / 4) * (R16_CHUNK >> 4) + (uint32_t)(ks % 4) * 2;
-    r16_mma_ss(d, a_k + o, b_k + o, idesc, ks > 0 ? 1u : 0u);
+    for (int ks = 0; ks < 4; ks++) {
+      const uint32_t o = (uint32_t)ks * 2;
+      r16_mma_ss(d, a_k + o, b_k + CH + o, idesc, ks > 0 ? 1u : 0u);
+      r16_mma_ss(d, a_k + CH + o, b_k + o, idesc, 1u);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ks++) r16_mma_ss(d, a_k + (uint32_t)ks * 2, b_k + (uint32_t)ks * 2, idesc, 1u);
+  } else {
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ks++) {
+      const uint32_t o = (uint32_t)(ks / 4) * CH + (uint32_t)(ks % 4) * 2;
+      r16_mma_ss(d, a_k + o, b_k + o, idesc, ks > 0 ? 1u : 0u);
+    }
   }
 }
 // D[128 x DP] (+)= A B over the 128 rows of B: A in tensor memory, B MN-major in shared memory. Where A lies over what it came from, a
 // row thread packs the results of its COLS columns over the first half of them: elements COLS t ... of the contraction are at COLS t.
-template <int DP, int COLS>
+// Two planes fill the place of what they came from, 32 columns at a time: 16 of h, 16 of l.
+template <int DP, int COLS, int PL>
 __device__ __forceinline__ void r16_gather(uint32_t d, uint32_t a, uint32_t b_mn, uint32_t accumulate) {
-  constexpr uint32_t idesc = r16_idesc(true, DP);
-  constexpr int STEPS = COLS / 16;
+  constexpr uint32_t idesc = r16_idesc(PL, true, DP);
+  constexpr int STEPS = (PL == 2 ? 32 : COLS) / 16, STRIDE = PL == 2 ? 32 : COLS;
+  if (PL == 2) {
+    // The small products first: the tensor core cuts off what a sum cannot hold at every addition.
 #pragma unroll
-  for (int ks = 0; ks < R16_T / 16; ks++)
-    r16_mma_ts(d, a + (uint32_t)((ks / STEPS) * COLS + (ks % STEPS) * 8), b_mn + (uint32_t)ks * 128u, idesc, ks > 0 ? 1u : accumulate);
+    for (int ks = 0; ks < R16_T / 16; ks++) {
+      const uint32_t h = a + (uint32_t)((ks / STEPS) * STRIDE + (ks % STEPS) * 8), b = b_mn + (uint32_t)ks * 128u;
+      r16_mma_ts(d, h, b + (R16_CHUNK >> 4), idesc, ks > 0 ? 1u : accumulate);
+      r16_mma_ts(d, h + 16u, b, idesc, 1u);
+    }
+  }
+#pragma unroll
+  for (int ks = 0; ks < R16_T / 16; ks++) {
+    const uint32_t h = a + (uint32_t)((ks / STEPS) * STRIDE + (ks % STEPS) * 8), b = b_mn + (uint32_t)ks * 128u;
+    r16_mma_ts(d, h, b, idesc, PL == 2 || ks > 0 ? 1u : accumulate);
+  }
 }
-template <int DP>
+__device__ __forceinline__ void r16_add_whole(uint32_t whole, uint32_t (&o)[32]) {
+  uint32_t w[32];
+  tmem_ld_32x32b_x32(whole, w);
+  tmem_ld_wait();
+#pragma unroll
+  for (int u = 0; u < 32; u++) o[u] = __float_as_uint(__uint_as_float(w[u]) + __uint_as_float(o[u]));
+}
+// Two planes: the tensor core's own sums over a walk of thousands would lose digits (8 additions that are cut off, a tile, 2e-7; 192
+// of them 5e-6), so each step's product is a sum of its own, which the rows add to the whole in fp32: whole = (whole + step) factor,
+// COLS columns of both in tensor memory.
+template <int COLS>
+__device__ __forceinline__ void r16_fold(uint32_t whole, uint32_t step, bool first, float factor) {
+#pragma unroll 1
+  for (int c = 0; c < COLS; c += 16) {
+    uint32_t a[16], b[16];
+    tmem_ld_32x32b_x16(step + (uint32_t)c, a);
+    if (!first) tmem_ld_32x32b_x16(whole + (uint32_t)c, b);
+    tmem_ld_wait();
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+      const float sum = first ? __uint_as_float(a[u]) : __uint_as_float(b[u]) + __uint_as_float(a[u]);
+      a[u] = __float_as_uint(sum * factor);
+    }
+    r16_st16(whole + (uint32_t)c, a);
+  }
+}
+// 32 results into tensor memory as operands: packed bfloat16, or two planes of halves.
+__device__ __forceinline__ uint32_t r16_pack_half(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void r16_take_apart(float a, float b, uint32_t* h, uint32_t* l) {
+  const __half2 hh = __floats2half2_rn(a, b);
+  const float2 back = __half22float2(hh);
+  *h = *reinterpret_cast<const uint32_t*>(&hh);
+  *l = r16_pack_half(a - back.x, b - back.y);
+}
+template <int DP, int PL>
 __device__ __forceinline__ void r16_load_tile(uint8_t* dst, const CUtensorMap* map, int row0, int head, int batch, uint64_t* bar) {
 #pragma unroll
-  for (int c = 0; c < DP / 64; c++) tma_load_4d(dst + c * R16_CHUNK, map, c * 64, row0, head, batch, bar);
+  for (int c = 0; c < (PL == 2 ? 2 : DP / 64); c++) tma_load_4d(dst + c * R16_CHUNK, map, c * 64, row0, head, batch, bar);
 }
 
 __device__ __forceinline__ void r16_load_rows(float* dst, const float* src, uint64_t* bar) {
@@ -195,11 +265,12 @@ __device__ __forceinline__ float r16_max3(float a, float b, float c) {
 struct R16Score {
   float scale, turns, cap, slope;                        // turns: of the tanh's argument, 2 log2 e scale / cap
 };
+// unit: of the products (1, or the powers of two that the planes were divided by).
 template <int MODE>
-__device__ __forceinline__ R16Score r16_score_of(const RuleArgs& r, int head) {
+__device__ __forceinline__ R16Score r16_score_of(const RuleArgs& r, int head, float unit) {
   R16Score c;
-  c.scale = r.scale * R16_LOG2E;
-  c.turns = 2.f * R16_LOG2E * r.scale * r.inv_softcap;
+  c.scale = r.scale * unit * R16_LOG2E;
+  c.turns = 2.f * R16_LOG2E * r.scale * unit * r.inv_softcap;
   c.cap = r.softcap * R16_LOG2E;
   c.slope = MODE > 0 && r.slopes ? r.slopes[head] * R16_LOG2E : 0.f;
   return c;
@@ -264,6 +335,8 @@ struct R16Fwd {
   float* part;                    // [splits][b * h * lq][d] and [splits][b * h * lq] (maximum, sum) where splits > 1
   float2* part_ml;
   long long rows;                 // b * h * lq
+  const float* units;             // two planes: [4][b * hkv] powers of two that q, k, v, g were divided by, and the flag that they were not
+  const int32_t* plain;
   int32_t* status;
 };
 
@@ -283,22 +356,22 @@ __device__ __forceinline__ int r16_plan(uint16_t* steps, int tiles, int lane, F 
   return n;
 }
 
-template <int DP>
+template <int DP, int PL>
 struct R16FwdShape {
-  static constexpr int TILE = DP / 64 * R16_CHUNK;
-  static constexpr int STAGES = DP == 128 ? 4 : 8;       // of K and V tiles in turn
-  static constexpr bool APART = DP == 64;                // the weights have columns of their own
+  static constexpr int TILE = r16_tile_bytes<DP, PL>();
+  static constexpr int STAGES = TILE > R16_CHUNK ? 4 : 8; // of K and V tiles in turn
+  static constexpr bool APART = DP == 64 && PL == 1;                // the weights have columns of their own
   static constexpr int RULES = (2 + STAGES) * TILE;
   static constexpr int PLAN = RULES + 128;
   static constexpr int BARS = PLAN + R16_PLAN * 2 + 16;
   static constexpr int SMEM = BARS + 512;
 };
 
-template <int DP, int MODE>
+template <int DP, int MODE, int PL>
 __global__ void __launch_bounds__(R16_THREADS, 1)
 rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const __grid_constant__ R16Fwd p) {
-  typedef R16FwdShape<DP> W;
+  typedef R16FwdShape<DP, PL> W;
   // Scores of query tile g at 128 g, weights at 128 g too or at 256 + 64 g, O behind.
   constexpr uint32_t COL_S = 0, COL_P = W::APART ? 256 : 0, P_STEP = W::APART ? 64 : 128, COL_O = W::APART ? 384 : 256, O_STEP = W::APART ? 64 : 128;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -372,15 +445,17 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int walk = (int)steps[R16_PLAN];
 
   bool ok = true;
-  if (warp == R16_ROW_WARPS + 1) {
+  if (PL == 2 && ld_global(p.plain) != 0) {
+    // values beyond what two halves hold: the fp32 kernel behind does the call
+  } else if (warp == R16_ROW_WARPS + 1) {
     if (lane == 0) {
       if (p.packed) {
-        mbar_expect_tx(bar_q, (uint32_t)(DP / 64) * (uint32_t)(group * r.lq) * 128u);
-        r16_load_tile<DP>(slot_q, &map_q, 0, hi, bi, bar_q);
+        mbar_expect_tx(bar_q, (uint32_t)(W::TILE / R16_CHUNK) * (uint32_t)(group * r.lq) * 128u);
+        r16_load_tile<DP, PL>(slot_q, &map_q, 0, hi, bi, bar_q);
       } else {
         mbar_expect_tx(bar_q, (uint32_t)W::TILE * (both ? 2u : 1u));
-        r16_load_tile<DP>(slot_q, &map_q, i0, hi, bi, bar_q);
-        if (both) r16_load_tile<DP>(slot_q + W::TILE, &map_q, i0 + R16_T, hi, bi, bar_q);
+        r16_load_tile<DP, PL>(slot_q, &map_q, i0, hi, bi, bar_q);
+        if (both) r16_load_tile<DP, PL>(slot_q + W::TILE, &map_q, i0 + R16_T, hi, bi, bar_q);
       }
       int s = 0;
       uint32_t phase = 0;
@@ -391,7 +466,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (again) ok = r16_bar(&bar_empty[s], phase ^ 1u, abort_flag, p.status, 61);
           if (!ok) break;
           mbar_expect_tx(&bar_full[s], W::TILE);
-          r16_load_tile<DP>(ring + s * W::TILE, kv ? &map_v : &map_k, (first + r16_tile_of(step)) * R16_T, hk, bi, &bar_full[s]);
+          r16_load_tile<DP, PL>(ring + s * W::TILE, kv ? &map_v : &map_k, (first + r16_tile_of(step)) * R16_T, hk, bi, &bar_full[s]);
           if (++s == W::STAGES) {
             s = 0;
             phase ^= 1u;
@@ -421,7 +496,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (!ok) return;
         }
         tc_fence_after();
-        r16_scores<DP>(tmem + COL_S + 128u * t, r16_desc_k(slot_q + t * W::TILE), r16_desc_k(ring + ks * W::TILE));
+        r16_scores<DP, PL>(tmem + COL_S + 128u * t, r16_desc_k(slot_q + t * W::TILE), r16_desc_k(ring + ks * W::TILE));
         umma_commit(&bar_s[t]);
         scored[t]++;
       };
@@ -429,7 +504,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ok = r16_bar(&bar_p[t], summed[t] & 1u, abort_flag, p.status, 65);
         if (!ok) return;
         tc_fence_after();
-        r16_gather<DP, 128>(tmem + COL_O + O_STEP * t, tmem + COL_P + P_STEP * t, r16_desc_mn(ring + vs * W::TILE), summed[t] > 0 ? 1u : 0u);
+        r16_gather<DP, 128, PL>(tmem + COL_O + O_STEP * t, tmem + COL_P + P_STEP * t, r16_desc_mn(ring + vs * W::TILE), PL == 1 && summed[t] > 0 ? 1u : 0u);
         umma_commit(&bar_o[t]);
         summed[t]++;
       };
@@ -472,12 +547,14 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       i = valid ? row - gi * r.lq : 0;
       head = valid ? hi + gi : hi;
     }
-    const R16Score score = r16_score_of<MODE>(r, head);
+    const int at_unit = bi * p.hkv + hk, n_units = (int)(p.rows / ((long long)p.h * r.lq)) * p.hkv;
+    const float unit = PL == 2 ? p.units[at_unit] * p.units[n_units + at_unit] : 1.f, unit_v = PL == 2 ? p.units[2 * n_units + at_unit] : 1.f;
+    const R16Score score = r16_score_of<MODE>(r, head, unit);
     const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
     const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
     const uint32_t t_s = lane_base + COL_S + 128u * g, t_p = lane_base + COL_P + P_STEP * g, t_o = lane_base + COL_O + O_STEP * g;
-    const float mult = MODE ? 1.f : r.scale * R16_LOG2E;
+    const float mult = MODE ? 1.f : r.scale * unit * R16_LOG2E;
     const uint64_t mult2 = r16_two(mult, mult);
     float m = -INFINITY, l = 0.f;
     uint32_t count = 0;
@@ -526,11 +603,13 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (!(ok = r16_wait(&bar_o[g], (count - 1) & 1u, abort_flag, p.status, 69))) break;
         tc_fence_after();
       }
-      if (__any_sync(0xffffffffu, grown)) {
+      if (PL == 2 || __any_sync(0xffffffffu, grown)) {
         const float shrink = grown ? r16_ex2(m - top) : 1.f;      // m = -inf: 0
         if (grown) m = top;
         l *= shrink;
-        if (count > 0) {
+        if (PL == 2) {
+          if (count > 0) r16_fold<DP>(t_o + 64u, t_o, count == 1, shrink);
+        } else if (count > 0) {
 #pragma unroll 1
           for (int c = 0; c < DP; c += 32) {
             uint32_t o[32];
@@ -542,7 +621,8 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           }
         }
       }
-      const float base = m == -INFINITY ? 0.f : m;
+      // Two planes: weights times 2^7, at most 2^15, so that small ones keep their digits (the row's sum has the same factor).
+      const float base = (m == -INFINITY ? 0.f : m) - (PL == 2 ? 7.f : 0.f);
       const uint64_t base2 = r16_two(-base, -base);
       uint64_t sum[2] = {0ull, 0ull};
       {
@@ -553,7 +633,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         for (int c = 0; c < 4; c++) {
           uint32_t(&v)[32] = x[c & 1];
           if (c < 3) tmem_ld_32x32b_x32(t_s + 32u * (c + 1), x[(c + 1) & 1]);
-          uint32_t w[16];
+          uint32_t w[16], wl[16];
 #pragma unroll
           for (int u = 0; u < 16; u++) {
             float a, b;
@@ -561,11 +641,13 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             a = r16_ex2(a);
             b = r16_ex2(b);
             sum[u & 1] = r16_add2(sum[u & 1], a, b);
-            w[u] = r16_pack(a, b);
+            if (PL == 2) r16_take_apart(a, b, &w[u], &wl[u]);
+            else w[u] = r16_pack(a, b);
           }
           if (c < 3) tmem_ld_wait();                      // what the weights may lie over has been read
           if (W::APART && c == 2) r16_arrive_warp(&bar_read[g], lane);
-          r16_st16(t_p + 16u * c, w);
+          r16_st16(t_p + (PL == 2 ? 32u : 16u) * c, w);
+          if (PL == 2) r16_st16(t_p + 32u * c + 16u, wl);
         }
       }
       const float2 s0 = *reinterpret_cast<const float2*>(&sum[0]), s1 = *reinterpret_cast<const float2*>(&sum[1]);
@@ -578,18 +660,18 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (ok) {
       tc_fence_after();
       const long long at_row = ((long long)bi * p.h + head) * r.lq + i;
-      float inv = l == 0.f ? 0.f : 1.f / l;
+      float inv = l == 0.f ? 0.f : unit_v / l;
       float* out = p.out;
       __nv_bfloat16* out16 = p.out16;
       long long at = bi * p.os.batch + head * p.os.head + (long long)i * p.os.row;
       if (p.splits > 1) {
-        inv = 1.f;
+        inv = unit_v;
         out = p.part;
         out16 = nullptr;
         at = ((long long)split * p.rows + at_row) * p.d;
-        if (valid) p.part_ml[(long long)split * p.rows + at_row] = make_float2(m, l);
+        if (valid) p.part_ml[(long long)split * p.rows + at_row] = make_float2(PL == 2 ? m - 7.f : m, l);
       } else if (p.lse && valid) {
-        p.lse[at_row] = l == 0.f ? -INFINITY : (m + log2f(l)) * R16_LN2;
+        p.lse[at_row] = l == 0.f ? -INFINITY : ((PL == 2 ? m - 7.f : m) + log2f(l)) * R16_LN2;
       }
       if (g == 0 || both) {
 #pragma unroll 1
@@ -600,6 +682,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
             tmem_ld_wait();
           }
+          if (PL == 2 && count > 1) r16_add_whole(t_o + 64u + (uint32_t)c, o);
           if (count == 0 || l == 0.f) {
 #pragma unroll
             for (int u = 0; u < 32; u++) o[u] = 0u;
@@ -621,6 +704,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 __global__ void __launch_bounds__(256)
 rule16_join_kernel(const __grid_constant__ R16Fwd p) {
   pdl_enter();
+  if (p.plain && ld_global(p.plain) != 0) return;
   const int lane = threadIdx.x & 31;
   for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < p.rows; row += (long long)gridDim.x * 8) {
     float m = -INFINITY;
@@ -665,15 +749,18 @@ struct R16Bwd {
   float *d0, *d1;                 // dv and dk, or dq and nothing
   __nv_bfloat16 *d0_16, *d1_16;
   R16Strides s0, s1;
+  const float* units;             // as in R16Fwd
+  int units_n;                    // b * hkv
+  const int32_t* plain;
   int32_t* status;
 };
 
 // Two stationary tiles, a ring of the tiles that two products read, the second one late (Q, or K), and a ring of the others (dO, or V).
 // dQ's kernel has room for a third K at 128 columns; with two, the next scores waited for a load that waited for the product before.
-template <int DP, bool KEYS>
+template <int DP, int PL, bool KEYS>
 struct R16BwdShape {
-  static constexpr int TILE = DP / 64 * R16_CHUNK;
-  static constexpr int RING_A = DP == 64 ? 4 : KEYS ? 2 : 3, RING_B = DP == 64 ? 4 : 2;
+  static constexpr int TILE = r16_tile_bytes<DP, PL>();
+  static constexpr int RING_A = TILE == R16_CHUNK ? 4 : KEYS ? 2 : 3, RING_B = TILE == R16_CHUNK ? 4 : 2;
   static constexpr int ROWS = (2 + RING_A + RING_B) * TILE;     // the queries' log-sum-exps and row dots, 1 KB a stage
   static constexpr int RULES = ROWS + (KEYS ? RING_A * 1024 : 0);
   static constexpr int PLAN = RULES + 64;
@@ -683,8 +770,8 @@ struct R16BwdShape {
 
 // Scores of one row (32 of them, a quarter of a tile) to weights: packed as bfloat16 in w where they are wanted, and in x, times the
 // cap's derivative, for r16_gradients. Rows are keys (COLUMNS: the log-sum-exps go with the columns) or queries.
-template <int MODE, bool COLUMNS>
-__device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)[32], uint32_t (&w)[16], const float* lses, float lse, float far, float mult,
+template <int MODE, bool COLUMNS, int PL>
+__device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)[32], uint32_t (&w)[16], uint32_t (&wl)[16], const float* lses, float lse, float lift, float far, float mult,
                                             bool partial, const R16Row& seen, int at, const int32_t* docs) {
   float dcap[MODE == 2 ? 32 : 1];
   if (MODE) {
@@ -703,18 +790,21 @@ __device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)
     }
 #pragma unroll
     for (int t = 0; t < 4; t += 2) {
-      r16_fma2(p[t], p[t + 1], x[u + t], x[u + t + 1], mult2, r16_two(-e[t], -e[t + 1]));
+      r16_fma2(p[t], p[t + 1], x[u + t], x[u + t + 1], mult2, PL == 2 && COLUMNS ? r16_two(lift - e[t], lift - e[t + 1]) : r16_two(-e[t], -e[t + 1]));
       p[t] = r16_ex2(p[t]);
       p[t + 1] = r16_ex2(p[t + 1]);
-      if (COLUMNS) w[(u + t) / 2] = r16_pack(p[t], p[t + 1]);
+      if (COLUMNS && PL == 2) r16_take_apart(p[t], p[t + 1], &w[(u + t) / 2], &wl[(u + t) / 2]);
+      else if (COLUMNS) w[(u + t) / 2] = r16_pack(p[t], p[t + 1]);
     }
 #pragma unroll
     for (int t = 0; t < 4; t++) x[u + t] = __float_as_uint(MODE == 2 ? p[t] == 0.f ? 0.f : p[t] * dcap[MODE == 2 ? u + t : 0] : p[t]);
   }
 }
 // dS = weight (dP - dot), 32 of them, packed. partial: some are hidden, and 0 whatever dP is there.
-template <bool COLUMNS>
-__device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uint32_t (&dp)[32], uint32_t (&w)[16], const float* dots, float dot, bool partial) {
+// Two planes: dP comes times `down`, the dots times dot_down, and the gradients go into w and wl.
+template <bool COLUMNS, int PL>
+__device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uint32_t (&dp)[32], uint32_t (&w)[16], uint32_t (&wl)[16], const float* dots, float dot,
+                                              float down, float dot_down, bool partial) {
   float v[32];
 #pragma unroll
   for (int u = 0; u < 32; u += 4) {
@@ -724,21 +814,25 @@ __device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uin
       d[0] = f.x; d[1] = f.y; d[2] = f.z; d[3] = f.w;
     }
 #pragma unroll
-    for (int t = 0; t < 4; t++) v[u + t] = __uint_as_float(x[u + t]) * (__uint_as_float(dp[u + t]) - d[t]);
+    for (int t = 0; t < 4; t++)
+      v[u + t] = __uint_as_float(x[u + t]) * (PL == 2 ? fmaf(__uint_as_float(dp[u + t]), down, -(d[t] * dot_down)) : __uint_as_float(dp[u + t]) - d[t]);
   }
   if (partial) {
 #pragma unroll
     for (int u = 0; u < 32; u++) v[u] = x[u] == 0u ? 0.f : v[u];
   }
 #pragma unroll
-  for (int u = 0; u < 32; u += 2) w[u / 2] = r16_pack(v[u], v[u + 1]);
+  for (int u = 0; u < 32; u += 2) {
+    if (PL == 2) r16_take_apart(v[u], v[u + 1], &w[u / 2], &wl[u / 2]);
+    else w[u / 2] = r16_pack(v[u], v[u + 1]);
+  }
 }
 
-template <int DP, int MODE>
+template <int DP, int MODE, int PL>
 __global__ void __launch_bounds__(R16_THREADS, 1)
 rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const __grid_constant__ CUtensorMap map_g, const __grid_constant__ R16Bwd p) {
-  typedef R16BwdShape<DP, true> W;
+  typedef R16BwdShape<DP, PL, true> W;
   constexpr uint32_t COL_S = 0 /* and P over it */, COL_DP = 128 /* and dS */, COL_DV = 256, COL_DK = 384;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *slot_k = smem, *slot_v = smem + W::TILE, *ring_q = smem + 2 * W::TILE, *ring_g = ring_q + W::RING_A * W::TILE;
@@ -805,11 +899,13 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   };
 
   bool ok = true;
-  if (warp == R16_ROW_WARPS + 1) {
+  if (PL == 2 && ld_global(p.plain) != 0) {
+    // values beyond what two halves hold: the fp32 kernel behind does the call
+  } else if (warp == R16_ROW_WARPS + 1) {
     if (lane == 0) {
       mbar_expect_tx(bar_kv, 2 * W::TILE);
-      r16_load_tile<DP>(slot_k, &map_k, j0, hk, bi, bar_kv);
-      r16_load_tile<DP>(slot_v, &map_v, j0, hk, bi, bar_kv);
+      r16_load_tile<DP, PL>(slot_k, &map_k, j0, hk, bi, bar_kv);
+      r16_load_tile<DP, PL>(slot_v, &map_v, j0, hk, bi, bar_kv);
       for (int n = 0; ok && n < walk; n++) {
         const uint32_t step = forth();
         const int a = n % W::RING_A, head = hk * group + gi, at = first + r16_tile_of(step);
@@ -818,12 +914,12 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (n >= W::RING_A) ok = r16_bar(&empty_q[a], before, abort_flag, p.status, 71);
         if (!ok) break;
         mbar_expect_tx(&full_q[a], W::TILE + 1024);
-        r16_load_tile<DP>(ring_q + a * W::TILE, &map_q, at * R16_T, head, bi, &full_q[a]);
+        r16_load_tile<DP, PL>(ring_q + a * W::TILE, &map_q, at * R16_T, head, bi, &full_q[a]);
         r16_load_rows(ring_rows + a * 256, p.rows + (((long long)bi * p.h + head) * p.tiles + at) * 256, &full_q[a]);
         if (n >= W::RING_A) ok = r16_bar(&empty_g[a], before, abort_flag, p.status, 72);
         if (!ok) break;
         mbar_expect_tx(&full_g[a], W::TILE);
-        r16_load_tile<DP>(ring_g + a * W::TILE, &map_g, at * R16_T, head, bi, &full_g[a]);
+        r16_load_tile<DP, PL>(ring_g + a * W::TILE, &map_g, at * R16_T, head, bi, &full_g[a]);
       }
     }
   } else if (warp == R16_ROW_WARPS) {
@@ -834,7 +930,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ok = ok && r16_bar(&full[a], (n / W::RING_A) & 1u, abort_flag, p.status, 74);
         if (!ok) return;
         tc_fence_after();
-        r16_scores<DP>(tmem + col, r16_desc_k(keep), r16_desc_k(ring + a * W::TILE));
+        r16_scores<DP, PL>(tmem + col, r16_desc_k(keep), r16_desc_k(ring + a * W::TILE));
         umma_commit(bar);
       };
       if (ok && walk > 0) {
@@ -848,7 +944,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // dV += P^T dO, then the next scores as soon as it has read P, which lies over these.
         if (!(ok = r16_bar(bar_p, phase, abort_flag, p.status, 76))) break;
         tc_fence_after();
-        r16_gather<DP, 64>(tmem + COL_DV, tmem + COL_S, r16_desc_mn(ring_g + a * W::TILE), n > 0 ? 1u : 0u);
+        r16_gather<DP, 64, PL>(tmem + COL_DV, tmem + COL_S, r16_desc_mn(ring_g + a * W::TILE), PL == 1 && n > 0 ? 1u : 0u);
         umma_commit(bar_dv);
         umma_commit(&empty_g[a]);
         if (more) {
@@ -858,7 +954,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // dK += dS^T Q, then the next dP.
         if (!(ok = ok && r16_bar(bar_ds, phase, abort_flag, p.status, 78))) break;
         tc_fence_after();
-        r16_gather<DP, 64>(tmem + COL_DK, tmem + COL_DP, r16_desc_mn(ring_q + a * W::TILE), n > 0 ? 1u : 0u);
+        r16_gather<DP, 64, PL>(tmem + COL_DK, tmem + COL_DP, r16_desc_mn(ring_q + a * W::TILE), PL == 1 && n > 0 ? 1u : 0u);
         umma_commit(bar_dk);
         umma_commit(&empty_q[a]);
         if (more) {
@@ -875,38 +971,50 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t t_s = lane_base + COL_S + 64u * half, t_dp = lane_base + COL_DP + 64u * half;
     const R16Row seen = r16_key_row(r, prefix, bi, min(j, r.lk - 1));
     const int32_t* docs = r.q_docs ? r.q_docs + (long long)bi * r.lq : nullptr;
-    const float mult = MODE ? 1.f : r.scale * R16_LOG2E;
+    // Units of the planes. Weights are kept times 2^14, gradients of scores over a power of two that is at least 2^-15 of their bound,
+    // 2 max |g| max |v|: both stay below 2^15 whatever the values are, and small ones keep their digits.
+    const int at_unit = bi * p.hkv + hk, n_units = p.units_n;
+    const float unit_q = PL == 2 ? p.units[at_unit] : 1.f, unit_k = PL == 2 ? p.units[n_units + at_unit] : 1.f, unit_v = PL == 2 ? p.units[2 * n_units + at_unit] : 1.f,
+                unit_g = PL == 2 ? p.units[3 * n_units + at_unit] : 1.f, unit = unit_q * unit_k, up = PL == 2 ? p.units[4 * n_units + at_unit] : 1.f;
+    const float lift = PL == 2 ? 14.f : 0.f, dot_down = PL == 2 ? 0x1p-14f / up : 1.f, down = PL == 2 ? dot_down * (unit_g * unit_v) : 1.f;
+    const float mult = MODE ? 1.f : r.scale * unit * R16_LOG2E;
     for (int n = 0; ok && n < walk; n++) {
       const uint32_t step = forth(), phase = n & 1u;
       const int a = n % W::RING_A, at = (first + r16_tile_of(step)) * R16_T + half * 64;
       const bool partial = r16_sees_of(step, 0) == 1;
-      const R16Score score = r16_score_of<MODE>(r, hk * group + gi);
+      const R16Score score = r16_score_of<MODE>(r, hk * group + gi, unit);
       const float* rows = ring_rows + a * 256 + half * 64;
       // The queries' log-sum-exps came with the queries, which the scores have waited for; this wait makes them seen here.
       if (!(ok = r16_wait(&full_q[a], (n / W::RING_A) & 1u, abort_flag, p.status, 94) && r16_wait(bar_s, phase, abort_flag, p.status, 80))) break;
       tc_fence_after();
-      uint32_t x[2][32], w[16];
+      // The scores came after the product before, and the next one waits for these weights.
+      if (PL == 2 && n > 0) r16_fold<32>(lane_base + COL_DV + 64u + 32u * half, lane_base + COL_DV + 32u * half, n == 1, 1.f);
+      uint32_t x[2][32], w[16], wl[16];
       tmem_ld_32x32b_x32(t_s, x[0]);
       tmem_ld_32x32b_x32(t_s + 32u, x[1]);
       tmem_ld_wait();
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        r16_weights<MODE, true>(score, x[c], w, rows + c * 32, 0.f, (float)(at + c * 32 + r.q_offset - j), mult, partial, seen, at + c * 32, docs);
-        r16_st16(t_s + 16u * c, w);
+        r16_weights<MODE, true, PL>(score, x[c], w, wl, rows + c * 32, 0.f, lift, (float)(at + c * 32 + r.q_offset - j), mult, partial, seen, at + c * 32, docs);
+        r16_st16(t_s + (PL == 2 ? 32u : 16u) * c, w);
+        if (PL == 2) r16_st16(t_s + 32u * c + 16u, wl);
       }
       r16_st_wait();
       r16_arrive_warp(bar_p, lane);
       if (!(ok = r16_wait(bar_dp, phase, abort_flag, p.status, 81))) break;
       tc_fence_after();
+      if (PL == 2 && n > 0) r16_fold<32>(lane_base + COL_DK + 64u + 32u * half, lane_base + COL_DK + 32u * half, n == 1, 1.f);
       uint32_t dp[2][32];
       tmem_ld_32x32b_x32(t_dp, dp[0]);
       tmem_ld_wait();
       tmem_ld_32x32b_x32(t_dp + 32u, dp[1]);
-      r16_gradients<true>(x[0], dp[0], w, rows + 128, 0.f, partial);
+      r16_gradients<true, PL>(x[0], dp[0], w, wl, rows + 128, 0.f, down, dot_down, partial);
       tmem_ld_wait();
       r16_st16(t_dp, w);
-      r16_gradients<true>(x[1], dp[1], w, rows + 160, 0.f, partial);
-      r16_st16(t_dp + 16u, w);
+      if (PL == 2) r16_st16(t_dp + 16u, wl);
+      r16_gradients<true, PL>(x[1], dp[1], w, wl, rows + 160, 0.f, down, dot_down, partial);
+      r16_st16(t_dp + (PL == 2 ? 32u : 16u), w);
+      if (PL == 2) r16_st16(t_dp + 48u, wl);
       r16_st_wait();
       r16_arrive_warp(bar_ds, lane);
     }
@@ -925,11 +1033,12 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (walk > 0) {
             tmem_ld_32x32b_x32(lane_base + (half == 0 ? COL_DV : COL_DK) + (uint32_t)c, o);
             tmem_ld_wait();
+            if (PL == 2 && walk > 1) r16_add_whole(lane_base + (half == 0 ? COL_DV : COL_DK) + 64u + (uint32_t)c, o);
           } else {
 #pragma unroll
             for (int u = 0; u < 32; u++) o[u] = 0u;
           }
-          if (j < r.lk) r16_write(o, half == 0 ? 1.f : r.scale, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
+          if (j < r.lk) r16_write(o, half == 0 ? unit_g * (PL == 2 ? 0x1p-14f : 1.f) : r.scale * unit_q * up, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
         }
       }
     }
@@ -942,11 +1051,11 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   }
 }
 
-template <int DP, int MODE>
+template <int DP, int MODE, int PL>
 __global__ void __launch_bounds__(R16_THREADS, 1)
 rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_g, const __grid_constant__ R16Bwd p) {
-  typedef R16BwdShape<DP, false> W;
+  typedef R16BwdShape<DP, PL, false> W;
   constexpr uint32_t COL_S = 0 /* two places, and dS over either */, COL_DP = 256, COL_DQ = 384;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *slot_q = smem, *slot_g = smem + W::TILE, *ring_k = smem + 2 * W::TILE, *ring_v = ring_k + W::RING_A * W::TILE;
@@ -1005,21 +1114,23 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int walk = (int)steps[R16_PLAN];
 
   bool ok = true;
-  if (warp == R16_ROW_WARPS + 1) {
+  if (PL == 2 && ld_global(p.plain) != 0) {
+    // values beyond what two halves hold: the fp32 kernel behind does the call
+  } else if (warp == R16_ROW_WARPS + 1) {
     if (lane == 0) {
       mbar_expect_tx(bar_qg, 2 * W::TILE);
-      r16_load_tile<DP>(slot_q, &map_q, i0, hi, bi, bar_qg);
-      r16_load_tile<DP>(slot_g, &map_g, i0, hi, bi, bar_qg);
+      r16_load_tile<DP, PL>(slot_q, &map_q, i0, hi, bi, bar_qg);
+      r16_load_tile<DP, PL>(slot_g, &map_g, i0, hi, bi, bar_qg);
       for (int n = 0; ok && n < walk; n++) {
         const int a = n % W::RING_A, b = n % W::RING_B, at = (first + r16_tile_of(steps[n])) * R16_T;
         if (n >= W::RING_A) ok = r16_bar(&empty_k[a], ((n / W::RING_A) & 1u) ^ 1u, abort_flag, p.status, 83);
         if (!ok) break;
         mbar_expect_tx(&full_k[a], W::TILE);
-        r16_load_tile<DP>(ring_k + a * W::TILE, &map_k, at, hk, bi, &full_k[a]);
+        r16_load_tile<DP, PL>(ring_k + a * W::TILE, &map_k, at, hk, bi, &full_k[a]);
         if (n >= W::RING_B) ok = r16_bar(&empty_v[b], ((n / W::RING_B) & 1u) ^ 1u, abort_flag, p.status, 84);
         if (!ok) break;
         mbar_expect_tx(&full_v[b], W::TILE);
-        r16_load_tile<DP>(ring_v + b * W::TILE, &map_v, at, hk, bi, &full_v[b]);
+        r16_load_tile<DP, PL>(ring_v + b * W::TILE, &map_v, at, hk, bi, &full_v[b]);
       }
     }
   } else if (warp == R16_ROW_WARPS) {
@@ -1032,13 +1143,13 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         ok = r16_bar(&full_k[a], (n / W::RING_A) & 1u, abort_flag, p.status, 86) && (n < 2 || r16_bar(&bar_dq[place], ((n - 2) >> 1) & 1u, abort_flag, p.status, 87));
         if (!ok) return;
         tc_fence_after();
-        r16_scores<DP>(tmem + COL_S + 128u * place, r16_desc_k(slot_q), r16_desc_k(ring_k + a * W::TILE));
+        r16_scores<DP, PL>(tmem + COL_S + 128u * place, r16_desc_k(slot_q), r16_desc_k(ring_k + a * W::TILE));
         umma_commit(&bar_s[place]);
         // Once the rows have taken the dP before.
         ok = r16_bar(&full_v[b], (n / W::RING_B) & 1u, abort_flag, p.status, 88) && (n < 1 || r16_bar(read_dp, (n - 1) & 1u, abort_flag, p.status, 89));
         if (!ok) return;
         tc_fence_after();
-        r16_scores<DP>(tmem + COL_DP, r16_desc_k(slot_g), r16_desc_k(ring_v + b * W::TILE));
+        r16_scores<DP, PL>(tmem + COL_DP, r16_desc_k(slot_g), r16_desc_k(ring_v + b * W::TILE));
         umma_commit(bar_dp);
         umma_commit(&empty_v[b]);
       };
@@ -1048,7 +1159,7 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (n + 1 < walk) scores(n + 1);
         if (!(ok = ok && r16_bar(&bar_ds[place], (n >> 1) & 1u, abort_flag, p.status, 90))) break;
         tc_fence_after();
-        r16_gather<DP, 64>(tmem + COL_DQ, tmem + COL_S + 128u * place, r16_desc_mn(ring_k + (n % W::RING_A) * W::TILE), n > 0 ? 1u : 0u);
+        r16_gather<DP, 64, PL>(tmem + COL_DQ, tmem + COL_S + 128u * place, r16_desc_mn(ring_k + (n % W::RING_A) * W::TILE), PL == 1 && n > 0 ? 1u : 0u);
         umma_commit(&bar_dq[place]);
         umma_commit(&empty_k[n % W::RING_A]);
       }
@@ -1058,10 +1169,14 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   } else {
     const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane, i = i0 + row;
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), t_dp = lane_base + COL_DP + 64u * half;
-    const R16Score score = r16_score_of<MODE>(r, hi);
+    const int at_unit = bi * p.hkv + hk, n_units = p.units_n;    // as in rule16_dkv_kernel
+    const float unit_q = PL == 2 ? p.units[at_unit] : 1.f, unit_k = PL == 2 ? p.units[n_units + at_unit] : 1.f, unit_v = PL == 2 ? p.units[2 * n_units + at_unit] : 1.f,
+                unit_g = PL == 2 ? p.units[3 * n_units + at_unit] : 1.f, unit = unit_q * unit_k, up = PL == 2 ? p.units[4 * n_units + at_unit] : 1.f;
+    const float dot_down = PL == 2 ? 1.f / up : 1.f, down = PL == 2 ? dot_down * (unit_g * unit_v) : 1.f;
+    const R16Score score = r16_score_of<MODE>(r, hi, unit);
     const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
     const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
-    const float mult = MODE ? 1.f : r.scale * R16_LOG2E;
+    const float mult = MODE ? 1.f : r.scale * unit * R16_LOG2E;
     const float2 stat = rule_row(p.rows, (long long)bi * p.h + hi, r.lq, i);
     for (int n = 0; ok && n < walk; n++) {
       const uint32_t step = steps[n], place = n & 1u, phase = (n >> 1) & 1u, t_s = lane_base + COL_S + 128u * place + 64u * half;
@@ -1069,23 +1184,30 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const bool partial = r16_sees_of(step, 0) == 1;
       if (!(ok = r16_wait(&bar_s[place], phase, abort_flag, p.status, 91))) break;
       tc_fence_after();
-      uint32_t x[2][32], dp[2][32], w[16];
+      uint32_t x[2][32], dp[2][32], w[16], wl[16];
       tmem_ld_32x32b_x32(t_s, x[0]);
       tmem_ld_32x32b_x32(t_s + 32u, x[1]);
       tmem_ld_wait();
 #pragma unroll
       for (int c = 0; c < 2; c++)
-        r16_weights<MODE, false>(score, x[c], w, nullptr, stat.x, (float)(i + r.q_offset - at - c * 32), mult, partial, seen, at + c * 32, docs);
+        r16_weights<MODE, false, PL>(score, x[c], w, wl, nullptr, stat.x, 0.f, (float)(i + r.q_offset - at - c * 32), mult, partial, seen, at + c * 32, docs);
       if (!(ok = r16_wait(bar_dp, n & 1u, abort_flag, p.status, 92))) break;
       tc_fence_after();
+      if (PL == 2 && n > 0) {
+        // The product before; the next one waits for these gradients.
+        if (!(ok = r16_wait(&bar_dq[place ^ 1u], ((n - 1) >> 1) & 1u, abort_flag, p.status, 95))) break;
+        tc_fence_after();
+        r16_fold<32>(lane_base + COL_DQ + 64u + 32u * half, lane_base + COL_DQ + 32u * half, n == 1, 1.f);
+      }
       tmem_ld_32x32b_x32(t_dp, dp[0]);
       tmem_ld_32x32b_x32(t_dp + 32u, dp[1]);
       tmem_ld_wait();
       r16_arrive_warp(read_dp, lane);
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        r16_gradients<false>(x[c], dp[c], w, nullptr, stat.y, partial);
-        r16_st16(t_s + 16u * c, w);
+        r16_gradients<false, PL>(x[c], dp[c], w, wl, nullptr, stat.y, down, dot_down, partial);
+        r16_st16(t_s + (PL == 2 ? 32u : 16u) * c, w);
+        if (PL == 2) r16_st16(t_s + 32u * c + 16u, wl);
       }
       r16_st_wait();
       r16_arrive_warp(&bar_ds[place], lane);
@@ -1101,11 +1223,12 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (walk > 0) {
           tmem_ld_32x32b_x32(lane_base + COL_DQ + (uint32_t)c, o);
           tmem_ld_wait();
+          if (PL == 2 && walk > 1) r16_add_whole(lane_base + COL_DQ + 64u + (uint32_t)c, o);
         } else {
 #pragma unroll
           for (int u = 0; u < 32; u++) o[u] = 0u;
         }
-        if (i < r.lq) r16_write(o, r.scale, p.d0, p.d0_16, bi * p.s0.batch + hi * p.s0.head + (long long)i * p.s0.row + c, c, p.d);
+        if (i < r.lq) r16_write(o, r.scale * unit_k * up, p.d0, p.d0_16, bi * p.s0.batch + hi * p.s0.head + (long long)i * p.s0.row + c, c, p.d);
       }
     }
   }
@@ -1164,27 +1287,32 @@ static int32_t r16_room(om_ctx* ctx, K kernel, int smem) {
   return OM_OK;
 }
 
-template <int DP, int MODE>
+template <int DP, int MODE, int PL>
 static int32_t r16_fwd(om_ctx* ctx, dim3 grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const R16Fwd& p) {
-  OM_TRY(r16_room(ctx, rule16_fwd_kernel<DP, MODE>, R16FwdShape<DP>::SMEM));
-  launch_chained(ctx, rule16_fwd_kernel<DP, MODE>, grid, R16_THREADS, R16FwdShape<DP>::SMEM, mq, mk, mv, p);
+  OM_TRY(r16_room(ctx, rule16_fwd_kernel<DP, MODE, PL>, R16FwdShape<DP, PL>::SMEM));
+  launch_chained(ctx, rule16_fwd_kernel<DP, MODE, PL>, grid, R16_THREADS, R16FwdShape<DP, PL>::SMEM, mq, mk, mv, p);
   return OM_OK;
 }
 
-template <int DP>
+template <int DP, int PL>
 static int32_t r16_fwd_by_mode(om_ctx* ctx, dim3 grid, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const R16Fwd& p) {
-  if (p.r.softcap > 0.f) return r16_fwd<DP, 2>(ctx, grid, mq, mk, mv, p);
-  return p.r.slopes ? r16_fwd<DP, 1>(ctx, grid, mq, mk, mv, p) : r16_fwd<DP, 0>(ctx, grid, mq, mk, mv, p);
+  if (p.r.softcap > 0.f) return r16_fwd<DP, 2, PL>(ctx, grid, mq, mk, mv, p);
+  return p.r.slopes ? r16_fwd<DP, 1, PL>(ctx, grid, mq, mk, mv, p) : r16_fwd<DP, 0, PL>(ctx, grid, mq, mk, mv, p);
 }
 
 int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_strides* qs, const void* k, const om_head_strides* ks, const void* v,
-                   const om_head_strides* vs, float* out, void* out16, const om_head_strides* os, float* lse) {
+                   const om_head_strides* vs, float* out, void* out16, const om_head_strides* os, float* lse, const RulePlanes* planes) {
   const int group = c.h / c.hkv, lq = c.r.lq, lk = c.r.lk;
   R16Fwd p = {};
   p.r = c.r; p.h = c.h; p.hkv = c.hkv; p.d = c.d;
   p.out = out; p.out16 = reinterpret_cast<__nv_bfloat16*>(out16); p.os = r16_strides(os); p.lse = lse;
   p.rows = (long long)c.b * c.h * lq;
   p.status = ctx->status_dev;
+  const int width = planes ? 128 : c.d;                  // columns of the operands: those of two planes are full
+  if (planes) {
+    p.units = planes->units;
+    p.plain = planes->plain;
+  }
   // Heads that share keys as rows of one tile where they fit it: keys and values are read once for all of them.
   p.packed = (long long)group * lq <= R16_T && (group > 1);
   dim3 grid((unsigned)(c.b * (p.packed ? c.hkv : c.h)), p.packed ? 1u : (unsigned)ceil_div(lq, 2 * R16_T), 1);
@@ -1197,9 +1325,9 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
   p.splits = (int)std::max<int64_t>(p.splits, ceil_div(ceil_div(lk, R16_T) + 1, R16_PLAN));   // a part is at most a plan long
   grid.z = (unsigned)p.splits;
   CUtensorMap mq, mk, mv;
-  if (!r16_map(&mq, q, c.d, lq, c.h, c.b, qs, p.packed ? lq : R16_T, p.packed ? group : 1) || !r16_map(&mk, k, c.d, lk, c.hkv, c.b, ks, R16_T, 1) ||
-      !r16_map(&mv, v, c.d, lk, c.hkv, c.b, vs, R16_T, 1))
-    return fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the operands of om_rule_attention_fwd_bf16");
+  if (!r16_map(&mq, q, width, lq, c.h, c.b, qs, p.packed ? lq : R16_T, p.packed ? group : 1) || !r16_map(&mk, k, width, lk, c.hkv, c.b, ks, R16_T, 1) ||
+      !r16_map(&mv, v, width, lk, c.hkv, c.b, vs, R16_T, 1))
+    return fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the operands of om_rule_attention_fwd");
   char* part = nullptr;
   if (p.splits > 1) {
     const size_t ml = ((size_t)p.splits * p.rows * sizeof(float2) + 255) & ~(size_t)255;
@@ -1207,7 +1335,7 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
     p.part_ml = reinterpret_cast<float2*>(part);
     p.part = reinterpret_cast<float*>(part + ml);
   }
-  const int32_t st = c.d <= 64 ? r16_fwd_by_mode<64>(ctx, grid, mq, mk, mv, p) : r16_fwd_by_mode<128>(ctx, grid, mq, mk, mv, p);
+  const int32_t st = planes ? r16_fwd_by_mode<64, 2>(ctx, grid, mq, mk, mv, p) : c.d <= 64 ? r16_fwd_by_mode<64, 1>(ctx, grid, mq, mk, mv, p) : r16_fwd_by_mode<128, 1>(ctx, grid, mq, mk, mv, p);
   if (p.splits > 1) {
     if (st == OM_OK) launch_chained(ctx, rule16_join_kernel, grid_for(ctx, p.rows, 8), 256, 0, p);
     pool_free(ctx, part);
@@ -1217,49 +1345,216 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
   return OM_OK;
 }
 
-template <int DP, int MODE>
+template <int DP, int MODE, int PL>
 static int32_t r16_bwd(om_ctx* ctx, const RuleCall& c, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg,
                        const R16Bwd& kv, const R16Bwd& q) {
   if (kv.d0 || kv.d0_16 || kv.d1 || kv.d1_16) {
-    constexpr int smem = R16BwdShape<DP, true>::SMEM;
-    OM_TRY(r16_room(ctx, rule16_dkv_kernel<DP, MODE>, smem));
-    launch_chained(ctx, rule16_dkv_kernel<DP, MODE>, dim3((unsigned)(c.b * c.hkv), (unsigned)ceil_div(c.r.lk, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, kv);
+    constexpr int smem = R16BwdShape<DP, PL, true>::SMEM;
+    OM_TRY(r16_room(ctx, rule16_dkv_kernel<DP, MODE, PL>, smem));
+    launch_chained(ctx, rule16_dkv_kernel<DP, MODE, PL>, dim3((unsigned)(c.b * c.hkv), (unsigned)ceil_div(c.r.lk, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, kv);
   }
   if (q.d0 || q.d0_16) {
-    constexpr int smem = R16BwdShape<DP, false>::SMEM;
-    OM_TRY(r16_room(ctx, rule16_dq_kernel<DP, MODE>, smem));
-    launch_chained(ctx, rule16_dq_kernel<DP, MODE>, dim3((unsigned)(c.b * c.h), (unsigned)ceil_div(c.r.lq, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, q);
+    constexpr int smem = R16BwdShape<DP, PL, false>::SMEM;
+    OM_TRY(r16_room(ctx, rule16_dq_kernel<DP, MODE, PL>, smem));
+    launch_chained(ctx, rule16_dq_kernel<DP, MODE, PL>, dim3((unsigned)(c.b * c.h), (unsigned)ceil_div(c.r.lq, R16_T)), R16_THREADS, smem, mq, mk, mv, mg, q);
   }
   return OM_OK;
 }
 
-template <int DP>
+template <int DP, int PL>
 static int32_t r16_bwd_by_mode(om_ctx* ctx, const RuleCall& c, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const CUtensorMap& mg,
                                const R16Bwd& kv, const R16Bwd& q) {
-  if (c.r.softcap > 0.f) return r16_bwd<DP, 2>(ctx, c, mq, mk, mv, mg, kv, q);
-  return c.r.slopes ? r16_bwd<DP, 1>(ctx, c, mq, mk, mv, mg, kv, q) : r16_bwd<DP, 0>(ctx, c, mq, mk, mv, mg, kv, q);
+  if (c.r.softcap > 0.f) return r16_bwd<DP, 2, PL>(ctx, c, mq, mk, mv, mg, kv, q);
+  return c.r.slopes ? r16_bwd<DP, 1, PL>(ctx, c, mq, mk, mv, mg, kv, q) : r16_bwd<DP, 0, PL>(ctx, c, mq, mk, mv, mg, kv, q);
 }
 
 int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_strides* gs, const void* q, const om_head_strides* qs, const void* k,
                    const om_head_strides* ks, const void* v, const om_head_strides* vs, const float* rows, float* dq, void* dq16,
-                   const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs) {
-  const int lq = c.r.lq, lk = c.r.lk;
+                   const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs,
+                   const RulePlanes* planes) {
+  const int lq = c.r.lq, lk = c.r.lk, width = planes ? 128 : c.d;
   CUtensorMap mq, mk, mv, mg;
-  if (!r16_map(&mq, q, c.d, lq, c.h, c.b, qs, R16_T, 1) || !r16_map(&mk, k, c.d, lk, c.hkv, c.b, ks, R16_T, 1) ||
-      !r16_map(&mv, v, c.d, lk, c.hkv, c.b, vs, R16_T, 1) || !r16_map(&mg, g, c.d, lq, c.h, c.b, gs, R16_T, 1))
+  if (!r16_map(&mq, q, width, lq, c.h, c.b, qs, R16_T, 1) || !r16_map(&mk, k, width, lk, c.hkv, c.b, ks, R16_T, 1) ||
+      !r16_map(&mv, v, width, lk, c.hkv, c.b, vs, R16_T, 1) || !r16_map(&mg, g, width, lq, c.h, c.b, gs, R16_T, 1))
     return fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the operands of om_rule_attention_bwd_bf16");
   R16Bwd kv = {};
   kv.r = c.r; kv.h = c.h; kv.hkv = c.hkv; kv.d = c.d; kv.rows = rows; kv.tiles = rule_row_tiles(lq); kv.status = ctx->status_dev;
+  if (planes) {
+    kv.units = planes->units;
+    kv.units_n = c.b * c.hkv;
+    kv.plain = planes->plain;
+  }
   R16Bwd one = kv;
   kv.d0 = dv; kv.d1 = dk; kv.d0_16 = reinterpret_cast<__nv_bfloat16*>(dv16); kv.d1_16 = reinterpret_cast<__nv_bfloat16*>(dk16);
   if (dv || dv16) kv.s0 = r16_strides(dvs);
   if (dk || dk16) kv.s1 = r16_strides(dks);
   one.d0 = dq; one.d0_16 = reinterpret_cast<__nv_bfloat16*>(dq16);
   if (dq || dq16) one.s0 = r16_strides(dqs);
-  const int32_t st = c.d <= 64 ? r16_bwd_by_mode<64>(ctx, c, mq, mk, mv, mg, kv, one) : r16_bwd_by_mode<128>(ctx, c, mq, mk, mv, mg, kv, one);
+  const int32_t st = planes ? r16_bwd_by_mode<64, 2>(ctx, c, mq, mk, mv, mg, kv, one)
+                     : c.d <= 64 ? r16_bwd_by_mode<64, 1>(ctx, c, mq, mk, mv, mg, kv, one) : r16_bwd_by_mode<128, 1>(ctx, c, mq, mk, mv, mg, kv, one);
   OM_TRY(st);
   OM_LAUNCH_CHECK(ctx, "om_rule_attention_bwd_bf16");
   return OM_OK;
+}
+
+// ---- two planes -----------------------------------------------------------------------------------------------------------------
+
+struct R16Source {
+  const float* x;                 // [b, heads, l, d] through strides
+  R16Strides s;
+  __half* planes;                 // [b * heads][l][128]: h in columns 0 to 63, l behind, zeros beyond d
+  int heads, l, quads;
+};
+struct R16Split {
+  R16Source t[4];                 // q, k, v, g
+  int d, hkv, b;
+  uint32_t* top;                  // [4][b * hkv] bits of the largest absolute value, then [4][b * hkv] of the largest row's sum of squares
+  float* units;                   // [5][b * hkv]: of q, k, v, g and of the gradients of scores
+  int32_t* plain;
+};
+constexpr int R16_SPLIT_ROWS = 64;
+
+// A CTA has 64 rows of one head of one operand, four threads a row with 16 columns each.
+__device__ __forceinline__ void r16_fetch(const R16Split& p, const R16Source& t, int bh, int row, float (&v)[16]) {
+  const int c0 = (threadIdx.x & 3) * 16, bi = bh / t.heads, hi = bh - bi * t.heads;
+  const float* x = t.x + bi * t.s.batch + hi * t.s.head + (long long)row * t.s.row;
+#pragma unroll
+  for (int c = 0; c < 16; c += 4) {
+    if (row < t.l && t.quads && c0 + c < p.d) {
+      const float4 f = *reinterpret_cast<const float4*>(x + c0 + c);
+      v[c] = f.x; v[c + 1] = f.y; v[c + 2] = f.z; v[c + 3] = f.w;
+    } else {
+#pragma unroll
+      for (int u = 0; u < 4; u++) v[c + u] = row < t.l && c0 + c + u < p.d ? x[c0 + c + u] : 0.f;
+    }
+  }
+}
+__device__ __forceinline__ uint32_t r16_largest(const float (&v)[16]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int u = 0; u < 16; u++) m = max(m, __float_as_uint(v[u]) & 0x7fffffffu);   // of bits: what is not a number counts as the largest
+  return m;
+}
+__global__ void __launch_bounds__(256) rule16_largest_kernel(const __grid_constant__ R16Split p) {
+  pdl_enter();
+  const R16Source& t = p.t[blockIdx.z];
+  const int bh = blockIdx.x, row = blockIdx.y * R16_SPLIT_ROWS + (threadIdx.x >> 2);
+  if (!t.x || bh >= p.b * t.heads || (int)blockIdx.y * R16_SPLIT_ROWS >= t.l) return;
+  float v[16];
+  r16_fetch(p, t, bh, row, v);
+  uint32_t m = __reduce_max_sync(0xffffffffu, r16_largest(v));
+  float squares = 0.f;
+#pragma unroll
+  for (int u = 0; u < 16; u++) squares = fmaf(v[u], v[u], squares);
+  squares += __shfl_xor_sync(0xffffffffu, squares, 1);
+  squares += __shfl_xor_sync(0xffffffffu, squares, 2);
+  uint32_t s = __reduce_max_sync(0xffffffffu, __float_as_uint(squares) & 0x7fffffffu);
+  __shared__ uint32_t all[16];
+  if ((threadIdx.x & 31) == 0) {
+    all[threadIdx.x >> 5] = m;
+    all[8 + (threadIdx.x >> 5)] = s;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; w++) {
+      m = max(m, all[w]);
+      s = max(s, all[8 + w]);
+    }
+    const int bi = bh / t.heads, hk = (bh - bi * t.heads) / (t.heads / p.hkv);
+    const int at = ((int)blockIdx.z * p.b + bi) * p.hkv + hk;
+    atomicMax(&p.top[at], m);                            // whole numbers: the order does not matter
+    atomicMax(&p.top[4 * p.b * p.hkv + at], s);
+  }
+}
+__global__ void __launch_bounds__(256) rule16_split_kernel(const __grid_constant__ R16Split p) {
+  pdl_enter();
+  const R16Source& t = p.t[blockIdx.z];
+  const int bh = blockIdx.x, row = blockIdx.y * R16_SPLIT_ROWS + (threadIdx.x >> 2);
+  if (!t.x || bh >= p.b * t.heads || (int)blockIdx.y * R16_SPLIT_ROWS >= t.l) return;
+  float v[16];
+  r16_fetch(p, t, bh, row, v);
+  const int bi = bh / t.heads, hk = (bh - bi * t.heads) / (t.heads / p.hkv), at = ((int)blockIdx.z * p.b + bi) * p.hkv + hk;
+  const uint32_t top = ld_global(p.top + at);
+  uint32_t mine = r16_largest(v);
+  mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+  mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+  // The largest goes to 2^14 ... 2^15. Units beyond 2^+-60 would leave fp32 in their products.
+  const int e = top == 0 ? 0 : (int)(top >> 23) - 127 - 14;
+  const bool fits = top < 0x7f800000u && e >= -60 && e <= 60;
+  const bool far = mine != 0 && (mine >> 23) + 14 < (top >> 23);
+  if ((threadIdx.x & 3) == 0 && (!fits || far)) *p.plain = 1;
+  const float unit = __uint_as_float((uint32_t)((fits ? e : 0) + 127) << 23), to = __uint_as_float((uint32_t)(127 - (fits ? e : 0)) << 23);
+  if (threadIdx.x == 0) {
+    p.units[at] = unit;
+    if (blockIdx.z == 3) {
+      // |dP - dot| <= 2 max |g| max |v|, over 2^14 and up to the next power of two.
+      const int group = bi * p.hkv + hk, n = p.b * p.hkv;
+      const float bound = sqrtf(__uint_as_float(ld_global(p.top + 6 * n + group))) * sqrtf(__uint_as_float(ld_global(p.top + 7 * n + group)));
+      const int eb = (int)(__float_as_uint(bound) >> 23) + 1 - 13;
+      p.units[4 * n + group] = bound == 0.f ? 1.f : __uint_as_float((uint32_t)min(max(eb, 1), 254) << 23);
+    }
+  }
+  if (row >= t.l) return;
+  uint32_t h[8], l[8];
+#pragma unroll
+  for (int u = 0; u < 8; u++) r16_take_apart(v[2 * u] * to, v[2 * u + 1] * to, &h[u], &l[u]);
+  uint4* out = reinterpret_cast<uint4*>(t.planes + ((long long)bh * t.l + row) * 128 + (threadIdx.x & 3) * 16);
+  out[0] = make_uint4(h[0], h[1], h[2], h[3]);
+  out[1] = make_uint4(h[4], h[5], h[6], h[7]);
+  out[8] = make_uint4(l[0], l[1], l[2], l[3]);
+  out[9] = make_uint4(l[4], l[5], l[6], l[7]);
+}
+
+// fp32 calls that are worth the two passes over the operands in front: from about 2^28 multiplications on (the fp32 kernels take some
+// 60 us for a forward and a backward of that many, the passes and the tensor-pipe kernels' extra launches 20).
+bool rule16_planes_take(const RuleCall& c, bool backward) {
+  const double work = (double)c.b * c.h * c.r.lq * (double)c.r.lk * c.d;
+  return r16_shape(c) && c.d <= 64 && c.r.lk <= R16_PLAN * R16_T && (!backward || c.r.lq <= R16_PLAN * R16_T) && work >= 268435456.0 &&
+         ceil_div(std::max(c.r.lq, c.r.lk), R16_SPLIT_ROWS) <= 65535;
+}
+bool rule16_result_fits(const float* p, const om_head_strides* s) { return p == nullptr || r16_result(p, nullptr, s); }
+
+int32_t rule16_planes(om_ctx* ctx, const RuleCall& c, const float* q, const om_head_strides* qs, const float* k, const om_head_strides* ks, const float* v,
+                      const om_head_strides* vs, const float* g, const om_head_strides* gs, RulePlanes* out) {
+  const size_t nq = (size_t)c.b * c.h * c.r.lq * 128, nk = (size_t)c.b * c.hkv * c.r.lk * 128, units = (size_t)c.b * c.hkv * 4;
+  const size_t head = (8 * units + 4 + 255) & ~(size_t)255, bytes = sizeof(__half) * (nq * (g ? 2 : 1) + 2 * nk);
+  out->small = out->large = nullptr;
+  OM_TRY(pool_alloc(ctx, head, true, &out->small));
+  const int32_t st = pool_alloc(ctx, bytes + sizeof(float) * (units + units / 4), false, &out->large);
+  if (st != OM_OK) {
+    rule16_planes_end(ctx, out);
+    return st;
+  }
+  __half* at = reinterpret_cast<__half*>(out->large);
+  R16Split p = {};
+  p.d = c.d; p.hkv = c.hkv; p.b = c.b;
+  p.top = reinterpret_cast<uint32_t*>(out->small);
+  p.plain = reinterpret_cast<int32_t*>(p.top + 2 * units);
+  auto source = [&](const float* x, const om_head_strides* s, int heads, int l) {
+    R16Source t = {};
+    t.x = x; t.s = r16_strides(s); t.planes = at; t.heads = heads; t.l = l;
+    t.quads = c.d % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && s->row % 4 == 0 && s->head % 4 == 0 && s->batch % 4 == 0;
+    at += (size_t)c.b * heads * l * 128;
+    return t;
+  };
+  p.t[0] = source(q, qs, c.h, c.r.lq);
+  p.t[1] = source(k, ks, c.hkv, c.r.lk);
+  p.t[2] = source(v, vs, c.hkv, c.r.lk);
+  if (g) p.t[3] = source(g, gs, c.h, c.r.lq);
+  p.units = reinterpret_cast<float*>(at);
+  for (int i = 0; i < 4; i++) out->p[i] = p.t[i].planes;
+  out->q = om_head_strides{(int64_t)c.h * c.r.lq * 128, (int64_t)c.r.lq * 128, 128};
+  out->k = om_head_strides{(int64_t)c.hkv * c.r.lk * 128, (int64_t)c.r.lk * 128, 128};
+  out->units = p.units;
+  out->plain = p.plain;
+  const dim3 grid((unsigned)(c.b * c.h), (unsigned)ceil_div(std::max(c.r.lq, c.r.lk), R16_SPLIT_ROWS), g ? 4u : 3u);
+  launch_chained(ctx, rule16_largest_kernel, grid, 256, 0, p);
+  launch_chained(ctx, rule16_split_kernel, grid, 256, 0, p);
+  return OM_OK;
+}
+void rule16_planes_end(om_ctx* ctx, RulePlanes* planes) {
+  if (planes->small) pool_free(ctx, planes->small);
+  if (planes->large) pool_free(ctx, planes->large);
 }
 
 }  // namespace om

@@ -29,9 +29,15 @@ def visible(b, lq, lk, causal=False, window=0, q_offset=0, prefix=None, q_docs=N
     return seen
 
 
-def attention(q, k, v, g, seen, scale, softcap=0.0, slopes=None, q_offset=0, half=False):
+def attention(q, k, v, g, seen, scale, softcap=0.0, slopes=None, q_offset=0, half=False, planes=False):
     """Output, log-sum-exp and gradients of [B, H, L, D] arrays, and how far each may be off: with fp32 arithmetic (half False), or
-    with bfloat16 operands, where every weight, every score gradient, the saved output and each result is rounded once."""
+    with bfloat16 operands, where every weight, every score gradient, the saved output and each result is rounded once.
+
+    planes: fp32 calls that are done with two half-precision numbers a value. Such a pair is within 2^-22 of its value, and the product of
+    two pairs leaves out 2^-22 more, 12 * 2^-24 of a product in all: less than the 4 sqrt(d) * 2^-24 that a sum of d products is allowed
+    here. What the smallest half, 2^-24, adds: 2^-25 (half a step) of a value's unit, where units put the largest operand of a head group at
+    2^14 or more, weights of the forward at 2^7 for the row's largest, weights of the backward at 2^14 for one, and the scores' gradients'
+    bound 2 |g| |v| at 2^14 or more (their largest rows' norms)."""
     q, k, v, g = (np.asarray(a, np.float64) for a in (q, k, v, g))
     (b, h, lq, d), (hk, lk) = q.shape, k.shape[1:3]
     r = {n: np.zeros_like(a) for n, a in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
@@ -72,6 +78,12 @@ def attention(q, k, v, g, seen, scale, softcap=0.0, slopes=None, q_offset=0, hal
             r["dv"][n, j] += p.T @ g[n, i]
             # Relative error of a weight: its score's, the row maximum's share of it, the exponential's and the sum's.
             err = np.where(m, ds_err, 0.0)
+            if planes:
+                mine = slice(j * (h // hk), (j + 1) * (h // hk))
+                top = {x: np.abs(a).max() for x, a in (("q", q[n, mine]), ("k", k[n, j]), ("v", v[n, j]), ("g", g[n, mine]))}
+                norm = {x: np.sqrt((a * a).sum(-1).max()) for x, a in (("v", v[n, j]), ("g", g[n, mine]))}
+                low = 2.0 ** -39
+                err = err + np.where(m, 2 * abs(scale) * low * (np.abs(q[n, i]).sum(1)[:, None] * top["k"] + np.abs(k[n, j]).sum(1)[None, :] * top["q"]), 0.0)
             w = err + err.max(1, keepdims=True) + U32 * (8 + 4 * np.sqrt(lk) + 4 * np.abs(np.where(m, s, 0.0)).max(1, keepdims=True))
             u = U16 if half else 0.0
             pe = p * (w + u)
@@ -83,6 +95,14 @@ def attention(q, k, v, g, seen, scale, softcap=0.0, slopes=None, q_offset=0, hal
             tol["dq"][n, i] = abs(scale) * ze @ np.abs(k[n, j]) + 4 * U32 * np.sqrt(lk) * abs(scale) * np.abs(z) @ np.abs(k[n, j])
             tol["dk"][n, j] += abs(scale) * ze.T @ np.abs(q[n, i]) + 4 * U32 * np.sqrt(lq) * abs(scale) * np.abs(z).T @ np.abs(q[n, i])
             tol["dv"][n, j] += pe.T @ np.abs(g[n, i]) + 4 * U32 * np.sqrt(lq) * p.T @ np.abs(g[n, i])
+            if planes:
+                ds_low = 2.0 ** -38 * norm["g"] * norm["v"]
+                dp_low = 2 * low * (np.abs(g[n, i]).sum(1)[:, None] * top["v"] + np.abs(v[n, j]).sum(1)[None, :] * top["g"])
+                tol["out"][n, i] += 2.0 ** -32 * p.max(1, keepdims=True) * (m @ np.abs(v[n, j])) + low * top["v"]
+                tol["dv"][n, j] += low * (m.T @ np.abs(g[n, i])) + low * top["g"] * p.sum(0)[:, None]
+                ze = p * dp_low + ds_low * m
+                tol["dq"][n, i] += abs(scale) * (ze @ np.abs(k[n, j]) + low * top["k"] * np.abs(z).sum(1)[:, None])
+                tol["dk"][n, j] += abs(scale) * (ze.T @ np.abs(q[n, i]) + low * top["q"] * np.abs(z).sum(0)[:, None])
     for n in ("dq", "dk", "dv"):
         tol[n] += (U16 if half else U32) * np.abs(r[n])
     return r, {n: t + 1e-30 for n, t in tol.items()}

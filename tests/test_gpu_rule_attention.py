@@ -111,11 +111,13 @@ class Call:
         ctx.sync()
         return self
 
-    def check(self, backward=True):
+    def check(self, backward=True, planes=None):
         b, h, hk, lq, lk, d = self.dims
         seen = ref.visible(b, lq, lk, self.causal, self.window, self.q_offset, self.prefix, self.qd, self.kd)
         v = self.value
-        want, tol = ref.attention(v["q"], v["k"], v["v"], v["g"], seen, self.scale, self.softcap, self.slopes, self.q_offset, self.half)
+        if planes is None:
+            planes = not self.half and d <= 64 and b * h * lq * lk * d >= 2 ** 28
+        want, tol = ref.attention(v["q"], v["k"], v["v"], v["g"], seen, self.scale, self.softcap, self.slopes, self.q_offset, self.half, planes)
         names = (("o", "out"),) + ((("dq", "dq"), ("dk", "dk"), ("dv", "dv")) if backward else ())
         for n, full in names:
             got = self.get(n).astype(np.float64)
@@ -178,6 +180,38 @@ def test_widths(ctx, d, half):
 def test_shared_heads_and_layouts(ctx, h, hk, layout, half):
     r = np.random.default_rng(10 * h + hk)
     Call(ctx, r, 2, h, hk, 140, 140, 64, half=half, layout=layout, causal=True, docs=50, padded=5).run().check()
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("mask", ["all", "causal", "cap", "slopes", "everything", "documents-prefix"])
+@pytest.mark.parametrize("layout,d", [("packed", 64), ("heads", 40)])
+def test_calls_large_enough_for_the_tensor_pipe_in_both_precisions(ctx, layout, d, mask, half):
+    r = np.random.default_rng(50 + d)
+    m = dict(MASKS[mask])
+    m.update({k: v * 6 for k, v in m.items() if k in ("window", "docs", "padded")})
+    Call(ctx, r, 2, 8, 4, 750, 750, d, half=half, layout=layout, **m).run().check()
+
+
+def test_large_fp32_call_with_few_queries_and_a_split_walk(ctx):
+    r = np.random.default_rng(60)
+    Call(ctx, r, 2, 8, 2, 30, 20011, 64, causal=True).run(False).check(False)
+
+
+def test_values_far_apart_keep_their_precision(ctx):
+    """One value row 1e20 times the others: the rows that do not see it keep fp32 accuracy, in a call of the size that is otherwise done
+    with two half-precision numbers a value. The same for tiny rows of k and of the output's gradient."""
+    r = np.random.default_rng(61)
+    for name, at, factor in (("v", 700, 1e20), ("k", 3, 1e-9), ("g", 5, 1e-9), ("q", 8, 1e-8)):
+        c = Call(ctx, r, 2, 8, 4, 750, 750, 64, causal=True)
+        c.value[name][:, :, at] *= np.float32(factor)
+        c.dev[name] = c.put(c.value[name].transpose(0, 2, 1, 3))
+        c.run().check(planes=False)
+
+
+def test_more_keys_than_one_plan(ctx):
+    r = np.random.default_rng(62)
+    Call(ctx, r, 1, 2, 1, 2, 140003, 64, half=True, causal=True).run(False).check(False)
+    Call(ctx, r, 1, 1, 1, 3, 131200, 64, half=True, causal=True, window=700).run().check()
 
 
 @pytest.mark.parametrize("half", [False, True])
