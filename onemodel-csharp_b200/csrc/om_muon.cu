@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <algorithm>
 #include <vector>
 
 #include "om_tc.cuh"
@@ -29,6 +30,7 @@ constexpr float MU_A = 3.4445f, MU_B = -4.7750f, MU_C = 2.0315f;   // the quinti
 constexpr int MU_CHUNK = 8192;                                     // elements of one partial sum of squares
 constexpr int MU_BM = 128, MU_BK = 64;                             // rows of a tile of a product, terms of a stage
 constexpr float MU_SX = 1024.f, MU_SG = 4096.f;                    // X is stored times the first, G and Y times the second
+constexpr int MU_WIDE = 2;                                         // wide tiles an SM from which on they are taken
 constexpr int MU_EPI = 8;                                          // warps 0-7: results, half of a tile's columns each four; warp 8: MMA issue; warp 9: TMA
 constexpr int MU_THREADS = 32 * (MU_EPI + 2);
 
@@ -254,42 +256,93 @@ __device__ __forceinline__ void mu_load(void* dst, const CUtensorMap* map, int c
                "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
                : "memory");
 }
-// 32 values of a row of planes, as they lie (from a column that is a multiple of 8; the pitch is one too, so whole groups of 8 lie within
-// it), and their sums.
-struct MuonRow {
+// A warp moves blocks of 32 rows by 32 columns of planes with four lanes a row (64 bytes; a lane a row would touch 32 lines with each
+// access), and turns them to a row a lane through shared memory. Columns start at multiples of 8 and the pitch is one too, so whole
+// groups of 8 lie within it. `e` of the four: row 8 e + lane / 4, columns 8 (lane & 3) ...
+struct MuonBlock {
   uint4 h[4], l[4];
 };
-__device__ __forceinline__ void mu_fetch(const MuonPlanes& x, long long at, int valid, MuonRow& v) {
+__device__ __forceinline__ void mu_fetch(const MuonPlanes& x, int row0, int rows, int col, int cols, int lane, MuonBlock& v) {
 #pragma unroll
-  for (int c = 0; c < 4; c++) {
-    v.h[c] = v.l[c] = make_uint4(0, 0, 0, 0);
-    if (8 * c < valid) {
-      v.h[c] = *reinterpret_cast<const uint4*>(x.p + at + 8 * c);
-      v.l[c] = *reinterpret_cast<const uint4*>(x.p + x.plane + at + 8 * c);
+  for (int e = 0; e < 4; e++) {
+    const int r = row0 + 8 * e + (lane >> 2), c = col + 8 * (lane & 3);
+    v.h[e] = v.l[e] = make_uint4(0, 0, 0, 0);
+    if (r < rows && c < cols) {
+      const __half* at = x.p + (long long)r * x.ld + c;
+      v.h[e] = *reinterpret_cast<const uint4*>(at);
+      v.l[e] = *reinterpret_cast<const uint4*>(at + x.plane);
     }
   }
 }
-__device__ __forceinline__ float mu_value(const MuonRow& v, int u) {
-  return __half2float(reinterpret_cast<const __half*>(v.h)[u]) + __half2float(reinterpret_cast<const __half*>(v.l)[u]);
+constexpr int MU_PITCH = 5;                              // uint4 a row of 32 halves: four and a gap
+__device__ __forceinline__ void mu_to_rows(uint4* stage, int lane, const uint4 (&block)[4], uint4 (&row)[4]) {
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 4; e++) stage[(8 * e + (lane >> 2)) * MU_PITCH + (lane & 3)] = block[e];
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 4; e++) row[e] = stage[lane * MU_PITCH + e];
+}
+__device__ __forceinline__ void mu_put(uint4* stage, int lane, const uint32_t (&row)[16], __half* p, int ld, int row0, int rows, int col, int cols) {
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 4; e++) stage[lane * MU_PITCH + e] = make_uint4(row[4 * e], row[4 * e + 1], row[4 * e + 2], row[4 * e + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const int r = row0 + 8 * e + (lane >> 2), c = col + 8 * (lane & 3);
+    if (r < rows && c < cols) *reinterpret_cast<uint4*>(p + (long long)r * ld + c) = stage[(8 * e + (lane >> 2)) * MU_PITCH + (lane & 3)];
+  }
+}
+__device__ __forceinline__ float mu_value(const uint4 (&h)[4], const uint4 (&l)[4], int u) {
+  return __half2float(reinterpret_cast<const __half*>(h)[u]) + __half2float(reinterpret_cast<const __half*>(l)[u]);
 }
 
+// A tile's results are read back under the next tile's products where its two accumulators fit tensor memory twice.
 template <int BN>
 struct MuonShape {
   static constexpr int PLANE_A = MU_BM * MU_BK * 2, PLANE_B = BN * MU_BK * 2;
-  static constexpr int STAGE = 2 * (PLANE_A + PLANE_B), STAGES = BN == 256 ? 2 : 3;
-  static constexpr int SMEM = STAGES * STAGE + 128 + 1024;
+  static constexpr int STAGE = 2 * (PLANE_A + PLANE_B), STAGES = BN == 256 ? 2 : 3, PLACES = BN == 256 ? 1 : 2;
+  static constexpr int TURN = STAGES * STAGE, BARS = TURN + MU_EPI * 32 * MU_PITCH * 16;
+  static constexpr int SMEM = BARS + 256;
 };
 
-// Blocks of 128 rows by BN columns of one product over every matrix. KIND 0: gram = x x^T; 1: poly = B gram + C gram gram (both
-// symmetric: only what lies on and below the diagonal of blocks of 128, the rest mirrored from there); 2: x2 = A x + poly x.
+// Where item `tile` of a launch lies.
+struct MuonTile {
+  int which, r0, c0;
+};
+template <int KIND, int BN>
+__device__ __forceinline__ MuonTile mu_tile(const MuonList& l, long long tile) {
+  MuonTile m;
+  m.which = mu_find(l, tile, &tile);
+  if (KIND == 2) {
+    const int down = (l.t[m.which].mm + MU_BM - 1) / MU_BM;      // down the rows first: the CTAs of a round share columns of X
+    m.c0 = (int)(tile / down) * BN;
+    m.r0 = (int)(tile % down) * MU_BM;
+  } else {
+    int rb = 0;
+    for (;; rb++) {
+      const int across = ((rb + 1) * MU_BM + BN - 1) / BN;
+      if (tile < across) break;
+      tile -= across;
+    }
+    m.r0 = rb * MU_BM;
+    m.c0 = (int)tile * BN;
+  }
+  return m;
+}
+
+// Blocks of 128 rows by BN columns of one product over every matrix; a CTA takes every gridDim.x-th (one each with the wide tiles, where
+// nothing is gained by staying). KIND 0: gram = x x^T; 1: poly =
+// B gram + C gram gram (both symmetric: only what lies on and below the diagonal of blocks of 128, the rest mirrored from there); 2: x2 =
+// A x + poly x.
 template <int KIND, int BN>
 __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __grid_constant__ MuonList l, const __grid_constant__ MuonMaps maps) {
   typedef MuonShape<BN> W;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::STAGES * W::STAGE);
-  uint64_t *bar_full = bars, *bar_empty = bars + W::STAGES, *bar_done = bars + 2 * W::STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * W::STAGES + 1);
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
+  uint64_t *bar_full = bars, *bar_empty = bars + W::STAGES, *bar_done = bars + 2 * W::STAGES /* [PLACES] */, *bar_read = bar_done + W::PLACES;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_read + W::PLACES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -297,12 +350,15 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
       mbar_init(&bar_full[s], 1);
       mbar_init(&bar_empty[s], 1);
     }
-    mbar_init(bar_done, 1);
+    for (int s = 0; s < W::PLACES; s++) {
+      mbar_init(&bar_done[s], 1);
+      mbar_init(&bar_read[s], MU_EPI);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == MU_EPI) {
-    tmem_alloc(tmem_slot, 2 * BN);
+    tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -312,46 +368,32 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
   pdl_trigger();
   pdl_wait();
 
-  long long tile;
-  const int which = mu_find(l, blockIdx.x, &tile);
-  const MuonTensor& t = l.t[which];
-  const int M = t.mm, N = KIND == 2 ? t.nn : t.mm, K = KIND == 0 ? t.nn : t.mm;
-  int r0, c0;
-  if (KIND == 2) {
-    const int down = (M + MU_BM - 1) / MU_BM;            // down the rows first: the CTAs of a round share columns of X
-    c0 = (int)(tile / down) * BN;
-    r0 = (int)(tile % down) * MU_BM;
-  } else {
-    int rb = 0;
-    for (;; rb++) {
-      const int across = ((rb + 1) * MU_BM + BN - 1) / BN;
-      if (tile < across) break;
-      tile -= across;
-    }
-    r0 = rb * MU_BM;
-    c0 = (int)tile * BN;
-  }
-  const int steps = (K + MU_BK - 1) / MU_BK;
-
+  const long long tiles = l.end[l.count - 1];
+  bool ok = true;
   if (warp == MU_EPI + 1) {
     if (lane == 0) {
-      bool ok = true;
-      for (int k = 0; ok && k < steps; k++) {
-        const int s = k % W::STAGES;
-        if (k >= W::STAGES) ok = mbar_wait(&bar_empty[s], (uint32_t)((k / W::STAGES) & 1) ^ 1u, abort_flag, l.status, 101);
-        if (!ok) break;
-        uint8_t* at = smem + s * W::STAGE;
-        mbar_expect_tx(&bar_full[s], W::STAGE);
+      uint32_t n = 0;                                    // stages filled
+      for (long long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
+        const MuonTile m = mu_tile<KIND, BN>(l, tile);
+        const int steps = ((KIND == 0 ? l.t[m.which].nn : l.t[m.which].mm) + MU_BK - 1) / MU_BK;
+        const CUtensorMap *map_a = &maps.a[m.which], *map_b = KIND == 2 ? &maps.b[m.which] : map_a;
+        for (int k = 0; ok && k < steps; k++, n++) {
+          const uint32_t s = n % W::STAGES;
+          if (n >= W::STAGES) ok = mbar_wait(&bar_empty[s], ((n / W::STAGES) & 1u) ^ 1u, abort_flag, l.status, 101);
+          if (!ok) break;
+          uint8_t* at = smem + s * W::STAGE;
+          mbar_expect_tx(&bar_full[s], W::STAGE);
 #pragma unroll
-        for (int plane = 0; plane < 2; plane++) {
-          mu_load(at + plane * W::PLANE_A, &maps.a[which], k * MU_BK, r0, plane, &bar_full[s]);
-          uint8_t* b = at + 2 * W::PLANE_A + plane * W::PLANE_B;
-          if (KIND == 2) {
+          for (int plane = 0; plane < 2; plane++) {
+            mu_load(at + plane * W::PLANE_A, map_a, k * MU_BK, m.r0, plane, &bar_full[s]);
+            uint8_t* b = at + 2 * W::PLANE_A + plane * W::PLANE_B;
+            if (KIND == 2) {
 #pragma unroll
-            for (int c = 0; c < BN / 64; c++) mu_load(b + c * 64 * 128, &maps.b[which], c0 + c * 64, k * MU_BK, plane, &bar_full[s]);
-          } else {
+              for (int c = 0; c < BN / 64; c++) mu_load(b + c * 64 * 128, map_b, m.c0 + c * 64, k * MU_BK, plane, &bar_full[s]);
+            } else {
 #pragma unroll
-            for (int c = 0; c < BN / 128; c++) mu_load(b + c * 128 * 128, &maps.a[which], k * MU_BK, c0 + c * 128, plane, &bar_full[s]);
+              for (int c = 0; c < BN / 128; c++) mu_load(b + c * 128 * 128, map_b, k * MU_BK, m.c0 + c * 128, plane, &bar_full[s]);
+            }
           }
         }
       }
@@ -361,53 +403,65 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
       // Half-precision operands, fp32 sums; B is K-major (rows of the same matrix) or MN-major (X as it lies).
       constexpr uint32_t idesc = (1u << 4) | ((KIND == 2 ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(MU_BM >> 4) << 24);
       constexpr uint32_t lbo_b = KIND == 2 ? ((64u * 128u) >> 4) << 16 : 1u << 16, step_b = KIND == 2 ? (16u * 128u) >> 4 : 2u;
-      bool ok = true;
-      for (int k = 0; ok && k < steps; k++) {
-        const int s = k % W::STAGES;
-        if (!(ok = mbar_wait(&bar_full[s], (uint32_t)(k / W::STAGES) & 1u, abort_flag, l.status, 102))) break;
-        tc_fence_after();
-        const uint32_t a_h = (smem_u32(smem + s * W::STAGE) >> 4) | 1u << 16, a_l = a_h + (W::PLANE_A >> 4);
-        const uint32_t b_h = (smem_u32(smem + s * W::STAGE + 2 * W::PLANE_A) >> 4) | lbo_b, b_l = b_h + (W::PLANE_B >> 4);
+      uint32_t n = 0, j = 0;                             // stages used, tiles begun
+      for (long long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, j++) {
+        const MuonTensor& t = l.t[mu_tile<KIND, BN>(l, tile).which];
+        const int steps = ((KIND == 0 ? t.nn : t.mm) + MU_BK - 1) / MU_BK;
+        const uint32_t place = j % W::PLACES, acc = tmem + place * 2 * BN;
+        if (j >= W::PLACES && !(ok = mbar_wait(&bar_read[place], ((j / W::PLACES) & 1u) ^ 1u, abort_flag, l.status, 104))) break;
+        for (int k = 0; ok && k < steps; k++, n++) {
+          const uint32_t s = n % W::STAGES;
+          if (!(ok = mbar_wait(&bar_full[s], (n / W::STAGES) & 1u, abort_flag, l.status, 102))) break;
+          tc_fence_after();
+          const uint32_t a_h = (smem_u32(smem + s * W::STAGE) >> 4) | 1u << 16, a_l = a_h + (W::PLANE_A >> 4);
+          const uint32_t b_h = (smem_u32(smem + s * W::STAGE + 2 * W::PLANE_A) >> 4) | lbo_b, b_l = b_h + (W::PLANE_B >> 4);
 #pragma unroll
-        for (int ks = 0; ks < MU_BK / 16; ks++) {
-          const uint32_t ao = ks * 2u, bo = ks * step_b;
-          const uint32_t more = (k > 0 || ks > 0) ? 1u : 0u;
-          mu_mma(tmem, a_h + ao, b_h + bo, idesc, more);
-          mu_mma(tmem + BN, a_h + ao, b_l + bo, idesc, more);
-          mu_mma(tmem + BN, a_l + ao, b_h + bo, idesc, 1u);
+          for (int ks = 0; ks < MU_BK / 16; ks++) {
+            const uint32_t ao = ks * 2u, bo = ks * step_b, more = (k > 0 || ks > 0) ? 1u : 0u;
+            mu_mma(acc, a_h + ao, b_h + bo, idesc, more);
+            mu_mma(acc + BN, a_h + ao, b_l + bo, idesc, more);
+            mu_mma(acc + BN, a_l + ao, b_h + bo, idesc, 1u);
+          }
+          umma_commit(&bar_empty[s]);
         }
-        umma_commit(&bar_empty[s]);
+        if (ok) umma_commit(&bar_done[place]);
       }
-      if (ok) umma_commit(bar_done);
-      else *abort_flag = 1;
+      if (!ok) *abort_flag = 1;
     }
   } else {
-    const int r = r0 + (warp & 3) * 32 + lane, first = (warp >> 2) * (BN / 2);
-    const uint32_t t_acc = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const MuonPlanes& out = KIND == 0 ? t.gram : KIND == 1 ? t.poly : t.x2;
-    const MuonPlanes& in = KIND == 1 ? t.gram : t.x;
-    // What the result adds to is fetched a block of 32 columns ahead, the first one under the products.
-    MuonRow next;
-    if (KIND != 0) mu_fetch(in, (long long)r * in.ld + c0 + first, r < M ? N - (c0 + first) : 0, next);
-    bool ok = true;
-    if (lane == 0) ok = mbar_wait(bar_done, 0, abort_flag, l.status, 103);
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
+    uint32_t j = 0;
+    for (long long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, j++) {
+      const MuonTile m = mu_tile<KIND, BN>(l, tile);
+      const MuonTensor& t = l.t[m.which];
+      const int M = t.mm, N = KIND == 2 ? t.nn : t.mm;
+      const int r = m.r0 + (warp & 3) * 32 + lane, first = (warp >> 2) * (BN / 2);
+      const uint32_t place = j % W::PLACES, t_acc = tmem + place * 2 * BN + ((uint32_t)((warp & 3) * 32) << 16);
+      const MuonPlanes& out = KIND == 0 ? t.gram : KIND == 1 ? t.poly : t.x2;
+      const MuonPlanes& in = KIND == 1 ? t.gram : t.x;
+      // What the result adds to is fetched a block of 32 columns ahead, the first one under the products.
+      const int row0 = m.r0 + (warp & 3) * 32;
+      uint4* stage = reinterpret_cast<uint4*>(smem + W::TURN) + warp * 32 * MU_PITCH;
+      MuonBlock next;
+      if (KIND != 0) mu_fetch(in, row0, M, m.c0 + first, N, lane, next);
+      ok = true;
+      if (lane == 0) ok = mbar_wait(&bar_done[place], (j / W::PLACES) & 1u, abort_flag, l.status, 103);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
       tc_fence_after();
 #pragma unroll 1
       for (int c = first; c < first + BN / 2; c += 32) {
-        const int col = c0 + c;
-        if (col >= N || (KIND != 2 && col >= r0 + MU_BM)) break;   // the same for the whole warp
+        const int col = m.c0 + c;
+        if (col >= N || (KIND != 2 && col >= m.r0 + MU_BM)) break;   // the same for the whole warp
         uint32_t acc[32], small[32];
         __syncwarp();
         tmem_ld_32x32b_x32(t_acc + (uint32_t)c, acc);
         tmem_ld_32x32b_x32(t_acc + (uint32_t)(BN + c), small);
         tmem_ld_wait();
-        const long long at = (long long)r * out.ld + col;
-        MuonRow v;
+        uint4 vh[4], vl[4];
         if (KIND != 0) {
-          v = next;
-          if (c + 32 < first + BN / 2) mu_fetch(in, at + 32, r < M ? N - (col + 32) : 0, next);
+          mu_to_rows(stage, lane, next.h, vh);
+          mu_to_rows(stage, lane, next.l, vl);
+          if (c + 32 < first + BN / 2) mu_fetch(in, row0, M, col + 32, N, lane, next);
         }
         uint32_t hi[16], lo[16];
 #pragma unroll
@@ -416,20 +470,17 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
 #pragma unroll
           for (int e = 0; e < 2; e++) {
             const float x = __uint_as_float(acc[u + e]) + __uint_as_float(small[u + e]);
-            const float y = KIND == 0 ? x * (MU_SG / (MU_SX * MU_SX)) : KIND == 1 ? fmaf(MU_C / MU_SG, x, MU_B * mu_value(v, u + e)) : fmaf(1.f / MU_SG, x, MU_A * mu_value(v, u + e));
+            const float y = KIND == 0 ? x * (MU_SG / (MU_SX * MU_SX))
+                            : KIND == 1 ? fmaf(MU_C / MU_SG, x, MU_B * mu_value(vh, vl, u + e)) : fmaf(1.f / MU_SG, x, MU_A * mu_value(vh, vl, u + e));
             mu_split(y, &h[e], &w[e]);
           }
           hi[u / 2] = (uint32_t)__half_as_ushort(h[0]) | (uint32_t)__half_as_ushort(h[1]) << 16;
           lo[u / 2] = (uint32_t)__half_as_ushort(w[0]) | (uint32_t)__half_as_ushort(w[1]) << 16;
         }
+        mu_put(stage, lane, hi, out.p, out.ld, row0, M, col, N);
+        mu_put(stage, lane, lo, out.p + out.plane, out.ld, row0, M, col, N);
         if (r < M) {
-#pragma unroll
-          for (int u = 0; u < 32; u += 8)
-            if (col + u < N) {                            // the pitch holds whole groups of 8
-              *reinterpret_cast<uint4*>(out.p + at + u) = make_uint4(hi[u / 2], hi[u / 2 + 1], hi[u / 2 + 2], hi[u / 2 + 3]);
-              *reinterpret_cast<uint4*>(out.p + out.plane + at + u) = make_uint4(lo[u / 2], lo[u / 2 + 1], lo[u / 2 + 2], lo[u / 2 + 3]);
-            }
-          if (KIND != 2 && col / MU_BM < r0 / MU_BM) {
+          if (KIND != 2 && col / MU_BM < m.r0 / MU_BM) {
             // Mirrored: the lanes of a warp are adjacent there.
 #pragma unroll
             for (int u = 0; u < 32; u++) {
@@ -441,13 +492,16 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
           }
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_read[place])) : "memory");
     }
   }
   tc_fence_before();
   __syncthreads();
   if (warp == MU_EPI) {
     tc_fence_after();
-    tmem_dealloc(tmem, 2 * BN);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -477,11 +531,11 @@ static int32_t mu_launch(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
     return all;
   });
   OM_CUDA(ctx, cudaFuncSetAttribute(muon_product_kernel<KIND, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, MuonShape<BN>::SMEM));
-  launch_chained(ctx, muon_product_kernel<KIND, BN>, (unsigned)n, MU_THREADS, MuonShape<BN>::SMEM, l, maps);
+  launch_chained(ctx, muon_product_kernel<KIND, BN>, (unsigned)(MuonShape<BN>::PLACES > 1 ? std::min<int64_t>(n, ctx->sm_count) : n), MU_THREADS, MuonShape<BN>::SMEM, l, maps);
   return OM_OK;
 }
-// Tiles of 128 x 256 use a stage's operands for twice the products, and a product of 256 columns is the tensor pipe's full rate; tiles
-// of 128 x 128 where the wider ones would leave SMs without one.
+// Tiles of 128 x 256 where every CTA has two of them at least: a stage's operands serve twice the products, and a product of 256 columns
+// is the tensor pipe's full rate. Else tiles of 128 x 128, more even over the SMs and read back under the next tile's products.
 template <int KIND>
 static int32_t mu_product(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
   int64_t wide = 0;
@@ -489,7 +543,7 @@ static int32_t mu_product(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
     const int64_t rb = ceil_div(l.t[i].mm, MU_BM), nb = ceil_div(KIND == 2 ? l.t[i].nn : l.t[i].mm, 256);
     wide += KIND == 2 ? rb * nb : (rb * nb + rb) / 2;
   }
-  return wide >= ctx->sm_count ? mu_launch<KIND, 256>(ctx, l, maps) : mu_launch<KIND, 128>(ctx, l, maps);
+  return wide >= MU_WIDE * ctx->sm_count ? mu_launch<KIND, 256>(ctx, l, maps) : mu_launch<KIND, 128>(ctx, l, maps);
 }
 
 }  // namespace om
@@ -518,7 +572,11 @@ int32_t om_optim_muon_step(om_ctx* ctx, int32_t n_tensors, float* const* p_host,
     bytes += 20.0 * mm * nn;
   }
   ProfileScope prof(ctx, "om_optim_muon_step", flops, bytes);
-  for (int at = 0; at < n_tensors;) {
+  // The longest sums first, so that no CTA begins one when the others are done (each matrix's result is its own).
+  std::vector<int> order(n_tensors);
+  for (int i = 0; i < n_tensors; i++) order[i] = i;
+  std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return std::max(rows_host[a], cols_host[a]) > std::max(rows_host[b], cols_host[b]); });
+  for (int next = 0; next < n_tensors;) {
     MuonList l = {};
     l.hyper = *hyper_host;
     l.hyper_dev = hyper_dev;
@@ -530,7 +588,8 @@ int32_t om_optim_muon_step(om_ctx* ctx, int32_t n_tensors, float* const* p_host,
       total += (n + 255) & ~(size_t)255;
       return o;
     };
-    for (; at < n_tensors && l.count < MU_TENSORS; at++) {
+    for (; next < n_tensors && l.count < MU_TENSORS; next++) {
+      const int at = order[next];
       if (rows_host[at] == 0 || cols_host[at] == 0) continue;
       MuonTensor& t = l.t[l.count++];
       t.p = p_host[at]; t.g = g_host[at]; t.m = m_host[at]; t.p16 = p16_host ? p16_host[at] : nullptr;
