@@ -558,7 +558,8 @@ int32_t om_attention_bwd_bf16(om_ctx* ctx, const uint16_t* g16, const float* g, 
  *   score(i, j)   = s - slopes[head] * |i + q_offset - j|  with  s = scale q_i . k_j, or softcap * tanh(scale q_i . k_j / softcap)
  * A row that sees no key gives zeros, a log-sum-exp of minus infinity and no gradients. A hidden score is never looked at, but
  * rows of k and v (and of the output's gradient) have to be finite wherever they lie in range: a weight of zero times an
- * infinite value is not a number, here as in the plain product. All pointers are device pointers and may be NULL. */
+ * infinite value is not a number, here as in the plain product. The fp32 entry points take rows of no document for zeros, whatever
+ * they hold. All pointers are device pointers and may be NULL. */
 typedef struct om_attention_rule {
   int32_t causal;
   int32_t window;             /* 0: none; else a positive number of positions */
@@ -571,7 +572,10 @@ typedef struct om_attention_rule {
 } om_attention_rule;
 /* out = softmax(score) v over the visible keys, with h query heads over hkv key heads (h a multiple of hkv: query head i reads
  * key head i / (h / hkv)); stands beside om_attention_fwd_strided, which takes a stored mask and equal heads. Activations are
- * addressed through om_head_strides; d is 1 to 256. Products, sums and exponentials are fp32 whatever the context's flags.
+ * addressed through om_head_strides; d is 1 to 256. Operands, sums and exponentials keep fp32 accuracy whatever the context's flags:
+ * products are fp32, or, where d is a multiple of 8 up to 64 and there are 96 keys (backward: keys or queries) or more, tensor products
+ * of two half-precision numbers a value, 22 bits. Which of the two depends on nothing but sizes, alignment and, for each head of k
+ * and v by itself, on whether its rows are within 2^14 of the largest.
  * lse [b, h, lq] (may be NULL) receives the row log-sum-exp for the backward. lk == 0 gives zeros. */
 int32_t om_rule_attention_fwd(om_ctx* ctx, const om_attention_rule* rule, const float* q, const om_head_strides* qs, const float* k,
                               const om_head_strides* ks, const float* v, const om_head_strides* vs, int32_t b, int32_t h,

@@ -30,7 +30,6 @@ constexpr float MU_A = 3.4445f, MU_B = -4.7750f, MU_C = 2.0315f;   // the quinti
 constexpr int MU_CHUNK = 8192;                                     // elements of one partial sum of squares
 constexpr int MU_BM = 128, MU_BK = 64;                             // rows of a tile of a product, terms of a stage
 constexpr float MU_SX = 1024.f, MU_SG = 4096.f;                    // X is stored times the first, G and Y times the second
-constexpr int MU_WIDE = 2;                                         // wide tiles an SM from which on they are taken
 constexpr int MU_EPI = 8;                                          // warps 0-7: results, half of a tile's columns each four; warp 8: MMA issue; warp 9: TMA
 constexpr int MU_THREADS = 32 * (MU_EPI + 2);
 
@@ -534,8 +533,10 @@ static int32_t mu_launch(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
   launch_chained(ctx, muon_product_kernel<KIND, BN>, (unsigned)(MuonShape<BN>::PLACES > 1 ? std::min<int64_t>(n, ctx->sm_count) : n), MU_THREADS, MuonShape<BN>::SMEM, l, maps);
   return OM_OK;
 }
-// Tiles of 128 x 256 where every CTA has two of them at least: a stage's operands serve twice the products, and a product of 256 columns
-// is the tensor pipe's full rate. Else tiles of 128 x 128, more even over the SMs and read back under the next tile's products.
+// Tiles of 128 x 256 where there are two for every SM: a stage's operands serve twice the products. Else tiles of 128 x 128, more even
+// over the SMs and read back under the next tile's products. One square matrix, five steps, narrow against wide: 1024 260 and 419 us,
+// 2048 (128 wide tiles in Y X) 510 and 681, 2560 (200) 1090 and 1073, 4096 (512) 4041 and 3944, 5120 7988 and 7619. 24 matrices of
+// 384 x 384 to 1536 (240, sums of 384): 338 and 390.
 template <int KIND>
 static int32_t mu_product(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
   int64_t wide = 0;
@@ -543,7 +544,7 @@ static int32_t mu_product(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
     const int64_t rb = ceil_div(l.t[i].mm, MU_BM), nb = ceil_div(KIND == 2 ? l.t[i].nn : l.t[i].mm, 256);
     wide += KIND == 2 ? rb * nb : (rb * nb + rb) / 2;
   }
-  return wide >= MU_WIDE * ctx->sm_count ? mu_launch<KIND, 256>(ctx, l, maps) : mu_launch<KIND, 128>(ctx, l, maps);
+  return wide >= 2 * ctx->sm_count ? mu_launch<KIND, 256>(ctx, l, maps) : mu_launch<KIND, 128>(ctx, l, maps);
 }
 
 }  // namespace om

@@ -172,7 +172,7 @@ struct RulePlanes {
   const void* p[4];               // q, k, v, g
   om_head_strides q, k;           // of q and g, of k and v
   const float* units;
-  const int32_t* plain;
+  const int32_t* plain;           // [b * hkv]
   void *small, *large;
 };
 // The tensor-pipe kernels for bfloat16 operands (om_rule_attention16.cu): whether they take a call, and the call. Pointers to
@@ -189,8 +189,8 @@ int32_t rule16_bwd(om_ctx* ctx, const RuleCall& c, const void* g, const om_head_
                    const om_head_strides* dqs, float* dk, void* dk16, const om_head_strides* dks, float* dv, void* dv16, const om_head_strides* dvs,
                    const RulePlanes* planes);
 // fp32 operands as two planes of halves for the same kernels: whether a call is taken, the planes (freed by rule16_planes_end once
-// what reads them is queued), and whether a result can be written. Where the flag `plain` gets set on the device the kernels leave
-// the call to the fp32 ones, which have to be queued behind them with that flag.
+// what reads them is queued), and whether a result can be written. Where the flag of a head of k and v gets set in `plain` on the device,
+// the kernels leave the heads that share it to the fp32 ones, which have to be queued behind them with the flags.
 bool rule16_planes_take(const RuleCall& c, bool backward);
 bool rule16_result_fits(const float* p, const om_head_strides* s);
 int32_t rule16_planes(om_ctx* ctx, const RuleCall& c, const float* q, const om_head_strides* qs, const float* k, const om_head_strides* ks, const float* v,

@@ -1,5 +1,6 @@
-// Attention by rule, forward and backward, with fp32 products: the exact tier of om_rule_attention_*, and every call with
-// bfloat16 operands that the tensor-pipe kernels do not take (their layout rules are in om_rule_attention16.cu).
+// Attention by rule, forward and backward, with fp32 products: the calls of om_rule_attention_* that the tensor-pipe kernels do not
+// take (short or oddly shaped fp32 calls, heads beyond 64 columns in fp32, fp32 heads whose values lie too far apart for two
+// half-precision numbers, bfloat16 layouts that a tile copy cannot address). The host side of both is here.
 //
 // One pass over the keys with the running maximum and sum of the softmax: a CTA holds a tile of queries and walks the tiles of
 // keys that the rule lets it see, so neither scores nor mask exist in memory. The backward recomputes the weights from the
@@ -119,16 +120,16 @@ struct RaStrides {
 };
 static RaStrides ra_strides(const om_head_strides* s) { return RaStrides{s->batch, s->head, s->row}; }
 
-// A tile of BM rows, zero beyond the tensor's rows and columns, as fp32 with DP + 4 floats a row: rows a quarter apart in the
+// A tile of BM rows, zero beyond the tensor's rows and columns and in rows of no document, as fp32 with DP + 4 floats a row: rows a quarter apart in the
 // banks, so that 16 threads reading 16 rows at one column, 16 bytes each, meet no conflict.
 template <typename T, int BM, int DP>
-__device__ __forceinline__ void ra_load(float* dst, const T* base, long long row_stride, int row0, int rows, int d, bool vec) {
+__device__ __forceinline__ void ra_load(float* dst, const T* base, long long row_stride, int row0, int rows, int d, bool vec, const int32_t* docs) {
   if (vec) {
     constexpr int N = 4;
     for (int e = threadIdx.x; e < BM * (DP / N); e += 256) {
       const int r = e / (DP / N), c = (e % (DP / N)) * N;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (row0 + r < rows && c < d) {
+      if (row0 + r < rows && c < d && !(docs && docs[row0 + r] < 0)) {
         if (sizeof(T) == 4) {
           v = *reinterpret_cast<const float4*>(base + (long long)(row0 + r) * row_stride + c);
         } else {
@@ -141,7 +142,7 @@ __device__ __forceinline__ void ra_load(float* dst, const T* base, long long row
   } else {
     for (int e = threadIdx.x; e < BM * DP; e += 256) {
       const int r = e / DP, c = e % DP;
-      dst[r * (DP + 4) + c] = (row0 + r < rows && c < d) ? ra_value<T>(base[(long long)(row0 + r) * row_stride + c]) : 0.f;
+      dst[r * (DP + 4) + c] = (row0 + r < rows && c < d && !(docs && docs[row0 + r] < 0)) ? ra_value<T>(base[(long long)(row0 + r) * row_stride + c]) : 0.f;
     }
   }
 }
@@ -231,14 +232,14 @@ struct RaParams {
   float *dq, *dk, *dv;
   __nv_bfloat16 *dq16, *dk16, *dv16;
   RaStrides dqs, dks, dvs;
-  const int32_t* plain;           // not NULL: the tensor-pipe kernels in front have done the call unless this is set
+  const int32_t* plain;           // not NULL: [b * hkv], the tensor-pipe kernels in front have done the heads for which this is not set
   float unit;                     // of the log-sum-exps in `rows` (log2 e where those kernels read them too)
 };
 
 template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
-  if (p.plain && ld_global(p.plain) == 0) return;
+  if (p.plain && ld_global(p.plain + blockIdx.y / (p.h / p.hkv)) == 0) return;
   extern __shared__ __align__(16) float sm[];
   constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *Q = sm, *K = Q + BM * LD, *V = K + BM * LD, *P = V + BM * LD;
@@ -248,8 +249,9 @@ rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
   const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * BM;      // the longest rows of a causal mask first
   const int bh = blockIdx.y, bi = bh / p.h, hi = bh - bi * p.h, hk = hi / (p.h / p.hkv);
   const int prefix = r.prefix ? r.prefix[bi] : 0;
+  const int32_t *q_rows = r.q_docs ? r.q_docs + (long long)bi * r.lq : nullptr, *k_rows = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
   const float slope = r.slopes ? r.slopes[hi] : 0.f;
-  ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + hi * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec);
+  ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + hi * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec, q_rows);
   float m[R], l[R], acc[R][RaCols<DP>::N];
   int qdoc[R];
 #pragma unroll
@@ -268,8 +270,8 @@ rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
     // The document ranges go by 64 rows: a tile of 32 asks for the 64 that hold it.
     if (rule_see<false>(tile, j0 / RULE_GRAIN * RULE_GRAIN, 1) == 0) continue;
     __syncthreads();
-    ra_load<T, BM, DP>(K, p.k + bi * p.ks.batch + hk * p.ks.head, p.ks.row, j0, r.lk, p.d, p.vec);
-    ra_load<T, BM, DP>(V, p.v + bi * p.vs.batch + hk * p.vs.head, p.vs.row, j0, r.lk, p.d, p.vec);
+    ra_load<T, BM, DP>(K, p.k + bi * p.ks.batch + hk * p.ks.head, p.ks.row, j0, r.lk, p.d, p.vec, k_rows);
+    ra_load<T, BM, DP>(V, p.v + bi * p.vs.batch + hk * p.vs.head, p.vs.row, j0, r.lk, p.d, p.vec, k_rows);
     if (r.k_docs)
       for (int e = threadIdx.x; e < BM; e += 256) kdoc[e] = j0 + e < r.lk ? r.k_docs[(long long)bi * r.lk + j0 + e] : -1;
     __syncthreads();
@@ -415,7 +417,7 @@ __device__ __forceinline__ void ra_gradients(const RaParams<T>& p, const float* 
 template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
-  if (p.plain && ld_global(p.plain) == 0) return;
+  if (p.plain && ld_global(p.plain + blockIdx.y) == 0) return;
   extern __shared__ __align__(16) float sm[];
   constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *K = sm, *V = K + BM * LD, *Q = V + BM * LD, *G = Q + BM * LD, *P = G + BM * LD, *S = P + BM * LW;
@@ -425,8 +427,9 @@ rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
   const int j0 = (int)blockIdx.x * BM;
   const int bk = blockIdx.y, bi = bk / p.hkv, hk = bk - bi * p.hkv, group = p.h / p.hkv;
   const int prefix = r.prefix ? r.prefix[bi] : 0;
-  ra_load<T, BM, DP>(K, p.k + bi * p.ks.batch + hk * p.ks.head, p.ks.row, j0, r.lk, p.d, p.vec);
-  ra_load<T, BM, DP>(V, p.v + bi * p.vs.batch + hk * p.vs.head, p.vs.row, j0, r.lk, p.d, p.vec);
+  const int32_t *q_rows = r.q_docs ? r.q_docs + (long long)bi * r.lq : nullptr, *k_rows = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
+  ra_load<T, BM, DP>(K, p.k + bi * p.ks.batch + hk * p.ks.head, p.ks.row, j0, r.lk, p.d, p.vec, k_rows);
+  ra_load<T, BM, DP>(V, p.v + bi * p.vs.batch + hk * p.vs.head, p.vs.row, j0, r.lk, p.d, p.vec, k_rows);
   if (r.k_docs)
     for (int e = threadIdx.x; e < BM; e += 256) kdoc[e] = j0 + e < r.lk ? r.k_docs[(long long)bi * r.lk + j0 + e] : -1;
   float dk[R][RaCols<DP>::N], dv[R][RaCols<DP>::N];
@@ -443,8 +446,8 @@ rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
     for (int i0 = lo / BM * BM; i0 < hi; i0 += BM) {
       if (rule_see<false>(tile, i0 / RULE_GRAIN * RULE_GRAIN, 1) == 0) continue;
       __syncthreads();
-      ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + head * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec);
-      ra_load<T, BM, DP>(G, p.g + bi * p.gs.batch + head * p.gs.head, p.gs.row, i0, r.lq, p.d, p.vec);
+      ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + head * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec, q_rows);
+      ra_load<T, BM, DP>(G, p.g + bi * p.gs.batch + head * p.gs.head, p.gs.row, i0, r.lq, p.d, p.vec, q_rows);
       if (r.q_docs)
         for (int e = threadIdx.x; e < BM; e += 256) qdoc[e] = i0 + e < r.lq ? r.q_docs[(long long)bi * r.lq + i0 + e] : -1;
       __syncthreads();
@@ -461,7 +464,7 @@ rule_attention_dkv_kernel(const __grid_constant__ RaParams<T> p) {
 template <typename T, int BM, int DP>
 __global__ void __launch_bounds__(256)
 rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
-  if (p.plain && ld_global(p.plain) == 0) return;
+  if (p.plain && ld_global(p.plain + blockIdx.y / (p.h / p.hkv)) == 0) return;
   extern __shared__ __align__(16) float sm[];
   constexpr int R = BM / 16, LD = DP + 4, LW = BM + 4;
   float *Q = sm, *G = Q + BM * LD, *K = G + BM * LD, *V = K + BM * LD, *S = V + BM * LD;
@@ -471,9 +474,10 @@ rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
   const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * BM;
   const int bh = blockIdx.y, bi = bh / p.h, hi = bh - bi * p.h, hk = hi / (p.h / p.hkv);
   const int prefix = r.prefix ? r.prefix[bi] : 0;
+  const int32_t *q_rows = r.q_docs ? r.q_docs + (long long)bi * r.lq : nullptr, *k_rows = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
   const float slope = r.slopes ? r.slopes[hi] : 0.f;
-  ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + hi * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec);
-  ra_load<T, BM, DP>(G, p.g + bi * p.gs.batch + hi * p.gs.head, p.gs.row, i0, r.lq, p.d, p.vec);
+  ra_load<T, BM, DP>(Q, p.q + bi * p.qs.batch + hi * p.qs.head, p.qs.row, i0, r.lq, p.d, p.vec, q_rows);
+  ra_load<T, BM, DP>(G, p.g + bi * p.gs.batch + hi * p.gs.head, p.gs.row, i0, r.lq, p.d, p.vec, q_rows);
   if (r.q_docs)
     for (int e = threadIdx.x; e < BM; e += 256) qdoc[e] = i0 + e < r.lq ? r.q_docs[(long long)bi * r.lq + i0 + e] : -1;
   float dq[R][RaCols<DP>::N];
@@ -487,8 +491,8 @@ rule_attention_dq_kernel(const __grid_constant__ RaParams<T> p) {
   for (int j0 = first; j0 < last; j0 += BM) {
     if (rule_see<false>(tile, j0 / RULE_GRAIN * RULE_GRAIN, 1) == 0) continue;
     __syncthreads();
-    ra_load<T, BM, DP>(K, p.k + bi * p.ks.batch + hk * p.ks.head, p.ks.row, j0, r.lk, p.d, p.vec);
-    ra_load<T, BM, DP>(V, p.v + bi * p.vs.batch + hk * p.vs.head, p.vs.row, j0, r.lk, p.d, p.vec);
+    ra_load<T, BM, DP>(K, p.k + bi * p.ks.batch + hk * p.ks.head, p.ks.row, j0, r.lk, p.d, p.vec, k_rows);
+    ra_load<T, BM, DP>(V, p.v + bi * p.vs.batch + hk * p.vs.head, p.vs.row, j0, r.lk, p.d, p.vec, k_rows);
     if (r.k_docs)
       for (int e = threadIdx.x; e < BM; e += 256) kdoc[e] = j0 + e < r.lk ? r.k_docs[(long long)bi * r.lk + j0 + e] : -1;
     __syncthreads();

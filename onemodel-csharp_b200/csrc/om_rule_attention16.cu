@@ -445,8 +445,8 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   const int walk = (int)steps[R16_PLAN];
 
   bool ok = true;
-  if (PL == 2 && ld_global(p.plain) != 0) {
-    // values beyond what two halves hold: the fp32 kernel behind does the call
+  if (PL == 2 && ld_global(p.plain + bi * p.hkv + hk) != 0) {
+    // values beyond what two halves hold: the fp32 kernel behind does these heads
   } else if (warp == R16_ROW_WARPS + 1) {
     if (lane == 0) {
       if (p.packed) {
@@ -704,9 +704,11 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 __global__ void __launch_bounds__(256)
 rule16_join_kernel(const __grid_constant__ R16Fwd p) {
   pdl_enter();
-  if (p.plain && ld_global(p.plain) != 0) return;
   const int lane = threadIdx.x & 31;
   for (long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); row < p.rows; row += (long long)gridDim.x * 8) {
+    const long long bh = row / p.r.lq;
+    const int i = (int)(row - bh * p.r.lq), bi = (int)(bh / p.h), hi = (int)(bh - (long long)bi * p.h);
+    if (p.plain && ld_global(p.plain + bi * p.hkv + hi / (p.h / p.hkv)) != 0) continue;
     float m = -INFINITY;
     for (int s = 0; s < p.splits; s++) {
       const float2 v = p.part_ml[s * p.rows + row];
@@ -726,8 +728,6 @@ rule16_join_kernel(const __grid_constant__ R16Fwd p) {
         acc = make_float4(fmaf(o.x, f, acc.x), fmaf(o.y, f, acc.y), fmaf(o.z, f, acc.z), fmaf(o.w, f, acc.w));
       }
     }
-    const long long bh = row / p.r.lq;
-    const int i = (int)(row - bh * p.r.lq), bi = (int)(bh / p.h), hi = (int)(bh - (long long)bi * p.h);
     const float inv = l == 0.f ? 0.f : 1.f / l;
     if (c < p.d) {
       const long long at = bi * p.os.batch + hi * p.os.head + (long long)i * p.os.row + c;
@@ -899,8 +899,8 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   };
 
   bool ok = true;
-  if (PL == 2 && ld_global(p.plain) != 0) {
-    // values beyond what two halves hold: the fp32 kernel behind does the call
+  if (PL == 2 && ld_global(p.plain + bi * p.hkv + hk) != 0) {
+    // values beyond what two halves hold: the fp32 kernel behind does these heads
   } else if (warp == R16_ROW_WARPS + 1) {
     if (lane == 0) {
       mbar_expect_tx(bar_kv, 2 * W::TILE);
@@ -1114,8 +1114,8 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   const int walk = (int)steps[R16_PLAN];
 
   bool ok = true;
-  if (PL == 2 && ld_global(p.plain) != 0) {
-    // values beyond what two halves hold: the fp32 kernel behind does the call
+  if (PL == 2 && ld_global(p.plain + bi * p.hkv + hk) != 0) {
+    // values beyond what two halves hold: the fp32 kernel behind does these heads
   } else if (warp == R16_ROW_WARPS + 1) {
     if (lane == 0) {
       mbar_expect_tx(bar_qg, 2 * W::TILE);
@@ -1404,13 +1404,14 @@ struct R16Source {
   R16Strides s;
   __half* planes;                 // [b * heads][l][128]: h in columns 0 to 63, l behind, zeros beyond d
   int heads, l, quads;
+  const int32_t* docs;            // [b, l] or NULL: rows of no document are taken for zeros, so that what they hold changes nothing
 };
 struct R16Split {
   R16Source t[4];                 // q, k, v, g
   int d, hkv, b;
   uint32_t* top;                  // [4][b * hkv] bits of the largest absolute value, then [4][b * hkv] of the largest row's sum of squares
   float* units;                   // [5][b * hkv]: of q, k, v, g and of the gradients of scores
-  int32_t* plain;
+  int32_t* plain;                 // [b * hkv]
 };
 constexpr int R16_SPLIT_ROWS = 64;
 
@@ -1418,14 +1419,15 @@ constexpr int R16_SPLIT_ROWS = 64;
 __device__ __forceinline__ void r16_fetch(const R16Split& p, const R16Source& t, int bh, int row, float (&v)[16]) {
   const int c0 = (threadIdx.x & 3) * 16, bi = bh / t.heads, hi = bh - bi * t.heads;
   const float* x = t.x + bi * t.s.batch + hi * t.s.head + (long long)row * t.s.row;
+  const bool some = row < t.l && (!t.docs || ld_global(t.docs + (long long)bi * t.l + row) >= 0);
 #pragma unroll
   for (int c = 0; c < 16; c += 4) {
-    if (row < t.l && t.quads && c0 + c < p.d) {
+    if (some && t.quads && c0 + c < p.d) {
       const float4 f = *reinterpret_cast<const float4*>(x + c0 + c);
       v[c] = f.x; v[c + 1] = f.y; v[c + 2] = f.z; v[c + 3] = f.w;
     } else {
 #pragma unroll
-      for (int u = 0; u < 4; u++) v[c + u] = row < t.l && c0 + c + u < p.d ? x[c0 + c + u] : 0.f;
+      for (int u = 0; u < 4; u++) v[c + u] = some && c0 + c + u < p.d ? x[c0 + c + u] : 0.f;
     }
   }
 }
@@ -1482,7 +1484,7 @@ __global__ void __launch_bounds__(256) rule16_split_kernel(const __grid_constant
   const int e = top == 0 ? 0 : (int)(top >> 23) - 127 - 14;
   const bool fits = top < 0x7f800000u && e >= -60 && e <= 60;
   const bool far = mine != 0 && (mine >> 23) + 14 < (top >> 23);
-  if ((threadIdx.x & 3) == 0 && (!fits || far)) *p.plain = 1;
+  if ((threadIdx.x & 3) == 0 && (!fits || far)) p.plain[bi * p.hkv + hk] = 1;
   const float unit = __uint_as_float((uint32_t)((fits ? e : 0) + 127) << 23), to = __uint_as_float((uint32_t)(127 - (fits ? e : 0)) << 23);
   if (threadIdx.x == 0) {
     p.units[at] = unit;
@@ -1505,19 +1507,22 @@ __global__ void __launch_bounds__(256) rule16_split_kernel(const __grid_constant
   out[9] = make_uint4(l[4], l[5], l[6], l[7]);
 }
 
-// fp32 calls that are worth the two passes over the operands in front: from about 2^28 multiplications on (the fp32 kernels take some
-// 60 us for a forward and a backward of that many, the passes and the tensor-pipe kernels' extra launches 20).
+// fp32 calls that are worth the two passes over the operands in front. What decides is the longest walk of a block: the fp32 kernels take
+// 0.2 to 0.4 us for each key or query of it, however little else there is, these a fixed 22 us forward and 55 us both ways and hardly more
+// for a long walk. Forward and backward of 12 heads of 64, fp32 kernels against these: length 64, one batch 58 and 61 us, 64 batches
+// 225 and 266; 96, 16 batches 181 and 114; 128, one batch 120 and 78; 256 163 and 77; 1024 822 and 145. One query to 512 keys 171 and 78.
+// 96 is where both directions together come out even or better with every number of batches and with heads of 8 to 64.
+constexpr int R16_WALK = 96;
 bool rule16_planes_take(const RuleCall& c, bool backward) {
-  const double work = (double)c.b * c.h * c.r.lq * (double)c.r.lk * c.d;
-  return r16_shape(c) && c.d <= 64 && c.r.lk <= R16_PLAN * R16_T && (!backward || c.r.lq <= R16_PLAN * R16_T) && work >= 268435456.0 &&
-         ceil_div(std::max(c.r.lq, c.r.lk), R16_SPLIT_ROWS) <= 65535;
+  return r16_shape(c) && c.d <= 64 && c.r.lk <= R16_PLAN * R16_T && (!backward || c.r.lq <= R16_PLAN * R16_T) &&
+         (backward ? std::max(c.r.lq, c.r.lk) : c.r.lk) >= R16_WALK && ceil_div(std::max(c.r.lq, c.r.lk), R16_SPLIT_ROWS) <= 65535;
 }
 bool rule16_result_fits(const float* p, const om_head_strides* s) { return p == nullptr || r16_result(p, nullptr, s); }
 
 int32_t rule16_planes(om_ctx* ctx, const RuleCall& c, const float* q, const om_head_strides* qs, const float* k, const om_head_strides* ks, const float* v,
                       const om_head_strides* vs, const float* g, const om_head_strides* gs, RulePlanes* out) {
   const size_t nq = (size_t)c.b * c.h * c.r.lq * 128, nk = (size_t)c.b * c.hkv * c.r.lk * 128, units = (size_t)c.b * c.hkv * 4;
-  const size_t head = (8 * units + 4 + 255) & ~(size_t)255, bytes = sizeof(__half) * (nq * (g ? 2 : 1) + 2 * nk);
+  const size_t head = sizeof(uint32_t) * (2 * units + units / 4), bytes = sizeof(__half) * (nq * (g ? 2 : 1) + 2 * nk);
   out->small = out->large = nullptr;
   OM_TRY(pool_alloc(ctx, head, true, &out->small));
   const int32_t st = pool_alloc(ctx, bytes + sizeof(float) * (units + units / 4), false, &out->large);
@@ -1530,17 +1535,17 @@ int32_t rule16_planes(om_ctx* ctx, const RuleCall& c, const float* q, const om_h
   p.d = c.d; p.hkv = c.hkv; p.b = c.b;
   p.top = reinterpret_cast<uint32_t*>(out->small);
   p.plain = reinterpret_cast<int32_t*>(p.top + 2 * units);
-  auto source = [&](const float* x, const om_head_strides* s, int heads, int l) {
+  auto source = [&](const float* x, const om_head_strides* s, int heads, int l, const int32_t* docs) {
     R16Source t = {};
-    t.x = x; t.s = r16_strides(s); t.planes = at; t.heads = heads; t.l = l;
+    t.x = x; t.s = r16_strides(s); t.planes = at; t.heads = heads; t.l = l; t.docs = docs;
     t.quads = c.d % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && s->row % 4 == 0 && s->head % 4 == 0 && s->batch % 4 == 0;
     at += (size_t)c.b * heads * l * 128;
     return t;
   };
-  p.t[0] = source(q, qs, c.h, c.r.lq);
-  p.t[1] = source(k, ks, c.hkv, c.r.lk);
-  p.t[2] = source(v, vs, c.hkv, c.r.lk);
-  if (g) p.t[3] = source(g, gs, c.h, c.r.lq);
+  p.t[0] = source(q, qs, c.h, c.r.lq, c.r.q_docs);
+  p.t[1] = source(k, ks, c.hkv, c.r.lk, c.r.k_docs);
+  p.t[2] = source(v, vs, c.hkv, c.r.lk, c.r.k_docs);
+  if (g) p.t[3] = source(g, gs, c.h, c.r.lq, c.r.q_docs);
   p.units = reinterpret_cast<float*>(at);
   for (int i = 0; i < 4; i++) out->p[i] = p.t[i].planes;
   out->q = om_head_strides{(int64_t)c.h * c.r.lq * 128, (int64_t)c.r.lq * 128, 128};

@@ -94,8 +94,14 @@ class Call:
 
     def run(self, backward=True):
         b, h, hk, lq, lk, d = self.dims
-        ctx, rule = self.ctx, self.rule()
-        self.lse = ctx.empty((b, h, lq))
+        self.the_rule, self.lse = self.rule(), self.ctx.empty((b, h, lq))
+        self.queue(backward)
+        self.ctx.sync()
+        return self
+
+    def queue(self, backward=True):
+        b, h, hk, lq, lk, d = self.dims
+        ctx, rule = self.ctx, self.the_rule
         sizes = [i32(n) for n in self.dims] + [f32(self.scale)]
         w = lambda n: (self.where(n)[0], C.byref(self.where(n)[1]))   # noqa: E731
         o, os = w("o")
@@ -108,15 +114,13 @@ class Call:
                 p, s = w(n)
                 grads += ([None] if self.half else []) + [p, s]
             ctx.call("om_rule_attention_bwd" + ("_bf16" if self.half else ""), ctx.handle, C.byref(rule), *w("g"), *qkv, o, os, self.lse.ptr, *sizes, *grads)
-        ctx.sync()
-        return self
 
     def check(self, backward=True, planes=None):
         b, h, hk, lq, lk, d = self.dims
         seen = ref.visible(b, lq, lk, self.causal, self.window, self.q_offset, self.prefix, self.qd, self.kd)
         v = self.value
         if planes is None:
-            planes = not self.half and d <= 64 and b * h * lq * lk * d >= 2 ** 28
+            planes = not self.half and d <= 64 and d % 8 == 0 and max(lq, lk) >= 96
         want, tol = ref.attention(v["q"], v["k"], v["v"], v["g"], seen, self.scale, self.softcap, self.slopes, self.q_offset, self.half, planes)
         names = (("o", "out"),) + ((("dq", "dq"), ("dk", "dk"), ("dv", "dv")) if backward else ())
         for n, full in names:
@@ -279,6 +283,44 @@ def test_same_bits_twice_and_gradients_one_by_one(ctx):
                      *sizes, *args)
             ctx.sync()
             assert np.array_equal(first[only], c.get(only)), only
+
+
+def test_a_sequence_does_not_depend_on_its_neighbours(ctx):
+    """One sequence of an fp32 batch is made to hold values far apart (another kind of kernel does it): the others keep every bit. So do
+    all when rows of no document are filled with what is not a number."""
+    r = np.random.default_rng(23)
+    c = Call(ctx, r, 3, 4, 2, 200, 200, 64, causal=True, docs=200, padded=0)
+    c.qd[:, 180:] = -1
+    c.kd[:, 180:] = -1
+    first = {n: c.run().get(n).copy() for n in ("o", "dq", "dk", "dv")}
+    for n in ("q", "k", "v", "g"):
+        c.value[n][:, :, 180:] = np.nan
+        c.value[n][1, :, 7] *= np.float32(1e-9)
+        c.dev[n] = c.put(c.value[n].transpose(0, 2, 1, 3))
+    c.run()
+    for n, a in first.items():
+        assert np.array_equal(a[[0, 2]], c.get(n)[[0, 2]]), n
+        assert np.isfinite(c.get(n)).all(), n
+
+
+def test_large_fp32_call_in_a_graph(ctx):
+    """Captured once, replayed over other values: the units and the choice of kernels follow the values, not the capture."""
+    r = np.random.default_rng(24)
+    c = Call(ctx, r, 2, 4, 2, 300, 300, 64, causal=True).run()
+    graph = C.c_void_p()
+    ctx.call("om_graph_begin", ctx.handle)
+    c.queue()
+    ctx.call("om_graph_end", ctx.handle, C.byref(graph))
+    try:
+        for n, factor, planes in (("q", 1.0, True), ("v", 300.0, True), ("k", 1e-12, False)):
+            c.value[n][:, :, 5:9] = (c.value[n][:, :, 5:9] * np.float32(factor)).astype(np.float32)
+            host = np.ascontiguousarray(c.value[n].transpose(0, 2, 1, 3))
+            ctx.call("om_memcpy_h2d", ctx.handle, c.dev[n].ptr, host.ctypes.data_as(C.c_void_p), C.c_size_t(host.nbytes))
+            ctx.call("om_graph_launch", ctx.handle, graph)
+            ctx.sync()
+            c.check(planes=planes)
+    finally:
+        ctx.call("om_graph_destroy", ctx.handle, graph)
 
 
 def test_both_forms_of_a_result(ctx):
