@@ -328,11 +328,13 @@ struct R16Fwd {
   int h, hkv, d;
   int packed;                     // rows of a tile are (head of the group, query): h / hkv * lq of them
   int splits;
+  int twin;                       // one row tile a CTA: its two groups of row warps take steps in turn and leave a part each
+  int parts;                      // 1, or what rule16_join_kernel joins: splits, or twice that
   float* out;
   __nv_bfloat16* out16;
   R16Strides os;
   float* lse;
-  float* part;                    // [splits][b * h * lq][d] and [splits][b * h * lq] (maximum, sum) where splits > 1
+  float* part;                    // [parts][b * h * lq][d] and [parts][b * h * lq] (maximum, sum) where parts > 1
   float2* part_ml;
   long long rows;                 // b * h * lq
   const float* units;             // two planes: [4][b * hkv] powers of two that q, k, v, g were divided by, and the flag that they were not
@@ -341,16 +343,18 @@ struct R16Fwd {
 };
 
 // A CTA's plan: the tiles of 128 of the other axis that some row tile sees anything of, in order, with rule_see's answer for each row
-// tile (two bits, from bit 10 on). Made by one warp; returns their number.
+// tile (two bits, from bit 10 on). Made by one warp; returns their number. twin: the rows of both row tiles are the same, and the
+// steps fall to the two in turn.
 __device__ __forceinline__ int r16_tile_of(uint32_t step) { return (int)(step & (R16_PLAN - 1)); }
 __device__ __forceinline__ int r16_sees_of(uint32_t step, int tile) { return (int)(step >> (10 + 2 * tile)) & 3; }
 template <typename F>
-__device__ __forceinline__ int r16_plan(uint16_t* steps, int tiles, int lane, F see) {
+__device__ __forceinline__ int r16_plan(uint16_t* steps, int tiles, int lane, bool twin, F see) {
   int n = 0;
   for (int t0 = 0; t0 < tiles; t0 += 32) {
     const int t = t0 + lane;
     const uint32_t a = t < tiles ? see(t) : 0u, some = __ballot_sync(0xffffffffu, a != 0);
-    if (a) steps[n + __popc(some & ((1u << lane) - 1u))] = (uint16_t)((uint32_t)t | a << 10);
+    const int at = n + __popc(some & ((1u << lane) - 1u));
+    if (a) steps[at] = (uint16_t)((uint32_t)t | a << (twin && (at & 1) ? 12 : 10));
     n += __popc(some);
   }
   return n;
@@ -436,8 +440,8 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   last = min(first + per, last);
   __syncthreads();
   if (warp == 0) {
-    const int n = r16_plan(steps, last - first, lane, [&](int t) {
-      return (uint32_t)(rule_see<true>(tiles[0], (first + t) * R16_T, 2) | rule_see<true>(tiles[1], (first + t) * R16_T, 2) << 2);
+    const int n = r16_plan(steps, last - first, lane, p.twin, [&](int t) {
+      return (uint32_t)(rule_see<true>(tiles[0], (first + t) * R16_T, 2) | (p.twin ? 0 : rule_see<true>(tiles[1], (first + t) * R16_T, 2) << 2));
     });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
@@ -496,7 +500,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (!ok) return;
         }
         tc_fence_after();
-        r16_scores<DP, PL>(tmem + COL_S + 128u * t, r16_desc_k(slot_q + t * W::TILE), r16_desc_k(ring + ks * W::TILE));
+        r16_scores<DP, PL>(tmem + COL_S + 128u * t, r16_desc_k(slot_q + (p.twin ? 0 : t) * W::TILE), r16_desc_k(ring + ks * W::TILE));
         umma_commit(&bar_s[t]);
         scored[t]++;
       };
@@ -519,7 +523,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const bool more = n + 1 < walk;
         const uint32_t ahead = more ? steps[n + 1] : 0u;
         const int vs = take(), ks = more ? take() : 0;
-        if (W::APART) {
+        if (W::APART || p.twin) {                         // twins: the step ahead is the other group's, so nothing of this one is in its way
           if (ok && r16_sees_of(ahead, 0)) scores(0, ks);
           if (ok && r16_sees_of(ahead, 1)) scores(1, ks);
           if (ok && r16_sees_of(step, 0)) product(0, vs);
@@ -539,11 +543,11 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
   } else {
     const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
-    int i = i0 + g * R16_T + row, head = hi;
+    int i = i0 + (p.twin ? 0 : g * R16_T) + row, head = hi;
     bool valid = i < r.lq;
     if (p.packed) {
       const int gi = row / r.lq;
-      valid = g == 0 && gi < group;
+      valid = (g == 0 || p.twin) && gi < group;
       i = valid ? row - gi * r.lq : 0;
       head = valid ? hi + gi : hi;
     }
@@ -664,16 +668,17 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       float* out = p.out;
       __nv_bfloat16* out16 = p.out16;
       long long at = bi * p.os.batch + head * p.os.head + (long long)i * p.os.row;
-      if (p.splits > 1) {
+      if (p.parts > 1) {
+        const int part = p.twin ? 2 * split + g : split;
         inv = unit_v;
         out = p.part;
         out16 = nullptr;
-        at = ((long long)split * p.rows + at_row) * p.d;
-        if (valid) p.part_ml[(long long)split * p.rows + at_row] = make_float2(PL == 2 ? m - 7.f : m, l);
+        at = ((long long)part * p.rows + at_row) * p.d;
+        if (valid) p.part_ml[(long long)part * p.rows + at_row] = make_float2(PL == 2 ? m - 7.f : m, l);
       } else if (p.lse && valid) {
         p.lse[at_row] = l == 0.f ? -INFINITY : ((PL == 2 ? m - 7.f : m) + log2f(l)) * R16_LN2;
       }
-      if (g == 0 || both) {
+      if (g == 0 || both || p.twin) {
 #pragma unroll 1
         for (int c = 0; c < DP; c += 32) {
           uint32_t o[32];
@@ -700,7 +705,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   }
 }
 
-// The parts of split walks: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s in increasing order of the splits. A warp per row.
+// The parts of split walks: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s in increasing order of the parts. A warp per row.
 __global__ void __launch_bounds__(256)
 rule16_join_kernel(const __grid_constant__ R16Fwd p) {
   pdl_enter();
@@ -710,7 +715,7 @@ rule16_join_kernel(const __grid_constant__ R16Fwd p) {
     const int i = (int)(row - bh * p.r.lq), bi = (int)(bh / p.h), hi = (int)(bh - (long long)bi * p.h);
     if (p.plain && ld_global(p.plain + bi * p.hkv + hi / (p.h / p.hkv)) != 0) continue;
     float m = -INFINITY;
-    for (int s = 0; s < p.splits; s++) {
+    for (int s = 0; s < p.parts; s++) {
       const float2 v = p.part_ml[s * p.rows + row];
       if (v.y != 0.f) m = fmaxf(m, v.x);
     }
@@ -718,7 +723,7 @@ rule16_join_kernel(const __grid_constant__ R16Fwd p) {
     float l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     const int c = lane * 4;
-    for (int s = 0; s < p.splits; s++) {
+    for (int s = 0; s < p.parts; s++) {
       const float2 v = p.part_ml[s * p.rows + row];
       if (v.y == 0.f) continue;                       // this part saw nothing
       const float f = r16_ex2(v.x - base);
@@ -883,7 +888,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   __syncthreads();
   const int first = tile->lo / R16_T, tiles = max(0, (min(tile->hi, r.lq) + R16_T - 1) / R16_T - first);
   if (warp == 0) {
-    const int n = r16_plan(steps, tiles, lane, [&](int t) { return (uint32_t)rule_see<false>(*tile, (first + t) * R16_T, 2); });
+    const int n = r16_plan(steps, tiles, lane, false, [&](int t) { return (uint32_t)rule_see<false>(*tile, (first + t) * R16_T, 2); });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
@@ -1107,7 +1112,7 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __syncthreads();
   const int first = tile->pre > 0 ? 0 : tile->lo / R16_T, tiles = max(0, (min(max(tile->pre, tile->hi), r.lk) + R16_T - 1) / R16_T - first);
   if (warp == 0) {
-    const int n = r16_plan(steps, tiles, lane, [&](int t) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T, 2); });
+    const int n = r16_plan(steps, tiles, lane, false, [&](int t) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T, 2); });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
@@ -1324,19 +1329,21 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count / std::max<int64_t>(ctas, 1), tiles / 4));
   p.splits = (int)std::max<int64_t>(p.splits, ceil_div(ceil_div(lk, R16_T) + 1, R16_PLAN));   // a part is at most a plan long
   grid.z = (unsigned)p.splits;
+  p.twin = (p.packed || lq <= R16_T) && (p.splits > 1 || tiles >= 8);
+  p.parts = p.splits << p.twin;
   CUtensorMap mq, mk, mv;
   if (!r16_map(&mq, q, width, lq, c.h, c.b, qs, p.packed ? lq : R16_T, p.packed ? group : 1) || !r16_map(&mk, k, width, lk, c.hkv, c.b, ks, R16_T, 1) ||
       !r16_map(&mv, v, width, lk, c.hkv, c.b, vs, R16_T, 1))
     return fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the operands of om_rule_attention_fwd");
   char* part = nullptr;
-  if (p.splits > 1) {
-    const size_t ml = ((size_t)p.splits * p.rows * sizeof(float2) + 255) & ~(size_t)255;
-    OM_TRY(pool_alloc(ctx, ml + (size_t)p.splits * p.rows * c.d * sizeof(float), false, (void**)&part));
+  if (p.parts > 1) {
+    const size_t ml = ((size_t)p.parts * p.rows * sizeof(float2) + 255) & ~(size_t)255;
+    OM_TRY(pool_alloc(ctx, ml + (size_t)p.parts * p.rows * c.d * sizeof(float), false, (void**)&part));
     p.part_ml = reinterpret_cast<float2*>(part);
     p.part = reinterpret_cast<float*>(part + ml);
   }
   const int32_t st = planes ? r16_fwd_by_mode<64, 2>(ctx, grid, mq, mk, mv, p) : c.d <= 64 ? r16_fwd_by_mode<64, 1>(ctx, grid, mq, mk, mv, p) : r16_fwd_by_mode<128, 1>(ctx, grid, mq, mk, mv, p);
-  if (p.splits > 1) {
+  if (p.parts > 1) {
     if (st == OM_OK) launch_chained(ctx, rule16_join_kernel, grid_for(ctx, p.rows, 8), 256, 0, p);
     pool_free(ctx, part);
   }

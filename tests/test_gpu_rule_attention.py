@@ -201,6 +201,23 @@ def test_large_fp32_call_with_few_queries_and_a_split_walk(ctx):
     Call(ctx, r, 2, 8, 2, 30, 20011, 64, causal=True).run(False).check(False)
 
 
+@pytest.mark.parametrize("half,b,h,hk,lq,lk,d,kw", [
+    (True, 75, 4, 2, 1, 1100, 128, {}),                                           # more heads than SMs, not split
+    (True, 75, 4, 2, 1, 1100, 64, dict(softcap=5.0, slopes=True)),
+    (False, 75, 4, 2, 1, 1100, 64, {}),
+    (True, 80, 2, 2, 100, 1300, 128, dict(causal=True)),                          # one tile of queries with its own keys
+    (True, 1, 2, 2, 100, 1300, 128, dict(causal=True, window=20)),                # two or three tiles in sight
+    (True, 2, 8, 1, 5, 3000, 64, dict(docs=40, padded=200, causal=True)),         # tiles in sight next to hidden ones
+    (False, 2, 8, 1, 5, 3000, 64, dict(docs=40, padded=200, causal=True)),
+    (True, 2, 4, 2, 3, 1200, 128, dict(causal=True, q_offset=5)),                 # one tile in sight: half the rows' warps have none
+    (False, 2, 4, 2, 3, 1200, 64, dict(causal=True, q_offset=5)),
+    (True, 2, 4, 2, 3, 1200, 96, dict(causal=True, q_offset=-10)),                # none
+])
+def test_one_tile_of_queries_walks_twice_as_fast(ctx, half, b, h, hk, lq, lk, d, kw):
+    r = np.random.default_rng(63)
+    Call(ctx, r, b, h, hk, lq, lk, d, half=half, **kw).run(False).check(False)
+
+
 def test_values_far_apart_keep_their_precision(ctx):
     """One value row 1e20 times the others: the rows that do not see it keep fp32 accuracy, in a call of the size that is otherwise done
     with two half-precision numbers a value. The same for tiny rows of k and of the output's gradient."""
