@@ -795,7 +795,7 @@ int32_t om_optim_adam_step_b16(om_ctx* ctx, int32_t n_tensors, float* const* p_h
  * Products, norms and the state keep fp32 accuracy whatever the context's flags. p16_host (may be NULL, as may be its entries):
  * the bfloat16 copies of the weights, refreshed by the update. hyper_dev (may be NULL): a device copy that the kernels read
  * in place of hyper_host (so that a captured update follows a schedule); steps is always taken from hyper_host. A matrix with
- * no elements is left alone; p, g and m of one call may not overlap. steps is 1 to 10, sides are at most 65536. */
+ * no elements is left alone; p, m and p16 of one call overlap nothing (OM_ERR_ARG). steps is 1 to 10, sides are at most 65536. */
 typedef struct om_muon_hyper {
   float lr, momentum, weight_decay, eps, grad_scale;
   int32_t nesterov, steps, match_rms;

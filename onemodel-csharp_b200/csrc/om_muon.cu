@@ -572,6 +572,28 @@ int32_t om_optim_muon_step(om_ctx* ctx, int32_t n_tensors, float* const* p_host,
     flops += hyper_host->steps * (4.0 * mm * mm * nn + 2.0 * mm * mm * mm);
     bytes += 20.0 * mm * nn;
   }
+  // Two matrices over one memory would be updated at the same time: refused.
+  struct Span {
+    uintptr_t begin, end;
+    bool written;
+  };
+  std::vector<Span> spans;
+  for (int i = 0; i < n_tensors; i++) {
+    const size_t n = (size_t)rows_host[i] * (size_t)cols_host[i];
+    if (n == 0) continue;
+    auto span = [&](const void* p, size_t size, bool written) { spans.push_back(Span{reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + n * size, written}); };
+    span(p_host[i], 4, true);
+    span(m_host[i], 4, true);
+    span(g_host[i], 4, false);
+    if (p16_host && p16_host[i]) span(p16_host[i], 2, true);
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+  uintptr_t end = 0, end_written = 0;
+  for (const Span& s : spans) {
+    if (s.begin < (s.written ? end : end_written)) return fail(ctx, OM_ERR_ARG, "om_optim_muon_step: weights, momentum and gradients overlap");
+    end = std::max(end, s.end);
+    if (s.written) end_written = std::max(end_written, s.end);
+  }
   ProfileScope prof(ctx, "om_optim_muon_step", flops, bytes);
   // The longest sums first, so that no CTA begins one when the others are done (each matrix's result is its own).
   std::vector<int> order(n_tensors);

@@ -145,6 +145,18 @@ def test_captured_step_follows_its_numbers_on_the_device(ctx):
     ctx.call("om_graph_destroy", ctx.handle, graph)
 
 
+def test_workspaces_under_the_checked_flag(ctx):
+    """Poisoned workspaces with guard bytes behind them: nothing is read that was not written, nothing written behind an end."""
+    ctx.set_flags(omb.OM_CHECKED)
+    try:
+        r = np.random.default_rng(31)
+        mats = [make(r, *s) for s in ((33, 65), (129, 31), (257, 130), (1, 5))]
+        for got, mat in zip(step(ctx, mats), mats):
+            check(got, mat)
+    finally:
+        ctx.set_flags(0)
+
+
 def test_refusals(ctx):
     A = ctx.zeros((16,))
     one = (C.c_void_p * 1)(A.ptr.value)
@@ -163,6 +175,18 @@ def test_refusals(ctx):
     call(8, hyper=omb.MuonHyper(steps=11))
     call(1, rows=-1)
     call(1, cols=65537)
+    call(8)                                                # one memory for everything
+    at = lambda *n: (C.c_void_p * len(n))(*[A.ptr.value + 4 * x for x in n])   # noqa: E731
+    big = ctx.zeros((64,))
+    on = lambda *n: (C.c_void_p * len(n))(*[big.ptr.value + 4 * x for x in n])   # noqa: E731
+    for p, g, m in ((on(0, 0), on(16, 16), on(32, 48)), (on(0, 15), on(32, 32), on(40, 48)), (on(0, 16), on(8, 48), on(32, 56))):
+        with pytest.raises(omb.OmError) as e:
+            ctx.call("om_optim_muon_step", ctx.handle, i32(2), p, g, m, None, omb.int_array([2, 2]), omb.int_array([8, 4]),
+                     C.byref(omb.MuonHyper(**(DEFAULT | dict(grad_scale=1.0)))), None)
+        assert e.value.status == 8
+    ctx.call("om_optim_muon_step", ctx.handle, i32(2), on(0, 16), at(0, 0), on(32, 48), None, omb.int_array([2, 2]), omb.int_array([8, 8]),
+             C.byref(omb.MuonHyper(**(DEFAULT | dict(grad_scale=1.0)))), None)                     # one gradient for two matrices
+    ctx.sync()
     t = lambda *s: omb.Tensor.from_numpy(np.zeros(s, np.float32), requires_grad=True)   # noqa: E731
     with pytest.raises(omb.ShapeError):
         omb.Optimizer.muon([t(3)])

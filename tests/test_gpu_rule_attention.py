@@ -340,6 +340,18 @@ def test_large_fp32_call_in_a_graph(ctx):
         ctx.call("om_graph_destroy", ctx.handle, graph)
 
 
+def test_workspaces_under_the_checked_flag(ctx):
+    """Poisoned workspaces with guard bytes behind them: nothing is read that was not written, nothing written behind an end."""
+    ctx.set_flags(omb.OM_CHECKED)
+    try:
+        r = np.random.default_rng(25)
+        for half in (False, True):
+            for lq, lk, d, kw in ((130, 130, 64, dict(causal=True, docs=50, padded=9)), (1, 2050, 64, {}), (77, 300, 40, dict(softcap=4.0, slopes=True)), (5, 7, 33, {})):
+                Call(ctx, r, 2, 4, 2, lq, lk, d, half=half, **kw).run().check()
+    finally:
+        ctx.set_flags(0)
+
+
 def test_both_forms_of_a_result(ctx):
     """The bfloat16 entry points write fp32, bfloat16 or both; the bfloat16 values are the fp32 ones rounded."""
     r = np.random.default_rng(22)
