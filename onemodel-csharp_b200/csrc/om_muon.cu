@@ -84,17 +84,40 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constan
     const float u = h.nesterov ? fmaf(m, h.momentum, g) : m;
     return u * u;
   };
+  // What a thread needs comes in front of what it writes: between a store and a load behind it the compiler keeps the order.
   if (t.quads) {
-#pragma unroll 4
-    for (long long e = e0 + 4 * threadIdx.x; e < e1; e += 1024) {
-      const float4 g = *reinterpret_cast<const float4*>(t.g + e);
-      float4 m = *reinterpret_cast<float4*>(t.m + e);
-      const float a = one(g.x, m.x), b = one(g.y, m.y), c = one(g.z, m.z), d = one(g.w, m.w);
-      *reinterpret_cast<float4*>(t.m + e) = m;
-      sum += ((double)a + b) + ((double)c + d);
+    for (long long e = e0 + 4 * threadIdx.x; e < e1; e += 4096) {
+      float4 g[4], m[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        if (e + 1024 * u < e1) {
+          g[u] = *reinterpret_cast<const float4*>(t.g + e + 1024 * u);
+          m[u] = *reinterpret_cast<const float4*>(t.m + e + 1024 * u);
+        }
+#pragma unroll
+      for (int u = 0; u < 4; u++)
+        if (e + 1024 * u < e1) {
+          const float a = one(g[u].x, m[u].x), b = one(g[u].y, m[u].y), c = one(g[u].z, m[u].z), d = one(g[u].w, m[u].w);
+          *reinterpret_cast<float4*>(t.m + e + 1024 * u) = m[u];
+          sum += ((double)a + b) + ((double)c + d);
+        }
     }
   } else {
-    for (long long e = e0 + threadIdx.x; e < e1; e += 256) sum += one(t.g[e], t.m[e]);
+    for (long long e = e0 + threadIdx.x; e < e1; e += 2048) {
+      float g[8], m[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        if (e + 256 * u < e1) {
+          g[u] = t.g[e + 256 * u];
+          m[u] = t.m[e + 256 * u];
+        }
+#pragma unroll
+      for (int u = 0; u < 8; u++)
+        if (e + 256 * u < e1) {
+          sum += one(g[u], m[u]);
+          t.m[e + 256 * u] = m[u];
+        }
+    }
   }
   __shared__ double s[8];
 #pragma unroll
@@ -154,7 +177,7 @@ __global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__
       block[a][b + 3] = one(m.w, g.w);
     }
   } else {
-#pragma unroll 4
+#pragma unroll 16
     for (int e = threadIdx.x; e < 64 * 64; e += 256) {
       const int r = r0 + e / 64, c = c0 + e % 64;
       if (r >= t.rows || c >= t.cols) continue;
@@ -212,27 +235,39 @@ __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant_
     return *reinterpret_cast<const uint16_t*>(&b);
   };
   if (t.quads) {
+    float4 p[4];
 #pragma unroll
-    for (int e = threadIdx.x; e < 64 * 16; e += 256) {
-      const int a = e / 16, b = e % 16 * 4;
+    for (int u = 0; u < 4; u++) {
+      const int a = (int)threadIdx.x / 16 + 16 * u, b = threadIdx.x % 16 * 4;
+      if (r0 + a < t.rows && c0 + b < t.cols) p[u] = *reinterpret_cast<const float4*>(t.p + (long long)(r0 + a) * t.cols + c0 + b);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      const int a = (int)threadIdx.x / 16 + 16 * u, b = threadIdx.x % 16 * 4;
       if (r0 + a >= t.rows || c0 + b >= t.cols) continue;
       const long long at = (long long)(r0 + a) * t.cols + c0 + b;
-      float4 p = *reinterpret_cast<float4*>(t.p + at);
-      p = make_float4(fmaf(-rate, block[a][b], p.x * keep), fmaf(-rate, block[a][b + 1], p.y * keep), fmaf(-rate, block[a][b + 2], p.z * keep),
-                      fmaf(-rate, block[a][b + 3], p.w * keep));
-      *reinterpret_cast<float4*>(t.p + at) = p;
+      const float4 q = make_float4(fmaf(-rate, block[a][b], p[u].x * keep), fmaf(-rate, block[a][b + 1], p[u].y * keep), fmaf(-rate, block[a][b + 2], p[u].z * keep),
+                                   fmaf(-rate, block[a][b + 3], p[u].w * keep));
+      *reinterpret_cast<float4*>(t.p + at) = q;
       if (t.p16)
-        *reinterpret_cast<uint2*>(t.p16 + at) = make_uint2((uint32_t)half16(p.x) | (uint32_t)half16(p.y) << 16, (uint32_t)half16(p.z) | (uint32_t)half16(p.w) << 16);
+        *reinterpret_cast<uint2*>(t.p16 + at) = make_uint2((uint32_t)half16(q.x) | (uint32_t)half16(q.y) << 16, (uint32_t)half16(q.z) | (uint32_t)half16(q.w) << 16);
     }
   } else {
-#pragma unroll 4
-    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-      const int r = r0 + e / 64, c = c0 + e % 64;
-      if (r >= t.rows || c >= t.cols) continue;
-      const long long at = (long long)r * t.cols + c;
-      const float p = fmaf(-rate, block[e / 64][e % 64], t.p[at] * keep);
-      t.p[at] = p;
-      if (t.p16) t.p16[at] = half16(p);
+    float p[16];
+    const int b = threadIdx.x % 64;
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+      const int a = (int)threadIdx.x / 64 + 4 * u;
+      if (r0 + a < t.rows && c0 + b < t.cols) p[u] = t.p[(long long)(r0 + a) * t.cols + c0 + b];
+    }
+#pragma unroll
+    for (int u = 0; u < 16; u++) {
+      const int a = (int)threadIdx.x / 64 + 4 * u;
+      if (r0 + a >= t.rows || c0 + b >= t.cols) continue;
+      const long long at = (long long)(r0 + a) * t.cols + c0 + b;
+      const float q = fmaf(-rate, block[a][b], p[u] * keep);
+      t.p[at] = q;
+      if (t.p16) t.p16[at] = half16(q);
     }
   }
 }
