@@ -1,14 +1,13 @@
 // Attention by rule with bfloat16 operands on the tensor pipe (tcgen05), forward and backward, for head dimensions up to 128.
 //
-// Forward: a CTA holds 256 queries as two tiles of 128 and walks the tiles of 128 keys that the rule lets them see. Four warps per query
-// tile keep the running maximum and sum of a row per thread; while one tile's rows turn scores into weights the tensor pipe works on
-// the other's: S = Q K^T in fp32 in tensor memory -> weights exp2(S - m), rounded to bfloat16, in tensor memory -> O += P V with P read
-// from there. Up to a head dimension of 64 the weights have a place of their own, so the next scores come while the rows are still at
-// these; with 128 columns of O they lie over the scores they came from, and the next scores wait for the product that reads them.
-// O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 over the one in use, which changes no
-// result: numerator and denominator share the factor. Rows go through their scores twice, 32 at a time (128 in registers would spill,
-// and what spills does not fit the L1 that the operands leave). Steps of 64 keys, with everything in places of its own, were measured
-// too and slower at 128 columns: a product of 128 x 64 takes the tensor pipe as long as one of 128 x 128.
+// Forward: a CTA holds 128 queries and walks the tiles of 128 keys that the rule lets them see. Two warps share 32 rows, a half of a step's
+// keys each: the running maximum goes between them through shared memory, the sums meet at the end. S = Q K^T in fp32 in tensor memory
+// -> weights exp2(S - m), rounded to bfloat16, in tensor memory -> O += P V with P read from there. Scores and weights have two places
+// each, so the tensor pipe is a step ahead and the rows never wait for a product: at 128 columns a step takes 2260 cycles, of which the
+// rows' exponentials 1250, maximum 350, waits 400; the pipe's two products 1500. (Two tiles of queries a CTA with one place each, rows
+// through their scores twice: 8 x 32 single tokens 66 us instead of 61, three documents' batches forward 66 instead of 50, a window
+// 207 instead of 226, 4 x 16 x 4096^2 344 instead of 372.) O stays in tensor memory; it is rescaled only when a row's maximum has grown
+// by more than 2^8 over the one in use, which changes no result: numerator and denominator share the factor.
 // With few rows the walk over the keys is split over CTAs that leave their sums, maxima and O for rule16_join_kernel, and the query
 // heads that share a key head become rows of one tile, so that keys and values are read once.
 //
@@ -328,13 +327,11 @@ struct R16Fwd {
   int h, hkv, d;
   int packed;                     // rows of a tile are (head of the group, query): h / hkv * lq of them
   int splits;
-  int twin;                       // one row tile a CTA: its two groups of row warps take steps in turn and leave a part each
-  int parts;                      // 1, or what rule16_join_kernel joins: splits, or twice that
   float* out;
   __nv_bfloat16* out16;
   R16Strides os;
   float* lse;
-  float* part;                    // [parts][b * h * lq][d] and [parts][b * h * lq] (maximum, sum) where parts > 1
+  float* part;                    // [splits][b * h * lq][d] and [splits][b * h * lq] (maximum, sum) where splits > 1
   float2* part_ml;
   long long rows;                 // b * h * lq
   const float* units;             // two planes: [4][b * hkv] powers of two that q, k, v, g were divided by, and the flag that they were not
@@ -343,18 +340,16 @@ struct R16Fwd {
 };
 
 // A CTA's plan: the tiles of 128 of the other axis that some row tile sees anything of, in order, with rule_see's answer for each row
-// tile (two bits, from bit 10 on). Made by one warp; returns their number. twin: the rows of both row tiles are the same, and the
-// steps fall to the two in turn.
+// tile (two bits, from bit 10 on). Made by one warp; returns their number.
 __device__ __forceinline__ int r16_tile_of(uint32_t step) { return (int)(step & (R16_PLAN - 1)); }
-__device__ __forceinline__ int r16_sees_of(uint32_t step, int tile) { return (int)(step >> (10 + 2 * tile)) & 3; }
+__device__ __forceinline__ int r16_sees_of(uint32_t step) { return (int)(step >> 10) & 3; }
 template <typename F>
-__device__ __forceinline__ int r16_plan(uint16_t* steps, int tiles, int lane, bool twin, F see) {
+__device__ __forceinline__ int r16_plan(uint16_t* steps, int tiles, int lane, F see) {
   int n = 0;
   for (int t0 = 0; t0 < tiles; t0 += 32) {
     const int t = t0 + lane;
     const uint32_t a = t < tiles ? see(t) : 0u, some = __ballot_sync(0xffffffffu, a != 0);
-    const int at = n + __popc(some & ((1u << lane) - 1u));
-    if (a) steps[at] = (uint16_t)((uint32_t)t | a << (twin && (at & 1) ? 12 : 10));
+    if (a) steps[n + __popc(some & ((1u << lane) - 1u))] = (uint16_t)((uint32_t)t | a << 10);
     n += __popc(some);
   }
   return n;
@@ -363,26 +358,29 @@ __device__ __forceinline__ int r16_plan(uint16_t* steps, int tiles, int lane, bo
 template <int DP, int PL>
 struct R16FwdShape {
   static constexpr int TILE = r16_tile_bytes<DP, PL>();
-  static constexpr int STAGES = TILE > R16_CHUNK ? 4 : 8; // of K and V tiles in turn
-  static constexpr bool APART = DP == 64 && PL == 1;                // the weights have columns of their own
-  static constexpr int RULES = (2 + STAGES) * TILE;
-  static constexpr int PLAN = RULES + 128;
+  static constexpr int STAGES = TILE > R16_CHUNK ? 5 : 8; // of K and V tiles
+  static constexpr int TURN = (1 + STAGES) * TILE;        // what the two warps of a row tell each other, [place][half][row]
+  static constexpr int RULES = TURN + 4096;
+  static constexpr int PLAN = RULES + 64;
   static constexpr int BARS = PLAN + R16_PLAN * 2 + 16;
   static constexpr int SMEM = BARS + 512;
 };
+// The two warps of a row. Both come here once a step whatever has happened to either, so neither waits for one that has left.
+__device__ __forceinline__ void r16_meet(int barrier) { asm volatile("bar.sync %0, 64;" ::"r"(barrier) : "memory"); }
 
 template <int DP, int MODE, int PL>
 __global__ void __launch_bounds__(R16_THREADS, 1)
 rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                   const __grid_constant__ R16Fwd p) {
   typedef R16FwdShape<DP, PL> W;
-  // Scores of query tile g at 128 g, weights at 128 g too or at 256 + 64 g, O behind.
-  constexpr uint32_t COL_S = 0, COL_P = W::APART ? 256 : 0, P_STEP = W::APART ? 64 : 128, COL_O = W::APART ? 384 : 256, O_STEP = W::APART ? 64 : 128;
+  // Scores in two places, O, and the weights in two places of their own; two planes of weights lie over the scores they came from, and
+  // their O has a step's sum and the whole side by side.
+  constexpr uint32_t COL_S = 0, COL_O = 256, COL_P = PL == 1 ? 384 : 0, P_STEP = PL == 1 ? 64 : 128;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t *slot_q = smem, *ring = smem + 2 * W::TILE;
+  uint8_t *slot_q = smem, *ring = smem + W::TILE;
   uint16_t* steps = reinterpret_cast<uint16_t*>(smem + W::PLAN);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
-  uint64_t *bar_q = bars, *bar_s = bars + 1 /* [tile] */, *bar_read = bars + 3 /* [tile] */, *bar_p = bars + 5 /* [tile] */, *bar_o = bars + 7 /* [tile] */,
+  uint64_t *bar_q = bars, *bar_s = bars + 1 /* [place] */, *bar_read = bars + 3 /* [place] */, *bar_p = bars + 5 /* [place] */, *bar_o = bars + 7 /* [place] */,
            *bar_full = bars + 9 /* [STAGES] */, *bar_empty = bar_full + W::STAGES;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_empty + W::STAGES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -400,16 +398,15 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     bi = blockIdx.x / p.h;
     hi = blockIdx.x - bi * p.h;
     hk = hi / group;
-    i0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 2 * R16_T;      // the longest walks of a causal mask first
+    i0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * R16_T;      // the longest walks of a causal mask first
   }
-  const int both = !p.packed && i0 + R16_T < r.lq;
 
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 1);
     for (int a = 0; a < 2; a++) {
       mbar_init(&bar_s[a], 1);
-      mbar_init(&bar_read[a], R16_ROW_WARPS / 2);
-      mbar_init(&bar_p[a], R16_ROW_WARPS / 2);
+      mbar_init(&bar_read[a], R16_ROW_WARPS);
+      mbar_init(&bar_p[a], R16_ROW_WARPS);
       mbar_init(&bar_o[a], 1);
     }
     for (int a = 0; a < W::STAGES; a++) {
@@ -431,18 +428,16 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   pdl_wait();
 
   const int prefix = r.prefix ? r.prefix[bi] : 0;
-  RuleTile* tiles = reinterpret_cast<RuleTile*>(smem + W::RULES);
-  if (threadIdx.x < 64 && lane == 0) tiles[warp] = rule_query_tile(r, prefix, bi, warp == 0 ? i0 : both ? i0 + R16_T : r.lq, 2);
-  const RuleSpan span = rule_keys(r, prefix, i0, min(p.packed ? r.lq : i0 + 2 * R16_T, r.lq));
+  RuleTile* tile = reinterpret_cast<RuleTile*>(smem + W::RULES);
+  if (threadIdx.x == 0) *tile = rule_query_tile(r, prefix, bi, i0, 2);
+  const RuleSpan span = rule_keys(r, prefix, i0, min(p.packed ? r.lq : i0 + R16_T, r.lq));
   int first = span.prefix > 0 ? 0 : span.lo / R16_T, last = (max(span.prefix, span.hi) + R16_T - 1) / R16_T;
   const int per = max(0, last - first + p.splits - 1) / p.splits;
   first += split * per;
   last = min(first + per, last);
   __syncthreads();
   if (warp == 0) {
-    const int n = r16_plan(steps, last - first, lane, p.twin, [&](int t) {
-      return (uint32_t)(rule_see<true>(tiles[0], (first + t) * R16_T, 2) | (p.twin ? 0 : rule_see<true>(tiles[1], (first + t) * R16_T, 2) << 2));
-    });
+    const int n = r16_plan(steps, last - first, lane, [&](int t) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T, 2); });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
@@ -453,37 +448,34 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     // values beyond what two halves hold: the fp32 kernel behind does these heads
   } else if (warp == R16_ROW_WARPS + 1) {
     if (lane == 0) {
-      if (p.packed) {
-        mbar_expect_tx(bar_q, (uint32_t)(W::TILE / R16_CHUNK) * (uint32_t)(group * r.lq) * 128u);
-        r16_load_tile<DP, PL>(slot_q, &map_q, 0, hi, bi, bar_q);
-      } else {
-        mbar_expect_tx(bar_q, (uint32_t)W::TILE * (both ? 2u : 1u));
-        r16_load_tile<DP, PL>(slot_q, &map_q, i0, hi, bi, bar_q);
-        if (both) r16_load_tile<DP, PL>(slot_q + W::TILE, &map_q, i0 + R16_T, hi, bi, bar_q);
-      }
+      mbar_expect_tx(bar_q, p.packed ? (uint32_t)(W::TILE / R16_CHUNK) * (uint32_t)(group * r.lq) * 128u : (uint32_t)W::TILE);
+      r16_load_tile<DP, PL>(slot_q, &map_q, i0, hi, bi, bar_q);
       int s = 0;
       uint32_t phase = 0;
       bool again = false;
-      for (int n = 0; ok && n < walk; n++) {
-        const uint32_t step = steps[n];
-        for (int kv = 0; kv < 2 && ok; kv++) {
-          if (again) ok = r16_bar(&bar_empty[s], phase ^ 1u, abort_flag, p.status, 61);
-          if (!ok) break;
-          mbar_expect_tx(&bar_full[s], W::TILE);
-          r16_load_tile<DP, PL>(ring + s * W::TILE, kv ? &map_v : &map_k, (first + r16_tile_of(step)) * R16_T, hk, bi, &bar_full[s]);
-          if (++s == W::STAGES) {
-            s = 0;
-            phase ^= 1u;
-            again = true;
-          }
+      auto load = [&](const CUtensorMap* map, int n) {
+        if (again) ok = ok && r16_bar(&bar_empty[s], phase ^ 1u, abort_flag, p.status, 61);
+        if (!ok) return;
+        mbar_expect_tx(&bar_full[s], W::TILE);
+        r16_load_tile<DP, PL>(ring + s * W::TILE, map, (first + r16_tile_of(steps[n])) * R16_T, hk, bi, &bar_full[s]);
+        if (++s == W::STAGES) {
+          s = 0;
+          phase ^= 1u;
+          again = true;
         }
+      };
+      // In the order that the products take them.
+      if (walk > 0) load(&map_k, 0);
+      for (int n = 0; ok && n < walk; n++) {
+        if (n + 1 < walk) load(&map_k, n + 1);
+        load(&map_v, n);
       }
     }
   } else if (warp == R16_ROW_WARPS) {
     if (lane == 0) {
       ok = r16_bar(bar_q, 0, abort_flag, p.status, 62);
       int s = 0;                                          // the ring's next tile
-      uint32_t phase = 0, scored[2] = {0, 0}, summed[2] = {0, 0};
+      uint32_t phase = 0;
       auto take = [&]() {
         const int at = s;
         ok = ok && r16_bar(&bar_full[s], phase, abort_flag, p.status, 63);
@@ -493,61 +485,37 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         }
         return at;
       };
-      auto scores = [&](const int t, int ks) {
-        if (scored[t] > 0) {
-          // APART: the rows have taken the scores before. Else the product that reads the weights over them is complete.
-          ok = W::APART ? r16_bar(&bar_read[t], (scored[t] - 1) & 1u, abort_flag, p.status, 64) : r16_bar(&bar_o[t], (summed[t] - 1) & 1u, abort_flag, p.status, 64);
-          if (!ok) return;
-        }
-        tc_fence_after();
-        r16_scores<DP, PL>(tmem + COL_S + 128u * t, r16_desc_k(slot_q + (p.twin ? 0 : t) * W::TILE), r16_desc_k(ring + ks * W::TILE));
-        umma_commit(&bar_s[t]);
-        scored[t]++;
-      };
-      auto product = [&](const int t, int vs) {
-        ok = r16_bar(&bar_p[t], summed[t] & 1u, abort_flag, p.status, 65);
+      auto scores = [&](int n) {
+        const int place = n & 1, ks = take();
+        // The rows have the scores before last, or (two planes) the product that reads the weights over them is complete.
+        if (n >= 2) ok = ok && r16_bar(PL == 1 ? &bar_read[place] : &bar_o[place], ((n - 2) >> 1) & 1u, abort_flag, p.status, 64);
         if (!ok) return;
         tc_fence_after();
-        r16_gather<DP, 128, PL>(tmem + COL_O + O_STEP * t, tmem + COL_P + P_STEP * t, r16_desc_mn(ring + vs * W::TILE), PL == 1 && summed[t] > 0 ? 1u : 0u);
-        umma_commit(&bar_o[t]);
-        summed[t]++;
+        r16_scores<DP, PL>(tmem + COL_S + 128u * place, r16_desc_k(slot_q), r16_desc_k(ring + ks * W::TILE));
+        umma_commit(&bar_s[place]);
+        umma_commit(&bar_empty[ks]);
       };
-      uint32_t step = walk > 0 ? steps[0] : 0u;
-      if (ok && walk > 0) {
-        const int ks = take();
-        if (ok && r16_sees_of(step, 0)) scores(0, ks);
-        if (ok && r16_sees_of(step, 1)) scores(1, ks);
-        if (ok) umma_commit(&bar_empty[ks]);
-      }
+      if (ok && walk > 0) scores(0);
       for (int n = 0; ok && n < walk; n++) {
-        const bool more = n + 1 < walk;
-        const uint32_t ahead = more ? steps[n + 1] : 0u;
-        const int vs = take(), ks = more ? take() : 0;
-        if (W::APART || p.twin) {                         // twins: the step ahead is the other group's, so nothing of this one is in its way
-          if (ok && r16_sees_of(ahead, 0)) scores(0, ks);
-          if (ok && r16_sees_of(ahead, 1)) scores(1, ks);
-          if (ok && r16_sees_of(step, 0)) product(0, vs);
-          if (ok && r16_sees_of(step, 1)) product(1, vs);
-        } else {
-          if (ok && r16_sees_of(step, 0)) product(0, vs);
-          if (ok && r16_sees_of(ahead, 0)) scores(0, ks);
-          if (ok && r16_sees_of(step, 1)) product(1, vs);
-          if (ok && r16_sees_of(ahead, 1)) scores(1, ks);
-        }
+        const int place = n & 1;
+        if (n + 1 < walk) scores(n + 1);
+        const int vs = take();
+        ok = ok && r16_bar(&bar_p[place], (n >> 1) & 1u, abort_flag, p.status, 65);
         if (!ok) break;
+        tc_fence_after();
+        r16_gather<DP, 128, PL>(tmem + COL_O, tmem + COL_P + P_STEP * place, r16_desc_mn(ring + vs * W::TILE), PL == 1 && n > 0 ? 1u : 0u);
+        umma_commit(&bar_o[place]);
         umma_commit(&bar_empty[vs]);
-        if (more) umma_commit(&bar_empty[ks]);
-        step = ahead;
       }
       if (!ok) *abort_flag = 1;
     }
   } else {
-    const int g = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
-    int i = i0 + (p.twin ? 0 : g * R16_T) + row, head = hi;
+    const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    int i = i0 + row, head = hi;
     bool valid = i < r.lq;
     if (p.packed) {
       const int gi = row / r.lq;
-      valid = (g == 0 || p.twin) && gi < group;
+      valid = gi < group;
       i = valid ? row - gi * r.lq : 0;
       head = valid ? hi + gi : hi;
     }
@@ -556,66 +524,90 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const R16Score score = r16_score_of<MODE>(r, head, unit);
     const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
     const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
-    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16);
-    const uint32_t t_s = lane_base + COL_S + 128u * g, t_p = lane_base + COL_P + P_STEP * g, t_o = lane_base + COL_O + O_STEP * g;
+    const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), t_o = lane_base + COL_O + (uint32_t)(DP / 2) * half;   // its half of O's columns
+    float2* turn = reinterpret_cast<float2*>(smem + W::TURN);
+    const int mine = half * 128 + row, other = (half ^ 1) * 128 + row;
     const float mult = MODE ? 1.f : r.scale * unit * R16_LOG2E;
     const uint64_t mult2 = r16_two(mult, mult);
-    float m = -INFINITY, l = 0.f;
-    uint32_t count = 0;
-    for (int n = 0; ok && n < walk; n++) {
-      const uint32_t step = steps[n];
-      const int sees = r16_sees_of(step, g);
-      if (!sees) continue;
-      const int j0 = (first + r16_tile_of(step)) * R16_T;
-      if (!(ok = r16_wait(&bar_s[g], count & 1u, abort_flag, p.status, 66))) break;
+    float m = -INFINITY, l = 0.f;                        // l: of its half
+    bool gone = false;                                   // both warps of a row know it
+    for (int n = 0; n < walk; n++) {
+      const uint32_t step = steps[n], place = n & 1u;
+      const int sees = r16_sees_of(step), at = (first + r16_tile_of(step)) * R16_T + 64 * half;
+      const uint32_t t_s = lane_base + COL_S + 128u * place + 64u * half, t_p = lane_base + COL_P + P_STEP * place + (PL == 1 ? 32u : 64u) * half;
+      ok = ok && r16_wait(&bar_s[place], (n >> 1) & 1u, abort_flag, p.status, 66);
       tc_fence_after();
-      float tops[4];
-      {
-        uint32_t x[2][32];
-        tmem_ld_32x32b_x32(t_s, x[0]);
-        tmem_ld_wait();
+      uint32_t x[2][32];
+      tmem_ld_32x32b_x32(t_s, x[0]);
+      tmem_ld_32x32b_x32(t_s + 32u, x[1]);
+      tmem_ld_wait();
+      if (PL == 1) r16_arrive_warp(&bar_read[place], lane);
+      float tops[2];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          uint32_t(&v)[32] = x[c & 1];
-          if (c < 3) tmem_ld_32x32b_x32(t_s + 32u * (c + 1), x[(c + 1) & 1]);
-          if (MODE) {
-            const float far = (float)(i + r.q_offset - j0 - 32 * c);
+      for (int c = 0; c < 2; c++) {
+        uint32_t(&v)[32] = x[c];
+        if (MODE) {
+          const float far = (float)(i + r.q_offset - at - 32 * c);
 #pragma unroll
-            for (int u = 0; u < 32; u++) {
-              float dcap;
-              v[u] = __float_as_uint(r16_score<MODE>(score, far - (float)u, __uint_as_float(v[u]), &dcap));
-            }
+          for (int u = 0; u < 32; u++) {
+            float dcap;
+            v[u] = __float_as_uint(r16_score<MODE>(score, far - (float)u, __uint_as_float(v[u]), &dcap));
           }
-          if (sees == 1) r16_hide(v, r16_bits(seen, j0 + c * 32, docs));
-          if (MODE || sees == 1) r16_st32(t_s + 32u * c, v);
-          float t[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            t[e] = fmaxf(__uint_as_float(v[8 * e]), __uint_as_float(v[8 * e + 1]));
-#pragma unroll
-            for (int u = 2; u < 8; u += 2) t[e] = r16_max3(t[e], __uint_as_float(v[8 * e + u]), __uint_as_float(v[8 * e + u + 1]));
-          }
-          tops[c] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-          if (c < 3) tmem_ld_wait();
         }
-        if (MODE || sees == 1) r16_st_wait();
+        if (sees == 1) r16_hide(v, r16_bits(seen, at + 32 * c, docs));
+        float t[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          t[e] = fmaxf(__uint_as_float(v[8 * e]), __uint_as_float(v[8 * e + 1]));
+#pragma unroll
+          for (int u = 2; u < 8; u += 2) t[e] = r16_max3(t[e], __uint_as_float(v[8 * e + u]), __uint_as_float(v[8 * e + u + 1]));
+        }
+        tops[c] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       }
-      const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * mult;
+      // The other half's, by turns in two places: whoever writes one again has met the other warp since it was read. A wait that ran out is
+      // told here.
+      const float part_top = fmaxf(tops[0], tops[1]);
+      turn[place * 256 + mine] = make_float2(part_top, ok ? 1.f : 0.f);
+      r16_meet(1 + quad);
+      const float2 theirs = turn[place * 256 + other];
+      gone = !__all_sync(0xffffffffu, ok && theirs.y != 0.f);
+      if (gone) break;
+      const float top = fmaxf(part_top, theirs.x) * mult;
       const bool grown = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
-      // The product before has read the weights' place and is in O (in the other layout these scores came after it anyway).
-      if (W::APART && count > 0) {
-        if (!(ok = r16_wait(&bar_o[g], (count - 1) & 1u, abort_flag, p.status, 69))) break;
-        tc_fence_after();
+      const float shrink = grown ? r16_ex2(m - top) : 1.f;      // m = -inf: 0
+      if (grown) m = top;
+      // Two planes: weights times 2^7, at most 2^15, so that small ones keep their digits (the row's sum has the same factor).
+      const float base = (m == -INFINITY ? 0.f : m) - (PL == 2 ? 7.f : 0.f);
+      const uint64_t base2 = r16_two(-base, -base);
+      uint64_t sum[2] = {0ull, 0ull};
+      // These scores came after the product before last, so its weights' place is free.
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        uint32_t w[16], wl[16];
+#pragma unroll
+        for (int u = 0; u < 16; u++) {
+          float a, b;
+          r16_fma2(a, b, x[c][2 * u], x[c][2 * u + 1], mult2, base2);
+          a = r16_ex2(a);
+          b = r16_ex2(b);
+          sum[u & 1] = r16_add2(sum[u & 1], a, b);
+          if (PL == 2) r16_take_apart(a, b, &w[u], &wl[u]);
+          else w[u] = r16_pack(a, b);
+        }
+        r16_st16(t_p + (PL == 2 ? 32u : 16u) * c, w);
+        if (PL == 2) r16_st16(t_p + 32u * c + 16u, wl);
       }
-      if (PL == 2 || __any_sync(0xffffffffu, grown)) {
-        const float shrink = grown ? r16_ex2(m - top) : 1.f;      // m = -inf: 0
-        if (grown) m = top;
-        l *= shrink;
+      const float2 s0 = *reinterpret_cast<const float2*>(&sum[0]), s1 = *reinterpret_cast<const float2*>(&sum[1]);
+      l = l * shrink + ((s0.x + s0.y) + (s1.x + s1.y));
+      // O, before the product that adds these weights to it and after the one before: rescaled, or the step before added to the whole.
+      if (n > 0 && (PL == 2 || __any_sync(0xffffffffu, grown))) {
+        ok = r16_wait(&bar_o[place ^ 1u], ((n - 1) >> 1) & 1u, abort_flag, p.status, 69);
+        tc_fence_after();
         if (PL == 2) {
-          if (count > 0) r16_fold<DP>(t_o + 64u, t_o, count == 1, shrink);
-        } else if (count > 0) {
+          r16_fold<DP / 2>(t_o + 64u, t_o, n == 1, shrink);
+        } else {
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
+          for (int c = 0; c < DP / 2; c += 32) {
             uint32_t o[32];
             tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
             tmem_ld_wait();
@@ -625,75 +617,47 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           }
         }
       }
-      // Two planes: weights times 2^7, at most 2^15, so that small ones keep their digits (the row's sum has the same factor).
-      const float base = (m == -INFINITY ? 0.f : m) - (PL == 2 ? 7.f : 0.f);
-      const uint64_t base2 = r16_two(-base, -base);
-      uint64_t sum[2] = {0ull, 0ull};
-      {
-        uint32_t x[2][32];
-        tmem_ld_32x32b_x32(t_s, x[0]);
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          uint32_t(&v)[32] = x[c & 1];
-          if (c < 3) tmem_ld_32x32b_x32(t_s + 32u * (c + 1), x[(c + 1) & 1]);
-          uint32_t w[16], wl[16];
-#pragma unroll
-          for (int u = 0; u < 16; u++) {
-            float a, b;
-            r16_fma2(a, b, v[2 * u], v[2 * u + 1], mult2, base2);
-            a = r16_ex2(a);
-            b = r16_ex2(b);
-            sum[u & 1] = r16_add2(sum[u & 1], a, b);
-            if (PL == 2) r16_take_apart(a, b, &w[u], &wl[u]);
-            else w[u] = r16_pack(a, b);
-          }
-          if (c < 3) tmem_ld_wait();                      // what the weights may lie over has been read
-          if (W::APART && c == 2) r16_arrive_warp(&bar_read[g], lane);
-          r16_st16(t_p + (PL == 2 ? 32u : 16u) * c, w);
-          if (PL == 2) r16_st16(t_p + 32u * c + 16u, wl);
-        }
-      }
-      const float2 s0 = *reinterpret_cast<const float2*>(&sum[0]), s1 = *reinterpret_cast<const float2*>(&sum[1]);
-      l += (s0.x + s0.y) + (s1.x + s1.y);
       r16_st_wait();
-      r16_arrive_warp(&bar_p[g], lane);
-      count++;
+      r16_arrive_warp(&bar_p[place], lane);
     }
-    if (ok && count > 0) ok = r16_wait(&bar_o[g], (count - 1) & 1u, abort_flag, p.status, 67);
-    if (ok) {
+    if (!gone) {
+      // The row's sum is both halves'.
+      if (walk > 0) ok = ok && r16_wait(&bar_o[(walk - 1) & 1], ((walk - 1) >> 1) & 1u, abort_flag, p.status, 67);
+      turn[(walk & 1) * 256 + mine] = make_float2(l, 0.f);
+      r16_meet(1 + quad);
+      l += turn[(walk & 1) * 256 + other].x;
+    }
+    if (ok && !gone) {
       tc_fence_after();
       const long long at_row = ((long long)bi * p.h + head) * r.lq + i;
       float inv = l == 0.f ? 0.f : unit_v / l;
       float* out = p.out;
       __nv_bfloat16* out16 = p.out16;
       long long at = bi * p.os.batch + head * p.os.head + (long long)i * p.os.row;
-      if (p.parts > 1) {
-        const int part = p.twin ? 2 * split + g : split;
+      if (p.splits > 1) {
         inv = unit_v;
         out = p.part;
         out16 = nullptr;
-        at = ((long long)part * p.rows + at_row) * p.d;
-        if (valid) p.part_ml[(long long)part * p.rows + at_row] = make_float2(PL == 2 ? m - 7.f : m, l);
-      } else if (p.lse && valid) {
+        at = ((long long)split * p.rows + at_row) * p.d;
+        if (valid && half == 0) p.part_ml[(long long)split * p.rows + at_row] = make_float2(PL == 2 ? m - 7.f : m, l);
+      } else if (p.lse && valid && half == 0) {
         p.lse[at_row] = l == 0.f ? -INFINITY : ((PL == 2 ? m - 7.f : m) + log2f(l)) * R16_LN2;
       }
-      if (g == 0 || both || p.twin) {
 #pragma unroll 1
-        for (int c = 0; c < DP; c += 32) {
-          uint32_t o[32];
-          __syncwarp();
-          if (count > 0) {
-            tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
-            tmem_ld_wait();
-          }
-          if (PL == 2 && count > 1) r16_add_whole(t_o + 64u + (uint32_t)c, o);
-          if (count == 0 || l == 0.f) {
-#pragma unroll
-            for (int u = 0; u < 32; u++) o[u] = 0u;
-          }
-          if (valid) r16_write(o, inv, out, out16, at + c, c, p.d);
+      for (int c = 0; c < DP / 2; c += 32) {
+        uint32_t o[32];
+        __syncwarp();
+        if (walk > 0) {
+          tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
+          tmem_ld_wait();
         }
+        if (PL == 2 && walk > 1) r16_add_whole(t_o + 64u + (uint32_t)c, o);
+        if (walk == 0 || l == 0.f) {
+#pragma unroll
+          for (int u = 0; u < 32; u++) o[u] = 0u;
+        }
+        const int col = half * (DP / 2) + c;
+        if (valid) r16_write(o, inv, out, out16, at + col, col, p.d);
       }
     }
   }
@@ -705,7 +669,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   }
 }
 
-// The parts of split walks: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s in increasing order of the parts. A warp per row.
+// The parts of split walks: out = sum 2^(m_s - m) O_s / sum 2^(m_s - m) l_s in increasing order of the splits. A warp per row.
 __global__ void __launch_bounds__(256)
 rule16_join_kernel(const __grid_constant__ R16Fwd p) {
   pdl_enter();
@@ -715,7 +679,7 @@ rule16_join_kernel(const __grid_constant__ R16Fwd p) {
     const int i = (int)(row - bh * p.r.lq), bi = (int)(bh / p.h), hi = (int)(bh - (long long)bi * p.h);
     if (p.plain && ld_global(p.plain + bi * p.hkv + hi / (p.h / p.hkv)) != 0) continue;
     float m = -INFINITY;
-    for (int s = 0; s < p.parts; s++) {
+    for (int s = 0; s < p.splits; s++) {
       const float2 v = p.part_ml[s * p.rows + row];
       if (v.y != 0.f) m = fmaxf(m, v.x);
     }
@@ -723,7 +687,7 @@ rule16_join_kernel(const __grid_constant__ R16Fwd p) {
     float l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     const int c = lane * 4;
-    for (int s = 0; s < p.parts; s++) {
+    for (int s = 0; s < p.splits; s++) {
       const float2 v = p.part_ml[s * p.rows + row];
       if (v.y == 0.f) continue;                       // this part saw nothing
       const float f = r16_ex2(v.x - base);
@@ -888,7 +852,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   __syncthreads();
   const int first = tile->lo / R16_T, tiles = max(0, (min(tile->hi, r.lq) + R16_T - 1) / R16_T - first);
   if (warp == 0) {
-    const int n = r16_plan(steps, tiles, lane, false, [&](int t) { return (uint32_t)rule_see<false>(*tile, (first + t) * R16_T, 2); });
+    const int n = r16_plan(steps, tiles, lane, [&](int t) { return (uint32_t)rule_see<false>(*tile, (first + t) * R16_T, 2); });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
@@ -986,7 +950,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     for (int n = 0; ok && n < walk; n++) {
       const uint32_t step = forth(), phase = n & 1u;
       const int a = n % W::RING_A, at = (first + r16_tile_of(step)) * R16_T + half * 64;
-      const bool partial = r16_sees_of(step, 0) == 1;
+      const bool partial = r16_sees_of(step) == 1;
       const R16Score score = r16_score_of<MODE>(r, hk * group + gi, unit);
       const float* rows = ring_rows + a * 256 + half * 64;
       // The queries' log-sum-exps came with the queries, which the scores have waited for; this wait makes them seen here.
@@ -1112,7 +1076,7 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __syncthreads();
   const int first = tile->pre > 0 ? 0 : tile->lo / R16_T, tiles = max(0, (min(max(tile->pre, tile->hi), r.lk) + R16_T - 1) / R16_T - first);
   if (warp == 0) {
-    const int n = r16_plan(steps, tiles, lane, false, [&](int t) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T, 2); });
+    const int n = r16_plan(steps, tiles, lane, [&](int t) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T, 2); });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
@@ -1186,7 +1150,7 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     for (int n = 0; ok && n < walk; n++) {
       const uint32_t step = steps[n], place = n & 1u, phase = (n >> 1) & 1u, t_s = lane_base + COL_S + 128u * place + 64u * half;
       const int at = (first + r16_tile_of(step)) * R16_T + half * 64;
-      const bool partial = r16_sees_of(step, 0) == 1;
+      const bool partial = r16_sees_of(step) == 1;
       if (!(ok = r16_wait(&bar_s[place], phase, abort_flag, p.status, 91))) break;
       tc_fence_after();
       uint32_t x[2][32], dp[2][32], w[16], wl[16];
@@ -1320,7 +1284,7 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
   }
   // Heads that share keys as rows of one tile where they fit it: keys and values are read once for all of them.
   p.packed = (long long)group * lq <= R16_T && (group > 1);
-  dim3 grid((unsigned)(c.b * (p.packed ? c.hkv : c.h)), p.packed ? 1u : (unsigned)ceil_div(lq, 2 * R16_T), 1);
+  dim3 grid((unsigned)(c.b * (p.packed ? c.hkv : c.h)), p.packed ? 1u : (unsigned)ceil_div(lq, R16_T), 1);
   // A walk is split where the CTAs leave SMs without one, four tiles of keys a part at least: a part costs its CTA's start and a
   // row of O per query in memory, twice.
   const int64_t ctas = (int64_t)grid.x * grid.y;
@@ -1329,21 +1293,19 @@ int32_t rule16_fwd(om_ctx* ctx, const RuleCall& c, const void* q, const om_head_
   p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count / std::max<int64_t>(ctas, 1), tiles / 4));
   p.splits = (int)std::max<int64_t>(p.splits, ceil_div(ceil_div(lk, R16_T) + 1, R16_PLAN));   // a part is at most a plan long
   grid.z = (unsigned)p.splits;
-  p.twin = (p.packed || lq <= R16_T) && (p.splits > 1 || tiles >= 8);
-  p.parts = p.splits << p.twin;
   CUtensorMap mq, mk, mv;
   if (!r16_map(&mq, q, width, lq, c.h, c.b, qs, p.packed ? lq : R16_T, p.packed ? group : 1) || !r16_map(&mk, k, width, lk, c.hkv, c.b, ks, R16_T, 1) ||
       !r16_map(&mv, v, width, lk, c.hkv, c.b, vs, R16_T, 1))
     return fail(ctx, OM_ERR_CUDA, "cuTensorMapEncodeTiled failed for the operands of om_rule_attention_fwd");
   char* part = nullptr;
-  if (p.parts > 1) {
-    const size_t ml = ((size_t)p.parts * p.rows * sizeof(float2) + 255) & ~(size_t)255;
-    OM_TRY(pool_alloc(ctx, ml + (size_t)p.parts * p.rows * c.d * sizeof(float), false, (void**)&part));
+  if (p.splits > 1) {
+    const size_t ml = ((size_t)p.splits * p.rows * sizeof(float2) + 255) & ~(size_t)255;
+    OM_TRY(pool_alloc(ctx, ml + (size_t)p.splits * p.rows * c.d * sizeof(float), false, (void**)&part));
     p.part_ml = reinterpret_cast<float2*>(part);
     p.part = reinterpret_cast<float*>(part + ml);
   }
   const int32_t st = planes ? r16_fwd_by_mode<64, 2>(ctx, grid, mq, mk, mv, p) : c.d <= 64 ? r16_fwd_by_mode<64, 1>(ctx, grid, mq, mk, mv, p) : r16_fwd_by_mode<128, 1>(ctx, grid, mq, mk, mv, p);
-  if (p.parts > 1) {
+  if (p.splits > 1) {
     if (st == OM_OK) launch_chained(ctx, rule16_join_kernel, grid_for(ctx, p.rows, 8), 256, 0, p);
     pool_free(ctx, part);
   }

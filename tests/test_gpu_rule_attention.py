@@ -213,7 +213,7 @@ def test_large_fp32_call_with_few_queries_and_a_split_walk(ctx):
     (False, 2, 4, 2, 3, 1200, 64, dict(causal=True, q_offset=5)),
     (True, 2, 4, 2, 3, 1200, 96, dict(causal=True, q_offset=-10)),                # none
 ])
-def test_one_tile_of_queries_walks_twice_as_fast(ctx, half, b, h, hk, lq, lk, d, kw):
+def test_few_queries_and_many_keys(ctx, half, b, h, hk, lq, lk, d, kw):
     r = np.random.default_rng(63)
     Call(ctx, r, b, h, hk, lq, lk, d, half=half, **kw).run(False).check(False)
 
