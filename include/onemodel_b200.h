@@ -575,7 +575,8 @@ typedef struct om_attention_rule {
  * addressed through om_head_strides; d is 1 to 256. Operands, sums and exponentials keep fp32 accuracy whatever the context's flags:
  * products are fp32, or, where d is a multiple of 8 up to 64 and there are 96 keys (backward: keys or queries) or more, tensor products
  * of two half-precision numbers a value, 22 bits. Which of the two depends on nothing but sizes, alignment and, for each head of k
- * and v by itself, on whether its rows are within 2^14 of the largest.
+ * and v by itself, on whether its rows (and those of its queries and output gradients) are within 2^14 of the largest of their tensor,
+ * which itself lies within 2^-46 to 2^45.
  * lse [b, h, lq] (may be NULL) receives the row log-sum-exp for the backward. lk == 0 gives zeros. */
 int32_t om_rule_attention_fwd(om_ctx* ctx, const om_attention_rule* rule, const float* q, const om_head_strides* qs, const float* k,
                               const om_head_strides* ks, const float* v, const om_head_strides* vs, int32_t b, int32_t h,

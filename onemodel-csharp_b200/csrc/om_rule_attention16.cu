@@ -21,7 +21,7 @@
 // h + l, 22 significant bits, side by side in a row of 128 columns where two blocks of 64 lie otherwise, and a product as h h' + h l' +
 // l h'. Weights and gradients of scores are taken apart the same way. A power of two per (batch, key head) brings each operand's
 // largest value to 2^14 ... 2^15, so values down to 2^-14 of it keep all 22 bits; rule16_split_kernel, which makes the planes, sets a flag
-// where a row's own largest is smaller than that (or not finite), and then these kernels do nothing and the fp32 ones behind them work.
+// where a row's own largest is smaller than that (or the largest of all beyond 2^45, or not finite), and then these kernels do nothing and the fp32 ones behind them work.
 //
 // What a CTA sees of the other axis is worked out before its walk, a byte per 128 indices: worked out along the way it cost the rows as
 // much as their exponentials. Every wait is bounded (om_tc.cuh). All sums are fp32 in an order that the shapes alone decide.
@@ -1449,9 +1449,10 @@ __global__ void __launch_bounds__(256) rule16_split_kernel(const __grid_constant
   uint32_t mine = r16_largest(v);
   mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
   mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
-  // The largest goes to 2^14 ... 2^15. Units beyond 2^+-60 would leave fp32 in their products.
+  // The largest goes to 2^14 ... 2^15. Units below 2^-60 would leave fp32 in their products, and so would, above 2^30 (values of 2^45), the
+  // squares of a row and what is bounded by their roots.
   const int e = top == 0 ? 0 : (int)(top >> 23) - 127 - 14;
-  const bool fits = top < 0x7f800000u && e >= -60 && e <= 60;
+  const bool fits = top < 0x7f800000u && e >= -60 && e <= 30;
   const bool far = mine != 0 && (mine >> 23) + 14 < (top >> 23);
   if ((threadIdx.x & 3) == 0 && (!fits || far)) p.plain[bi * p.hkv + hk] = 1;
   const float unit = __uint_as_float((uint32_t)((fits ? e : 0) + 127) << 23), to = __uint_as_float((uint32_t)(127 - (fits ? e : 0)) << 23);

@@ -1,0 +1,43 @@
+"""Attention by rule where values are far apart, huge or tiny, caps large and padding not a number: against the formulas in 64 bits, with
+bounds that follow from the precision promised and not from how a kernel gets there."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import om_binding as omb
+import rule_reference as ref
+from om_binding import f32, i32
+from test_gpu_rule_attention import Call
+
+pytestmark = pytest.mark.gpu
+
+
+def put(c, name, value):
+    """Another value of one operand of a call in the layout of rows."""
+    c.value[name] = ref.from_bf16(ref.to_bf16(value)) if c.half else value.astype(np.float32)
+    c.dev[name] = c.put(c.value[name].transpose(0, 2, 1, 3))
+
+
+def wanted(c):
+    b, h, hk, lq, lk, d = c.dims
+    seen = ref.visible(b, lq, lk, c.causal, c.window, c.q_offset, c.prefix, c.qd, c.kd)
+    v = c.value
+    return ref.attention(v["q"], v["k"], v["v"], v["g"], seen, c.scale, c.softcap, c.slopes, c.q_offset, c.half)
+
+
+def row_errors(got, want):
+    """Each row's error over the row, in the Euclidean norm."""
+    return np.linalg.norm(got - want, axis=-1) / np.maximum(np.linalg.norm(want, axis=-1), 1e-300)
+
+
+@pytest.mark.parametrize("names,size", [("v", 1e19), ("g", 1e20), ("v", 1e22), ("q", 1e19), ("vg", 3e17)])
+def test_huge_values_in_every_row(ctx, names, size):
+    """All rows alike, so nothing is far apart, in a call long enough for two half-precision numbers a value."""
+    r = np.random.default_rng(70)
+    c = Call(ctx, r, 1, 4, 2, 300, 300, 64, causal=True)
+    for n in names:
+        put(c, n, c.value[n] * np.float32(size))
+    if names == "q":
+        put(c, "k", c.value["k"] * np.float32(1 / size))
+    c.run().check(planes=False)
