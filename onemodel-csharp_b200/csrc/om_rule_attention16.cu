@@ -19,9 +19,10 @@
 //
 // fp32 operands of heads up to 64 columns run on the same kernels (PL = 2) with fp32 accuracy: every value as two half-precision numbers
 // h + l, 22 significant bits, side by side in a row of 128 columns where two blocks of 64 lie otherwise, and a product as h h' + h l' +
-// l h'. Weights and gradients of scores are taken apart the same way. A power of two per (batch, key head) brings each operand's
-// largest value to 2^14 ... 2^15, so values down to 2^-14 of it keep all 22 bits; rule16_split_kernel, which makes the planes, sets a flag
-// where a row's own largest is smaller than that (or the largest of all beyond 2^45, or not finite), and then these kernels do nothing and the fp32 ones behind them work.
+// l h'. Weights and gradients of scores are taken apart the same way, the gradients of each row and step over a power of two of their own. A
+// power of two per (batch, key head) brings each operand's largest value to 2^14 ... 2^15, so values down to 2^-14 of it keep all 22 bits;
+// rule16_split_kernel, which makes the planes, sets a flag where a row's own largest is smaller than that (or the largest of all beyond
+// 2^45, or not finite), and then these kernels do nothing and the fp32 ones behind them work.
 //
 // What a CTA sees of the other axis is worked out before its walk, a byte per 128 indices: worked out along the way it cost the rows as
 // much as their exponentials. Every wait is bounded (om_tc.cuh). All sums are fp32 in an order that the shapes alone decide.
@@ -152,18 +153,24 @@ __device__ __forceinline__ void r16_gather(uint32_t d, uint32_t a, uint32_t b_mn
     r16_mma_ts(d, h, b, idesc, PL == 2 || ks > 0 ? 1u : accumulate);
   }
 }
-__device__ __forceinline__ void r16_add_whole(uint32_t whole, uint32_t (&o)[32]) {
+// The last step, which is in o: o = whole keep + o unit.
+__device__ __forceinline__ void r16_add_whole(uint32_t whole, uint32_t (&o)[32], bool only, float keep, float unit) {
   uint32_t w[32];
-  tmem_ld_32x32b_x32(whole, w);
-  tmem_ld_wait();
+  if (!only) {
+    tmem_ld_32x32b_x32(whole, w);
+    tmem_ld_wait();
+  }
 #pragma unroll
-  for (int u = 0; u < 32; u++) o[u] = __float_as_uint(__uint_as_float(w[u]) + __uint_as_float(o[u]));
+  for (int u = 0; u < 32; u++) {
+    const float mine = __uint_as_float(o[u]) * unit;
+    o[u] = __float_as_uint(only ? mine : fmaf(__uint_as_float(w[u]), keep, mine));
+  }
 }
 // Two planes: the tensor core's own sums over a walk of thousands would lose digits (8 additions that are cut off, a tile, 2e-7; 192
-// of them 5e-6), so each step's product is a sum of its own, which the rows add to the whole in fp32: whole = (whole + step) factor,
+// of them 5e-6), so each step's product is a sum of its own, which the rows add to the whole in fp32: whole = whole keep + step unit,
 // COLS columns of both in tensor memory.
 template <int COLS>
-__device__ __forceinline__ void r16_fold(uint32_t whole, uint32_t step, bool first, float factor) {
+__device__ __forceinline__ void r16_fold(uint32_t whole, uint32_t step, bool first, float keep, float unit) {
 #pragma unroll 1
   for (int c = 0; c < COLS; c += 16) {
     uint32_t a[16], b[16];
@@ -172,8 +179,8 @@ __device__ __forceinline__ void r16_fold(uint32_t whole, uint32_t step, bool fir
     tmem_ld_wait();
 #pragma unroll
     for (int u = 0; u < 16; u++) {
-      const float sum = first ? __uint_as_float(a[u]) : __uint_as_float(b[u]) + __uint_as_float(a[u]);
-      a[u] = __float_as_uint(sum * factor);
+      const float mine = __uint_as_float(a[u]) * unit;
+      a[u] = __float_as_uint(first ? mine : fmaf(__uint_as_float(b[u]), keep, mine));
     }
     r16_st16(whole + (uint32_t)c, a);
   }
@@ -604,7 +611,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ok = r16_wait(&bar_o[place ^ 1u], ((n - 1) >> 1) & 1u, abort_flag, p.status, 69);
         tc_fence_after();
         if (PL == 2) {
-          r16_fold<DP / 2>(t_o + 64u, t_o, n == 1, shrink);
+          r16_fold<DP / 2>(t_o + 64u, t_o, n == 1, shrink, shrink);
         } else {
 #pragma unroll 1
           for (int c = 0; c < DP / 2; c += 32) {
@@ -651,7 +658,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
           tmem_ld_wait();
         }
-        if (PL == 2 && walk > 1) r16_add_whole(t_o + 64u + (uint32_t)c, o);
+        if (PL == 2 && walk > 0) r16_add_whole(t_o + 64u + (uint32_t)c, o, walk == 1, 1.f, 1.f);
         if (walk == 0 || l == 0.f) {
 #pragma unroll
           for (int u = 0; u < 32; u++) o[u] = 0u;
@@ -731,7 +738,8 @@ struct R16BwdShape {
   static constexpr int TILE = r16_tile_bytes<DP, PL>();
   static constexpr int RING_A = TILE == R16_CHUNK ? 4 : KEYS ? 2 : 3, RING_B = TILE == R16_CHUNK ? 4 : 2;
   static constexpr int ROWS = (2 + RING_A + RING_B) * TILE;     // the queries' log-sum-exps and row dots, 1 KB a stage
-  static constexpr int RULES = ROWS + (KEYS ? RING_A * 1024 : 0);
+  static constexpr int TURN = ROWS + (KEYS ? RING_A * 1024 : 0);   // two planes: what the two warps of a row tell each other, [place][half][row]
+  static constexpr int RULES = TURN + (PL == 2 ? 512 : 0);
   static constexpr int PLAN = RULES + 64;
   static constexpr int BARS = PLAN + R16_PLAN * 2 + 16;
   static constexpr int SMEM = BARS + 256;
@@ -769,12 +777,9 @@ __device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)
     for (int t = 0; t < 4; t++) x[u + t] = __float_as_uint(MODE == 2 ? p[t] == 0.f ? 0.f : p[t] * dcap[MODE == 2 ? u + t : 0] : p[t]);
   }
 }
-// dS = weight (dP - dot), 32 of them, packed. partial: some are hidden, and 0 whatever dP is there.
-// Two planes: dP comes times `down`, the dots times dot_down, and the gradients go into w and wl.
+// dS = weight (dP - dot), 32 of them, in v. partial: some are hidden, and 0 whatever dP is there. dP comes over `unit` (two planes).
 template <bool COLUMNS, int PL>
-__device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uint32_t (&dp)[32], uint32_t (&w)[16], uint32_t (&wl)[16], const float* dots, float dot,
-                                              float down, float dot_down, bool partial) {
-  float v[32];
+__device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uint32_t (&dp)[32], float (&v)[32], const float* dots, float dot, float unit, bool partial) {
 #pragma unroll
   for (int u = 0; u < 32; u += 4) {
     float d[4] = {dot, dot, dot, dot};
@@ -784,17 +789,52 @@ __device__ __forceinline__ void r16_gradients(const uint32_t (&x)[32], const uin
     }
 #pragma unroll
     for (int t = 0; t < 4; t++)
-      v[u + t] = __uint_as_float(x[u + t]) * (PL == 2 ? fmaf(__uint_as_float(dp[u + t]), down, -(d[t] * dot_down)) : __uint_as_float(dp[u + t]) - d[t]);
+      v[u + t] = __uint_as_float(x[u + t]) * (PL == 2 ? fmaf(__uint_as_float(dp[u + t]), unit, -d[t]) : __uint_as_float(dp[u + t]) - d[t]);
   }
   if (partial) {
 #pragma unroll
     for (int u = 0; u < 32; u++) v[u] = x[u] == 0u ? 0.f : v[u];
   }
+}
+template <bool COLUMNS>
+__device__ __forceinline__ void r16_gradients16(const uint32_t (&x)[32], const uint32_t (&dp)[32], uint32_t (&w)[16], const float* dots, float dot, bool partial) {
+  float v[32];
+  r16_gradients<COLUMNS, 1>(x, dp, v, dots, dot, 1.f, partial);
+#pragma unroll
+  for (int u = 0; u < 32; u += 2) w[u / 2] = r16_pack(v[u], v[u + 1]);
+}
+// Two planes: a row's gradients of a step over a power of two of their own, which brings the largest of them to 2^14 ... 2^15, whatever
+// it is: a unit for the whole head, from bounds of |dO| and |V|, left few digits to the rows far below the bound (a row of dO at 2^-13 of the
+// largest: its dQ off by 2e-4). The row's two warps tell each other the exponent of the largest, in a byte; 255: a wait ran out.
+struct R16Unit {
+  float to, back;                                        // the power of two that the row is multiplied with, and the one that undoes it
+};
+__device__ __forceinline__ R16Unit r16_unit(uint32_t exponent) {
+  const uint32_t e = max(exponent, 15u);
+  return R16Unit{__uint_as_float((268u - e) << 23), __uint_as_float((e - 14u) << 23)};
+}
+__device__ __forceinline__ bool r16_share(uint8_t* turn, int half, int row, int quad, bool ok, uint32_t& exponent) {
+  exponent = min(exponent, 254u);
+  turn[128 * half + row] = (uint8_t)(ok ? exponent : 255u);
+  r16_meet(1 + quad);
+  const uint32_t theirs = turn[128 * (half ^ 1) + row];
+  exponent = max(exponent, theirs);
+  return __all_sync(0xffffffffu, ok && theirs != 255u);
+}
+template <bool COLUMNS>
+__device__ __forceinline__ void r16_gradients2(uint32_t (&x)[32], const uint32_t (&dp)[32], const float* dots, float dot, float unit, bool partial, float& largest) {
+  float v[32];
+  r16_gradients<COLUMNS, 2>(x, dp, v, dots, dot, unit, partial);
 #pragma unroll
   for (int u = 0; u < 32; u += 2) {
-    if (PL == 2) r16_take_apart(v[u], v[u + 1], &w[u / 2], &wl[u / 2]);
-    else w[u / 2] = r16_pack(v[u], v[u + 1]);
+    largest = r16_max3(largest, fabsf(v[u]), fabsf(v[u + 1]));
+    x[u] = __float_as_uint(v[u]);
+    x[u + 1] = __float_as_uint(v[u + 1]);
   }
+}
+__device__ __forceinline__ void r16_apart(const uint32_t (&x)[32], float to, uint32_t (&h)[16], uint32_t (&l)[16]) {
+#pragma unroll
+  for (int u = 0; u < 32; u += 2) r16_take_apart(__uint_as_float(x[u]) * to, __uint_as_float(x[u + 1]) * to, &h[u / 2], &l[u / 2]);
 }
 
 template <int DP, int MODE, int PL>
@@ -940,12 +980,13 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t t_s = lane_base + COL_S + 64u * half, t_dp = lane_base + COL_DP + 64u * half;
     const R16Row seen = r16_key_row(r, prefix, bi, min(j, r.lk - 1));
     const int32_t* docs = r.q_docs ? r.q_docs + (long long)bi * r.lq : nullptr;
-    // Units of the planes. Weights are kept times 2^14, gradients of scores over a power of two that is at least 2^-15 of their bound,
-    // 2 max |g| max |v|: both stay below 2^15 whatever the values are, and small ones keep their digits.
+    // Units of the planes. Weights are kept times 2^14.
     const int at_unit = bi * p.hkv + hk, n_units = p.units_n;
     const float unit_q = PL == 2 ? p.units[at_unit] : 1.f, unit_k = PL == 2 ? p.units[n_units + at_unit] : 1.f, unit_v = PL == 2 ? p.units[2 * n_units + at_unit] : 1.f,
-                unit_g = PL == 2 ? p.units[3 * n_units + at_unit] : 1.f, unit = unit_q * unit_k, up = PL == 2 ? p.units[4 * n_units + at_unit] : 1.f;
-    const float lift = PL == 2 ? 14.f : 0.f, dot_down = PL == 2 ? 0x1p-14f / up : 1.f, down = PL == 2 ? dot_down * (unit_g * unit_v) : 1.f;
+                unit_g = PL == 2 ? p.units[3 * n_units + at_unit] : 1.f, unit = unit_q * unit_k;
+    const float lift = PL == 2 ? 14.f : 0.f;
+    uint8_t* turn = smem + W::TURN;
+    float unit_dk = 1.f;                                   // of the step's product that is not yet added to the whole
     const float mult = MODE ? 1.f : r.scale * unit * R16_LOG2E;
     for (int n = 0; ok && n < walk; n++) {
       const uint32_t step = forth(), phase = n & 1u;
@@ -954,10 +995,11 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       const R16Score score = r16_score_of<MODE>(r, hk * group + gi, unit);
       const float* rows = ring_rows + a * 256 + half * 64;
       // The queries' log-sum-exps came with the queries, which the scores have waited for; this wait makes them seen here.
-      if (!(ok = r16_wait(&full_q[a], (n / W::RING_A) & 1u, abort_flag, p.status, 94) && r16_wait(bar_s, phase, abort_flag, p.status, 80))) break;
+      ok = r16_wait(&full_q[a], (n / W::RING_A) & 1u, abort_flag, p.status, 94) && r16_wait(bar_s, phase, abort_flag, p.status, 80);
+      if (PL == 1 && !ok) break;                           // two planes: both warps of a row leave together, below
       tc_fence_after();
       // The scores came after the product before, and the next one waits for these weights.
-      if (PL == 2 && n > 0) r16_fold<32>(lane_base + COL_DV + 64u + 32u * half, lane_base + COL_DV + 32u * half, n == 1, 1.f);
+      if (PL == 2 && n > 0) r16_fold<32>(lane_base + COL_DV + 64u + 32u * half, lane_base + COL_DV + 32u * half, n == 1, 1.f, 1.f);
       uint32_t x[2][32], w[16], wl[16];
       tmem_ld_32x32b_x32(t_s, x[0]);
       tmem_ld_32x32b_x32(t_s + 32u, x[1]);
@@ -970,20 +1012,40 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
       r16_st_wait();
       r16_arrive_warp(bar_p, lane);
-      if (!(ok = r16_wait(bar_dp, phase, abort_flag, p.status, 81))) break;
+      ok = ok && r16_wait(bar_dp, phase, abort_flag, p.status, 81);
+      if (PL == 1 && !ok) break;
       tc_fence_after();
-      if (PL == 2 && n > 0) r16_fold<32>(lane_base + COL_DK + 64u + 32u * half, lane_base + COL_DK + 32u * half, n == 1, 1.f);
-      uint32_t dp[2][32];
-      tmem_ld_32x32b_x32(t_dp, dp[0]);
-      tmem_ld_wait();
-      tmem_ld_32x32b_x32(t_dp + 32u, dp[1]);
-      r16_gradients<true, PL>(x[0], dp[0], w, wl, rows + 128, 0.f, down, dot_down, partial);
-      tmem_ld_wait();
-      r16_st16(t_dp, w);
-      if (PL == 2) r16_st16(t_dp + 16u, wl);
-      r16_gradients<true, PL>(x[1], dp[1], w, wl, rows + 160, 0.f, down, dot_down, partial);
-      r16_st16(t_dp + (PL == 2 ? 32u : 16u), w);
-      if (PL == 2) r16_st16(t_dp + 48u, wl);
+      if (PL == 2) {
+        if (n > 0) r16_fold<32>(lane_base + COL_DK + 64u + 32u * half, lane_base + COL_DK + 32u * half, n == 1, 1.f, unit_dk);
+        float largest = 0.f;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          uint32_t dp[32];
+          tmem_ld_32x32b_x32(t_dp + 32u * c, dp);
+          tmem_ld_wait();
+          r16_gradients2<true>(x[c], dp, rows + 128 + 32 * c, 0.f, unit_g * unit_v, partial, largest);
+        }
+        uint32_t exponent = __float_as_uint(largest) >> 23;
+        if (!(ok = r16_share(turn + 256 * phase, half, row, quad, ok, exponent))) break;
+        const R16Unit step_unit = r16_unit(exponent);
+        unit_dk = step_unit.back * 0x1p-14f;               // the weights' factor is in them
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          r16_apart(x[c], step_unit.to, w, wl);
+          r16_st16(t_dp + 32u * c, w);
+          r16_st16(t_dp + 32u * c + 16u, wl);
+        }
+      } else {
+        uint32_t dp[2][32];
+        tmem_ld_32x32b_x32(t_dp, dp[0]);
+        tmem_ld_wait();
+        tmem_ld_32x32b_x32(t_dp + 32u, dp[1]);
+        r16_gradients16<true>(x[0], dp[0], w, rows + 128, 0.f, partial);
+        tmem_ld_wait();
+        r16_st16(t_dp, w);
+        r16_gradients16<true>(x[1], dp[1], w, rows + 160, 0.f, partial);
+        r16_st16(t_dp + 16u, w);
+      }
       r16_st_wait();
       r16_arrive_warp(bar_ds, lane);
     }
@@ -1002,12 +1064,12 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (walk > 0) {
             tmem_ld_32x32b_x32(lane_base + (half == 0 ? COL_DV : COL_DK) + (uint32_t)c, o);
             tmem_ld_wait();
-            if (PL == 2 && walk > 1) r16_add_whole(lane_base + (half == 0 ? COL_DV : COL_DK) + 64u + (uint32_t)c, o);
+            if (PL == 2) r16_add_whole(lane_base + (half == 0 ? COL_DV : COL_DK) + 64u + (uint32_t)c, o, walk == 1, 1.f, half == 0 ? 1.f : unit_dk);
           } else {
 #pragma unroll
             for (int u = 0; u < 32; u++) o[u] = 0u;
           }
-          if (j < r.lk) r16_write(o, half == 0 ? unit_g * (PL == 2 ? 0x1p-14f : 1.f) : r.scale * unit_q * up, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
+          if (j < r.lk) r16_write(o, half == 0 ? unit_g * (PL == 2 ? 0x1p-14f : 1.f) : r.scale * unit_q, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
         }
       }
     }
@@ -1140,8 +1202,9 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint32_t lane_base = tmem + ((uint32_t)(quad * 32) << 16), t_dp = lane_base + COL_DP + 64u * half;
     const int at_unit = bi * p.hkv + hk, n_units = p.units_n;    // as in rule16_dkv_kernel
     const float unit_q = PL == 2 ? p.units[at_unit] : 1.f, unit_k = PL == 2 ? p.units[n_units + at_unit] : 1.f, unit_v = PL == 2 ? p.units[2 * n_units + at_unit] : 1.f,
-                unit_g = PL == 2 ? p.units[3 * n_units + at_unit] : 1.f, unit = unit_q * unit_k, up = PL == 2 ? p.units[4 * n_units + at_unit] : 1.f;
-    const float dot_down = PL == 2 ? 1.f / up : 1.f, down = PL == 2 ? dot_down * (unit_g * unit_v) : 1.f;
+                unit_g = PL == 2 ? p.units[3 * n_units + at_unit] : 1.f, unit = unit_q * unit_k;
+    uint8_t* turn = smem + W::TURN;
+    float unit_dq = 1.f;
     const R16Score score = r16_score_of<MODE>(r, hi, unit);
     const R16Row seen = r16_query_row(r, prefix, bi, min(i, r.lq - 1));
     const int32_t* docs = r.k_docs ? r.k_docs + (long long)bi * r.lk : nullptr;
@@ -1151,32 +1214,56 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       const uint32_t step = steps[n], place = n & 1u, phase = (n >> 1) & 1u, t_s = lane_base + COL_S + 128u * place + 64u * half;
       const int at = (first + r16_tile_of(step)) * R16_T + half * 64;
       const bool partial = r16_sees_of(step) == 1;
-      if (!(ok = r16_wait(&bar_s[place], phase, abort_flag, p.status, 91))) break;
+      ok = r16_wait(&bar_s[place], phase, abort_flag, p.status, 91);
+      if (PL == 1 && !ok) break;                           // two planes: both warps of a row leave together, below
       tc_fence_after();
-      uint32_t x[2][32], dp[2][32], w[16], wl[16];
+      uint32_t x[2][32], w[16], wl[16];
       tmem_ld_32x32b_x32(t_s, x[0]);
       tmem_ld_32x32b_x32(t_s + 32u, x[1]);
       tmem_ld_wait();
 #pragma unroll
       for (int c = 0; c < 2; c++)
         r16_weights<MODE, false, PL>(score, x[c], w, wl, nullptr, stat.x, 0.f, (float)(i + r.q_offset - at - c * 32), mult, partial, seen, at + c * 32, docs);
-      if (!(ok = r16_wait(bar_dp, n & 1u, abort_flag, p.status, 92))) break;
+      ok = ok && r16_wait(bar_dp, n & 1u, abort_flag, p.status, 92);
+      if (PL == 1 && !ok) break;
       tc_fence_after();
-      if (PL == 2 && n > 0) {
-        // The product before; the next one waits for these gradients.
-        if (!(ok = r16_wait(&bar_dq[place ^ 1u], ((n - 1) >> 1) & 1u, abort_flag, p.status, 95))) break;
-        tc_fence_after();
-        r16_fold<32>(lane_base + COL_DQ + 64u + 32u * half, lane_base + COL_DQ + 32u * half, n == 1, 1.f);
-      }
-      tmem_ld_32x32b_x32(t_dp, dp[0]);
-      tmem_ld_32x32b_x32(t_dp + 32u, dp[1]);
-      tmem_ld_wait();
-      r16_arrive_warp(read_dp, lane);
+      if (PL == 2) {
+        if (n > 0) {
+          // The product before; the next one waits for these gradients.
+          ok = ok && r16_wait(&bar_dq[place ^ 1u], ((n - 1) >> 1) & 1u, abort_flag, p.status, 95);
+          tc_fence_after();
+          r16_fold<32>(lane_base + COL_DQ + 64u + 32u * half, lane_base + COL_DQ + 32u * half, n == 1, 1.f, unit_dq);
+        }
+        float largest = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; c++) {
-        r16_gradients<false, PL>(x[c], dp[c], w, wl, nullptr, stat.y, down, dot_down, partial);
-        r16_st16(t_s + (PL == 2 ? 32u : 16u) * c, w);
-        if (PL == 2) r16_st16(t_s + 32u * c + 16u, wl);
+        for (int c = 0; c < 2; c++) {
+          uint32_t dp[32];
+          tmem_ld_32x32b_x32(t_dp + 32u * c, dp);
+          tmem_ld_wait();
+          r16_gradients2<false>(x[c], dp, nullptr, stat.y, unit_g * unit_v, partial, largest);
+        }
+        r16_arrive_warp(read_dp, lane);
+        uint32_t exponent = __float_as_uint(largest) >> 23;
+        if (!(ok = r16_share(turn + 256 * place, half, row, quad, ok, exponent))) break;
+        const R16Unit step_unit = r16_unit(exponent);
+        unit_dq = step_unit.back;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          r16_apart(x[c], step_unit.to, w, wl);
+          r16_st16(t_s + 32u * c, w);
+          r16_st16(t_s + 32u * c + 16u, wl);
+        }
+      } else {
+        uint32_t dp[2][32];
+        tmem_ld_32x32b_x32(t_dp, dp[0]);
+        tmem_ld_32x32b_x32(t_dp + 32u, dp[1]);
+        tmem_ld_wait();
+        r16_arrive_warp(read_dp, lane);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          r16_gradients16<false>(x[c], dp[c], w, nullptr, stat.y, partial);
+          r16_st16(t_s + 16u * c, w);
+        }
       }
       r16_st_wait();
       r16_arrive_warp(&bar_ds[place], lane);
@@ -1192,12 +1279,12 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         if (walk > 0) {
           tmem_ld_32x32b_x32(lane_base + COL_DQ + (uint32_t)c, o);
           tmem_ld_wait();
-          if (PL == 2 && walk > 1) r16_add_whole(lane_base + COL_DQ + 64u + (uint32_t)c, o);
+          if (PL == 2) r16_add_whole(lane_base + COL_DQ + 64u + (uint32_t)c, o, walk == 1, 1.f, unit_dq);
         } else {
 #pragma unroll
           for (int u = 0; u < 32; u++) o[u] = 0u;
         }
-        if (i < r.lq) r16_write(o, r.scale * unit_k * up, p.d0, p.d0_16, bi * p.s0.batch + hi * p.s0.head + (long long)i * p.s0.row + c, c, p.d);
+        if (i < r.lq) r16_write(o, r.scale * unit_k, p.d0, p.d0_16, bi * p.s0.batch + hi * p.s0.head + (long long)i * p.s0.row + c, c, p.d);
       }
     }
   }
@@ -1378,8 +1465,8 @@ struct R16Source {
 struct R16Split {
   R16Source t[4];                 // q, k, v, g
   int d, hkv, b;
-  uint32_t* top;                  // [4][b * hkv] bits of the largest absolute value, then [4][b * hkv] of the largest row's sum of squares
-  float* units;                   // [5][b * hkv]: of q, k, v, g and of the gradients of scores
+  uint32_t* top;                  // [4][b * hkv] bits of the largest absolute value
+  float* units;                   // [4][b * hkv]: of q, k, v and g
   int32_t* plain;                 // [b * hkv]
 };
 constexpr int R16_SPLIT_ROWS = 64;
@@ -1414,27 +1501,14 @@ __global__ void __launch_bounds__(256) rule16_largest_kernel(const __grid_consta
   float v[16];
   r16_fetch(p, t, bh, row, v);
   uint32_t m = __reduce_max_sync(0xffffffffu, r16_largest(v));
-  float squares = 0.f;
-#pragma unroll
-  for (int u = 0; u < 16; u++) squares = fmaf(v[u], v[u], squares);
-  squares += __shfl_xor_sync(0xffffffffu, squares, 1);
-  squares += __shfl_xor_sync(0xffffffffu, squares, 2);
-  uint32_t s = __reduce_max_sync(0xffffffffu, __float_as_uint(squares) & 0x7fffffffu);
-  __shared__ uint32_t all[16];
-  if ((threadIdx.x & 31) == 0) {
-    all[threadIdx.x >> 5] = m;
-    all[8 + (threadIdx.x >> 5)] = s;
-  }
+  __shared__ uint32_t all[8];
+  if ((threadIdx.x & 31) == 0) all[threadIdx.x >> 5] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 8; w++) {
-      m = max(m, all[w]);
-      s = max(s, all[8 + w]);
-    }
+    for (int w = 1; w < 8; w++) m = max(m, all[w]);
     const int bi = bh / t.heads, hk = (bh - bi * t.heads) / (t.heads / p.hkv);
     const int at = ((int)blockIdx.z * p.b + bi) * p.hkv + hk;
     atomicMax(&p.top[at], m);                            // whole numbers: the order does not matter
-    atomicMax(&p.top[4 * p.b * p.hkv + at], s);
   }
 }
 __global__ void __launch_bounds__(256) rule16_split_kernel(const __grid_constant__ R16Split p) {
@@ -1450,22 +1524,13 @@ __global__ void __launch_bounds__(256) rule16_split_kernel(const __grid_constant
   mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
   mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
   // The largest goes to 2^14 ... 2^15. Units below 2^-60 would leave fp32 in their products, and so would, above 2^30 (values of 2^45), the
-  // squares of a row and what is bounded by their roots.
+  // gradients of scores times half-precision values of 2^15.
   const int e = top == 0 ? 0 : (int)(top >> 23) - 127 - 14;
   const bool fits = top < 0x7f800000u && e >= -60 && e <= 30;
   const bool far = mine != 0 && (mine >> 23) + 14 < (top >> 23);
   if ((threadIdx.x & 3) == 0 && (!fits || far)) p.plain[bi * p.hkv + hk] = 1;
   const float unit = __uint_as_float((uint32_t)((fits ? e : 0) + 127) << 23), to = __uint_as_float((uint32_t)(127 - (fits ? e : 0)) << 23);
-  if (threadIdx.x == 0) {
-    p.units[at] = unit;
-    if (blockIdx.z == 3) {
-      // |dP - dot| <= 2 max |g| max |v|, over 2^14 and up to the next power of two.
-      const int group = bi * p.hkv + hk, n = p.b * p.hkv;
-      const float bound = sqrtf(__uint_as_float(ld_global(p.top + 6 * n + group))) * sqrtf(__uint_as_float(ld_global(p.top + 7 * n + group)));
-      const int eb = (int)(__float_as_uint(bound) >> 23) + 1 - 13;
-      p.units[4 * n + group] = bound == 0.f ? 1.f : __uint_as_float((uint32_t)min(max(eb, 1), 254) << 23);
-    }
-  }
+  if (threadIdx.x == 0) p.units[at] = unit;
   if (row >= t.l) return;
   uint32_t h[8], l[8];
 #pragma unroll
@@ -1492,10 +1557,10 @@ bool rule16_result_fits(const float* p, const om_head_strides* s) { return p == 
 int32_t rule16_planes(om_ctx* ctx, const RuleCall& c, const float* q, const om_head_strides* qs, const float* k, const om_head_strides* ks, const float* v,
                       const om_head_strides* vs, const float* g, const om_head_strides* gs, RulePlanes* out) {
   const size_t nq = (size_t)c.b * c.h * c.r.lq * 128, nk = (size_t)c.b * c.hkv * c.r.lk * 128, units = (size_t)c.b * c.hkv * 4;
-  const size_t head = sizeof(uint32_t) * (2 * units + units / 4), bytes = sizeof(__half) * (nq * (g ? 2 : 1) + 2 * nk);
+  const size_t head = sizeof(uint32_t) * (units + units / 4), bytes = sizeof(__half) * (nq * (g ? 2 : 1) + 2 * nk);
   out->small = out->large = nullptr;
   OM_TRY(pool_alloc(ctx, head, true, &out->small));
-  const int32_t st = pool_alloc(ctx, bytes + sizeof(float) * (units + units / 4), false, &out->large);
+  const int32_t st = pool_alloc(ctx, bytes + sizeof(float) * units, false, &out->large);
   if (st != OM_OK) {
     rule16_planes_end(ctx, out);
     return st;
@@ -1504,7 +1569,7 @@ int32_t rule16_planes(om_ctx* ctx, const RuleCall& c, const float* q, const om_h
   R16Split p = {};
   p.d = c.d; p.hkv = c.hkv; p.b = c.b;
   p.top = reinterpret_cast<uint32_t*>(out->small);
-  p.plain = reinterpret_cast<int32_t*>(p.top + 2 * units);
+  p.plain = reinterpret_cast<int32_t*>(p.top + units);
   auto source = [&](const float* x, const om_head_strides* s, int heads, int l, const int32_t* docs) {
     R16Source t = {};
     t.x = x; t.s = r16_strides(s); t.planes = at; t.heads = heads; t.l = l; t.docs = docs;

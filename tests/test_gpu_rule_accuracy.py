@@ -41,3 +41,40 @@ def test_huge_values_in_every_row(ctx, names, size):
     if names == "q":
         put(c, "k", c.value["k"] * np.float32(1 / size))
     c.run().check(planes=False)
+
+
+# What fp32 arithmetic does to a row of a gradient whose terms are of like size: a product of two pairs of half-precision numbers is within
+# 12 * 2^-24, there are two in a row (dP, dS k), a weight is within 16 * 2^-24 for scores up to 4, and the row dot that is taken from dP has the
+# error of a sum of 64 products once more. 64 * 2^-24 holds them, in norm, whatever the size of the row.
+LIKE_FP32 = 64 * ref.U32
+
+
+@pytest.mark.parametrize("power", [-6, -10, -13])
+def test_a_small_gradient_row_keeps_its_digits(ctx, power):
+    r = np.random.default_rng(71)
+    c = Call(ctx, r, 1, 2, 1, 1024, 1024, 64)
+    rows = [5, 300, 1023]
+    g = c.value["g"].copy()
+    g[:, :, rows] *= np.float32(2.0 ** power)
+    put(c, "g", g)
+    c.run()
+    want, _ = wanted(c)
+    err = row_errors(c.get("dq"), want["dq"])
+    assert err.max() <= LIKE_FP32, (err.max(), err[:, :, rows])
+
+
+@pytest.mark.parametrize("name", ["g", "v"])
+@pytest.mark.parametrize("power", [-8, -13])
+def test_a_document_of_small_values_keeps_its_digits(ctx, name, power):
+    """The second of two documents has small values: its rows of every gradient are as exact as the first one's."""
+    r = np.random.default_rng(72)
+    c = Call(ctx, r, 1, 2, 1, 700, 700, 64, docs=700)
+    c.kd = c.qd = (np.arange(700)[None] >= 350).astype(np.int32)
+    a = c.value[name].copy()
+    a[:, :, 350:] *= np.float32(2.0 ** power)
+    put(c, name, a)
+    c.run()
+    want, _ = wanted(c)
+    for n in ("dq", "dk", "dv"):
+        err = row_errors(c.get(n), want[n])
+        assert err.max() <= LIKE_FP32, (n, err.max(), err[:, :, :350].max())
