@@ -19,7 +19,7 @@
 //
 // fp32 operands of heads up to 64 columns run on the same kernels (PL = 2) with fp32 accuracy: every value as two half-precision numbers
 // h + l, 22 significant bits, side by side in a row of 128 columns where two blocks of 64 lie otherwise, and a product as h h' + h l' +
-// l h'. Weights and gradients of scores are taken apart the same way, the gradients of each row and step over a power of two of their own. A
+// l h'. In the backward weights and gradients of scores are taken apart the same way, those of each row and step over a power of two of their own. A
 // power of two per (batch, key head) brings each operand's largest value to 2^14 ... 2^15, so values down to 2^-14 of it keep all 22 bits;
 // rule16_split_kernel, which makes the planes, sets a flag where a row's own largest is smaller than that (or the largest of all beyond
 // 2^45, or not finite), and then these kernels do nothing and the fp32 ones behind them work.
@@ -749,14 +749,14 @@ struct R16BwdShape {
 // cap's derivative, for r16_gradients. Rows are keys (COLUMNS: the log-sum-exps go with the columns) or queries.
 template <int MODE, bool COLUMNS, int PL>
 __device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)[32], uint32_t (&w)[16], uint32_t (&wl)[16], const float* lses, float lse, float lift, float far, float mult,
-                                            bool partial, const R16Row& seen, int at, const int32_t* docs) {
+                                            bool partial, uint32_t bits) {
   float dcap[MODE == 2 ? 32 : 1];
   if (MODE) {
 #pragma unroll
     for (int u = 0; u < 32; u++)
       x[u] = __float_as_uint(r16_score<MODE>(score, COLUMNS ? far + (float)u : far - (float)u, __uint_as_float(x[u]), &dcap[MODE == 2 ? u : 0]));
   }
-  if (partial) r16_hide(x, r16_bits(seen, at, docs));
+  if (partial) r16_hide(x, bits);
   const uint64_t mult2 = r16_two(mult, mult);
 #pragma unroll
   for (int u = 0; u < 32; u += 4) {
@@ -776,6 +776,19 @@ __device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)
 #pragma unroll
     for (int t = 0; t < 4; t++) x[u + t] = __float_as_uint(MODE == 2 ? p[t] == 0.f ? 0.f : p[t] * dcap[MODE == 2 ? u + t : 0] : p[t]);
   }
+}
+// The largest exponent of the 32 weights of a row whose columns have the log-sum-exps (the scores are formed twice: held, they would not
+// fit the registers beside the cap's derivatives).
+template <int MODE>
+__device__ __forceinline__ float r16_top(const R16Score& score, const uint32_t (&x)[32], const float* lses, float far, float mult, bool partial, uint32_t bits) {
+  float top = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < 32; u++) {
+    float dcap;
+    const float s = MODE ? r16_score<MODE>(score, far + (float)u, __uint_as_float(x[u]), &dcap) - lses[u] : fmaf(__uint_as_float(x[u]), mult, -lses[u]);
+    top = fmaxf(top, partial && !((bits >> u) & 1u) ? -INFINITY : s);
+  }
+  return top;
 }
 // dS = weight (dP - dot), 32 of them, in v. partial: some are hidden, and 0 whatever dP is there. dP comes over `unit` (two planes).
 template <bool COLUMNS, int PL>
@@ -980,13 +993,12 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const uint32_t t_s = lane_base + COL_S + 64u * half, t_dp = lane_base + COL_DP + 64u * half;
     const R16Row seen = r16_key_row(r, prefix, bi, min(j, r.lk - 1));
     const int32_t* docs = r.q_docs ? r.q_docs + (long long)bi * r.lq : nullptr;
-    // Units of the planes. Weights are kept times 2^14.
+    // Units of the planes. The weights of a row and step are kept over a power of two, too: the largest is brought to 2^13 ... 2^14.
     const int at_unit = bi * p.hkv + hk, n_units = p.units_n;
     const float unit_q = PL == 2 ? p.units[at_unit] : 1.f, unit_k = PL == 2 ? p.units[n_units + at_unit] : 1.f, unit_v = PL == 2 ? p.units[2 * n_units + at_unit] : 1.f,
                 unit_g = PL == 2 ? p.units[3 * n_units + at_unit] : 1.f, unit = unit_q * unit_k;
-    const float lift = PL == 2 ? 14.f : 0.f;
     uint8_t* turn = smem + W::TURN;
-    float unit_dk = 1.f;                                   // of the step's product that is not yet added to the whole
+    float lift = 0.f, unit_dv = 1.f, unit_dk = 1.f;        // the units: of the step's products that are not yet added to the whole
     const float mult = MODE ? 1.f : r.scale * unit * R16_LOG2E;
     for (int n = 0; ok && n < walk; n++) {
       const uint32_t step = forth(), phase = n & 1u;
@@ -999,14 +1011,28 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (PL == 1 && !ok) break;                           // two planes: both warps of a row leave together, below
       tc_fence_after();
       // The scores came after the product before, and the next one waits for these weights.
-      if (PL == 2 && n > 0) r16_fold<32>(lane_base + COL_DV + 64u + 32u * half, lane_base + COL_DV + 32u * half, n == 1, 1.f, 1.f);
+      if (PL == 2 && n > 0) r16_fold<32>(lane_base + COL_DV + 64u + 32u * half, lane_base + COL_DV + 32u * half, n == 1, 1.f, unit_dv);
       uint32_t x[2][32], w[16], wl[16];
       tmem_ld_32x32b_x32(t_s, x[0]);
       tmem_ld_32x32b_x32(t_s + 32u, x[1]);
       tmem_ld_wait();
+      uint32_t bits[2] = {~0u, ~0u};
+      if (partial) {
+        bits[0] = r16_bits(seen, at, docs);
+        bits[1] = r16_bits(seen, at + 32, docs);
+      }
+      if (PL == 2) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; c++) top = fmaxf(top, r16_top<MODE>(score, x[c], rows + c * 32, (float)(at + c * 32 + r.q_offset - j), mult, partial, bits[c]));
+        uint32_t up = (uint32_t)(min(max((int)ceilf(top), -110), 110) + 140);
+        if (!(ok = r16_share(turn, half, row, quad, ok, up))) break;
+        lift = 154.f - (float)up;                          // weights times 2^lift
+        unit_dv = __uint_as_float((up - 27u) << 23);
+      }
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        r16_weights<MODE, true, PL>(score, x[c], w, wl, rows + c * 32, 0.f, lift, (float)(at + c * 32 + r.q_offset - j), mult, partial, seen, at + c * 32, docs);
+        r16_weights<MODE, true, PL>(score, x[c], w, wl, rows + c * 32, 0.f, lift, (float)(at + c * 32 + r.q_offset - j), mult, partial, bits[c]);
         r16_st16(t_s + (PL == 2 ? 32u : 16u) * c, w);
         if (PL == 2) r16_st16(t_s + 32u * c + 16u, wl);
       }
@@ -1026,9 +1052,9 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           r16_gradients2<true>(x[c], dp, rows + 128 + 32 * c, 0.f, unit_g * unit_v, partial, largest);
         }
         uint32_t exponent = __float_as_uint(largest) >> 23;
-        if (!(ok = r16_share(turn + 256 * phase, half, row, quad, ok, exponent))) break;
+        if (!(ok = r16_share(turn + 256, half, row, quad, ok, exponent))) break;
         const R16Unit step_unit = r16_unit(exponent);
-        unit_dk = step_unit.back * 0x1p-14f;               // the weights' factor is in them
+        unit_dk = step_unit.back * unit_dv;                // the weights' factor is in them
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           r16_apart(x[c], step_unit.to, w, wl);
@@ -1064,12 +1090,12 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           if (walk > 0) {
             tmem_ld_32x32b_x32(lane_base + (half == 0 ? COL_DV : COL_DK) + (uint32_t)c, o);
             tmem_ld_wait();
-            if (PL == 2) r16_add_whole(lane_base + (half == 0 ? COL_DV : COL_DK) + 64u + (uint32_t)c, o, walk == 1, 1.f, half == 0 ? 1.f : unit_dk);
+            if (PL == 2) r16_add_whole(lane_base + (half == 0 ? COL_DV : COL_DK) + 64u + (uint32_t)c, o, walk == 1, 1.f, half == 0 ? unit_dv : unit_dk);
           } else {
 #pragma unroll
             for (int u = 0; u < 32; u++) o[u] = 0u;
           }
-          if (j < r.lk) r16_write(o, half == 0 ? unit_g * (PL == 2 ? 0x1p-14f : 1.f) : r.scale * unit_q, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
+          if (j < r.lk) r16_write(o, half == 0 ? unit_g : r.scale * unit_q, out, out16, bi * s.batch + hk * s.head + (long long)j * s.row + c, c, p.d);
         }
       }
     }
@@ -1223,7 +1249,8 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       tmem_ld_wait();
 #pragma unroll
       for (int c = 0; c < 2; c++)
-        r16_weights<MODE, false, PL>(score, x[c], w, wl, nullptr, stat.x, 0.f, (float)(i + r.q_offset - at - c * 32), mult, partial, seen, at + c * 32, docs);
+        r16_weights<MODE, false, PL>(score, x[c], w, wl, nullptr, stat.x, 0.f, (float)(i + r.q_offset - at - c * 32), mult, partial,
+                                     partial ? r16_bits(seen, at + c * 32, docs) : ~0u);
       ok = ok && r16_wait(bar_dp, n & 1u, abort_flag, p.status, 92);
       if (PL == 1 && !ok) break;
       tc_fence_after();

@@ -78,3 +78,34 @@ def test_a_document_of_small_values_keeps_its_digits(ctx, name, power):
     for n in ("dq", "dk", "dv"):
         err = row_errors(c.get(n), want[n])
         assert err.max() <= LIKE_FP32, (n, err.max(), err[:, :, :350].max())
+
+
+def test_gradients_of_hardly_seen_keys(ctx):
+    """Keys whose weights are about 2^-36 in every row. A weight's relative error is its score's absolute one: 25 here, four roundings of 2^-24
+    of it each, so 100 * 2^-24 more than above.
+
+    All queries lie in nearly one direction, so the terms of dK = sum dS q, whose signs differ, can cancel: a row's error is that of its terms,
+    independent of one another, and so is taken over the root of the sum of their squares (which is the row's norm where they do not cancel)."""
+    r = np.random.default_rng(73)
+    c = Call(ctx, r, 1, 2, 2, 500, 500, 64, scale=1.0)
+    q, k = 0.05 * c.value["q"], c.value["k"].copy()
+    q[..., 0], k[..., 0] = 5.0, 0.0
+    k[:, :, 200:210, 0] = -5.0
+    put(c, "q", q)
+    put(c, "k", k)
+    c.run()
+    want, _ = wanted(c)
+    q, k, v, g = (c.value[n].astype(np.float64) for n in "qkvg")
+    p = np.exp(np.einsum("bhid,bhjd->bhij", q, k) - want["lse"][..., None])
+    ds = p * (np.einsum("bhid,bhjd->bhij", g, v) - (g * want["out"]).sum(-1, keepdims=True))
+    for n, weight, rows in (("dv", p, g), ("dk", ds, q)):
+        terms = np.sqrt(np.einsum("bhij,bhi->bhj", weight ** 2, (rows ** 2).sum(-1)))
+        err = np.linalg.norm(c.get(n) - want[n], axis=-1) / terms
+        assert err.max() <= LIKE_FP32 + 100 * ref.U32, (n, err.max(), err[:, :, 200:210])
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_large_scores_against_64_bits(ctx, half):
+    """Scores of several hundred: almost all of a row's weight on one key."""
+    r = np.random.default_rng(77)
+    Call(ctx, r, 1, 2, 2, 260, 260, 64, half=half, causal=True, size=8.0).run().check(planes=False)
