@@ -19,7 +19,7 @@
 //
 // fp32 operands of heads up to 64 columns run on the same kernels (PL = 2) with fp32 accuracy: every value as two half-precision numbers
 // h + l, 22 significant bits, side by side in a row of 128 columns where two blocks of 64 lie otherwise, and a product as h h' + h l' +
-// l h'. In the backward weights and gradients of scores are taken apart the same way, those of each row and step over a power of two of their own. A
+// l h'. Weights and gradients of scores are taken apart the same way, those of each row and step over a unit of their own. A
 // power of two per (batch, key head) brings each operand's largest value to 2^14 ... 2^15, so values down to 2^-14 of it keep all 22 bits;
 // rule16_split_kernel, which makes the planes, sets a flag where a row's own largest is smaller than that (or the largest of all beyond
 // 2^45, or not finite), and then these kernels do nothing and the fp32 ones behind them work.
@@ -537,6 +537,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const float mult = MODE ? 1.f : r.scale * unit * R16_LOG2E;
     const uint64_t mult2 = r16_two(mult, mult);
     float m = -INFINITY, l = 0.f;                        // l: of its half
+    float keep = 1.f, unit_o = 1.f;                      // two planes: what the whole and the step's product are added up with, a step later
     bool gone = false;                                   // both warps of a row know it
     for (int n = 0; n < walk; n++) {
       const uint32_t step = steps[n], place = n & 1u;
@@ -580,11 +581,13 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       gone = !__all_sync(0xffffffffu, ok && theirs.y != 0.f);
       if (gone) break;
       const float top = fmaxf(part_top, theirs.x) * mult;
-      const bool grown = top > m + 8.f || (m == -INFINITY && top > -INFINITY);
+      const bool grown = top > (PL == 2 ? m : m + 8.f) || (m == -INFINITY && top > -INFINITY);
       const float shrink = grown ? r16_ex2(m - top) : 1.f;      // m = -inf: 0
       if (grown) m = top;
-      // Two planes: weights times 2^7, at most 2^15, so that small ones keep their digits (the row's sum has the same factor).
-      const float base = (m == -INFINITY ? 0.f : m) - (PL == 2 ? 7.f : 0.f);
+      // Two planes: weights over the step's own maximum, which goes to 2^15, so that small ones keep their digits however far the row's
+      // maximum is above them: thousands of them can add up to something. Their sum and product come back over the row's maximum.
+      const float step_unit = PL == 2 ? (top == -INFINITY ? 0.f : r16_ex2(top - m)) : 1.f;
+      const float base = PL == 2 ? (top == -INFINITY ? 0.f : top) - 15.f : m == -INFINITY ? 0.f : m;
       const uint64_t base2 = r16_two(-base, -base);
       uint64_t sum[2] = {0ull, 0ull};
       // These scores came after the product before last, so its weights' place is free.
@@ -605,13 +608,13 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         if (PL == 2) r16_st16(t_p + 32u * c + 16u, wl);
       }
       const float2 s0 = *reinterpret_cast<const float2*>(&sum[0]), s1 = *reinterpret_cast<const float2*>(&sum[1]);
-      l = l * shrink + ((s0.x + s0.y) + (s1.x + s1.y));
+      l = l * shrink + ((s0.x + s0.y) + (s1.x + s1.y)) * step_unit;
       // O, before the product that adds these weights to it and after the one before: rescaled, or the step before added to the whole.
       if (n > 0 && (PL == 2 || __any_sync(0xffffffffu, grown))) {
         ok = r16_wait(&bar_o[place ^ 1u], ((n - 1) >> 1) & 1u, abort_flag, p.status, 69);
         tc_fence_after();
         if (PL == 2) {
-          r16_fold<DP / 2>(t_o + 64u, t_o, n == 1, shrink, shrink);
+          r16_fold<DP / 2>(t_o + 64u, t_o, n == 1, keep, unit_o);
         } else {
 #pragma unroll 1
           for (int c = 0; c < DP / 2; c += 32) {
@@ -623,6 +626,10 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             r16_st32(t_o + (uint32_t)c, o);
           }
         }
+      }
+      if (PL == 2) {
+        keep = shrink;
+        unit_o = step_unit;
       }
       r16_st_wait();
       r16_arrive_warp(&bar_p[place], lane);
@@ -646,9 +653,9 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         out = p.part;
         out16 = nullptr;
         at = ((long long)split * p.rows + at_row) * p.d;
-        if (valid && half == 0) p.part_ml[(long long)split * p.rows + at_row] = make_float2(PL == 2 ? m - 7.f : m, l);
+        if (valid && half == 0) p.part_ml[(long long)split * p.rows + at_row] = make_float2(PL == 2 ? m - 15.f : m, l);
       } else if (p.lse && valid && half == 0) {
-        p.lse[at_row] = l == 0.f ? -INFINITY : ((PL == 2 ? m - 7.f : m) + log2f(l)) * R16_LN2;
+        p.lse[at_row] = l == 0.f ? -INFINITY : ((PL == 2 ? m - 15.f : m) + log2f(l)) * R16_LN2;
       }
 #pragma unroll 1
       for (int c = 0; c < DP / 2; c += 32) {
@@ -658,7 +665,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
           tmem_ld_32x32b_x32(t_o + (uint32_t)c, o);
           tmem_ld_wait();
         }
-        if (PL == 2 && walk > 0) r16_add_whole(t_o + 64u + (uint32_t)c, o, walk == 1, 1.f, 1.f);
+        if (PL == 2 && walk > 0) r16_add_whole(t_o + 64u + (uint32_t)c, o, walk == 1, keep, unit_o);
         if (walk == 0 || l == 0.f) {
 #pragma unroll
           for (int u = 0; u < 32; u++) o[u] = 0u;

@@ -104,6 +104,25 @@ def test_gradients_of_hardly_seen_keys(ctx):
         assert err.max() <= LIKE_FP32 + 100 * ref.U32, (n, err.max(), err[:, :, 200:210])
 
 
+def test_many_small_weights_add_up(ctx):
+    """One key has all but 2^-21 of the weight and a value of zero: the output is what the thousands of others add up to."""
+    r = np.random.default_rng(74)
+    c = Call(ctx, r, 1, 2, 2, 200, 5000, 64, scale=1.0, q_offset=0)
+    q, k, v = 0.05 * c.value["q"], 0.05 * c.value["k"], c.value["v"].copy()
+    q[..., 0], k[..., 0] = 5.0, 0.0
+    k[:, :, 17, 0] = 4.6                    # 23 above the others: 2^-33 each
+    v[:, :, :128] = 0.0
+    v[:, :, 128:, 0] = 1.0
+    put(c, "q", q)
+    put(c, "k", k)
+    put(c, "v", v)
+    c.run(False)
+    want, _ = wanted(c)
+    got = c.get("o").astype(np.float64)
+    err = np.abs(got[..., 0] - want["out"][..., 0]) / want["out"][..., 0]
+    assert err.max() <= LIKE_FP32 + 100 * ref.U32, err.max()
+
+
 @pytest.mark.parametrize("half", [False, True])
 def test_large_scores_against_64_bits(ctx, half):
     """Scores of several hundred: almost all of a row's weight on one key."""
