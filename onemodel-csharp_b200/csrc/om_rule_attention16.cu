@@ -269,28 +269,62 @@ __device__ __forceinline__ float r16_max3(float a, float b, float c) {
 // of two: scale, cap and slope come times log2 e. `far`: the signed distance of the first index of a run, as a float (a conversion for
 // every score would take the unit that the exponentials need).
 struct R16Score {
-  float scale, turns, cap, slope;                        // turns: of the tanh's argument, 2 log2 e scale / cap
+  float scale, angle, cap, slope;                        // angle: of the tanh's argument, scale / cap
 };
 // unit: of the products (1, or the powers of two that the planes were divided by).
 template <int MODE>
 __device__ __forceinline__ R16Score r16_score_of(const RuleArgs& r, int head, float unit) {
   R16Score c;
   c.scale = r.scale * unit * R16_LOG2E;
-  c.turns = 2.f * R16_LOG2E * r.scale * unit * r.inv_softcap;
+  c.angle = fminf(r.scale * unit * r.inv_softcap, 1e38f);   // a finite number, so that 0 times it is 0
   c.cap = r.softcap * R16_LOG2E;
   c.slope = MODE > 0 && r.slopes ? r.slopes[head] * R16_LOG2E : 0.f;
   return c;
 }
-template <int MODE>
+// tanh(x) = 1 - 2 / (exp(2 x) + 1) is off by 2^-22 at most, absolutely: 2^-20 of its value from |x| = 0.3 on. Below, the Taylor series of
+// tanh(x) / x, whose first term left out is 2^-24 there: the score times it, so that a cap far above the scores leaves them as they are
+// (with the first form alone, a cap of 1000 put errors of 1e-4 on every score, one of 10^8 made them meaningless). LOW: |x| is known to be.
+constexpr float R16_LOW = 0.3f;
+template <int MODE, bool LOW>
 __device__ __forceinline__ float r16_score(const R16Score& c, float far, float dot, float* dcap) {
   float s = dot * c.scale;
   if (MODE == 2) {
-    // tanh(x) = 1 - 2 / (exp(2 x) + 1): off by 2^-22 at most, absolutely, which the cap times it carries into a score.
-    const float t = fmaf(-2.f, r16_rcp(r16_ex2(dot * c.turns) + 1.f), 1.f);
+    const float x = dot * c.angle, x2 = x * x;
+    const float ratio = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+    float t = x * ratio;
+    s *= ratio;
+    if (!LOW && !(fabsf(x) < R16_LOW)) {
+      t = fmaf(-2.f, r16_rcp(r16_ex2(x * (2.f * R16_LOG2E)) + 1.f), 1.f);
+      s = c.cap * t;
+    }
     *dcap = fmaf(-t, t, 1.f);
-    s = c.cap * t;
   }
   return fmaf(-c.slope, fabsf(far), s);
+}
+// 32 scores of a row; use(u, score, derivative of the cap). step: of the signed distance from one to the next. Caps are mostly far above the
+// scores, so a warp looks first whether all of its own are low: 10 operations for each then, in place of two on the unit that the
+// exponentials need (three documents' batches both ways: 168 us with the first form alone, 187 with both for every score, 172 so).
+template <int MODE, typename F>
+__device__ __forceinline__ void r16_scores32(const R16Score& c, const uint32_t (&x)[32], float far, float step, F use) {
+  float dcap = 1.f;
+  if (MODE == 2) {
+    float big = 0.f;
+#pragma unroll
+    for (int u = 0; u < 32; u += 2) big = r16_max3(big, fabsf(__uint_as_float(x[u])), fabsf(__uint_as_float(x[u + 1])));
+    if (__all_sync(0xffffffffu, big * c.angle < R16_LOW)) {
+#pragma unroll
+      for (int u = 0; u < 32; u++) {
+        const float s = r16_score<MODE, true>(c, far + step * (float)u, __uint_as_float(x[u]), &dcap);
+        use(u, s, dcap);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 32; u++) {
+    const float s = r16_score<MODE, false>(c, far + step * (float)u, __uint_as_float(x[u]), &dcap);
+    use(u, s, dcap);
+  }
 }
 
 // A row of N fp32 values to fp32 and bfloat16 results, both 16 bytes at a time; columns behind d stay unwritten (d is a multiple of 8).
@@ -555,12 +589,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       for (int c = 0; c < 2; c++) {
         uint32_t(&v)[32] = x[c];
         if (MODE) {
-          const float far = (float)(i + r.q_offset - at - 32 * c);
-#pragma unroll
-          for (int u = 0; u < 32; u++) {
-            float dcap;
-            v[u] = __float_as_uint(r16_score<MODE>(score, far - (float)u, __uint_as_float(v[u]), &dcap));
-          }
+          r16_scores32<MODE>(score, v, (float)(i + r.q_offset - at - 32 * c), -1.f, [&](int u, float s, float) { v[u] = __float_as_uint(s); });
         }
         if (sees == 1) r16_hide(v, r16_bits(seen, at + 32 * c, docs));
         float t[4];
@@ -758,11 +787,11 @@ template <int MODE, bool COLUMNS, int PL>
 __device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)[32], uint32_t (&w)[16], uint32_t (&wl)[16], const float* lses, float lse, float lift, float far, float mult,
                                             bool partial, uint32_t bits) {
   float dcap[MODE == 2 ? 32 : 1];
-  if (MODE) {
-#pragma unroll
-    for (int u = 0; u < 32; u++)
-      x[u] = __float_as_uint(r16_score<MODE>(score, COLUMNS ? far + (float)u : far - (float)u, __uint_as_float(x[u]), &dcap[MODE == 2 ? u : 0]));
-  }
+  if (MODE)
+    r16_scores32<MODE>(score, x, far, COLUMNS ? 1.f : -1.f, [&](int u, float s, float d) {
+      x[u] = __float_as_uint(s);
+      if (MODE == 2) dcap[u] = d;
+    });
   if (partial) r16_hide(x, bits);
   const uint64_t mult2 = r16_two(mult, mult);
 #pragma unroll
@@ -784,16 +813,17 @@ __device__ __forceinline__ void r16_weights(const R16Score& score, uint32_t (&x)
     for (int t = 0; t < 4; t++) x[u + t] = __float_as_uint(MODE == 2 ? p[t] == 0.f ? 0.f : p[t] * dcap[MODE == 2 ? u + t : 0] : p[t]);
   }
 }
-// The largest exponent of the 32 weights of a row whose columns have the log-sum-exps (the scores are formed twice: held, they would not
-// fit the registers beside the cap's derivatives).
+// The largest exponent of the 32 weights of a row whose columns have the log-sum-exps (of 32 scores, which are formed and read
+// again for the weights).
 template <int MODE>
 __device__ __forceinline__ float r16_top(const R16Score& score, const uint32_t (&x)[32], const float* lses, float far, float mult, bool partial, uint32_t bits) {
   float top = -INFINITY;
+  auto take = [&](int u, float s) { top = fmaxf(top, partial && !((bits >> u) & 1u) ? -INFINITY : s); };
+  if (MODE) {
+    r16_scores32<MODE>(score, x, far, 1.f, [&](int u, float s, float) { take(u, s - lses[u]); });
+  } else {
 #pragma unroll
-  for (int u = 0; u < 32; u++) {
-    float dcap;
-    const float s = MODE ? r16_score<MODE>(score, far + (float)u, __uint_as_float(x[u]), &dcap) - lses[u] : fmaf(__uint_as_float(x[u]), mult, -lses[u]);
-    top = fmaxf(top, partial && !((bits >> u) & 1u) ? -INFINITY : s);
+    for (int u = 0; u < 32; u++) take(u, fmaf(__uint_as_float(x[u]), mult, -lses[u]));
   }
   return top;
 }
@@ -1020,9 +1050,11 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       // The scores came after the product before, and the next one waits for these weights.
       if (PL == 2 && n > 0) r16_fold<32>(lane_base + COL_DV + 64u + 32u * half, lane_base + COL_DV + 32u * half, n == 1, 1.f, unit_dv);
       uint32_t x[2][32], w[16], wl[16];
-      tmem_ld_32x32b_x32(t_s, x[0]);
-      tmem_ld_32x32b_x32(t_s + 32u, x[1]);
-      tmem_ld_wait();
+      if (PL == 1) {
+        tmem_ld_32x32b_x32(t_s, x[0]);
+        tmem_ld_32x32b_x32(t_s + 32u, x[1]);
+        tmem_ld_wait();
+      }
       uint32_t bits[2] = {~0u, ~0u};
       if (partial) {
         bits[0] = r16_bits(seen, at, docs);
@@ -1031,7 +1063,11 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (PL == 2) {
         float top = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < 2; c++) top = fmaxf(top, r16_top<MODE>(score, x[c], rows + c * 32, (float)(at + c * 32 + r.q_offset - j), mult, partial, bits[c]));
+        for (int c = 0; c < 2; c++) {
+          tmem_ld_32x32b_x32(t_s + 32u * c, x[c]);
+          tmem_ld_wait();
+          top = fmaxf(top, r16_top<MODE>(score, x[c], rows + c * 32, (float)(at + c * 32 + r.q_offset - j), mult, partial, bits[c]));
+        }
         uint32_t up = (uint32_t)(min(max((int)ceilf(top), -110), 110) + 140);
         if (!(ok = r16_share(turn, half, row, quad, ok, up))) break;
         lift = 154.f - (float)up;                          // weights times 2^lift
@@ -1039,6 +1075,10 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       }
 #pragma unroll
       for (int c = 0; c < 2; c++) {
+        if (PL == 2) {                                     // again: 64 scores and what becomes of them do not fit the registers
+          tmem_ld_32x32b_x32(t_s + 32u * c, x[c]);
+          tmem_ld_wait();
+        }
         r16_weights<MODE, true, PL>(score, x[c], w, wl, rows + c * 32, 0.f, lift, (float)(at + c * 32 + r.q_offset - j), mult, partial, bits[c]);
         r16_st16(t_s + (PL == 2 ? 32u : 16u) * c, w);
         if (PL == 2) r16_st16(t_s + 32u * c + 16u, wl);

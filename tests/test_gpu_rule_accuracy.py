@@ -123,6 +123,28 @@ def test_many_small_weights_add_up(ctx):
     assert err.max() <= LIKE_FP32 + 100 * ref.U32, err.max()
 
 
+@pytest.mark.parametrize("half,d", [(False, 64), (True, 64), (True, 128), (False, 80)])
+@pytest.mark.parametrize("softcap", [0.5, 50.0, 1e3, 1e6, 1e30, 3e38])
+def test_caps_of_every_size(ctx, half, d, softcap):
+    """A score's error is relative to the score. Where the cap is far above them it changes nothing: the scores are those of no cap."""
+    r = np.random.default_rng(75)
+    c = Call(ctx, r, 1, 2, 1, 260, 260, d, half=half, causal=True, softcap=softcap).run()
+    b, h, hk, lq, lk, _ = c.dims
+    v = {n: a.astype(np.float64) for n, a in c.value.items()}
+    s = c.scale * np.einsum("bhid,bhjd->bhij", v["q"], np.repeat(v["k"], h // hk, 1))
+    s = softcap * np.tanh(s / softcap)
+    s = np.where(np.arange(lk)[None] <= np.arange(lq)[:, None], s, -np.inf)
+    lse = np.log(np.exp(s - s.max(-1, keepdims=True)).sum(-1)) + s.max(-1)
+    # A score: d products as a random walk of four deviations of 2^-24 each times sqrt(d), the cap and its scale sixteen roundings, of scores below 8;
+    # the log-sum-exp is a mean of scores beside its own four roundings.
+    allowed = 8 * ref.U32 * (4 * np.sqrt(d) + 16 + 4)
+    assert np.abs(c.lse.numpy() - lse).max() <= allowed, np.abs(c.lse.numpy() - lse).max()
+    want, tol = (ref.attention(v["q"], v["k"], v["v"], v["g"], ref.visible(b, lq, lk, True), c.scale, 0.0, None, 0, half) if softcap >= 1e6 else (None, None))
+    if want:
+        for n, full in (("o", "out"), ("dq", "dq"), ("dk", "dk"), ("dv", "dv")):
+            assert (np.abs(c.get(n) - want[full]) <= tol[full]).all(), full
+
+
 @pytest.mark.parametrize("half", [False, True])
 def test_large_scores_against_64_bits(ctx, half):
     """Scores of several hundred: almost all of a row's weight on one key."""
