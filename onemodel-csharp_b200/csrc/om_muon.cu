@@ -480,6 +480,7 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
       ok = true;
       if (lane == 0) ok = mbar_wait(&bar_done[place], (j / W::PLACES) & 1u, abort_flag, l.status, 103);
       ok = __all_sync(0xffffffffu, ok);
+      __syncwarp();                                      // what the lane waited for is seen by the others: a vote orders no memory
       if (!ok) break;
       tc_fence_after();
 #pragma unroll 1

@@ -352,7 +352,9 @@ __device__ __forceinline__ bool r16_bar(uint64_t* bar, uint32_t parity, volatile
 __device__ __forceinline__ bool r16_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int where) {
   bool ok = true;
   if ((threadIdx.x & 31) == 0) ok = r16_bar(bar, parity, abort_flag, status, where);   // one lane asks: 32 asking alike cost the issue slots of the others
-  return __all_sync(0xffffffffu, ok);
+  ok = __all_sync(0xffffffffu, ok);
+  __syncwarp();                                          // what the lane waited for is seen by the others: a vote orders no memory
+  return ok;
 }
 // One arrival for a warp whose rows are done with tensor memory and shared memory.
 __device__ __forceinline__ void r16_arrive_warp(uint64_t* bar, int lane) {
