@@ -556,10 +556,10 @@ int32_t om_attention_bwd_bf16(om_ctx* ctx, const uint16_t* g16, const float* g, 
  *   visible(i, j) = (j < prefix[b]  or  ((not causal or j <= i + q_offset) and (window == 0 or |i + q_offset - j| < window)))
  *                   and q_documents[b, i] == k_documents[b, j] and q_documents[b, i] >= 0      (where documents are given)
  *   score(i, j)   = s - slopes[head] * |i + q_offset - j|  with  s = scale q_i . k_j, or softcap * tanh(scale q_i . k_j / softcap)
- * A row that sees no key gives zeros, a log-sum-exp of minus infinity and no gradients. A hidden score is never looked at, but
- * rows of k and v (and of the output's gradient) have to be finite wherever they lie in range: a weight of zero times an
- * infinite value is not a number, here as in the plain product. The fp32 entry points take rows of no document for zeros, whatever
- * they hold. All pointers are device pointers and may be NULL. */
+ * A row that sees no key gives zeros, a log-sum-exp of minus infinity and no gradients. A hidden score is never looked at, and
+ * rows of no document may hold anything: they are taken for zeros. All other rows have to be finite wherever they lie in range,
+ * seen or not: a weight of zero times an infinite value is not a number, here as in the plain product. All pointers are device
+ * pointers and may be NULL. */
 typedef struct om_attention_rule {
   int32_t causal;
   int32_t window;             /* 0: none; else a positive number of positions */

@@ -13,7 +13,8 @@ struct RuleArgs {
   const float* slopes;
   const int32_t* prefix;
   const int32_t *q_docs, *k_docs;
-  const int4 *q_ranges, *k_ranges;   // [b][ceil(l / 64)]: lowest and highest document (padding left out), the document if it is one only else -1
+  const int4 *q_ranges, *k_ranges;   // [b][ceil(l / 64)]: lowest and highest document (padding left out), the document if it is one only else -1, padding
+  const uint2 *q_pads, *k_pads;      // [b][ceil(l / 64)]: a bit for each row that is padding
   int lq, lk, nq64, nk64;
 };
 
@@ -130,6 +131,13 @@ __device__ __forceinline__ int rule_see(const RuleTile& t, int at, int n) {
   }
   if (hi < 0 || t.doc_hi < 0 || lo > t.doc_hi || hi < t.doc_lo) return 0;
   return all && same ? 2 : 1;
+}
+// Whether any of indices [at, at + 64 n) is padding.
+__device__ __forceinline__ bool rule_padding(const RuleTile& t, int at, int n) {
+  int pad = 0;
+  if (t.other)
+    for (int e = at / RULE_GRAIN; e < min(at / RULE_GRAIN + n, t.n64); e++) pad |= t.other[e].w;
+  return pad != 0;
 }
 // One pair, both inside the matrix; doc: the query's document (any value where there are none).
 __device__ __forceinline__ bool rule_visible(const RuleArgs& r, int prefix, int i, int j, int q_doc, int k_doc) {

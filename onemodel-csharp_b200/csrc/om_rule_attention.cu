@@ -22,9 +22,9 @@ __device__ __forceinline__ float ra_value(float v) { return v; }
 template <>
 __device__ __forceinline__ float ra_value(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// Lowest and highest document of every 64 rows, and the document itself where there is only one and no padding.
+// Lowest and highest document of every 64 rows, the document itself where there is only one and no padding, and which rows are padding.
 __global__ void __launch_bounds__(64)
-rule_ranges_kernel(const int32_t* docs, int l, int tiles, int4* __restrict__ ranges) {
+rule_ranges_kernel(const int32_t* docs, int l, int tiles, int4* __restrict__ ranges, uint2* __restrict__ pads) {
   pdl_enter();
   __shared__ int lo_s[2], hi_s[2], pad_s[2];
   const int t = blockIdx.x, b = blockIdx.y, i = t * RULE_GRAIN + threadIdx.x;
@@ -38,8 +38,8 @@ rule_ranges_kernel(const int32_t* docs, int l, int tiles, int4* __restrict__ ran
   for (int o = 16; o > 0; o >>= 1) {
     lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
     hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    pad |= __shfl_xor_sync(0xffffffffu, pad, o);
   }
+  pad = (int)__ballot_sync(0xffffffffu, pad != 0);
   if ((threadIdx.x & 31) == 0) {
     lo_s[threadIdx.x >> 5] = lo;
     hi_s[threadIdx.x >> 5] = hi;
@@ -49,7 +49,8 @@ rule_ranges_kernel(const int32_t* docs, int l, int tiles, int4* __restrict__ ran
   if (threadIdx.x == 0) {
     lo = min(lo_s[0], lo_s[1]);
     hi = max(hi_s[0], hi_s[1]);
-    ranges[(long long)b * tiles + t] = make_int4(lo, hi, (lo == hi && !(pad_s[0] | pad_s[1])) ? lo : -1, 0);
+    ranges[(long long)b * tiles + t] = make_int4(lo, hi, (lo == hi && !(pad_s[0] | pad_s[1])) ? lo : -1, (pad_s[0] | pad_s[1]) != 0);
+    pads[(long long)b * tiles + t] = make_uint2((uint32_t)pad_s[0], (uint32_t)pad_s[1]);
   }
 }
 
@@ -96,6 +97,7 @@ int32_t rule_begin(om_ctx* ctx, const om_attention_rule* rule, int b, int h, int
   r.q_docs = rule->q_documents;
   r.k_docs = rule->k_documents;
   r.q_ranges = r.k_ranges = nullptr;
+  r.q_pads = r.k_pads = nullptr;
   r.lq = lq;
   r.lk = lk;
   r.nq64 = (lq + RULE_GRAIN - 1) / RULE_GRAIN;
@@ -103,11 +105,15 @@ int32_t rule_begin(om_ctx* ctx, const om_attention_rule* rule, int b, int h, int
   call->b = b; call->h = h; call->hkv = hkv; call->d = d;
   call->ranges = nullptr;
   if (r.q_docs && lk > 0) {
-    OM_TRY(pool_alloc(ctx, sizeof(int4) * (size_t)b * ((size_t)r.nq64 + r.nk64), false, (void**)&call->ranges));
-    launch_chained(ctx, rule_ranges_kernel, dim3((unsigned)r.nq64, (unsigned)b), 64, 0, r.q_docs, lq, r.nq64, call->ranges);
-    launch_chained(ctx, rule_ranges_kernel, dim3((unsigned)r.nk64, (unsigned)b), 64, 0, r.k_docs, lk, r.nk64, call->ranges + (size_t)b * r.nq64);
+    const size_t nq = (size_t)b * r.nq64, n = nq + (size_t)b * r.nk64;
+    OM_TRY(pool_alloc(ctx, (sizeof(int4) + sizeof(uint2)) * n, false, (void**)&call->ranges));
+    uint2* pads = reinterpret_cast<uint2*>(call->ranges + n);
+    launch_chained(ctx, rule_ranges_kernel, dim3((unsigned)r.nq64, (unsigned)b), 64, 0, r.q_docs, lq, r.nq64, call->ranges, pads);
+    launch_chained(ctx, rule_ranges_kernel, dim3((unsigned)r.nk64, (unsigned)b), 64, 0, r.k_docs, lk, r.nk64, call->ranges + nq, pads + nq);
     r.q_ranges = call->ranges;
-    r.k_ranges = call->ranges + (size_t)b * r.nq64;
+    r.k_ranges = call->ranges + nq;
+    r.q_pads = pads;
+    r.k_pads = pads + nq;
   }
   return OM_OK;
 }

@@ -352,9 +352,8 @@ __device__ __forceinline__ bool r16_bar(uint64_t* bar, uint32_t parity, volatile
 __device__ __forceinline__ bool r16_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int where) {
   bool ok = true;
   if ((threadIdx.x & 31) == 0) ok = r16_bar(bar, parity, abort_flag, status, where);   // one lane asks: 32 asking alike cost the issue slots of the others
-  ok = __all_sync(0xffffffffu, ok);
   __syncwarp();                                          // what the lane waited for is seen by the others: a vote orders no memory
-  return ok;
+  return __all_sync(0xffffffffu, ok);
 }
 // One arrival for a warp whose rows are done with tensor memory and shared memory.
 __device__ __forceinline__ void r16_arrive_warp(uint64_t* bar, int lane) {
@@ -383,9 +382,29 @@ struct R16Fwd {
 };
 
 // A CTA's plan: the tiles of 128 of the other axis that some row tile sees anything of, in order, with rule_see's answer for each row
-// tile (two bits, from bit 10 on). Made by one warp; returns their number.
+// tile (two bits, from bit 10 on) and whether rows of it are padding (bit 12). Made by one warp; returns their number.
 __device__ __forceinline__ int r16_tile_of(uint32_t step) { return (int)(step & (R16_PLAN - 1)); }
 __device__ __forceinline__ int r16_sees_of(uint32_t step) { return (int)(step >> 10) & 3; }
+__device__ __forceinline__ bool r16_padded(uint32_t step) { return (step >> 12) & 1u; }
+template <bool FULL>
+__device__ __forceinline__ uint32_t r16_look(const RuleTile& t, int at) {
+  const uint32_t sees = (uint32_t)rule_see<FULL>(t, at, 2);
+  return sees == 1 && rule_padding(t, at, 2) ? 5u : sees;
+}
+// Padding of a bfloat16 tile that a product adds up over, to zeros: its weights are 0, but 0 times what is not a number is not one. A
+// row warp has 16 rows of the tile, which no product reads at the time, and then tells the product that does through a barrier as ever.
+template <int DP>
+__device__ __forceinline__ void r16_clear(uint8_t* tile, const uint2* pads, int at64, int n64, int warp, int lane) {
+  constexpr int PIECES = DP / 8;                         // of 16 bytes in a row
+  const uint2 v = at64 + (warp >> 2) < n64 ? pads[at64 + (warp >> 2)] : make_uint2(0u, 0u);
+  const uint32_t bits = ((warp & 2) ? v.y : v.x) >> (16 * (warp & 1));
+#pragma unroll
+  for (int e = lane; e < 16 * PIECES; e += 32) {
+    const int row = e / PIECES, c = e % PIECES;
+    if ((bits >> row) & 1u) *reinterpret_cast<uint4*>(tile + (c / 8) * R16_CHUNK + (16 * warp + row) * 128 + (c % 8) * 16) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
 template <typename F>
 __device__ __forceinline__ int r16_plan(uint16_t* steps, int tiles, int lane, F see) {
   int n = 0;
@@ -480,7 +499,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   last = min(first + per, last);
   __syncthreads();
   if (warp == 0) {
-    const int n = r16_plan(steps, last - first, lane, [&](int t) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T, 2); });
+    const int n = r16_plan(steps, last - first, lane, [&](int t) { return r16_look<true>(*tile, (first + t) * R16_T); });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
@@ -661,6 +680,11 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
       if (PL == 2) {
         keep = shrink;
         unit_o = step_unit;
+      }
+      if (PL == 1 && r16_padded(step)) {
+        const int stage = n + 1 < walk ? 2 * n + 2 : 2 * n + 1;   // of the values, in the order of the loads
+        ok = ok && r16_wait(&bar_full[stage % W::STAGES], (stage / W::STAGES) & 1u, abort_flag, p.status, 68);
+        if (ok) r16_clear<DP>(ring + stage % W::STAGES * W::TILE, r.k_pads + (long long)bi * r.nk64, (first + r16_tile_of(step)) * (R16_T / RULE_GRAIN), r.nk64, warp, lane);
       }
       r16_st_wait();
       r16_arrive_warp(&bar_p[place], lane);
@@ -944,7 +968,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
   __syncthreads();
   const int first = tile->lo / R16_T, tiles = max(0, (min(tile->hi, r.lq) + R16_T - 1) / R16_T - first);
   if (warp == 0) {
-    const int n = r16_plan(steps, tiles, lane, [&](int t) { return (uint32_t)rule_see<false>(*tile, (first + t) * R16_T, 2); });
+    const int n = r16_plan(steps, tiles, lane, [&](int t) { return r16_look<false>(*tile, (first + t) * R16_T); });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
@@ -1085,6 +1109,14 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         r16_st16(t_s + (PL == 2 ? 32u : 16u) * c, w);
         if (PL == 2) r16_st16(t_s + 32u * c + 16u, wl);
       }
+      if (PL == 1 && r16_padded(step)) {
+        // Both tiles, once the product that forms dP from one of them is complete (the scores are).
+        if (!(ok = r16_wait(bar_dp, phase, abort_flag, p.status, 96))) break;
+        const uint2* pads = r.q_pads + (long long)bi * r.nq64;
+        const int at64 = (first + r16_tile_of(step)) * (R16_T / RULE_GRAIN);
+        r16_clear<DP>(ring_g + a * W::TILE, pads, at64, r.nq64, warp, lane);
+        r16_clear<DP>(ring_q + a * W::TILE, pads, at64, r.nq64, warp, lane);
+      }
       r16_st_wait();
       r16_arrive_warp(bar_p, lane);
       ok = ok && r16_wait(bar_dp, phase, abort_flag, p.status, 81);
@@ -1213,7 +1245,7 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   __syncthreads();
   const int first = tile->pre > 0 ? 0 : tile->lo / R16_T, tiles = max(0, (min(max(tile->pre, tile->hi), r.lk) + R16_T - 1) / R16_T - first);
   if (warp == 0) {
-    const int n = r16_plan(steps, tiles, lane, [&](int t) { return (uint32_t)rule_see<true>(*tile, (first + t) * R16_T, 2); });
+    const int n = r16_plan(steps, tiles, lane, [&](int t) { return r16_look<true>(*tile, (first + t) * R16_T); });
     if (lane == 0) steps[R16_PLAN] = (uint16_t)n;
   }
   __syncthreads();
@@ -1341,6 +1373,8 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           r16_st16(t_s + 16u * c, w);
         }
       }
+      if (PL == 1 && r16_padded(step))
+        r16_clear<DP>(ring_k + n % W::RING_A * W::TILE, r.k_pads + (long long)bi * r.nk64, (first + r16_tile_of(step)) * (R16_T / RULE_GRAIN), r.nk64, warp, lane);
       r16_st_wait();
       r16_arrive_warp(&bar_ds[place], lane);
     }

@@ -145,6 +145,28 @@ def test_caps_of_every_size(ctx, half, d, softcap):
             assert (np.abs(c.get(n) - want[full]) <= tol[full]).all(), full
 
 
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("d,lq,lk,docs,padded", [(64, 200, 200, 90, 20), (128, 300, 300, 200, 130), (64, 1, 700, 400, 90), (40, 130, 130, 130, 1), (120, 5, 600, 50, 60)])
+def test_padding_of_bfloat16_calls_may_hold_anything(ctx, d, lq, lk, docs, padded, what):
+    r = np.random.default_rng(76)
+    c = Call(ctx, r, 2, 4, 2, lq, lk, d, half=True, causal=True, docs=docs, padded=padded)
+    if lk > 400:                             # padding between documents as well
+        c.kd[:, 130:150] = -1
+    c.qd = c.kd[:, -lq:].copy()
+    if lq == 1 or lq == 5:
+        c.qd[:] = c.kd[:, 100:101]
+        c.q_offset = lk
+    first = {n: c.run().get(n).copy() for n in ("o", "dq", "dk", "dv")}
+    c.check()
+    for n, ids in (("q", c.qd), ("k", c.kd), ("v", c.kd), ("g", c.qd)):
+        a = c.value[n].copy()
+        a.transpose(0, 2, 1, 3)[ids < 0] = what
+        put(c, n, a)
+    c.run()
+    for n, a in first.items():
+        assert np.array_equal(a, c.get(n)), n
+
+
 @pytest.mark.parametrize("half", [False, True])
 def test_large_scores_against_64_bits(ctx, half):
     """Scores of several hundred: almost all of a row's weight on one key."""
