@@ -626,11 +626,11 @@ static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* r
                         __nv_bfloat16* dq16, const om_head_strides* dqs, float* dk, __nv_bfloat16* dk16, const om_head_strides* dks, float* dv,
                         __nv_bfloat16* dv16, const om_head_strides* dvs) {
   OM_TRY(rule_check(ctx, who, rule, b, h, hkv, lq, lk, d, scale));
-  if ((int64_t)b * h == 0) return OM_OK;
-  if (dq || dq16) OM_TRY(rule_result(ctx, who, dqs, b, h, lq, d));
+  if (b == 0 || hkv == 0) return OM_OK;
+  if (h > 0 && (dq || dq16)) OM_TRY(rule_result(ctx, who, dqs, b, h, lq, d));
   if (dk || dk16) OM_TRY(rule_result(ctx, who, dks, b, hkv, lk, d));
   if (dv || dv16) OM_TRY(rule_result(ctx, who, dvs, b, hkv, lk, d));
-  if (lq == 0 || lk == 0) {
+  if (h == 0 || lq == 0 || lk == 0) {                      // zeros, for the key heads of no query head too
     if (lq > 0) {
       OM_TRY(ra_zero(ctx, dq, dqs, b, h, lq, d));
       OM_TRY(ra_zero(ctx, dq16, dqs, b, h, lq, d));

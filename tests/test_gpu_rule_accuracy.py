@@ -172,3 +172,18 @@ def test_large_scores_against_64_bits(ctx, half):
     """Scores of several hundred: almost all of a row's weight on one key."""
     r = np.random.default_rng(77)
     Call(ctx, r, 1, 2, 2, 260, 260, 64, half=half, causal=True, size=8.0).run().check(planes=False)
+
+
+@pytest.mark.parametrize("half", [False, True])
+def test_no_query_heads(ctx, half):
+    """Key heads that no query head shares get gradients of zero."""
+    r = np.random.default_rng(78)
+    c = Call(ctx, r, 2, 2, 2, 6, 9, 16, half=half).run()
+    rule, sizes = c.rule(), [i32(n) for n in (2, 0, 2, 6, 9, 16)] + [f32(c.scale)]
+    w = lambda n: (c.where(n)[0], C.byref(c.where(n)[1]))   # noqa: E731
+    for n in ("dk", "dv"):
+        c.dev[n] = c.poison(c.value[n[1]].size)
+    grads = [a for n in ("dq", "dk", "dv") for a in (([None] if half else []) + list(w(n)))]
+    ctx.call("om_rule_attention_bwd" + ("_bf16" if half else ""), ctx.handle, C.byref(rule), *w("g"), *w("q"), *w("k"), *w("v"), *w("o"), c.lse.ptr, *sizes, *grads)
+    ctx.sync()
+    assert (c.get("dk") == 0).all() and (c.get("dv") == 0).all()
