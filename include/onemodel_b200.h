@@ -793,7 +793,8 @@ int32_t om_optim_adam_step_b16(om_ctx* ctx, int32_t n_tensors, float* const* p_h
  *   m = momentum m + (1 - momentum) g;  u = nesterov ? momentum m + (1 - momentum) g : m;  X = u / max(|u|, eps) (Frobenius norm),
  *   steps times: G = X X^T (of the smaller side), X = 3.4445 X + (-4.7750 G + 2.0315 G G) X,
  *   p = (1 - lr weight_decay) p - lr s X, with s = match_rms ? 0.2 sqrt(max(rows, cols)) : sqrt(max(1, rows / cols)).
- * Products, norms and the state keep fp32 accuracy whatever the context's flags. p16_host (may be NULL, as may be its entries):
+ * Norms and the state are fp32 or more whatever the context's flags, and products have operands of 22 bits and sums in fp32: X is as
+ * exact as with fp32 products to within a factor of four. p16_host (may be NULL, as may be its entries):
  * the bfloat16 copies of the weights, refreshed by the update. hyper_dev (may be NULL): a device copy that the kernels read
  * in place of hyper_host (so that a captured update follows a schedule); steps is always taken from hyper_host. A matrix with
  * no elements is left alone; p, m and p16 of one call overlap nothing (OM_ERR_ARG). steps is 1 to 10, sides are at most 65536. */

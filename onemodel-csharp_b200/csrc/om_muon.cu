@@ -6,12 +6,13 @@
 // call go through each launch together: a launch covers the tiles of one product of up to MU_TENSORS matrices, whatever their
 // shapes, so a step costs three launches for a whole model.
 //
-// The products run on the tensor pipe with fp32 accuracy: a value v is kept as two half-precision numbers, h = half(v) and
-// l = half(v - h), 22 significant bits together, and a product is h h' + h l' + l h' (what is left out is 2^-22 of it). Five steps
-// raise an error in the direction of a small singular value up to 3.4445^5 = 485 times, which is why plain half or bfloat16
-// operands (2^-11, 2^-8) would leave few digits of the update. The tensor core cuts each sum it adds to off, an error that grows with the
-// number of additions: h h' has an accumulator of its own and the two small products another, a third of the additions
-// (4096 terms: the weights' error against 64 bits 8.7e-7 in one accumulator, 7.1e-7 in two, at the same speed). Every matrix of a step is bounded (|X| <= 1.2, |G| <= 1.5, |Y| <= 3 in the
+// The products run on the tensor pipe: a value v is kept as two half-precision numbers, h = half(v) and l = half(v - h), 22 significant
+// bits together, and a product is h h' + h l' + l h' (what is left out is 2^-22 of it). Five steps raise an error in the direction of a small
+// singular value up to 3.4445^5 = 485 times, which is why plain half or bfloat16 operands (2^-11, 2^-8) would leave few digits of the
+// update. The tensor core cuts off what a sum cannot hold at every addition, always towards zero: an error that grows with the length of
+// the sum (X off by 1.2e-5 for a long side of 1536 and 7.6e-5 for 16384, where fp32 products leave 2e-6). So its sums are of 256 terms
+// and are added up in fp32 (6e-6 and 2e-6), and h h' has an accumulator of its own, the two small products another. Sums of 128 terms: 4e-6, and
+// 24 matrices of 384 x 384 to 1536 368 us instead of 355. Every matrix of a step is bounded (|X| <= 1.2, |G| <= 1.5, |Y| <= 3 in the
 // spectral norm, so element by element), and is stored times a power of two that puts its usual elements in the middle of the
 // half's range. Three products at the 16-bit rate bound it: 3/1664 s a TFLOP; two planes of 2 bytes are what fp32 would read.
 #include <cuda_bf16.h>
@@ -29,6 +30,7 @@ constexpr int MU_TENSORS = 32;
 constexpr float MU_A = 3.4445f, MU_B = -4.7750f, MU_C = 2.0315f;   // the quintic's coefficients
 constexpr int MU_CHUNK = 8192;                                     // elements of one partial sum of squares
 constexpr int MU_BM = 128, MU_BK = 64;                             // rows of a tile of a product, terms of a stage
+constexpr int MU_SUM = 4;                                          // stages that one sum of the tensor core runs over
 constexpr float MU_SX = 1024.f, MU_SG = 4096.f;                    // X is stored times the first, G and Y times the second
 constexpr int MU_EPI = 8;                                          // warps 0-7: results, half of a tile's columns each four; warp 8: MMA issue; warp 9: TMA
 constexpr int MU_THREADS = 32 * (MU_EPI + 2);
@@ -332,59 +334,48 @@ __device__ __forceinline__ float mu_value(const uint4 (&h)[4], const uint4 (&l)[
   return __half2float(reinterpret_cast<const __half*>(h)[u]) + __half2float(reinterpret_cast<const __half*>(l)[u]);
 }
 
-// A tile's results are read back under the next tile's products where its two accumulators fit tensor memory twice.
-template <int BN>
-struct MuonShape {
-  static constexpr int PLANE_A = MU_BM * MU_BK * 2, PLANE_B = BN * MU_BK * 2;
-  static constexpr int STAGE = 2 * (PLANE_A + PLANE_B), STAGES = BN == 256 ? 2 : 3, PLACES = BN == 256 ? 1 : 2;
-  static constexpr int TURN = STAGES * STAGE, BARS = TURN + MU_EPI * 32 * MU_PITCH * 16;
-  static constexpr int SMEM = BARS + 256;
-};
+// Shared memory of a product's CTA. Tensor memory: two accumulators of the large products, which take the sums in turn, and two of the
+// small ones, which take the tiles in turn: what one holds is read back under the products of the other.
+constexpr int MU_PLANE = MU_BM * MU_BK * 2, MU_STAGE = 4 * MU_PLANE, MU_STAGES = 3;
+constexpr int MU_TURN = MU_STAGES * MU_STAGE, MU_BARS = MU_TURN + MU_EPI * 32 * MU_PITCH * 16, MU_SMEM = MU_BARS + 256;
 
 // Where item `tile` of a launch lies.
 struct MuonTile {
   int which, r0, c0;
 };
-template <int KIND, int BN>
+template <int KIND>
 __device__ __forceinline__ MuonTile mu_tile(const MuonList& l, long long tile) {
   MuonTile m;
   m.which = mu_find(l, tile, &tile);
   if (KIND == 2) {
     const int down = (l.t[m.which].mm + MU_BM - 1) / MU_BM;      // down the rows first: the CTAs of a round share columns of X
-    m.c0 = (int)(tile / down) * BN;
+    m.c0 = (int)(tile / down) * MU_BM;
     m.r0 = (int)(tile % down) * MU_BM;
   } else {
     int rb = 0;
-    for (;; rb++) {
-      const int across = ((rb + 1) * MU_BM + BN - 1) / BN;
-      if (tile < across) break;
-      tile -= across;
-    }
+    for (; tile > rb; rb++) tile -= rb + 1;
     m.r0 = rb * MU_BM;
-    m.c0 = (int)tile * BN;
+    m.c0 = (int)tile * MU_BM;
   }
   return m;
 }
 
-// Blocks of 128 rows by BN columns of one product over every matrix; a CTA takes every gridDim.x-th (one each with the wide tiles, where
-// nothing is gained by staying). KIND 0: gram = x x^T; 1: poly =
-// B gram + C gram gram (both symmetric: only what lies on and below the diagonal of blocks of 128, the rest mirrored from there); 2: x2 =
-// A x + poly x.
-template <int KIND, int BN>
+// Blocks of 128 rows by 128 columns of one product over every matrix; a CTA takes every gridDim.x-th. KIND 0: gram = x x^T; 1: poly = B gram +
+// C gram gram (both symmetric: only the blocks on and below the diagonal, the others mirrored from there); 2: x2 = A x + poly x.
+template <int KIND>
 __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __grid_constant__ MuonList l, const __grid_constant__ MuonMaps maps) {
-  typedef MuonShape<BN> W;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + W::BARS);
-  uint64_t *bar_full = bars, *bar_empty = bars + W::STAGES, *bar_done = bars + 2 * W::STAGES /* [PLACES] */, *bar_read = bar_done + W::PLACES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_read + W::PLACES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + MU_BARS);
+  uint64_t *bar_full = bars, *bar_empty = bars + MU_STAGES, *bar_done = bars + 2 * MU_STAGES /* [2] */, *bar_read = bar_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_read + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < W::STAGES; s++) {
+    for (int s = 0; s < MU_STAGES; s++) {
       mbar_init(&bar_full[s], 1);
       mbar_init(&bar_empty[s], 1);
     }
-    for (int s = 0; s < W::PLACES; s++) {
+    for (int s = 0; s < 2; s++) {
       mbar_init(&bar_done[s], 1);
       mbar_init(&bar_read[s], MU_EPI);
     }
@@ -408,25 +399,24 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
     if (lane == 0) {
       uint32_t n = 0;                                    // stages filled
       for (long long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x) {
-        const MuonTile m = mu_tile<KIND, BN>(l, tile);
+        const MuonTile m = mu_tile<KIND>(l, tile);
         const int steps = ((KIND == 0 ? l.t[m.which].nn : l.t[m.which].mm) + MU_BK - 1) / MU_BK;
         const CUtensorMap *map_a = &maps.a[m.which], *map_b = KIND == 2 ? &maps.b[m.which] : map_a;
         for (int k = 0; ok && k < steps; k++, n++) {
-          const uint32_t s = n % W::STAGES;
-          if (n >= W::STAGES) ok = mbar_wait(&bar_empty[s], ((n / W::STAGES) & 1u) ^ 1u, abort_flag, l.status, 101);
+          const uint32_t s = n % MU_STAGES;
+          if (n >= MU_STAGES) ok = mbar_wait(&bar_empty[s], ((n / MU_STAGES) & 1u) ^ 1u, abort_flag, l.status, 101);
           if (!ok) break;
-          uint8_t* at = smem + s * W::STAGE;
-          mbar_expect_tx(&bar_full[s], W::STAGE);
+          uint8_t* at = smem + s * MU_STAGE;
+          mbar_expect_tx(&bar_full[s], MU_STAGE);
 #pragma unroll
           for (int plane = 0; plane < 2; plane++) {
-            mu_load(at + plane * W::PLANE_A, map_a, k * MU_BK, m.r0, plane, &bar_full[s]);
-            uint8_t* b = at + 2 * W::PLANE_A + plane * W::PLANE_B;
+            mu_load(at + plane * MU_PLANE, map_a, k * MU_BK, m.r0, plane, &bar_full[s]);
+            uint8_t* b = at + (2 + plane) * MU_PLANE;
             if (KIND == 2) {
-#pragma unroll
-              for (int c = 0; c < BN / 64; c++) mu_load(b + c * 64 * 128, map_b, m.c0 + c * 64, k * MU_BK, plane, &bar_full[s]);
+              mu_load(b, map_b, m.c0, k * MU_BK, plane, &bar_full[s]);
+              mu_load(b + 64 * 128, map_b, m.c0 + 64, k * MU_BK, plane, &bar_full[s]);
             } else {
-#pragma unroll
-              for (int c = 0; c < BN / 128; c++) mu_load(b + c * 128 * 128, map_b, k * MU_BK, m.c0 + c * 128, plane, &bar_full[s]);
+              mu_load(b, map_b, k * MU_BK, m.c0, plane, &bar_full[s]);
             }
           }
         }
@@ -435,68 +425,108 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
   } else if (warp == MU_EPI) {
     if (lane == 0) {
       // Half-precision operands, fp32 sums; B is K-major (rows of the same matrix) or MN-major (X as it lies).
-      constexpr uint32_t idesc = (1u << 4) | ((KIND == 2 ? 1u : 0u) << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(MU_BM >> 4) << 24);
+      constexpr uint32_t idesc = (1u << 4) | ((KIND == 2 ? 1u : 0u) << 16) | ((uint32_t)(MU_BM >> 3) << 17) | ((uint32_t)(MU_BM >> 4) << 24);
       constexpr uint32_t lbo_b = KIND == 2 ? ((64u * 128u) >> 4) << 16 : 1u << 16, step_b = KIND == 2 ? (16u * 128u) >> 4 : 2u;
-      uint32_t n = 0, j = 0;                             // stages used, tiles begun
-      for (long long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, j++) {
-        const MuonTensor& t = l.t[mu_tile<KIND, BN>(l, tile).which];
+      uint32_t n = 0, j = 0, turn = 0;                   // stages used, sums begun, tiles
+      for (long long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, turn ^= 1u) {
+        const MuonTensor& t = l.t[mu_tile<KIND>(l, tile).which];
         const int steps = ((KIND == 0 ? t.nn : t.mm) + MU_BK - 1) / MU_BK;
-        const uint32_t place = j % W::PLACES, acc = tmem + place * 2 * BN;
-        if (j >= W::PLACES && !(ok = mbar_wait(&bar_read[place], ((j / W::PLACES) & 1u) ^ 1u, abort_flag, l.status, 104))) break;
+        const uint32_t small = tmem + (2 + turn) * MU_BM;
         for (int k = 0; ok && k < steps; k++, n++) {
-          const uint32_t s = n % W::STAGES;
-          if (!(ok = mbar_wait(&bar_full[s], (n / W::STAGES) & 1u, abort_flag, l.status, 102))) break;
+          const uint32_t s = n % MU_STAGES, place = j & 1u, acc = tmem + place * MU_BM;
+          // The sum before last has been read, and with it, where it was a tile's last, that tile's small products.
+          if (k % MU_SUM == 0 && j >= 2 && !(ok = mbar_wait(&bar_read[place], ((j >> 1) & 1u) ^ 1u, abort_flag, l.status, 104))) break;
+          if (!(ok = mbar_wait(&bar_full[s], (n / MU_STAGES) & 1u, abort_flag, l.status, 102))) break;
           tc_fence_after();
-          const uint32_t a_h = (smem_u32(smem + s * W::STAGE) >> 4) | 1u << 16, a_l = a_h + (W::PLANE_A >> 4);
-          const uint32_t b_h = (smem_u32(smem + s * W::STAGE + 2 * W::PLANE_A) >> 4) | lbo_b, b_l = b_h + (W::PLANE_B >> 4);
+          const uint32_t a_h = (smem_u32(smem + s * MU_STAGE) >> 4) | 1u << 16, a_l = a_h + (MU_PLANE >> 4);
+          const uint32_t b_h = (smem_u32(smem + s * MU_STAGE + 2 * MU_PLANE) >> 4) | lbo_b, b_l = b_h + (MU_PLANE >> 4);
 #pragma unroll
           for (int ks = 0; ks < MU_BK / 16; ks++) {
-            const uint32_t ao = ks * 2u, bo = ks * step_b, more = (k > 0 || ks > 0) ? 1u : 0u;
-            mu_mma(acc, a_h + ao, b_h + bo, idesc, more);
-            mu_mma(acc + BN, a_h + ao, b_l + bo, idesc, more);
-            mu_mma(acc + BN, a_l + ao, b_h + bo, idesc, 1u);
+            const uint32_t ao = ks * 2u, bo = ks * step_b;
+            mu_mma(acc, a_h + ao, b_h + bo, idesc, k % MU_SUM > 0 || ks > 0 ? 1u : 0u);
+            mu_mma(small, a_h + ao, b_l + bo, idesc, k > 0 || ks > 0 ? 1u : 0u);
+            mu_mma(small, a_l + ao, b_h + bo, idesc, 1u);
           }
           umma_commit(&bar_empty[s]);
+          if (k % MU_SUM == MU_SUM - 1 || k == steps - 1) {
+            umma_commit(&bar_done[place]);
+            j++;
+          }
         }
-        if (ok) umma_commit(&bar_done[place]);
       }
       if (!ok) *abort_flag = 1;
     }
   } else {
-    uint32_t j = 0;
-    for (long long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, j++) {
-      const MuonTile m = mu_tile<KIND, BN>(l, tile);
+    uint32_t j = 0, turn = 0;
+    for (long long tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, turn ^= 1u) {
+      const MuonTile m = mu_tile<KIND>(l, tile);
       const MuonTensor& t = l.t[m.which];
       const int M = t.mm, N = KIND == 2 ? t.nn : t.mm;
-      const int r = m.r0 + (warp & 3) * 32 + lane, first = (warp >> 2) * (BN / 2);
-      const uint32_t place = j % W::PLACES, t_acc = tmem + place * 2 * BN + ((uint32_t)((warp & 3) * 32) << 16);
+      const int steps = ((KIND == 0 ? t.nn : t.mm) + MU_BK - 1) / MU_BK, sums = (steps + MU_SUM - 1) / MU_SUM;
+      const int r = m.r0 + (warp & 3) * 32 + lane, first = (warp >> 2) * 64;
+      const uint32_t t_lane = tmem + (uint32_t)first + ((uint32_t)((warp & 3) * 32) << 16);
       const MuonPlanes& out = KIND == 0 ? t.gram : KIND == 1 ? t.poly : t.x2;
       const MuonPlanes& in = KIND == 1 ? t.gram : t.x;
-      // What the result adds to is fetched a block of 32 columns ahead, the first one under the products.
       const int row0 = m.r0 + (warp & 3) * 32;
-      uint4* stage = reinterpret_cast<uint4*>(smem + W::TURN) + warp * 32 * MU_PITCH;
+      uint4* stage = reinterpret_cast<uint4*>(smem + MU_TURN) + warp * 32 * MU_PITCH;
+      auto wait = [&]() {
+        if (lane == 0) ok = mbar_wait(&bar_done[j & 1u], (j >> 1) & 1u, abort_flag, l.status, 103);
+        __syncwarp();                                    // what the lane waited for is seen by the others: a vote orders no memory
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      };
+      auto read = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_read[j & 1u])) : "memory");
+      };
+      // What the result adds to is fetched a block of 32 columns ahead, the first one under the products.
       MuonBlock next;
       if (KIND != 0) mu_fetch(in, row0, M, m.c0 + first, N, lane, next);
-      ok = true;
-      if (lane == 0) ok = mbar_wait(&bar_done[place], (j / W::PLACES) & 1u, abort_flag, l.status, 103);
-      ok = __all_sync(0xffffffffu, ok);
-      __syncwarp();                                      // what the lane waited for is seen by the others: a vote orders no memory
+      wait();
+      if (sums > 1) {
+        // Added up in fp32, and what comes out put back in the place of the last, so that long and short sums end alike.
+        float sum[64];
+#pragma unroll
+        for (int u = 0; u < 64; u++) sum[u] = 0.f;
+        for (int q = 1; ok; q++) {
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            uint32_t acc[32];
+            tmem_ld_32x32b_x32(t_lane + (j & 1u) * MU_BM + (uint32_t)c, acc);
+            tmem_ld_wait();
+#pragma unroll
+            for (int u = 0; u < 32; u++) sum[c + u] += __uint_as_float(acc[u]);
+          }
+          if (q == sums) break;
+          read();
+          j++;
+          wait();
+        }
+#pragma unroll
+        for (int c = 0; c < 64; c += 32) {
+          uint32_t acc[32];
+#pragma unroll
+          for (int u = 0; u < 32; u++) acc[u] = __float_as_uint(sum[c + u]);
+          tmem_st_32x32b_x32(t_lane + (j & 1u) * MU_BM + (uint32_t)c, acc);
+        }
+        tmem_st_wait();
+      }
       if (!ok) break;
-      tc_fence_after();
 #pragma unroll 1
-      for (int c = first; c < first + BN / 2; c += 32) {
-        const int col = m.c0 + c;
-        if (col >= N || (KIND != 2 && col >= m.r0 + MU_BM)) break;   // the same for the whole warp
+      for (int b = 0; b < 64; b += 32) {
+        const int col = m.c0 + first + b;
+        if (col >= N) break;                             // the same for the whole warp
         uint32_t acc[32], small[32];
         __syncwarp();
-        tmem_ld_32x32b_x32(t_acc + (uint32_t)c, acc);
-        tmem_ld_32x32b_x32(t_acc + (uint32_t)(BN + c), small);
+        tmem_ld_32x32b_x32(t_lane + (j & 1u) * MU_BM + (uint32_t)b, acc);
+        tmem_ld_32x32b_x32(t_lane + (2 + turn) * MU_BM + (uint32_t)b, small);
         tmem_ld_wait();
         uint4 vh[4], vl[4];
         if (KIND != 0) {
           mu_to_rows(stage, lane, next.h, vh);
           mu_to_rows(stage, lane, next.l, vl);
-          if (c + 32 < first + BN / 2) mu_fetch(in, row0, M, col + 32, N, lane, next);
+          if (b == 0) mu_fetch(in, row0, M, col + 32, N, lane, next);
         }
         uint32_t hi[16], lo[16];
 #pragma unroll
@@ -527,9 +557,8 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
           }
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(&bar_read[place])) : "memory");
+      read();
+      j++;
     }
   }
   tc_fence_before();
@@ -556,31 +585,17 @@ static int64_t mu_items(MuonList& l, F items) {
   return end;
 }
 
-template <int KIND, int BN>
-static int32_t mu_launch(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
-  const int64_t n = mu_items(l, [](const MuonTensor& t) {
-    const int64_t rb = ceil_div(t.mm, MU_BM);
-    if (KIND == 2) return rb * ceil_div(t.nn, BN);
-    int64_t all = 0;
-    for (int64_t r = 0; r < rb; r++) all += ceil_div((r + 1) * MU_BM, BN);
-    return all;
-  });
-  OM_CUDA(ctx, cudaFuncSetAttribute(muon_product_kernel<KIND, BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, MuonShape<BN>::SMEM));
-  launch_chained(ctx, muon_product_kernel<KIND, BN>, (unsigned)(MuonShape<BN>::PLACES > 1 ? std::min<int64_t>(n, ctx->sm_count) : n), MU_THREADS, MuonShape<BN>::SMEM, l, maps);
-  return OM_OK;
-}
-// Tiles of 128 x 256 where there are two for every SM: a stage's operands serve twice the products. Else tiles of 128 x 128, more even
-// over the SMs and read back under the next tile's products. One square matrix, five steps, narrow against wide: 1024 260 and 419 us,
-// 2048 (128 wide tiles in Y X) 510 and 681, 2560 (200) 1090 and 1073, 4096 (512) 4041 and 3944, 5120 7988 and 7619. 24 matrices of
-// 384 x 384 to 1536 (240, sums of 384): 338 and 390.
+// Tiles of 128 x 256 gain nothing: twice as many sums a thread are read back no faster than they are made. One square matrix, five steps, those
+// against these: 1024 287 and 292 us, 2048 565 and 567, 4096 4080 and 3870.
 template <int KIND>
 static int32_t mu_product(om_ctx* ctx, MuonList& l, const MuonMaps& maps) {
-  int64_t wide = 0;
-  for (int i = 0; i < l.count; i++) {
-    const int64_t rb = ceil_div(l.t[i].mm, MU_BM), nb = ceil_div(KIND == 2 ? l.t[i].nn : l.t[i].mm, 256);
-    wide += KIND == 2 ? rb * nb : (rb * nb + rb) / 2;
-  }
-  return wide >= 2 * ctx->sm_count ? mu_launch<KIND, 256>(ctx, l, maps) : mu_launch<KIND, 128>(ctx, l, maps);
+  const int64_t n = mu_items(l, [](const MuonTensor& t) {
+    const int64_t rb = ceil_div(t.mm, MU_BM);
+    return KIND == 2 ? rb * ceil_div(t.nn, MU_BM) : rb * (rb + 1) / 2;
+  });
+  OM_CUDA(ctx, cudaFuncSetAttribute(muon_product_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, MU_SMEM));
+  launch_chained(ctx, muon_product_kernel<KIND>, (unsigned)std::min<int64_t>(n, ctx->sm_count), MU_THREADS, MU_SMEM, l, maps);
+  return OM_OK;
 }
 
 }  // namespace om

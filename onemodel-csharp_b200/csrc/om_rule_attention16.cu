@@ -88,16 +88,6 @@ __device__ __forceinline__ void r16_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo
       ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(R16_DESC_HI), "r"(0u)
       : "memory");
 }
-__device__ __forceinline__ void r16_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 __device__ __forceinline__ void r16_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
@@ -105,7 +95,6 @@ __device__ __forceinline__ void r16_st16(uint32_t taddr, const uint32_t (&r)[16]
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void r16_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bytes of a tile of 128 rows.
 template <int DP, int PL>
@@ -673,7 +662,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             tmem_ld_wait();
 #pragma unroll
             for (int u = 0; u < 32; u++) o[u] = __float_as_uint(__uint_as_float(o[u]) * shrink);
-            r16_st32(t_o + (uint32_t)c, o);
+            tmem_st_32x32b_x32(t_o + (uint32_t)c, o);
           }
         }
       }
@@ -686,7 +675,7 @@ rule16_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         ok = ok && r16_wait(&bar_full[stage % W::STAGES], (stage / W::STAGES) & 1u, abort_flag, p.status, 68);
         if (ok) r16_clear<DP>(ring + stage % W::STAGES * W::TILE, r.k_pads + (long long)bi * r.nk64, (first + r16_tile_of(step)) * (R16_T / RULE_GRAIN), r.nk64, warp, lane);
       }
-      r16_st_wait();
+      tmem_st_wait();
       r16_arrive_warp(&bar_p[place], lane);
     }
     if (!gone) {
@@ -1117,7 +1106,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         r16_clear<DP>(ring_g + a * W::TILE, pads, at64, r.nq64, warp, lane);
         r16_clear<DP>(ring_q + a * W::TILE, pads, at64, r.nq64, warp, lane);
       }
-      r16_st_wait();
+      tmem_st_wait();
       r16_arrive_warp(bar_p, lane);
       ok = ok && r16_wait(bar_dp, phase, abort_flag, p.status, 81);
       if (PL == 1 && !ok) break;
@@ -1153,7 +1142,7 @@ rule16_dkv_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         r16_gradients16<true>(x[1], dp[1], w, rows + 160, 0.f, partial);
         r16_st16(t_dp + 16u, w);
       }
-      r16_st_wait();
+      tmem_st_wait();
       r16_arrive_warp(bar_ds, lane);
     }
     if (ok) ok = r16_wait(bar_done, 0, abort_flag, p.status, 82);
@@ -1375,7 +1364,7 @@ rule16_dq_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       }
       if (PL == 1 && r16_padded(step))
         r16_clear<DP>(ring_k + n % W::RING_A * W::TILE, r.k_pads + (long long)bi * r.nk64, (first + r16_tile_of(step)) * (R16_T / RULE_GRAIN), r.nk64, warp, lane);
-      r16_st_wait();
+      tmem_st_wait();
       r16_arrive_warp(&bar_ds[place], lane);
     }
     if (ok) ok = r16_wait(bar_done, 0, abort_flag, p.status, 93);
