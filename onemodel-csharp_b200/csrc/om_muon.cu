@@ -72,7 +72,7 @@ __device__ __forceinline__ int mu_find(const MuonList& l, long long item, long l
 }
 
 // m = momentum m + (1 - momentum) g, and the sum of squares of u over this chunk (in double: the chunks of a large matrix
-// differ by orders of magnitude in what they add).
+// differ by orders of magnitude in what they add, and squares of u beyond 2^64 or below 2^-64 leave fp32).
 __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constant__ MuonList l) {
   pdl_enter();
   long long chunk;
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constan
   auto one = [&](float g, float& m) {
     g = g * h.grad_scale * (1.f - h.momentum);
     m = fmaf(m, h.momentum, g);
-    const float u = h.nesterov ? fmaf(m, h.momentum, g) : m;
+    const double u = h.nesterov ? fmaf(m, h.momentum, g) : m;
     return u * u;
   };
   // What a thread needs comes in front of what it writes: between a store and a load behind it the compiler keeps the order.
@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(256) muon_momentum_kernel(const __grid_constan
 #pragma unroll
       for (int u = 0; u < 4; u++)
         if (e + 1024 * u < e1) {
-          const float a = one(g[u].x, m[u].x), b = one(g[u].y, m[u].y), c = one(g[u].z, m[u].z), d = one(g[u].w, m[u].w);
+          const double a = one(g[u].x, m[u].x), b = one(g[u].y, m[u].y), c = one(g[u].z, m[u].z), d = one(g[u].w, m[u].w);
           *reinterpret_cast<float4*>(t.m + e + 1024 * u) = m[u];
-          sum += ((double)a + b) + ((double)c + d);
+          sum += (a + b) + (c + d);
         }
     }
   } else {
@@ -161,11 +161,13 @@ __global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__
   __syncthreads();
   sum = 0.0;
   for (int w = 0; w < 8; w++) sum += s[w];
-  const float norm = fmaxf((float)sqrt(sum), h.eps);
+  // A norm near fp32's end, or past it, is divided out 2^-64 of u at a time.
+  const double full = fmax(sqrt(sum), (double)h.eps);
+  const float part = full > 1e30 ? 0x1p-64f : 1.f, norm = (float)(full * part);
   int r0, c0;
   mu_block(t, tile, &r0, &c0);
   const bool turn = t.rows > t.cols;
-  auto one = [&](float m, float g) { return (h.nesterov ? fmaf(m, h.momentum, g * h.grad_scale * (1.f - h.momentum)) : m) / norm * MU_SX; };
+  auto one = [&](float m, float g) { return (h.nesterov ? fmaf(m, h.momentum, g * h.grad_scale * (1.f - h.momentum)) : m) * part / norm * MU_SX; };
   if (t.quads) {
 #pragma unroll
     for (int e = threadIdx.x; e < 64 * 16; e += 256) {

@@ -3,7 +3,8 @@ of 24 amount to. fp32 is numpy's here, with the products of a BLAS."""
 import numpy as np
 import pytest
 
-from test_gpu_muon import make, step
+import rule_reference as ref
+from test_gpu_muon import check, make, step
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +46,13 @@ def test_digits_of_many_large_matrices_in_one_launch(ctx):
     for i in list(range(8)) + [31]:
         err, allowed = digits(-got[i][0].astype(np.float64) / (0.2 * np.sqrt(max(shapes[i]))), mats[i][1].astype(np.float64))
         assert err <= allowed, (shapes[i], err, allowed)
+
+
+@pytest.mark.parametrize("size,eps", [(1e22, 1e-7), (1e35, 1e-7), (2e37, 1e-7), (1e-25, 1e-30), (1e-29, 1e-35)])
+def test_updates_of_any_size(ctx, size, eps):
+    """X depends on u / |u| alone, however large or small the squares of u are."""
+    r = np.random.default_rng(81)
+    for rows, cols in ((96, 160), (33, 7)):
+        p, g, m = make(r, rows, cols, 1.0)
+        mat = (p, (g * np.float32(size)).astype(np.float32), (m * np.float32(size)).astype(np.float32))
+        check(step(ctx, [mat], eps=eps)[0], mat, eps=eps)
