@@ -592,7 +592,10 @@ int32_t om_rule_attention_bwd(om_ctx* ctx, const om_attention_rule* rule, const 
                               const om_head_strides* dvs);
 /* The same with bfloat16 operands: scores, softmax statistics and sums in fp32, the weights and the scores' gradients rounded to
  * bfloat16 as operands of the products behind them. The forward writes out, out16 (same strides) or both, the backward each
- * gradient as fp32, bfloat16 or both; the backward takes the output as bfloat16. */
+ * gradient as fp32, bfloat16 or both. The backward takes the output as bfloat16, or, in the _out32 form, as fp32: its row dots
+ * with the output's gradient are subtracted from products that nearly equal them in a row which looks at one key almost alone, and
+ * the rounding of the output to bfloat16 can be all that is left of such a row's dq (dq as a whole, scores of a few: 4.8e-3 off with
+ * the one, 2.0e-3 with the other). */
 int32_t om_rule_attention_fwd_bf16(om_ctx* ctx, const om_attention_rule* rule, const uint16_t* q16, const om_head_strides* qs,
                                    const uint16_t* k16, const om_head_strides* ks, const uint16_t* v16, const om_head_strides* vs,
                                    int32_t b, int32_t h, int32_t hkv, int32_t lq, int32_t lk, int32_t d, float scale, float* out,
@@ -603,6 +606,12 @@ int32_t om_rule_attention_bwd_bf16(om_ctx* ctx, const om_attention_rule* rule, c
                                    const float* lse, int32_t b, int32_t h, int32_t hkv, int32_t lq, int32_t lk, int32_t d,
                                    float scale, float* dq, uint16_t* dq16, const om_head_strides* dqs, float* dk, uint16_t* dk16,
                                    const om_head_strides* dks, float* dv, uint16_t* dv16, const om_head_strides* dvs);
+int32_t om_rule_attention_bwd_bf16_out32(om_ctx* ctx, const om_attention_rule* rule, const uint16_t* g16, const om_head_strides* gs,
+                                         const uint16_t* q16, const om_head_strides* qs, const uint16_t* k16, const om_head_strides* ks,
+                                         const uint16_t* v16, const om_head_strides* vs, const float* out, const om_head_strides* os,
+                                         const float* lse, int32_t b, int32_t h, int32_t hkv, int32_t lq, int32_t lk, int32_t d,
+                                         float scale, float* dq, uint16_t* dq16, const om_head_strides* dqs, float* dk, uint16_t* dk16,
+                                         const om_head_strides* dks, float* dv, uint16_t* dv16, const om_head_strides* dvs);
 
 /* ---- rotary positions -------------------------------------------------------------------------------------------- */
 

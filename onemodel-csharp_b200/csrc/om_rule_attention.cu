@@ -329,14 +329,17 @@ rule_attention_fwd_kernel(const __grid_constant__ RaParams<T> p) {
 
 // Row dots rowsum(dO o O) beside the log-sum-exp times `unit` (log2 e for the kernels that work with powers of two); rows behind
 // the last query, and those that see no key, get plus infinity and 0, so that a weight recomputed from them is 0. A power of two of
-// lanes per row, each with 16 bytes at a time (N elements; one where rows do not start on that grid), two rows in flight per lane.
-template <typename T, int N>
+// lanes per row, each with 16 bytes of dO at a time (N elements; one where rows do not start on that grid), two rows in flight per lane.
+template <typename T, typename O, int N>
 __global__ void __launch_bounds__(256)
-rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float* lse, int h, int lq, int lq_pad, int d, int lanes, float unit,
+rule_rows_kernel(const T* g, RaStrides gs, const O* o, RaStrides os, const float* lse, int h, int lq, int lq_pad, int d, int lanes, float unit,
                  long long total, float* __restrict__ rows) {
   pdl_enter();
-  struct alignas(N * sizeof(T)) Vec {
+  struct alignas(N * sizeof(T)) VecG {
     T v[N];
+  };
+  struct alignas(N == 1 ? sizeof(O) : 16) VecO {
+    O v[N];
   };
   const int sub = threadIdx.x & (lanes - 1), per_cta = 256 / lanes;
   for (long long w0 = (long long)blockIdx.x * 2 * per_cta + threadIdx.x / lanes; w0 < total; w0 += (long long)gridDim.x * 2 * per_cta) {
@@ -352,11 +355,12 @@ rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float
         const long long bi = bhs[u] / h;
         const int hi = (int)(bhs[u] - bi * h);
         const T* gp = g + bi * gs.batch + hi * gs.head + (long long)is[u] * gs.row;
-        const T* op = o + bi * os.batch + hi * os.head + (long long)is[u] * os.row;
+        const O* op = o + bi * os.batch + hi * os.head + (long long)is[u] * os.row;
         for (int c = sub * N; c < d; c += lanes * N) {
-          const Vec a = *reinterpret_cast<const Vec*>(gp + c), b = *reinterpret_cast<const Vec*>(op + c);
+          const VecG a = *reinterpret_cast<const VecG*>(gp + c);
+          const VecO b = *reinterpret_cast<const VecO*>(op + c);
 #pragma unroll
-          for (int e = 0; e < N; e++) dot[u] = fmaf(ra_value<T>(a.v[e]), ra_value<T>(b.v[e]), dot[u]);
+          for (int e = 0; e < N; e++) dot[u] = fmaf(ra_value<T>(a.v[e]), ra_value<O>(b.v[e]), dot[u]);
         }
       }
     }
@@ -375,21 +379,21 @@ rule_rows_kernel(const T* g, RaStrides gs, const T* o, RaStrides os, const float
     }
   }
 }
-template <typename T>
-static void launch_rows(om_ctx* ctx, const T* g, const om_head_strides* gs, const T* o, const om_head_strides* os, const float* lse, int b, int h, int lq, int d,
+template <typename T, typename O>
+static void launch_rows(om_ctx* ctx, const T* g, const om_head_strides* gs, const O* o, const om_head_strides* os, const float* lse, int b, int h, int lq, int d,
                         float unit, float* rows) {
   const int lq_pad = rule_row_tiles(lq) * 128;
   const long long total = (long long)b * h * lq_pad;          // a multiple of 128: no warp runs over the end alone
   constexpr int N = 16 / sizeof(T);
-  auto grid16 = [&](const T* p, const om_head_strides* s) {
+  auto grid16 = [&](const void* p, const om_head_strides* s) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s->row % N == 0 && s->head % N == 0 && s->batch % N == 0;
   };
   const bool vec = d % N == 0 && grid16(g, gs) && grid16(o, os);
   int lanes = 1;
   while (lanes < 32 && lanes * (vec ? N : 1) < d) lanes *= 2;
   const int grid = grid_for(ctx, total, 2 * 256 / lanes, 16);
-  if (vec) launch_chained(ctx, rule_rows_kernel<T, N>, grid, 256, 0, g, ra_strides(gs), o, ra_strides(os), lse, h, lq, lq_pad, d, lanes, unit, total, rows);
-  else launch_chained(ctx, rule_rows_kernel<T, 1>, grid, 256, 0, g, ra_strides(gs), o, ra_strides(os), lse, h, lq, lq_pad, d, lanes, unit, total, rows);
+  if (vec) launch_chained(ctx, rule_rows_kernel<T, O, N>, grid, 256, 0, g, ra_strides(gs), o, ra_strides(os), lse, h, lq, lq_pad, d, lanes, unit, total, rows);
+  else launch_chained(ctx, rule_rows_kernel<T, O, 1>, grid, 256, 0, g, ra_strides(gs), o, ra_strides(os), lse, h, lq, lq_pad, d, lanes, unit, total, rows);
 }
 
 // The weights and the scores' gradients of one tile into P and S, [query][key].
@@ -622,7 +626,7 @@ static int32_t rule_fwd(om_ctx* ctx, const char* who, const om_attention_rule* r
 template <typename T>
 static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* rule, const T* g, const om_head_strides* gs, const T* q,
                         const om_head_strides* qs, const T* k, const om_head_strides* ks, const T* v, const om_head_strides* vs, const T* out,
-                        const om_head_strides* os, const float* lse, int b, int h, int hkv, int lq, int lk, int d, float scale, float* dq,
+                        const float* out32, const om_head_strides* os, const float* lse, int b, int h, int hkv, int lq, int lk, int d, float scale, float* dq,
                         __nv_bfloat16* dq16, const om_head_strides* dqs, float* dk, __nv_bfloat16* dk16, const om_head_strides* dks, float* dv,
                         __nv_bfloat16* dv16, const om_head_strides* dvs) {
   OM_TRY(rule_check(ctx, who, rule, b, h, hkv, lq, lk, d, scale));
@@ -648,7 +652,7 @@ static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   OM_TRY(rule_operand(ctx, who, q, qs, d));
   OM_TRY(rule_operand(ctx, who, k, ks, d));
   OM_TRY(rule_operand(ctx, who, v, vs, d));
-  OM_TRY(rule_operand(ctx, who, out, os, d));
+  OM_TRY(rule_operand(ctx, who, out32 ? (const void*)out32 : out, os, d));
   ProfileScope prof(ctx, "om_rule_attention_bwd", 10.0 * b * h * (double)lq * lk * d, sizeof(T) * (4.0 * b * h * (double)lq * d + 4.0 * b * hkv * (double)lk * d));
   RuleCall call;
   OM_TRY(rule_begin(ctx, rule, b, h, hkv, lq, lk, d, scale, &call));
@@ -658,7 +662,9 @@ static int32_t rule_bwd(om_ctx* ctx, const char* who, const om_attention_rule* r
   if (st == OM_OK) {
     const bool tensor = sizeof(T) == 2 && rule16_bwd_takes(call, g, gs, q, qs, k, ks, v, vs, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs);
     const bool apart = sizeof(T) == 4 && rule16_planes_take(call, true) && rule16_result_fits(dq, dqs) && rule16_result_fits(dk, dks) && rule16_result_fits(dv, dvs);
-    launch_rows<T>(ctx, g, gs, out, os, lse, b, h, lq, d, tensor || apart ? 1.4426950408889634f : 1.f, rows);
+    const float unit = tensor || apart ? 1.4426950408889634f : 1.f;
+    if (out32) launch_rows(ctx, g, gs, out32, os, lse, b, h, lq, d, unit, rows);
+    else launch_rows(ctx, g, gs, out, os, lse, b, h, lq, d, unit, rows);
     if (tensor) {
       st = rule16_bwd(ctx, call, g, gs, q, qs, k, ks, v, vs, rows, dq, dq16, dqs, dk, dk16, dks, dv, dv16, dvs, nullptr);
       pool_free(ctx, rows);
@@ -710,7 +716,7 @@ int32_t om_rule_attention_bwd(om_ctx* ctx, const om_attention_rule* rule, const 
                               int32_t d, float scale, float* dq, const om_head_strides* dqs, float* dk, const om_head_strides* dks, float* dv,
                               const om_head_strides* dvs) {
   OM_CHECK_CTX(ctx);
-  return rule_bwd<float>(ctx, "om_rule_attention_bwd", rule, g, gs, q, qs, k, ks, v, vs, out, os, lse, b, h, hkv, lq, lk, d, scale, dq, nullptr, dqs, dk,
+  return rule_bwd<float>(ctx, "om_rule_attention_bwd", rule, g, gs, q, qs, k, ks, v, vs, out, nullptr, os, lse, b, h, hkv, lq, lk, d, scale, dq, nullptr, dqs, dk,
                          nullptr, dks, dv, nullptr, dvs);
 }
 
@@ -731,8 +737,20 @@ int32_t om_rule_attention_bwd_bf16(om_ctx* ctx, const om_attention_rule* rule, c
   OM_CHECK_CTX(ctx);
   typedef __nv_bfloat16 T;
   return rule_bwd<T>(ctx, "om_rule_attention_bwd_bf16", rule, reinterpret_cast<const T*>(g16), gs, reinterpret_cast<const T*>(q16), qs,
-                     reinterpret_cast<const T*>(k16), ks, reinterpret_cast<const T*>(v16), vs, reinterpret_cast<const T*>(out16), os, lse, b, h, hkv, lq, lk, d,
-                     scale, dq, reinterpret_cast<T*>(dq16), dqs, dk, reinterpret_cast<T*>(dk16), dks, dv, reinterpret_cast<T*>(dv16), dvs);
+                     reinterpret_cast<const T*>(k16), ks, reinterpret_cast<const T*>(v16), vs, reinterpret_cast<const T*>(out16), nullptr, os, lse, b, h, hkv,
+                     lq, lk, d, scale, dq, reinterpret_cast<T*>(dq16), dqs, dk, reinterpret_cast<T*>(dk16), dks, dv, reinterpret_cast<T*>(dv16), dvs);
+}
+
+int32_t om_rule_attention_bwd_bf16_out32(om_ctx* ctx, const om_attention_rule* rule, const uint16_t* g16, const om_head_strides* gs, const uint16_t* q16,
+                                         const om_head_strides* qs, const uint16_t* k16, const om_head_strides* ks, const uint16_t* v16,
+                                         const om_head_strides* vs, const float* out, const om_head_strides* os, const float* lse, int32_t b, int32_t h,
+                                         int32_t hkv, int32_t lq, int32_t lk, int32_t d, float scale, float* dq, uint16_t* dq16, const om_head_strides* dqs,
+                                         float* dk, uint16_t* dk16, const om_head_strides* dks, float* dv, uint16_t* dv16, const om_head_strides* dvs) {
+  OM_CHECK_CTX(ctx);
+  typedef __nv_bfloat16 T;
+  return rule_bwd<T>(ctx, "om_rule_attention_bwd_bf16_out32", rule, reinterpret_cast<const T*>(g16), gs, reinterpret_cast<const T*>(q16), qs,
+                     reinterpret_cast<const T*>(k16), ks, reinterpret_cast<const T*>(v16), vs, nullptr, out, os, lse, b, h, hkv, lq, lk, d, scale, dq,
+                     reinterpret_cast<T*>(dq16), dqs, dk, reinterpret_cast<T*>(dk16), dks, dv, reinterpret_cast<T*>(dv16), dvs);
 }
 
 }  // extern "C"

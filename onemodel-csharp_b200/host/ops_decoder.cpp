@@ -207,8 +207,8 @@ void RuleAttentionBackward(BackwardRecord& r, const Tensor& g) {
   if (!dv.IsEmpty()) dvs = StridesOf(dv, keyHeads);
   float *dqp = dq.IsEmpty() ? nullptr : dq.Data(), *dkp = dk.IsEmpty() ? nullptr : dk.Data(), *dvp = dv.IsEmpty() ? nullptr : dv.Data();
   if (r.Ints[5]) {
-    Check(om_rule_attention_bwd_bf16(C(), &rule, gc.Bf16(), &gs, q.Bf16(), &qs, k.Bf16(), &ks, v.Bf16(), &vs, out.Bf16(), &os, lse.Data(), s.b, s.h, s.hkv,
-                                     s.lq, s.lk, s.d, scale, dqp, nullptr, &dqs, dkp, nullptr, &dks, dvp, nullptr, &dvs));
+    Check(om_rule_attention_bwd_bf16_out32(C(), &rule, gc.Bf16(), &gs, q.Bf16(), &qs, k.Bf16(), &ks, v.Bf16(), &vs, out.Data(), &os, lse.Data(), s.b, s.h,
+                                           s.hkv, s.lq, s.lk, s.d, scale, dqp, nullptr, &dqs, dkp, nullptr, &dks, dvp, nullptr, &dvs));
   } else {
     Check(om_rule_attention_bwd(C(), &rule, gc.Data(), &gs, q.Data(), &qs, k.Data(), &ks, v.Data(), &vs, out.Data(), &os, lse.Data(), s.b, s.h, s.hkv, s.lq,
                                 s.lk, s.d, scale, dqp, &dqs, dkp, &dks, dvp, &dvs));
