@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256) muon_start_kernel(const __grid_constant__
   for (int w = 0; w < 8; w++) sum += s[w];
   // A norm near fp32's end, or past it, is divided out 2^-64 of u at a time.
   const double full = fmax(sqrt(sum), (double)h.eps);
-  const float part = full > 1e30 ? 0x1p-64f : 1.f, norm = (float)(full * part);
+  const float part = full > 1e30 ? 0x1p-64f : 1.f, norm = full > 0.0 ? (float)(full * part) : 1.f;   // nothing over nothing: nothing
   int r0, c0;
   mu_block(t, tile, &r0, &c0);
   const bool turn = t.rows > t.cols;

@@ -3,7 +3,6 @@ of 24 amount to. fp32 is numpy's here, with the products of a BLAS."""
 import numpy as np
 import pytest
 
-import rule_reference as ref
 from test_gpu_muon import check, make, step
 
 pytestmark = pytest.mark.gpu
@@ -56,3 +55,11 @@ def test_updates_of_any_size(ctx, size, eps):
         p, g, m = make(r, rows, cols, 1.0)
         mat = (p, (g * np.float32(size)).astype(np.float32), (m * np.float32(size)).astype(np.float32))
         check(step(ctx, [mat], eps=eps)[0], mat, eps=eps)
+
+
+def test_an_update_of_zero_without_an_eps(ctx):
+    """X is zero, not zero over zero: the weights decay and nothing else."""
+    p = make(np.random.default_rng(82), 40, 70)[0]
+    zero = np.zeros_like(p)
+    got = step(ctx, [(p, zero, zero)], eps=0.0, lr=0.5)[0]
+    assert np.abs(got[0] - 0.95 * p.astype(np.float64)).max() <= 2.0 ** -23 * np.abs(p).max() and (got[1] == 0).all()
