@@ -6,10 +6,12 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <functional>
 #include <map>
 #include <string>
 #include <unordered_map>
+#include <utility>
 #include <vector>
 
 #include "../../include/onemodel_b200.h"
@@ -127,6 +129,28 @@ struct ProfileScope {
 constexpr int kArrivalSlots = 4096;
 
 static inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Whether two rows of d elements of a result [b, h, l, d] share memory. Strides are not negative and rows at least d apart.
+static inline bool heads_overlap(const om_head_strides& s, int64_t b, int64_t h, int64_t l, int64_t d) {
+  // Axes nested in one another, as in any view of a tensor in memory order, do not.
+  std::pair<int64_t, int64_t> axes[3] = {{s.batch, b}, {s.head, h}, {s.row, l}};
+  std::sort(axes, axes + 3);
+  int64_t span = d;
+  bool nested = true;
+  for (const auto& a : axes) {
+    if (a.second <= 1) continue;
+    nested = nested && a.first >= span;
+    span = a.first * (a.second - 1) + span;
+  }
+  if (nested) return false;
+  // Else two rows (i, j, k) apart are less than d elements apart, or none are.
+  for (int64_t i = 0; i < b; i++)
+    for (int64_t j = i ? 1 - h : 0; j < h; j++) {
+      const int64_t t = i * s.batch + j * s.head, k0 = -t / s.row;
+      for (int64_t k = k0 - 1; k <= k0 + 1; k++)
+        if ((i || j || k) && k > -l && k < l && t + k * s.row < d && t + k * s.row > -d) return true;
+    }
+  return false;
+}
 
 // ---- overlapped launches (programmatic dependent launch) ------------------------------------------------------------
 // A kernel that begins with pdl_enter() may be launched through launch_chained(): its CTAs

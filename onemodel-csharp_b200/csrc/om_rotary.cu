@@ -150,9 +150,8 @@ static int32_t rotary(om_ctx* ctx, const char* who, const T* x, const om_head_st
   if (b < 0 || h < 0 || l < 0 || d < 0) return fail(ctx, OM_ERR_SHAPE, "%s: b %d h %d l %d d %d", who, b, h, l, d);
   if (pairs < 1 || pairs > ROT_PAIRS || 2 * pairs > d)
     return fail(ctx, OM_ERR_SHAPE, "%s: %d pairs of columns do not fit heads of %d columns (at most %d pairs)", who, pairs, d, ROT_PAIRS);
-  if (!xs || !ys || xs->row < d || ys->row < d || xs->batch < 0 || xs->head < 0)
+  if (!xs || !ys || xs->row < d || ys->row < d || xs->batch < 0 || xs->head < 0 || (b > 1 && ys->batch < 0) || (h > 1 && ys->head < 0))
     return fail(ctx, OM_ERR_SHAPE, "%s: rows of an activation must be at least d = %d elements apart and strides non-negative", who, d);
-  if ((b > 1 && ys->batch < d) || (h > 1 && ys->head < d)) return fail(ctx, OM_ERR_SHAPE, "%s: the result's heads overlap", who);
   if (!inv_freq) return fail(ctx, OM_ERR_ARG, "%s: the frequencies are required", who);
   if (!isfinite(magnitude)) return fail(ctx, OM_ERR_ARG, "%s: the magnitude must be finite", who);
   if (positions && positions_batch_stride < 0) return fail(ctx, OM_ERR_SHAPE, "%s: a negative stride of the positions", who);
@@ -163,6 +162,7 @@ static int32_t rotary(om_ctx* ctx, const char* who, const T* x, const om_head_st
   const bool in_place = x == y;
   if (in_place && ((b > 1 && xs->batch != ys->batch) || (h > 1 && xs->head != ys->head) || (l > 1 && xs->row != ys->row)))
     return fail(ctx, OM_ERR_SHAPE, "%s: in place needs the same strides on both sides", who);
+  if (heads_overlap(*ys, b, h, l, d)) return fail(ctx, OM_ERR_SHAPE, "%s: rows of the result overlap", who);
   ProfileScope prof(ctx, "om_rotary", 3.0 * b * h * (double)l * 2 * pairs, 2.0 * sizeof(T) * b * h * (double)l * d);
   RotaryParams p;
   for (int j = 0; j < pairs; j++) p.inv_freq[j] = inv_freq[j];

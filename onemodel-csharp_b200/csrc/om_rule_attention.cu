@@ -80,7 +80,7 @@ int32_t rule_result(om_ctx* ctx, const char* who, const om_head_strides* s, int 
   if (l == 0) return OM_OK;     // nothing is written: strides of an empty tensor may be anything
   if (!s || s->row < d || s->batch < 0 || s->head < 0)
     return fail(ctx, OM_ERR_SHAPE, "%s: rows of a result must be at least d = %d elements apart and strides non-negative", who, d);
-  if ((b > 1 && s->batch < d) || (h > 1 && s->head < d)) return fail(ctx, OM_ERR_SHAPE, "%s: the result's heads overlap", who);
+  if (heads_overlap(*s, b, h, l, d)) return fail(ctx, OM_ERR_SHAPE, "%s: rows of a result overlap", who);
   return OM_OK;
 }
 

@@ -235,3 +235,35 @@ def test_a_row_that_looks_at_one_key_keeps_its_gradient(ctx, api):
     err = np.linalg.norm(got - want["dq"], axis=-1)
     over = err / (allowed + 1e-30)
     assert over[:, :, 1:].max() <= 2, (over[:, :, 1:].max(), over[:, :, 1:].argmax())
+
+
+def test_results_whose_rows_overlap_are_refused(ctx):
+    """Heads in each other's place, also where every stride is large enough by itself; heads between each other's rows are none of it."""
+    r = np.random.default_rng(83)
+    c = Call(ctx, r, 2, 2, 1, 3, 3, 8).run()
+    w = lambda n: (c.where(n)[0], C.byref(c.where(n)[1]))   # noqa: E731
+    room = ctx.zeros((4096,))
+    freq = (C.c_double * 4)(*[0.5] * 4)
+
+    def calls(strides):
+        s, lse = omb.HeadStrides(*strides), c.lse.ptr
+        sizes = [i32(n) for n in c.dims] + [f32(c.scale)]
+        rule = c.rule()
+        yield "om_rule_attention_fwd", [C.byref(rule), *w("q"), *w("k"), *w("v"), *sizes, room.ptr, C.byref(s), None]
+        yield "om_rule_attention_bwd", [C.byref(rule), *w("g"), *w("q"), *w("k"), *w("v"), *w("o"), lse, *sizes, room.ptr, C.byref(s), None, None, None, None]
+        yield "om_rotary", [*w("q"), None, C.c_int64(0), i32(0), i32(2), i32(2), i32(3), i32(8), freq, i32(4), i32(0), f32(1.0), i32(0), room.ptr, C.byref(s)]
+
+    for strides in ((64, 8, 8), (64, 16, 8), (40, 24, 8), (16, 64, 16), (100, 12, 8), (64, 4, 16)):
+        for name, args in calls(strides):
+            with pytest.raises(omb.OmError) as e:
+                ctx.call(name, ctx.handle, *args)
+            assert e.value.status == 1, (name, strides)
+    want = None
+    for strides in ((48, 24, 8), (48, 8, 16), (8, 64, 16), (200, 24, 16), (24, 8, 64)):     # nested; heads or sequences between rows
+        for name, args in calls(strides):
+            ctx.call(name, ctx.handle, *args)
+        ctx.sync()
+        at = sum(np.arange(n).reshape([-1 if a == i else 1 for a in range(4)]) * s for i, (n, s) in enumerate(zip((2, 2, 3, 8), (*strides, 1))))
+        got = room.numpy()[at]               # the last call's
+        assert want is None or np.array_equal(got, want)
+        want = got
