@@ -278,17 +278,6 @@ __global__ void __launch_bounds__(256) muon_finish_kernel(const __grid_constant_
 
 // ---- products ---------------------------------------------------------------------------------------------------------------------
 
-constexpr uint32_t MU_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);     // stride offset 1024 bytes, version 1, 128-byte swizzle
-__device__ __forceinline__ void mu_mma(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-      "mov.b64 da, {%1, %5};\n\t"
-      "mov.b64 db, {%2, %5};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n\t}"
-      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(MU_DESC_HI), "r"(0u)
-      : "memory");
-}
 __device__ __forceinline__ void mu_load(void* dst, const CUtensorMap* map, int c0, int c1, int c2, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)), "l"(map),
                "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
@@ -445,9 +434,9 @@ __global__ void __launch_bounds__(MU_THREADS, 1) muon_product_kernel(const __gri
 #pragma unroll
           for (int ks = 0; ks < MU_BK / 16; ks++) {
             const uint32_t ao = ks * 2u, bo = ks * step_b;
-            mu_mma(acc, a_h + ao, b_h + bo, idesc, k % MU_SUM > 0 || ks > 0 ? 1u : 0u);
-            mu_mma(small, a_h + ao, b_l + bo, idesc, k > 0 || ks > 0 ? 1u : 0u);
-            mu_mma(small, a_l + ao, b_h + bo, idesc, 1u);
+            umma_f16_ss(acc, a_h + ao, b_h + bo, idesc, k % MU_SUM > 0 || ks > 0 ? 1u : 0u);
+            umma_f16_ss(small, a_h + ao, b_l + bo, idesc, k > 0 || ks > 0 ? 1u : 0u);
+            umma_f16_ss(small, a_l + ao, b_h + bo, idesc, 1u);
           }
           umma_commit(&bar_empty[s]);
           if (k % MU_SUM == MU_SUM - 1 || k == steps - 1) {

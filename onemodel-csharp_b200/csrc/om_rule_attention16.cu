@@ -58,25 +58,13 @@ __device__ __forceinline__ uint32_t r16_pack(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Shared-memory descriptors share their upper word (stride offset 1024 bytes, version 1, 128-byte swizzle); the lower one is
-// (address >> 4) with the leading offset, one block of 64 columns for MN-major operands.
-constexpr uint32_t R16_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+// The lower word of a shared-memory descriptor: (address >> 4) with the leading offset, one block of 64 columns for MN-major operands.
 constexpr uint32_t R16_LBO_K = 1u << 16, R16_LBO_MN = ((uint32_t)R16_CHUNK >> 4) << 16;
 __device__ __forceinline__ uint32_t r16_desc_k(const void* p) { return (smem_u32(p) >> 4) | R16_LBO_K; }
 __device__ __forceinline__ uint32_t r16_desc_mn(const void* p) { return (smem_u32(p) >> 4) | R16_LBO_MN; }
 // kind::f16 with bfloat16 (PL = 1) or half-precision operands and fp32 sums, M = 128.
 __device__ __forceinline__ constexpr uint32_t r16_idesc(int pl, bool b_mn, int n) {
   return (1u << 4) | (pl == 1 ? (1u << 7) | (1u << 10) : 0u) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(R16_T >> 4) << 24);
-}
-__device__ __forceinline__ void r16_mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
-      "mov.b64 da, {%1, %5};\n\t"
-      "mov.b64 db, {%2, %5};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%6, %6, %6, %6}, p;\n\t}"
-      ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(R16_DESC_HI), "r"(0u)
-      : "memory");
 }
 // A from tensor memory: row r in lane r, elements 2 c and 2 c + 1 of the contraction in column c.
 __device__ __forceinline__ void r16_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
@@ -85,7 +73,7 @@ __device__ __forceinline__ void r16_mma_ts(uint32_t d, uint32_t a, uint32_t b_lo
       "mov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%6, %6, %6, %6}, p;\n\t}"
-      ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(R16_DESC_HI), "r"(0u)
+      ::"r"(d), "r"(a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(UMMA_DESC_HI), "r"(0u)
       : "memory");
 }
 __device__ __forceinline__ void r16_st16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -107,16 +95,16 @@ __device__ __forceinline__ void r16_scores(uint32_t d, uint32_t a_k, uint32_t b_
 #pragma unroll
     for (int ks = 0; ks < 4; ks++) {
       const uint32_t o = (uint32_t)ks * 2;
-      r16_mma_ss(d, a_k + o, b_k + CH + o, idesc, ks > 0 ? 1u : 0u);
-      r16_mma_ss(d, a_k + CH + o, b_k + o, idesc, 1u);
+      umma_f16_ss(d, a_k + o, b_k + CH + o, idesc, ks > 0 ? 1u : 0u);
+      umma_f16_ss(d, a_k + CH + o, b_k + o, idesc, 1u);
     }
 #pragma unroll
-    for (int ks = 0; ks < 4; ks++) r16_mma_ss(d, a_k + (uint32_t)ks * 2, b_k + (uint32_t)ks * 2, idesc, 1u);
+    for (int ks = 0; ks < 4; ks++) umma_f16_ss(d, a_k + (uint32_t)ks * 2, b_k + (uint32_t)ks * 2, idesc, 1u);
   } else {
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ks++) {
       const uint32_t o = (uint32_t)(ks / 4) * CH + (uint32_t)(ks % 4) * 2;
-      r16_mma_ss(d, a_k + o, b_k + o, idesc, ks > 0 ? 1u : 0u);
+      umma_f16_ss(d, a_k + o, b_k + o, idesc, ks > 0 ? 1u : 0u);
     }
   }
 }
