@@ -576,14 +576,16 @@ typedef struct om_attention_rule {
  * products are fp32, or, where d is a multiple of 8 up to 64 and there are 96 keys (backward: keys or queries) or more, tensor products
  * of two half-precision numbers a value, 22 bits. Which of the two depends on nothing but sizes, alignment and, for each head of k
  * and v by itself, on whether its rows (and those of its queries and output gradients) are within 2^14 of the largest of their tensor,
- * which itself lies within 2^-46 to 2^45.
+ * which itself lies within 2^-46 to 2^45; the fp32 products take up to six times as long. Errors are those of fp32 arithmetic over a
+ * row: an operand's value is exact to 22 bits or to 2^-39 of the largest of its tensor and head, whichever is more.
  * lse [b, h, lq] (may be NULL) receives the row log-sum-exp for the backward. lk == 0 gives zeros. */
 int32_t om_rule_attention_fwd(om_ctx* ctx, const om_attention_rule* rule, const float* q, const om_head_strides* qs, const float* k,
                               const om_head_strides* ks, const float* v, const om_head_strides* vs, int32_t b, int32_t h,
                               int32_t hkv, int32_t lq, int32_t lk, int32_t d, float scale, float* out, const om_head_strides* os,
                               float* lse);
 /* dq, dk, dv (each may be NULL) from g = dOut, the forward's output and its log-sum-exp; the gradient of a key head is the sum
- * over its query heads in increasing order. Beside om_attention_bwd_strided_out. */
+ * over its query heads in increasing order (zeros where there is none). Beside om_attention_bwd_strided_out. Tensor products are for at
+ * most 131072 queries and keys here and in the bfloat16 form. */
 int32_t om_rule_attention_bwd(om_ctx* ctx, const om_attention_rule* rule, const float* g, const om_head_strides* gs, const float* q,
                               const om_head_strides* qs, const float* k, const om_head_strides* ks, const float* v,
                               const om_head_strides* vs, const float* out, const om_head_strides* os, const float* lse, int32_t b,

@@ -15,7 +15,8 @@
 // all heads that share them; rows are keys: S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q) and once in rule16_dq_kernel (a
 // CTA per 128 queries walks the keys: dQ += dS K). Seven products for five, but no partial sums through memory: a part of dQ per
 // (query tile, key tile) is 128 KB of traffic against 0.3 us of tensor time for the two products that are done again.
-// P and dS are rounded to bfloat16 as operands (the only roundings of the backward besides the results').
+// P and dS are rounded to bfloat16 as operands; the row dots come from the output as the caller has kept it, fp32 or bfloat16. Other
+// roundings of the backward are the results' alone.
 //
 // fp32 operands of heads up to 64 columns run on the same kernels (PL = 2) with fp32 accuracy: every value as two half-precision numbers
 // h + l, 22 significant bits, side by side in a row of 128 columns where two blocks of 64 lie otherwise, and a product as h h' + h l' +
@@ -1630,10 +1631,10 @@ __global__ void __launch_bounds__(256) rule16_split_kernel(const __grid_constant
 }
 
 // fp32 calls that are worth the two passes over the operands in front. What decides is the longest walk of a block: the fp32 kernels take
-// 0.2 to 0.4 us for each key or query of it, however little else there is, these a fixed 22 us forward and 55 us both ways and hardly more
-// for a long walk. Forward and backward of 12 heads of 64, fp32 kernels against these: length 64, one batch 58 and 61 us, 64 batches
-// 225 and 266; 96, 16 batches 181 and 114; 128, one batch 120 and 78; 256 163 and 77; 1024 822 and 145. One query to 512 keys 171 and 78.
-// 96 is where both directions together come out even or better with every number of batches and with heads of 8 to 64.
+// 0.2 to 0.4 us for each key or query of it, however little else there is, these a fixed 25 us forward and 60 us both ways and hardly more
+// for a long walk. Forward and backward of 12 heads of 64, fp32 kernels against these: length 64, one batch 58 and 65 us, 64 batches
+// 225 and 275; 96, one batch 85 and 63, 16 batches 181 and 117; 128, one batch 92 and 66; 256 163 and 74; 1024 818 and 143. One query to 512
+// keys, forward, 68 and 25. 96 is where both directions together come out even or better with every number of batches and with heads of 8 to 64.
 constexpr int R16_WALK = 96;
 bool rule16_planes_take(const RuleCall& c, bool backward) {
   return r16_shape(c) && c.d <= 64 && c.r.lk <= R16_PLAN * R16_T && (!backward || c.r.lq <= R16_PLAN * R16_T) &&
